@@ -208,7 +208,7 @@ def _quantise(case, x):
     x = torch.nan_to_num(x, nan=0.0, posinf=_LIMIT, neginf=-_LIMIT).clamp(-_LIMIT, _LIMIT)
     x = x.unflatten(-1, (case["dim"] // case["group"], case["group"]))
     low = x.amin(-1, keepdim=True).half().float()
-    scale = ((x.amax(-1, keepdim=True) - low).clamp_min(0) / 15.0).half().float()
+    scale = ((x.amax(-1, keepdim=True) - low).clamp_min(0) / x.new_full((), 15.0)).half().float()
     code = torch.where(scale > 0, torch.round((x - low) / torch.where(scale > 0, scale, 1.0)), 0.0).clamp(0, 15)
     code = code.flatten(-2).to(torch.uint8)
     return code[..., 0::2] | (code[..., 1::2] << 4), torch.cat((scale, low), -1).half()
