@@ -73,7 +73,9 @@ typedef enum w4a16_status {
     W4A16_ERR_DEVICE_TIMEOUT = 15,   /* a kernel's bounded wait ran out (see w4a16_device_status) */
     W4A16_ERR_WORKSPACE = 16,        /* workspace missing, too small or misaligned */
     W4A16_ERR_FLAGS = 17,            /* flags holds bits that are not w4a16_flags values */
-    W4A16_ERR_TP_GROUP = 18          /* a w4a16_tp_group or an exchange's sizes are not usable */
+    W4A16_ERR_TP_GROUP = 18,         /* a w4a16_tp_group or an exchange's sizes are not usable */
+    W4A16_ERR_CACHE = 19,            /* a w4a16_cache, or the sizes of a call on it, are not usable */
+    W4A16_ERR_ACT_DTYPE = 20         /* dtype is not a w4a16_act_dtype value */
 } w4a16_status;
 
 typedef enum w4a16_flags {
@@ -260,6 +262,113 @@ w4a16_status w4a16_tp_allreduce(const w4a16_tp_group* group, uint64_t partial_of
  * == 0.  Replaces an NCCL all-gather and the copy into y's column order. */
 w4a16_status w4a16_tp_allgather(const w4a16_tp_group* group, uint64_t src_off, uint64_t y_off, int64_t M,
                                 int64_t N, void* stream);
+
+/* ------------------------------------------------------------------------------
+ * 4-bit key/value cache: append (with rotary positions), read back, attention.  No
+ * counterpart in the reference, which has the GEMM only; these are what a decoder served
+ * with it needs between its QKV and its output projection.
+ *
+ * Format.  The cache is paged: `data` holds num_pages x kv_heads blocks of
+ * page_size * (D + 8 * D / G) bytes, D = head_dim and G = group_size.  A block (one page,
+ * one head) is, one after the other: the codes of the keys [page_size][D / 2], the codes of
+ * the values [page_size][D / 2], the fp16 pairs (scale, minimum) of the keys
+ * [page_size][D / G][2] and those of the values.  Byte i of a token's codes holds value 2i
+ * in its low and value 2i + 1 in its high four bits.  A cached value is code * scale +
+ * minimum.  Slot s is row s % page_size of page s / page_size.
+ *
+ * Quantisation (per token, head and group of G values x, in fp32): NaN becomes 0, values are
+ * clamped to +-W4A16_CACHE_LIMIT (so everything read back is finite), minimum = fp16(min x),
+ * scale = fp16(max(max x - minimum, 0) / 15), code = clamp(round-half-even((x - minimum) /
+ * scale), 0, 15), or 0 where scale is 0.
+ *
+ * head_dim is 64 or 128, group_size 64 or 128 and at most head_dim, page_size 16, 32, 64,
+ * 128 or 256.  Activations are fp16 or bf16 (w4a16_act_dtype), their last dimension dense,
+ * pointers 16-byte aligned and strides (in elements) multiples of 8.  Calls follow the
+ * library's stream order: nothing is read before the previous kernel on the stream is done. */
+#define W4A16_CACHE_LIMIT 57344.0f
+
+typedef enum w4a16_act_dtype {
+    W4A16_ACT_F16 = 0,
+    W4A16_ACT_BF16 = 1
+} w4a16_act_dtype;
+
+typedef struct w4a16_cache {
+    void* data;              /* num_pages * kv_heads * w4a16_cache_page_bytes(...) bytes, 16-byte aligned */
+    int64_t num_pages;
+    int32_t page_size;
+    int32_t kv_heads;
+    int32_t head_dim;
+    int32_t group_size;
+} w4a16_cache;
+
+/* Rotary positions applied by an append to its keys, and to the queries that come with them.
+ * The pair of angle i (0 <= i < rotary_dim / 2) is values (i, i + rotary_dim / 2), or (2i, 2i
+ * + 1) if interleaved; values from rotary_dim on are left as they are.  (a, b) becomes (a c -
+ * b s, b c + a s) in fp32, c = cos_sin[p][i], s = cos_sin[p][rotary_dim / 2 + i], with p the
+ * token's position on the axis of angle i: the first sections[0] angles belong to axis 0, the
+ * next sections[1] to axis 1, the rest to axis 2.  Positions are clamped to [0, max_pos). */
+typedef struct w4a16_rotary {
+    const void* q;           /* [tokens][q_heads][head_dim], the append's dtype; NULL: keys only */
+    void* q_out;             /* dense [tokens][q_heads][head_dim]; may be q itself if q is dense */
+    int64_t q_token_stride, q_head_stride;
+    const int64_t* positions;          /* [axes][tokens] */
+    int64_t positions_axis_stride;
+    const float* cos_sin;    /* dense [max_pos][rotary_dim]: cosines, then sines; 16-byte aligned */
+    int64_t max_pos;
+    int32_t q_heads;
+    int32_t axes;            /* 1..3 */
+    int32_t sections[3];     /* angles of each axis; sum rotary_dim / 2 (ignored for one axis) */
+    int32_t rotary_dim;      /* head_dim or head_dim / 2 */
+    int32_t interleaved;
+} w4a16_rotary;
+
+typedef struct w4a16_cache_attention_args {
+    const void* q;           /* [q_tokens][q_heads][head_dim] */
+    void* out;               /* dense [q_tokens][q_heads][head_dim], same dtype */
+    float* lse;              /* dense [q_tokens][q_heads] or NULL: natural log of the sum of exp(score) */
+    int64_t q_token_stride, q_head_stride;
+    int64_t q_tokens;
+    const int32_t* page_table;         /* [batch][table_pages]: pages of each sequence in order */
+    int64_t page_table_stride;
+    const int32_t* seq_lens; /* [batch]: cached tokens, those of the queries included */
+    const int32_t* cu_q;     /* [batch + 1]: first query of each sequence; NULL: one query a sequence */
+    float scale;             /* of the scores, usually 1 / sqrt(head_dim) */
+    int32_t dtype;           /* w4a16_act_dtype of q and out */
+    int32_t q_heads;         /* a multiple of kv_heads */
+    int32_t batch;
+    int32_t table_pages;
+    int32_t max_q;           /* no sequence has more queries (1 if cu_q is NULL) */
+    int32_t causal;          /* 0: a query sees every cached token of its sequence */
+    int32_t window;          /* > 0: a query at position p sees tokens above p - window only */
+} w4a16_cache_attention_args;
+
+/* Bytes of one (page, head) block. */
+w4a16_status w4a16_cache_page_bytes(int32_t page_size, int32_t head_dim, int32_t group_size, uint64_t* bytes);
+
+/* Quantises k and v ([tokens][kv_heads][head_dim]) into the slots (int64 [tokens]; a slot
+ * outside the cache is skipped; of equal slots one, unspecified, is kept per value).
+ * rotary (may be NULL): keys are turned before they are quantised, and queries into q_out. */
+w4a16_status w4a16_cache_append(const w4a16_cache* cache, const void* k, const void* v, int64_t k_token_stride,
+                                int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, int32_t dtype,
+                                const int64_t* slots, int64_t tokens, const w4a16_rotary* rotary, void* stream);
+
+/* Reads slots back into dense k_out, v_out [tokens][kv_heads][head_dim] (code * scale +
+ * minimum in fp32, rounded once); a slot outside the cache gives zeros. */
+w4a16_status w4a16_cache_read(const w4a16_cache* cache, const int64_t* slots, int64_t tokens, void* k_out,
+                              void* v_out, int32_t dtype, void* stream);
+
+/* out = softmax(scale * q K^T + mask) V over each sequence's cached tokens.  Query i of the T
+ * of a sequence of L cached tokens has position L - T + i; with `causal` it sees tokens up to
+ * its position.  A query that sees no token gives zeros and lse -inf.  q_heads / kv_heads
+ * query heads share a key head (head h reads key head h / (q_heads / kv_heads)).  Entries of
+ * the page table past a sequence's end are not used; lengths are clamped to the table. */
+w4a16_status w4a16_cache_attention(const w4a16_cache* cache, const w4a16_cache_attention_args* args, void* workspace,
+                                   uint64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of a call with these sizes (pointers in args are not read): scratch, no
+ * initialisation, 256-byte aligned, one per concurrent call. */
+w4a16_status w4a16_cache_attention_workspace(const w4a16_cache* cache, const w4a16_cache_attention_args* args,
+                                             uint64_t* bytes);
 
 /* Reads the current device's status word, set by a kernel whose bounded wait
  * ran out (0 = none).  Synchronises the device.  reset != 0 clears it. */

@@ -30,6 +30,7 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3"]
 
+LIB_SOURCES = ["kernels.cu", "cache.cu", "capi.cpp"]
 LIB_PATH = os.path.join(OUT_DIR, "libw4a16.so")
 EXT_PATH = os.path.join(OUT_DIR, "_C" + sysconfig.get_config_var("EXT_SUFFIX"))
 
@@ -59,8 +60,8 @@ def build_library(force=False):
     if not force and not _stale(LIB_PATH, deps):
         return LIB_PATH
     tmp = LIB_PATH + ".tmp"
-    _run([NVCC, *ARCH_FLAGS, *NVCC_FLAGS, "-shared", "-I", INCLUDE,
-          os.path.join(CSRC, "kernels.cu"), os.path.join(CSRC, "capi.cpp"), "-o", tmp])
+    _run([NVCC, *ARCH_FLAGS, *NVCC_FLAGS, "--threads", "2", "-shared", "-I", INCLUDE,
+          *[os.path.join(CSRC, f) for f in LIB_SOURCES], "-o", tmp])
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 

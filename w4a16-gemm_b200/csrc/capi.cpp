@@ -419,6 +419,193 @@ w4a16_status w4a16_tp_allgather(const w4a16_tp_group* group, uint64_t src_off, u
     return tp_launch(true, group, src_off, y_off, M, N, stream);
 }
 
+// ------------------------------------------------------------------ 4-bit key/value cache
+namespace {
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+w4a16_status cuda_fail(cudaError_t err) {
+    return fail(W4A16_ERR_CUDA, std::string("kernel launch failed: ") + cudaGetErrorString(err));
+}
+
+w4a16_status check_cache_format(int32_t page_size, int32_t head_dim, int32_t group_size) {
+    if (head_dim != 64 && head_dim != 128)
+        return fail(W4A16_ERR_CACHE, "unsupported head_dim " + std::to_string(head_dim) + ", supported: 64, 128");
+    if ((group_size != 64 && group_size != 128) || group_size > head_dim)
+        return fail(W4A16_ERR_GROUP_SIZE, "unsupported group size " + std::to_string(group_size) +
+                                              ", supported: 64, 128, at most head_dim");
+    if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128 && page_size != 256)
+        return fail(W4A16_ERR_CACHE, "unsupported page_size " + std::to_string(page_size) +
+                                         ", supported: 16, 32, 64, 128, 256");
+    return ok();
+}
+
+w4a16_status check_cache(const w4a16_cache* c) {
+    if (!c) return fail(W4A16_ERR_NULL_POINTER, "cache must be non-null");
+    w4a16_status s = check_cache_format(c->page_size, c->head_dim, c->group_size);
+    if (s != W4A16_OK) return s;
+    if (c->kv_heads < 1 || c->kv_heads > 1024) return fail(W4A16_ERR_CACHE, "kv_heads must be in [1, 1024]");
+    if (c->num_pages < 1 || c->num_pages >= (1LL << 31)) return fail(W4A16_ERR_CACHE, "num_pages must be in [1, 2^31)");
+    return ok();
+}
+
+w4a16_status check_act_dtype(int32_t dtype) {
+    if (dtype != W4A16_ACT_F16 && dtype != W4A16_ACT_BF16)
+        return fail(W4A16_ERR_ACT_DTYPE, "dtype must be 0 (fp16) or 1 (bf16)");
+    return ok();
+}
+
+bool strides8(int64_t a, int64_t b) { return a % 8 == 0 && b % 8 == 0; }
+
+// Everything of an attention call but its pointers.
+w4a16_status check_attention_sizes(const w4a16_cache* c, const w4a16_cache_attention_args* a) {
+    w4a16_status s = check_cache(c);
+    if (s != W4A16_OK) return s;
+    if (!a) return fail(W4A16_ERR_NULL_POINTER, "args must be non-null");
+    if ((s = check_act_dtype(a->dtype)) != W4A16_OK) return s;
+    if (a->q_heads < 1 || a->q_heads % c->kv_heads || a->q_heads > 65536)
+        return fail(W4A16_ERR_CACHE, "q_heads must be a multiple of kv_heads");
+    if (a->batch < 0 || a->batch > 65535 || a->table_pages < 0)
+        return fail(W4A16_ERR_CACHE, "batch must be in [0, 65535] and table_pages must not be negative");
+    if (a->q_tokens < 0 || a->q_tokens * a->q_heads >= (1LL << 31))
+        return fail(W4A16_ERR_DIM_RANGE, "q_tokens * q_heads must fit in int32");
+    if (a->max_q < 0 || a->max_q > a->q_tokens) return fail(W4A16_ERR_CACHE, "max_q must be in [0, q_tokens]");
+    if ((int64_t)a->table_pages * c->page_size >= (1LL << 31))
+        return fail(W4A16_ERR_DIM_RANGE, "a sequence's tokens (table_pages * page_size) must fit in int32");
+    if (a->window < 0) return fail(W4A16_ERR_CACHE, "window must not be negative (0: none)");
+    if (!(a->scale == a->scale)) return fail(W4A16_ERR_CACHE, "scale must be a number");
+    return ok();
+}
+
+}  // namespace
+
+w4a16_status w4a16_cache_page_bytes(int32_t page_size, int32_t head_dim, int32_t group_size, uint64_t* bytes) {
+    w4a16_status s = check_cache_format(page_size, head_dim, group_size);
+    if (s != W4A16_OK) return s;
+    if (!bytes) return fail(W4A16_ERR_NULL_POINTER, "bytes must be non-null");
+    *bytes = (uint64_t)page_size * (uint64_t)(head_dim + 8 * (head_dim / group_size));
+    return ok();
+}
+
+w4a16_status w4a16_cache_append(const w4a16_cache* cache, const void* k, const void* v, int64_t k_token_stride,
+                                int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, int32_t dtype,
+                                const int64_t* slots, int64_t tokens, const w4a16_rotary* rotary, void* stream) {
+    w4a16_status s = check_cache(cache);
+    if (s != W4A16_OK) return s;
+    if ((s = check_act_dtype(dtype)) != W4A16_OK) return s;
+    const int64_t q_heads = rotary && rotary->q ? rotary->q_heads : 0;
+    if (tokens < 0 || tokens * (cache->kv_heads + q_heads) >= (1LL << 31))
+        return fail(W4A16_ERR_DIM_RANGE, "tokens * heads must fit in int32");
+    if (rotary) {
+        const w4a16_rotary& r = *rotary;
+        if (r.rotary_dim != cache->head_dim && r.rotary_dim != cache->head_dim / 2)
+            return fail(W4A16_ERR_CACHE, "rotary_dim must be head_dim or head_dim / 2");
+        if (r.axes < 1 || r.axes > 3) return fail(W4A16_ERR_CACHE, "positions must have 1 to 3 axes");
+        if (r.axes > 1) {
+            int64_t sum = 0;
+            for (int i = 0; i < r.axes; ++i) {
+                if (r.sections[i] < 0) return fail(W4A16_ERR_CACHE, "sections must not be negative");
+                sum += r.sections[i];
+            }
+            if (sum != r.rotary_dim / 2) return fail(W4A16_ERR_CACHE, "sections must add up to rotary_dim / 2");
+        }
+        if (r.max_pos < 1) return fail(W4A16_ERR_CACHE, "cos_sin must hold at least one position");
+        if (r.q && (r.q_heads < 1 || r.q_heads > 65536)) return fail(W4A16_ERR_CACHE, "q_heads must be at least 1");
+    }
+    if (tokens == 0) return ok();
+    if (!cache->data || !k || !v || !slots) return fail(W4A16_ERR_NULL_POINTER, "cache data, k, v and slots must be non-null");
+    if (!aligned16(cache->data) || !aligned16(k) || !aligned16(v))
+        return fail(W4A16_ERR_ALIGNMENT, "cache data, k and v must be 16-byte aligned");
+    if (!strides8(k_token_stride, k_head_stride) || !strides8(v_token_stride, v_head_stride))
+        return fail(W4A16_ERR_ALIGNMENT, "strides of k and v must be multiples of 8 elements");
+    if (rotary) {
+        const w4a16_rotary& r = *rotary;
+        if (!r.positions || !r.cos_sin || (r.q && !r.q_out))
+            return fail(W4A16_ERR_NULL_POINTER, "positions, cos_sin and q_out must be non-null");
+        if (!aligned16(r.cos_sin) || !aligned16(r.q) || !aligned16(r.q_out) ||
+            (r.q && !strides8(r.q_token_stride, r.q_head_stride)))
+            return fail(W4A16_ERR_ALIGNMENT, "cos_sin, q and q_out must be 16-byte aligned, q's strides multiples of 8 elements");
+    }
+    w4a16::DeviceInfo d;
+    if ((s = check_device(&d)) != W4A16_OK) return s;
+    w4a16::CacheAppendArgs a = {};
+    a.c = *cache;
+    a.k = k;
+    a.v = v;
+    a.k_token_stride = k_token_stride;
+    a.k_head_stride = k_head_stride;
+    a.v_token_stride = v_token_stride;
+    a.v_head_stride = v_head_stride;
+    a.bf16 = dtype == W4A16_ACT_BF16;
+    a.slots = slots;
+    a.tokens = tokens;
+    a.rotate = rotary != nullptr;
+    if (rotary) a.r = *rotary;
+    a.stream = static_cast<cudaStream_t>(stream);
+    a.pdl = pdl_enabled();
+    const cudaError_t err = w4a16::launch_cache_append(a);
+    return err == cudaSuccess ? ok() : cuda_fail(err);
+}
+
+w4a16_status w4a16_cache_read(const w4a16_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out,
+                              int32_t dtype, void* stream) {
+    w4a16_status s = check_cache(cache);
+    if (s != W4A16_OK) return s;
+    if ((s = check_act_dtype(dtype)) != W4A16_OK) return s;
+    if (tokens < 0 || tokens * cache->kv_heads >= (1LL << 31))
+        return fail(W4A16_ERR_DIM_RANGE, "tokens * heads must fit in int32");
+    if (tokens == 0) return ok();
+    if (!cache->data || !slots || !k_out || !v_out)
+        return fail(W4A16_ERR_NULL_POINTER, "cache data, slots, k_out and v_out must be non-null");
+    if (!aligned16(cache->data) || !aligned16(k_out) || !aligned16(v_out))
+        return fail(W4A16_ERR_ALIGNMENT, "cache data, k_out and v_out must be 16-byte aligned");
+    w4a16::DeviceInfo d;
+    if ((s = check_device(&d)) != W4A16_OK) return s;
+    const cudaError_t err = w4a16::launch_cache_read(*cache, slots, tokens, k_out, v_out, dtype == W4A16_ACT_BF16,
+                                                     static_cast<cudaStream_t>(stream), pdl_enabled());
+    return err == cudaSuccess ? ok() : cuda_fail(err);
+}
+
+w4a16_status w4a16_cache_attention_workspace(const w4a16_cache* cache, const w4a16_cache_attention_args* args,
+                                             uint64_t* bytes) {
+    w4a16_status s = check_attention_sizes(cache, args);
+    if (s != W4A16_OK) return s;
+    if (!bytes) return fail(W4A16_ERR_NULL_POINTER, "bytes must be non-null");
+    *bytes = 0;
+    if (args->batch == 0 || args->q_tokens == 0 || args->max_q == 0) return ok();
+    w4a16::DeviceInfo d;
+    if ((s = check_device(&d)) != W4A16_OK) return s;
+    *bytes = w4a16::cache_attention_workspace(*cache, *args, d);
+    return ok();
+}
+
+w4a16_status w4a16_cache_attention(const w4a16_cache* cache, const w4a16_cache_attention_args* args, void* workspace,
+                                   uint64_t workspace_bytes, void* stream) {
+    w4a16_status s = check_attention_sizes(cache, args);
+    if (s != W4A16_OK) return s;
+    if (args->batch == 0 || args->q_tokens == 0 || args->max_q == 0) return ok();
+    if (!cache->data || !args->q || !args->out || !args->seq_lens || (!args->page_table && args->table_pages > 0))
+        return fail(W4A16_ERR_NULL_POINTER, "cache data, q, out, page_table and seq_lens must be non-null");
+    if (!args->cu_q && args->max_q != 1) return fail(W4A16_ERR_CACHE, "without cu_q every sequence has one query: max_q must be 1");
+    if (!aligned16(cache->data) || !aligned16(args->q) || !aligned16(args->out))
+        return fail(W4A16_ERR_ALIGNMENT, "cache data, q and out must be 16-byte aligned");
+    if (!strides8(args->q_token_stride, args->q_head_stride))
+        return fail(W4A16_ERR_ALIGNMENT, "strides of q must be multiples of 8 elements");
+    w4a16::DeviceInfo d;
+    if ((s = check_device(&d)) != W4A16_OK) return s;
+    const size_t need = w4a16::cache_attention_workspace(*cache, *args, d);
+    if (need > 0) {
+        if (!workspace) return fail(W4A16_ERR_WORKSPACE, "this call needs a workspace of " + std::to_string(need) + " bytes");
+        if (workspace_bytes < need)
+            return fail(W4A16_ERR_WORKSPACE, "workspace too small: " + std::to_string(workspace_bytes) + " < " +
+                                                 std::to_string(need) + " bytes");
+        if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(W4A16_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+    }
+    const cudaError_t err = w4a16::launch_cache_attention(*cache, *args, d, workspace, static_cast<cudaStream_t>(stream),
+                                                          pdl_enabled());
+    return err == cudaSuccess ? ok() : cuda_fail(err);
+}
+
 w4a16_status w4a16_device_status(int32_t* code, int32_t reset) {
     if (!code) return fail(W4A16_ERR_NULL_POINTER, "code must be non-null");
     int c = 0;
@@ -467,6 +654,8 @@ const char* w4a16_status_string(w4a16_status status) {
         case W4A16_ERR_WORKSPACE: return "W4A16_ERR_WORKSPACE";
         case W4A16_ERR_FLAGS: return "W4A16_ERR_FLAGS";
         case W4A16_ERR_TP_GROUP: return "W4A16_ERR_TP_GROUP";
+        case W4A16_ERR_CACHE: return "W4A16_ERR_CACHE";
+        case W4A16_ERR_ACT_DTYPE: return "W4A16_ERR_ACT_DTYPE";
     }
     return "W4A16_ERR_UNKNOWN";
 }

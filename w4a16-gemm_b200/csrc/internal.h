@@ -103,6 +103,29 @@ cudaError_t launch_tp_exchange(bool gather, bool push, const TpPtrs& p, int rank
                                uint64_t y_off, uint64_t recv_off, uint64_t slot_bytes, int M, int N,
                                cudaStream_t stream);
 
+// ---------------------------------------------------------------- 4-bit key/value cache (cache.cu)
+struct CacheAppendArgs {
+    w4a16_cache c;
+    const void *k, *v;
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    bool bf16;
+    const int64_t* slots;
+    int64_t tokens;
+    bool rotate;
+    w4a16_rotary r;       // set if rotate
+    cudaStream_t stream;
+    bool pdl;
+};
+cudaError_t launch_cache_append(const CacheAppendArgs& a);
+cudaError_t launch_cache_read(const w4a16_cache& c, const int64_t* slots, int64_t tokens, void* k, void* v, bool bf16,
+                              cudaStream_t stream, bool pdl);
+// Workspace bytes and launch of one validated attention call (rows of q > 0, batch > 0).
+size_t cache_attention_workspace(const w4a16_cache& c, const w4a16_cache_attention_args& a, const DeviceInfo& dev);
+cudaError_t launch_cache_attention(const w4a16_cache& c, const w4a16_cache_attention_args& a, const DeviceInfo& dev,
+                                   void* workspace, cudaStream_t stream, bool pdl);
+// read_device_status for cache.cu's status word (no synchronisation of its own).
+cudaError_t read_cache_device_status(int* code, bool reset);
+
 // ---------------------------------------------------------------- debug dequant
 cudaError_t launch_dequant(const void* wp, const void* scales, void* out, int N, int K, int G,
                            cudaStream_t stream);

@@ -1,4 +1,4 @@
-// The single device-code translation unit: decode, prefill, dequant and format kernels,
+// The GEMM's device code (the 4-bit cache's is in cache.cu): decode, prefill, dequant and format kernels,
 // the device status word, and the host helpers they need (device properties,
 // shared-memory opt-in, TMA tensor maps).
 #include <cuda.h>
@@ -67,10 +67,15 @@ cudaError_t ensure_max_dynamic_smem(const void* func) {
 cudaError_t read_device_status(int* code, bool reset) {
     cudaError_t err = cudaDeviceSynchronize();
     if (err != cudaSuccess) return err;
+    int cache_code = 0;
+    if ((err = read_cache_device_status(&cache_code, reset)) != cudaSuccess) return err;
     err = cudaMemcpyFromSymbol(code, w4a16_device_status, sizeof(int));
-    if (err != cudaSuccess || !reset) return err;
-    const int zero = 0;
-    return cudaMemcpyToSymbol(w4a16_device_status, &zero, sizeof(int));
+    if (err == cudaSuccess && reset) {
+        const int zero = 0;
+        err = cudaMemcpyToSymbol(w4a16_device_status, &zero, sizeof(int));
+    }
+    if (*code == 0) *code = cache_code;
+    return err;
 }
 
 // One thread waits for phase 0 of an mbarrier that nothing arrives at, with the wait the

@@ -25,11 +25,12 @@ enum DeviceError : int {
     kDevTimeoutPipeline = 4,     // prefill: a producer/consumer barrier never completed
     kDevTimeoutDrain = 5,        // error path: in-flight copies did not land in time
     kDevTimeoutPeer = 7,         // tensor-parallel exchange: a peer rank never arrived
+    kDevTimeoutCache = 8,        // cache attention: a pipeline barrier never completed
 };
 
-// Per-device status word (one definition: this header is included by the single
-// device-code translation unit, kernels.cu).
-__device__ int w4a16_device_status = 0;
+// Per-device status word of this translation unit (kernels.cu and cache.cu have one each;
+// the entry point that reads them reports the first that is set).
+static __device__ int w4a16_device_status = 0;
 
 __device__ __forceinline__ void record_device_error(int code) {
     atomicCAS(&w4a16_device_status, 0, code);

@@ -8,10 +8,12 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <climits>
 #include <map>
 #include <vector>
 #include <mutex>
+#include <tuple>
 #include <utility>
 
 #include "../../include/w4a16.h"
@@ -194,6 +196,188 @@ pybind11::dict query_route_py(int64_t M, int64_t N, int64_t K, int64_t groups, i
     return d;
 }
 
+// ------------------------------------------------------------------ 4-bit key/value cache
+w4a16_cache cache_of(const torch::Tensor& data, int64_t head_dim, int64_t page_size, int64_t group_size) {
+    TORCH_CHECK(data.is_cuda() && data.dtype() == torch::kUInt8 && data.dim() == 3 && data.is_contiguous(),
+                "the cache must be a contiguous CUDA uint8 [pages, kv_heads, page_bytes] tensor");
+    TORCH_CHECK(head_dim > 0 && head_dim <= 1024 && page_size > 0 && page_size <= 4096 && group_size > 0 && group_size <= 1024,
+                "head_dim, page_size and group_size must be positive");
+    uint64_t bytes = 0;
+    check(w4a16_cache_page_bytes((int32_t)page_size, (int32_t)head_dim, (int32_t)group_size, &bytes));
+    TORCH_CHECK((uint64_t)data.size(2) == bytes, "the cache's blocks must hold ", bytes, " bytes, not ", data.size(2));
+    TORCH_CHECK(data.size(1) <= INT_MAX, "dimensions must fit in int32");
+    return w4a16_cache{data.data_ptr(), data.size(0), (int32_t)page_size, (int32_t)data.size(1), (int32_t)head_dim,
+                       (int32_t)group_size};
+}
+
+int32_t act_dtype(torch::ScalarType t, const char* what) {
+    TORCH_CHECK(t == torch::kHalf || t == torch::kBFloat16, what, " must be fp16 or bf16");
+    return t == torch::kHalf ? W4A16_ACT_F16 : W4A16_ACT_BF16;
+}
+
+// [tokens, heads, head_dim] activations with a dense last dimension, on the cache's device.
+void check_act(const torch::Tensor& x, const torch::Tensor& data, int64_t tokens, int64_t heads, int64_t dim,
+               const char* what) {
+    TORCH_CHECK(x.is_cuda() && x.device() == data.device(), what, " must be a CUDA tensor on the cache's device");
+    TORCH_CHECK(x.dim() == 3 && x.size(0) == tokens && x.size(1) == heads && x.size(2) == dim, what, " must be [", tokens,
+                ", ", heads, ", ", dim, "]");
+    TORCH_CHECK(x.stride(2) == 1, what, "'s last dimension must be contiguous");
+}
+
+void check_slots(const torch::Tensor& slots, const torch::Tensor& data) {
+    TORCH_CHECK(slots.is_cuda() && slots.device() == data.device() && slots.dtype() == torch::kInt64 && slots.dim() == 1 &&
+                    slots.is_contiguous(),
+                "slots must be a contiguous int64 [tokens] tensor on the cache's device");
+}
+
+c10::optional<torch::Tensor> cache_append_py(torch::Tensor data, int64_t head_dim, int64_t page_size, int64_t group_size,
+                                             torch::Tensor k, torch::Tensor v, torch::Tensor slots,
+                                             c10::optional<torch::Tensor> q, c10::optional<torch::Tensor> positions,
+                                             c10::optional<torch::Tensor> cos_sin,
+                                             c10::optional<std::vector<int64_t>> sections, bool interleaved) {
+    const w4a16_cache c = cache_of(data, head_dim, page_size, group_size);
+    check_slots(slots, data);
+    const int64_t tokens = slots.size(0);
+    check_act(k, data, tokens, c.kv_heads, head_dim, "k");
+    check_act(v, data, tokens, c.kv_heads, head_dim, "v");
+    const int32_t dtype = act_dtype(k.scalar_type(), "k");
+    TORCH_CHECK(v.scalar_type() == k.scalar_type(), "k and v must have one dtype");
+    const at::cuda::CUDAGuard guard(data.device());
+    w4a16_rotary r = {};
+    torch::Tensor q_out;
+    TORCH_CHECK(positions.has_value() == cos_sin.has_value(), "positions and cos_sin go together");
+    TORCH_CHECK(positions.has_value() || (!q.has_value() && !sections.has_value()),
+                "q and sections need positions and cos_sin");
+    if (positions.has_value()) {
+        const torch::Tensor& p = *positions;
+        const torch::Tensor& t = *cos_sin;
+        TORCH_CHECK(p.is_cuda() && p.device() == data.device() && p.dtype() == torch::kInt64 &&
+                        (p.dim() == 1 || p.dim() == 2) && p.size(-1) == tokens && (tokens < 2 || p.stride(-1) == 1),
+                    "positions must be int64 [tokens] or [axes, tokens] on the cache's device");
+        TORCH_CHECK(t.is_cuda() && t.device() == data.device() && t.dtype() == torch::kFloat && t.dim() == 2 && t.is_contiguous(),
+                    "cos_sin must be a contiguous fp32 [positions, rotary_dim] tensor on the cache's device");
+        TORCH_CHECK(t.size(1) <= INT_MAX, "dimensions must fit in int32");
+        r.positions = p.data_ptr<int64_t>();
+        r.axes = p.dim() == 2 ? (int32_t)std::min<int64_t>(p.size(0), 4) : 1;   // above 3: rejected below the ABI
+        r.positions_axis_stride = p.dim() == 2 ? p.stride(0) : 0;
+        r.cos_sin = t.data_ptr<float>();
+        r.max_pos = t.size(0);
+        r.rotary_dim = (int32_t)t.size(1);
+        r.interleaved = interleaved;
+        TORCH_CHECK(r.axes == 1 || sections.has_value(), "positions of several axes need sections");
+        if (sections.has_value()) {
+            TORCH_CHECK((int64_t)sections->size() == r.axes, "sections must have one entry for each axis");
+            for (size_t i = 0; i < sections->size() && i < 3; ++i)
+                r.sections[i] = (int32_t)std::min<int64_t>(std::max<int64_t>((*sections)[i], -1), INT_MAX);
+        }
+        if (q.has_value()) {
+            TORCH_CHECK(q->dim() == 3 && q->scalar_type() == k.scalar_type(), "q must be [tokens, q_heads, head_dim] of k's dtype");
+            check_act(*q, data, tokens, q->size(1), head_dim, "q");
+            TORCH_CHECK(q->size(1) >= 1 && q->size(1) <= INT_MAX, "q_heads must be at least 1");
+            q_out = torch::empty({tokens, q->size(1), head_dim}, q->options());
+            r.q = q->data_ptr();
+            r.q_out = q_out.data_ptr();
+            r.q_token_stride = q->stride(0);
+            r.q_head_stride = q->stride(1);
+            r.q_heads = (int32_t)q->size(1);
+        }
+    }
+    check(w4a16_cache_append(&c, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), dtype,
+                             slots.data_ptr<int64_t>(), tokens, positions.has_value() ? &r : nullptr,
+                             at::cuda::getCurrentCUDAStream().stream()));
+    if (q_out.defined()) return q_out;
+    return c10::nullopt;
+}
+
+std::tuple<torch::Tensor, torch::Tensor> cache_read_py(torch::Tensor data, int64_t head_dim, int64_t page_size,
+                                                       int64_t group_size, torch::Tensor slots, bool bf16) {
+    const w4a16_cache c = cache_of(data, head_dim, page_size, group_size);
+    check_slots(slots, data);
+    const at::cuda::CUDAGuard guard(data.device());
+    const auto opts = data.options().dtype(bf16 ? torch::kBFloat16 : torch::kHalf);
+    auto k = torch::empty({slots.size(0), c.kv_heads, head_dim}, opts);
+    auto v = torch::empty({slots.size(0), c.kv_heads, head_dim}, opts);
+    check(w4a16_cache_read(&c, slots.data_ptr<int64_t>(), slots.size(0), k.data_ptr(), v.data_ptr(),
+                           bf16 ? W4A16_ACT_BF16 : W4A16_ACT_F16, at::cuda::getCurrentCUDAStream().stream()));
+    return {k, v};
+}
+
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> cache_attention_py(
+    torch::Tensor q, torch::Tensor data, int64_t head_dim, int64_t page_size, int64_t group_size, torch::Tensor page_table,
+    torch::Tensor seq_lens, c10::optional<torch::Tensor> cu_q, int64_t max_q, double scale, bool causal, int64_t window,
+    bool return_lse, c10::optional<torch::Tensor> out, c10::optional<torch::Tensor> workspace) {
+    const w4a16_cache c = cache_of(data, head_dim, page_size, group_size);
+    TORCH_CHECK(q.dim() == 3, "q must be [tokens, q_heads, head_dim]");
+    check_act(q, data, q.size(0), q.size(1), head_dim, "q");
+    auto ints = [&](const torch::Tensor& t, int64_t dim) {
+        return t.is_cuda() && t.device() == data.device() && t.dtype() == torch::kInt32 && t.dim() == dim &&
+               (t.size(dim - 1) < 2 || t.stride(dim - 1) == 1);
+    };
+    TORCH_CHECK(ints(page_table, 2), "page_table must be int32 [batch, pages] on the cache's device");
+    TORCH_CHECK(ints(seq_lens, 1) && seq_lens.size(0) == page_table.size(0), "seq_lens must be int32 [batch] on the cache's device");
+    const int64_t batch = seq_lens.size(0);
+    if (cu_q.has_value()) {
+        TORCH_CHECK(ints(*cu_q, 1) && cu_q->size(0) == batch + 1, "cu_q must be int32 [batch + 1] on the cache's device");
+    } else {
+        TORCH_CHECK(q.size(0) == batch, "without cu_q, q must hold one token for each sequence");
+    }
+    TORCH_CHECK(q.size(1) <= INT_MAX && batch <= INT_MAX && page_table.size(1) <= INT_MAX && max_q >= 0 && max_q <= INT_MAX &&
+                    window >= 0 && window <= INT_MAX, "sizes must fit in int32 and must not be negative");
+    const at::cuda::CUDAGuard guard(data.device());
+    w4a16_cache_attention_args a = {};
+    a.dtype = act_dtype(q.scalar_type(), "q");
+    torch::Tensor y, lse;
+    if (out.has_value()) {
+        y = *out;
+        TORCH_CHECK(y.is_cuda() && y.device() == q.device() && y.scalar_type() == q.scalar_type() && y.sizes() == q.sizes() &&
+                        y.is_contiguous(), "out must be a contiguous tensor of q's shape, dtype and device");
+    } else {
+        y = torch::empty(q.sizes(), q.options());
+    }
+    if (return_lse) {
+        lse = torch::empty({q.size(0), q.size(1)}, q.options().dtype(torch::kFloat));
+        a.lse = lse.data_ptr<float>();
+    }
+    a.q = q.data_ptr();
+    a.out = y.data_ptr();
+    a.q_token_stride = q.stride(0);
+    a.q_head_stride = q.stride(1);
+    a.q_tokens = q.size(0);
+    a.page_table = page_table.data_ptr<int32_t>();
+    a.page_table_stride = page_table.stride(0);
+    a.seq_lens = seq_lens.data_ptr<int32_t>();
+    a.cu_q = cu_q.has_value() ? cu_q->data_ptr<int32_t>() : nullptr;
+    a.scale = (float)scale;
+    a.q_heads = (int32_t)q.size(1);
+    a.batch = (int32_t)batch;
+    a.table_pages = (int32_t)page_table.size(1);
+    a.max_q = (int32_t)max_q;
+    a.causal = causal;
+    a.window = (int32_t)window;
+    cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
+    uint64_t ws_bytes = 0;
+    torch::Tensor ws;
+    if (workspace.has_value()) {
+        ws = *workspace;
+        TORCH_CHECK(ws.is_cuda() && ws.device() == data.device() && ws.is_contiguous(),
+                    "workspace must be a contiguous CUDA tensor on the cache's device");
+        ws_bytes = (uint64_t)ws.numel() * ws.element_size();
+    } else {
+        check(w4a16_cache_attention_workspace(&c, &a, &ws_bytes));
+        ws = workspace_for(data, ws_bytes, stream);
+    }
+    check(w4a16_cache_attention(&c, &a, ws.defined() ? ws.data_ptr() : nullptr, ws_bytes, stream));
+    return {y, return_lse ? c10::optional<torch::Tensor>(lse) : c10::nullopt};
+}
+
+int64_t cache_page_bytes_py(int64_t page_size, int64_t head_dim, int64_t group_size) {
+    TORCH_CHECK(head_dim > 0 && head_dim <= 1024 && page_size > 0 && page_size <= 4096 && group_size > 0 && group_size <= 1024,
+                "head_dim, page_size and group_size must be positive");
+    uint64_t bytes = 0;
+    check(w4a16_cache_page_bytes((int32_t)page_size, (int32_t)head_dim, (int32_t)group_size, &bytes));
+    return (int64_t)bytes;
+}
+
 int64_t device_status_py(bool reset) {
     int32_t code = 0;
     w4a16_status s = w4a16_device_status(&code, reset ? 1 : 0);
@@ -221,5 +405,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("pack", &pack_py, "uint8 codes [N, K] -> packed int32 words (GPU)", pybind11::arg("q"));
     m.def("quantize", &quantize_py, "fp32/fp16 W [N, K] -> (codes or packed words, fp16 scales [K/G, N]) (GPU)",
           pybind11::arg("W"), pybind11::arg("group_size"), pybind11::arg("pack") = false);
+    m.def("cache_page_bytes", &cache_page_bytes_py, "bytes of one (page, head) block of a 4-bit cache");
+    m.def("cache_append", &cache_append_py, "quantise keys and values into a 4-bit cache, with rotary positions");
+    m.def("cache_read", &cache_read_py, "read slots of a 4-bit cache back");
+    m.def("cache_attention", &cache_attention_py, "attention over a 4-bit cache");
     m.attr("ABI_VERSION") = w4a16_abi_version();
 }

@@ -30,6 +30,7 @@ except ImportError as exc:  # pragma: no cover - exercised only when unbuilt
     ) from exc
 
 from .format import dequantize_w4, pack_int4, quantize_pack, quantize_w4, unpack_int4  # noqa: E402
+from .kvcache import Int4KVCache, cache_append, cache_attention, cache_read  # noqa: E402
 
 LIBRARY_PATH = os.path.join(_HERE, "libw4a16.so")
 ABI_VERSION = _C.ABI_VERSION
@@ -97,5 +98,6 @@ __all__ = [
     "w4a16_gemm", "w4a16_gemm_out", "w4a16_dequant", "query_route", "device_status",
     "workspace_bytes", "make_workspace",
     "pack_int4", "unpack_int4", "quantize_w4", "quantize_pack", "dequantize_w4",
+    "Int4KVCache", "cache_append", "cache_read", "cache_attention",
     "LIBRARY_PATH", "ABI_VERSION", "PREFILL_VARIANTS",
 ]

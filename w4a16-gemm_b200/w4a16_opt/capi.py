@@ -24,6 +24,7 @@ STATUS_NAMES = {
     8: "W4A16_ERR_WP_SIZE", 9: "W4A16_ERR_ALIGNMENT", 10: "W4A16_ERR_GROUP_SIZE",
     11: "W4A16_ERR_DECODE_SHAPE", 12: "W4A16_ERR_OUT_DTYPE", 13: "W4A16_ERR_DEVICE", 14: "W4A16_ERR_CUDA",
     15: "W4A16_ERR_DEVICE_TIMEOUT", 16: "W4A16_ERR_WORKSPACE", 17: "W4A16_ERR_FLAGS", 18: "W4A16_ERR_TP_GROUP",
+    19: "W4A16_ERR_CACHE", 20: "W4A16_ERR_ACT_DTYPE",
 }
 TP_MAX_RANKS = 8
 TP_CTRL_BYTES = 8192
@@ -47,6 +48,28 @@ class TpGroup(ctypes.Structure):
     _fields_ = [("rank", ctypes.c_int32), ("world", ctypes.c_int32), ("buf", ctypes.c_void_p * TP_MAX_RANKS),
                 ("buf_bytes", ctypes.c_uint64), ("recv_off", ctypes.c_uint64), ("recv_bytes", ctypes.c_uint64)]
 
+
+class Cache(ctypes.Structure):
+    """w4a16_cache: a paged 4-bit key/value cache."""
+    _fields_ = [("data", _vp), ("num_pages", _i64), ("page_size", _i32), ("kv_heads", _i32), ("head_dim", _i32),
+                ("group_size", _i32)]
+
+
+class Rotary(ctypes.Structure):
+    """w4a16_rotary: positions and tables of an append's rotary embedding."""
+    _fields_ = [("q", _vp), ("q_out", _vp), ("q_token_stride", _i64), ("q_head_stride", _i64), ("positions", _vp),
+                ("positions_axis_stride", _i64), ("cos_sin", _vp), ("max_pos", _i64), ("q_heads", _i32),
+                ("axes", _i32), ("sections", _i32 * 3), ("rotary_dim", _i32), ("interleaved", _i32)]
+
+
+class CacheAttentionArgs(ctypes.Structure):
+    """w4a16_cache_attention_args: one attention call over a cache."""
+    _fields_ = [("q", _vp), ("out", _vp), ("lse", _vp), ("q_token_stride", _i64), ("q_head_stride", _i64),
+                ("q_tokens", _i64), ("page_table", _vp), ("page_table_stride", _i64), ("seq_lens", _vp), ("cu_q", _vp),
+                ("scale", ctypes.c_float), ("dtype", _i32), ("q_heads", _i32), ("batch", _i32), ("table_pages", _i32),
+                ("max_q", _i32), ("causal", _i32), ("window", _i32)]
+
+
 # name -> (restype, argtypes), one entry per declaration in include/w4a16.h
 EXPORTS = {
     "w4a16_abi_version": (_i32, []),
@@ -67,6 +90,13 @@ EXPORTS = {
     "w4a16_peer_free": (_i32, [_vp]),
     "w4a16_tp_allreduce": (_i32, [ctypes.POINTER(TpGroup), _u64, _u64, _i64, _i64, _vp]),
     "w4a16_tp_allgather": (_i32, [ctypes.POINTER(TpGroup), _u64, _u64, _i64, _i64, _vp]),
+    "w4a16_cache_page_bytes": (_i32, [_i32, _i32, _i32, ctypes.POINTER(_u64)]),
+    "w4a16_cache_append": (_i32, [ctypes.POINTER(Cache), _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i64,
+                                  ctypes.POINTER(Rotary), _vp]),
+    "w4a16_cache_read": (_i32, [ctypes.POINTER(Cache), _vp, _i64, _vp, _vp, _i32, _vp]),
+    "w4a16_cache_attention": (_i32, [ctypes.POINTER(Cache), ctypes.POINTER(CacheAttentionArgs), _vp, _u64, _vp]),
+    "w4a16_cache_attention_workspace": (_i32, [ctypes.POINTER(Cache), ctypes.POINTER(CacheAttentionArgs),
+                                               ctypes.POINTER(_u64)]),
     "w4a16_device_status": (_i32, [ctypes.POINTER(_i32), _i32]),
     "w4a16_check_wait_limits": (_i32, [ctypes.POINTER(_i32)]),
     "w4a16_status_string": (ctypes.c_char_p, [_i32]),
