@@ -8,6 +8,8 @@
 #include "ptx.cuh"
 #include "cache_format.cuh"
 #include "cache_attention.cuh"
+#include "cache_decode.cuh"
+#include "cache_rows.cuh"
 
 namespace w4a16 {
 
@@ -135,19 +137,66 @@ static AttentionParams attention_params(const w4a16_cache& c, const w4a16_cache_
     return p;
 }
 
+// How an attention call is run: by rows (query heads of a key head times queries).
+struct AttentionPlan {
+    int nt;              // 8-row tiles of the decode kernel; 0: more rows than it takes
+    int grid;
+    size_t workspace;
+};
+
+template <int D, int G, int NT>
+static AttentionPlan plan_decode_t(const w4a16_cache& c, const w4a16_cache_attention_args& a, const DeviceInfo& dev) {
+    using C = CdCfg<D, G, NT>;
+    const int64_t segments = (int64_t)a.batch * c.kv_heads;
+    const int64_t tiles = ((int64_t)a.table_pages * c.page_size + kCdTile - 1) / kCdTile;
+    AttentionPlan p;
+    p.nt = NT;
+    p.grid = (int)std::max<int64_t>(1, std::min<int64_t>(segments * tiles, (int64_t)C::CTAS * dev.num_sms));
+    p.workspace = cd_info_bytes(segments) + 2 * (size_t)p.grid * cd_slot_floats(C::ROWS, D) * sizeof(float);
+    return p;
+}
+
+static AttentionPlan plan_attention(const w4a16_cache& c, const w4a16_cache_attention_args& a, const DeviceInfo& dev) {
+    const int64_t rows = (int64_t)a.max_q * (a.q_heads / c.kv_heads);
+    AttentionPlan p = {};
+    if (rows > 16) return p;
+    with_format(c, [&](auto d, auto g) {
+        p = rows <= 8 ? plan_decode_t<d.value, g.value, 1>(c, a, dev) : plan_decode_t<d.value, g.value, 2>(c, a, dev);
+        return cudaSuccess;
+    });
+    return p;
+}
+
 size_t cache_attention_workspace(const w4a16_cache& c, const w4a16_cache_attention_args& a, const DeviceInfo& dev) {
-    (void)c; (void)a; (void)dev;
-    return 0;
+    return plan_attention(c, a, dev).workspace;
+}
+
+template <int D, int G, int NT>
+static cudaError_t launch_decode_t(const AttentionParams& ap, const AttentionPlan& plan, cudaStream_t stream, bool pdl) {
+    using C = CdCfg<D, G, NT>;
+    auto kern = cache_decode_kernel<D, G, NT>;
+    cudaError_t err = ensure_max_dynamic_smem(reinterpret_cast<const void*>(kern));
+    if (err != cudaSuccess) return err;
+    err = launch(kern, dim3(plan.grid), kCdThreads, C::SMEM, stream, pdl, ap);
+    if (err != cudaSuccess) return err;
+    // threads of a combine block: enough slices of the parts that a segment may have
+    const int64_t segments = (int64_t)ap.batch * ap.c.kv_heads;
+    const int threads = plan.grid / segments >= 64 ? 512 : 128;
+    const int rows = std::min(C::ROWS, ap.max_q * ap.shared);
+    return launch(cache_decode_combine_kernel<D>, dim3((unsigned)segments, (unsigned)rows), threads, 0, stream, pdl, ap,
+                  (int)C::ROWS);
 }
 
 cudaError_t launch_cache_attention(const w4a16_cache& c, const w4a16_cache_attention_args& a, const DeviceInfo& dev,
                                    void* workspace, cudaStream_t stream, bool pdl) {
-    (void)dev; (void)workspace;
-    const AttentionParams p = attention_params(c, a);
-    const int64_t warps = (int64_t)a.batch * a.max_q * a.q_heads;
-    const dim3 grid((unsigned)((warps + 7) / 8));
+    AttentionParams p = attention_params(c, a);
+    p.workspace = static_cast<char*>(workspace);
+    const AttentionPlan plan = plan_attention(c, a, dev);
     return with_format(c, [&](auto d, auto g) {
-        return launch(cache_attention_kernel<d.value, g.value>, grid, 256, 0, stream, pdl, p);
+        if (plan.nt == 1) return launch_decode_t<d.value, g.value, 1>(p, plan, stream, pdl);
+        if (plan.nt == 2) return launch_decode_t<d.value, g.value, 2>(p, plan, stream, pdl);
+        const int64_t warps = (int64_t)a.batch * a.max_q * a.q_heads;
+        return launch(cache_attention_kernel<d.value, g.value>, dim3((unsigned)((warps + 7) / 8)), 256, 0, stream, pdl, p);
     });
 }
 

@@ -1,0 +1,701 @@
+// Attention of few rows (query heads of a key head times queries of a sequence, at most 16)
+// over the 4-bit cache: one pass over the codes, bound by memory.  Included by cache.cu only.
+//
+// Work.  A unit is 128 cached tokens of one (sequence, key head).  All units of the call,
+// sequence by sequence and head by head, are cut into equal contiguous ranges, one a CTA, so
+// that ragged batches load every SM alike whatever the lengths; lengths are read on the device.
+// A range holds whole segments (a (sequence, head) pair), whose results are written at once,
+// and at most two parts of segments, whose sums go to the workspace for combine_kernel.
+//
+// A CTA is one producer warp, which walks the page table and fills a ring of stages with bulk
+// copies (the runs of key codes, value codes and pairs of each page), and four consumer warps,
+// each with 32 tokens of every stage and its own softmax state; the four states are merged at the
+// end of a segment.
+//
+// Products on the tensor cores, with the codes as they are: a nibble masked in place is the
+// fp16 subnormal c 2^-24 (bits 0-3) or c 2^-20 (bits 4-7), an exact operand, so eight codes cost
+// one shift and four masks.  The odd power of two goes to where it is free: for q K^T into the
+// query fragment, for P V into the result's row.  Scales and minima stay in fp32, outside the
+// products:  q.K_t = s_t (q.c_t) + m_t sum(q),  out = sum_t (w_t s_t) c_t + sum_t w_t m_t.
+// Queries become fp16 after their row is scaled by a power of two (nothing is lost from fp16
+// or bf16 inputs within 2^-24 of the row's largest); w_t s_t becomes fp16 (2^-11 relative) after a
+// power of two taken from the largest s_t seen keeps it within [2^-18, 2^14] for weights
+// down to 2^-24 of the row's largest.  So that its rounding acts on the values' spread and not on
+// their distance from the minimum, the same rounded weights are also multiplied with a constant
+// 8, which is taken from the codes' product and put back in fp32:
+//     out = sum_t fp16(w_t s_t) (c_t - 8) + sum_t w_t (m_t + 8 s_t).
+//
+// Order of the contraction index: lane t of a quad holds G / 4 neighbouring values of a key's
+// group, in the order of the nibbles, and the query fragment follows it; token index i of an
+// 8-token block is row (i >> 1) + 4 (i & 1), so that the value loads of a quad hit both halves
+// of the banks.
+#pragma once
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "cache_attention.cuh"
+
+namespace w4a16 {
+
+constexpr int kCdTile = 128;        // tokens of a unit
+constexpr int kCdWarps = 4;         // consumer warps
+constexpr int kCdWarpTokens = kCdTile / kCdWarps;
+constexpr int kCdThreads = (kCdWarps + 1) * 32;
+
+// What the producer tells the consumers about a stage.
+struct __align__(16) CdStage {
+    int tok0;        // first token of the unit
+    int b, head;
+    int flags;       // 1: first unit of this CTA's part of the segment, 2: last, 4: the part is not all of it
+    int len, nq, q0;
+    int slot;        // workspace slot of the part
+};
+
+template <int D, int G, int NT>
+struct CdCfg {
+    using F = CacheFmt<D, G>;
+    static constexpr int CODES = kCdTile * F::CODE;
+    static constexpr int PAIRS = kCdTile * F::PAIR;
+    static constexpr int STAGE = 2 * (CODES + PAIRS);
+    static constexpr int ROWS = 8 * NT;
+    static constexpr int STAGES = D == 64 ? 5 : 3;
+    static constexpr int LD = D + 4;                               // floats of a row in the merge buffer
+    static constexpr int MERGE = kCdWarps * ROWS * LD * 4;         // [warp][row][LD]: sums, then maximum and sum of weights
+    static constexpr int HDR = STAGES * (int)sizeof(CdStage);
+    static constexpr int SMEM = STAGES * STAGE + MERGE + HDR + 256;
+    static constexpr int CTAS = NT == 1 ? 3 : 2;                   // resident on an SM (shared memory and registers)
+};
+
+// Units of one sequence and key head.
+__device__ __forceinline__ int cd_first_tile(const AttentionParams& p, const SeqSpan& s) {
+    return seen_lo(p, s.len - s.nq) / kCdTile;
+}
+__device__ __forceinline__ int cd_tiles(const AttentionParams& p, const SeqSpan& s) {
+    if (s.nq == 0 || s.len == 0) return 0;
+    return (s.len + kCdTile - 1) / kCdTile - cd_first_tile(p, s);
+}
+
+// Workspace: per (sequence, key head) the CTAs {first, last, first one's slot, 0} that hold
+// parts of it, then 2 slots a CTA of ROWS x (D + 2) floats: sums, maxima, sums of weights.
+__host__ __device__ __forceinline__ size_t cd_info_bytes(int64_t segments) {
+    return (size_t)(segments * 16 + 255) / 256 * 256;
+}
+__host__ __device__ __forceinline__ size_t cd_slot_floats(int rows, int D) {
+    return (size_t)rows * (D + 2);
+}
+
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+
+template <int D, int G, int NT>
+__global__ void __launch_bounds__(kCdThreads, CdCfg<D, G, NT>::CTAS)
+cache_decode_kernel(const __grid_constant__ AttentionParams p) {
+    using C = CdCfg<D, G, NT>;
+    using F = CacheFmt<D, G>;
+    constexpr int NG = F::NG, ST = C::STAGES, ROWS = C::ROWS;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint8_t* merge_p = smem + ST * C::STAGE;
+    CdStage* hdr = reinterpret_cast<CdStage*>(merge_p + C::MERGE);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(hdr + ST);
+    const uint32_t bar0 = smem_u32(bars);
+    auto full = [&](int s) { return bar0 + 8u * s; };
+    auto empty = [&](int s) { return bar0 + 8u * (ST + s); };
+    const uint32_t merge_bar = bar0 + 8u * (2 * ST);
+    long long* found = reinterpret_cast<long long*>(bars + 2 * ST + 2);    // total units, first sequence's base, sequence
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), kCdWarps);
+        }
+        mbar_init(merge_bar, kCdWarps * 32);
+        fence_mbar_init();
+    }
+    pdl_wait();
+    pdl_launch_dependents();
+
+    // ---- this CTA's range of units: a scan over the sequences
+    const int hk = p.c.kv_heads;
+    {
+        long long* warp_sum = found + 4;
+        const int per = (p.batch + kCdThreads - 1) / kCdThreads;
+        const int b0 = min((int)threadIdx.x * per, p.batch), b1 = min(b0 + per, p.batch);
+        long long mine = 0;
+        for (int b = b0; b < b1; ++b) mine += cd_tiles(p, seq_span(p, b));
+        mine *= hk;
+        long long incl = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const long long o = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += o;
+        }
+        if (lane == 31) warp_sum[warp] = incl;
+        __syncthreads();
+        long long before = 0, total = 0;
+#pragma unroll
+        for (int w = 0; w < kCdWarps + 1; ++w) {
+            if (w < warp) before += warp_sum[w];
+            total += warp_sum[w];
+        }
+        const long long u0 = total * blockIdx.x / max(min((long long)gridDim.x, total), 1LL);
+        long long base = before + incl - mine;
+        if (threadIdx.x == 0) found[0] = total;
+        if (u0 >= base && u0 < base + mine) {
+            int b = b0;
+            for (; b < b1; ++b) {
+                const long long n = (long long)cd_tiles(p, seq_span(p, b)) * hk;
+                if (u0 < base + n) break;
+                base += n;
+            }
+            found[1] = base;
+            found[2] = b;
+        }
+        __syncthreads();
+    }
+    const long long total = found[0];
+    const long long ctas = min((long long)gridDim.x, total);      // those with work: a unit at least
+    if (blockIdx.x >= ctas) return;
+    const long long u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
+
+    if (warp == kCdWarps) {
+        // ------------------------------------------------------------ producer
+        const int ps_log = p.c.page_shift;
+        const int rows = min(1 << ps_log, kCdTile);             // tokens of a run
+        const int part = lane & 3, run = lane >> 2;             // this lane's copy: K codes, V codes, K pairs, V pairs
+        const uint32_t unit_b = part < 2 ? F::CODE : F::PAIR;
+        const uint32_t run_bytes = (uint32_t)rows * unit_b;
+        const uint32_t dst_off = (part < 2 ? part * C::CODES : 2 * C::CODES + (part - 2) * C::PAIRS) + run * run_bytes;
+        const uint32_t src_part = part < 2 ? (uint32_t)(part * F::CODE) << ps_log
+                                           : (uint32_t)(2 * F::CODE + (part - 2) * F::PAIR) << ps_log;
+        int b = (int)found[2];
+        long long base = found[1];
+        SeqSpan s = seq_span(p, b);
+        int nt = cd_tiles(p, s), first = cd_first_tile(p, s);
+        int local = (int)(u0 - base);
+        int head = local / nt, tile = local % nt;
+        bool begins = true;
+        long long seg0 = u0 - tile;                              // first unit of the segment
+        int4* info = reinterpret_cast<int4*>(p.workspace);
+        long long it = 0;
+        bool ok = true;
+        for (long long u = u0; u < u1; ++u, ++it) {
+            const int st = (int)(it % ST);
+            const int tok0 = (first + tile) * kCdTile;
+            const int tok = tok0 + run * rows;
+            const bool valid = run * rows < kCdTile && tok < s.len && tok + rows > seen_lo(p, s.len - s.nq);
+            const int64_t page = valid ? page_of(p, b, tok >> ps_log) : 0;
+            const uint8_t* src = cache_block(p.c, page, head) + src_part + (uint32_t)(tok & ((1 << ps_log) - 1)) * unit_b;
+            const bool got = mbar_wait(empty(st), (uint32_t)((it / ST) & 1) ^ 1, kDevTimeoutCache);
+            if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
+            const int runs = __popc(__ballot_sync(0xffffffffu, valid)) / 4;
+            const bool ends = tile + 1 == nt || u + 1 == u1;
+            if (lane == 0) {
+                const bool part_of = seg0 < u0 || seg0 + nt > u1;
+                CdStage h;
+                h.tok0 = tok0; h.b = b; h.head = head;
+                h.flags = (begins ? 1 : 0) | (ends ? 2 : 0) | (part_of ? 4 : 0);
+                h.len = s.len; h.nq = s.nq; h.q0 = s.q0;
+                h.slot = 2 * (int)blockIdx.x + (seg0 > u0 ? 1 : 0);
+                hdr[st] = h;
+                if (tile == 0)
+                    info[(int64_t)b * hk + head] = make_int4((int)blockIdx.x,
+                        (int)(((seg0 + nt) * ctas - 1) / total), seg0 > u0 ? 1 : 0, 0);
+                mbar_arrive_expect_tx(full(st), (uint32_t)(runs * rows * F::TOKEN));
+            }
+            __syncwarp();
+            if (valid) bulk_load(smem_u32(smem + st * C::STAGE) + dst_off, src, run_bytes, full(st));
+            begins = ends;
+            if (++tile == nt) {
+                tile = 0;
+                seg0 = u + 1;
+                if (++head == hk && u + 1 < u1) {
+                    head = 0;
+                    do { s = seq_span(p, ++b); nt = cd_tiles(p, s); } while (nt == 0);
+                    first = cd_first_tile(p, s);
+                }
+            }
+        }
+        if (!ok) {
+            // Error path: the last stages that were issued may still be landing.
+            for (long long j = it > ST ? it - ST : 0; j < it; ++j)
+                mbar_wait(full((int)(j % ST)), (uint32_t)((j / ST) & 1), kDevTimeoutDrain);
+        }
+        return;
+    }
+
+    // ---------------------------------------------------------------- consumers
+    const int g = lane >> 2, t = lane & 3;
+    const int krow = (g >> 1) + 4 * (g & 1);                     // cache row of token index g of an 8-token block
+    constexpr uint32_t LO = 0x000F000Fu, HI = 0x00F000F0u;
+    constexpr int KW = D / 32, VW = D / 64;                      // words of a key / value row that a lane holds
+    float* merge = reinterpret_cast<float*>(merge_p);
+    uint32_t merge_phase = 0;
+
+    uint32_t qf[2 * KW][NT][2];                                  // query fragments, contraction steps of 16
+    float o[4 * VW][NT][4];                                      // sums: (value 2j, rows 2t, 2t+1), (value 2j+1, ...)
+    float oc[NG][NT][4];                                         // the same weights times 8
+    float m[NT][2], thr[NT][2], sum[NT][2], msum[NG][NT][2];
+    float r24[NT][2], qs[NG][NT][2];                             // score = r24 (s (q'.c) + m qs)
+    int lo[NT][2], hi[NT][2];
+    float vlim = 0.f, vmul = 1.f;                                // s_t <= vlim; w_t s_t vmul is what fp16 holds
+    int lo_all = 0, lo_max = 0, hi_min = 0;
+
+    const long long n_units = u1 - u0;
+    for (long long it = 0; it < n_units; ++it) {
+        const int st = (int)(it % ST);
+        if (!__all_sync(0xffffffffu, mbar_wait(full(st), (uint32_t)((it / ST) & 1), kDevTimeoutCache))) return;
+        const CdStage h = hdr[st];
+        if (h.flags & 1) {
+            // ---- a new segment: queries, masks, empty state
+            const int rows = h.nq * p.shared;
+            const int pos0 = h.len - h.nq;
+            lo_all = seen_lo(p, pos0);
+            lo_max = seen_lo(p, h.len - 1);
+            hi_min = seen_hi(p, pos0, h.len);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int row = g + 8 * n;
+                uint4 raw[NG][G / 32];
+                uint32_t amax = 0;
+#pragma unroll
+                for (int a = 0; a < NG; ++a)
+#pragma unroll
+                    for (int j = 0; j < G / 32; ++j) {
+                        raw[a][j] = make_uint4(0, 0, 0, 0);
+                        if (row < rows)
+                            raw[a][j] = __ldg(reinterpret_cast<const uint4*>(
+                                p.q + (int64_t)(h.q0 + row / p.shared) * p.q_token +
+                                (int64_t)(h.head * p.shared + row % p.shared) * p.q_head + a * G + t * (G / 4)) + j);
+                    }
+                float f[NG][G / 4];
+#pragma unroll
+                for (int a = 0; a < NG; ++a)
+#pragma unroll
+                    for (int j = 0; j < G / 32; ++j) {
+                        float x[8];
+                        if (p.bf16) unpack8<true>(raw[a][j], x);
+                        else unpack8<false>(raw[a][j], x);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            f[a][8 * j + e] = x[e];
+                            amax = max(amax, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+                        }
+                    }
+                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                // the row's power of two: its largest value comes to [2^13, 2^14)
+                const int ex = min(max((int)(amax >> 23), 24), 250);
+                const float down = __uint_as_float((uint32_t)(267 - ex) << 23 & 0x7F800000u);   // 2^(140 - ex)
+                const float back = __uint_as_float((uint32_t)(ex - 13) << 23);                  // 2^(ex - 140)
+                float total_q[NG];
+#pragma unroll
+                for (int a = 0; a < NG; ++a) {
+                    total_q[a] = 0.f;
+#pragma unroll
+                    for (int e = 0; e < G / 4; ++e) {
+                        f[a][e] *= down;
+                        total_q[a] += __half2float(__float2half_rn(f[a][e]));
+                    }
+                    total_q[a] += __shfl_xor_sync(0xffffffffu, total_q[a], 1);
+                    total_q[a] += __shfl_xor_sync(0xffffffffu, total_q[a], 2);
+#pragma unroll
+                    for (int w = 0; w < G / 32; ++w) {
+                        const float* x = &f[a][8 * w];
+                        const int c = 2 * (a * (G / 32) + w);
+                        qf[c][n][0] = pack16(x[0], x[4], false);
+                        qf[c][n][1] = pack16(x[1] * 0.0625f, x[5] * 0.0625f, false);
+                        qf[c + 1][n][0] = pack16(x[2], x[6], false);
+                        qf[c + 1][n][1] = pack16(x[3] * 0.0625f, x[7] * 0.0625f, false);
+                    }
+                }
+                const float r = back * p.scale_log2 * 16777216.f;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int from = 8 * t + 4 * e, mine = 2 * t + e + 8 * n;
+                    r24[n][e] = __shfl_sync(0xffffffffu, r, from);
+#pragma unroll
+                    for (int a = 0; a < NG; ++a) qs[a][n][e] = __shfl_sync(0xffffffffu, total_q[a], from) * 5.9604644775390625e-8f;
+                    const int pos = pos0 + mine / p.shared;
+                    hi[n][e] = mine < rows ? seen_hi(p, pos, h.len) : h.len;
+                    lo[n][e] = mine < rows ? seen_lo(p, pos) : 0;
+                    m[n][e] = 0.f;
+                    thr[n][e] = -3.0e38f;                        // nothing seen yet: any score sets the maximum
+                    sum[n][e] = 0.f;
+#pragma unroll
+                    for (int a = 0; a < NG; ++a) msum[a][n][e] = 0.f;
+                }
+#pragma unroll
+                for (int j = 0; j < 4 * VW; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][n][e] = 0.f;
+#pragma unroll
+                for (int a = 0; a < NG; ++a)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) oc[a][n][e] = 0.f;
+            }
+            vlim = 0.f;
+            vmul = 1.f;
+        }
+
+        const int w0 = warp * kCdWarpTokens, tok = h.tok0 + w0;  // this warp's first token
+        if (tok < h.len && tok + kCdWarpTokens > lo_all) {
+            const uint32_t sb = smem_u32(smem + st * C::STAGE);
+            const bool inside = tok >= lo_max && tok + kCdWarpTokens <= hi_min;
+            float x[2][NT][4];                                   // [block][..][token g rows 2t, 2t+1; token g+8]
+            __half2 vp[2][2][NG];                                // value pairs of this lane's tokens
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk) {
+                uint32_t kw[2][KW];
+                __half2 kp[2][NG];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t row = (uint32_t)(w0 + blk * 16 + e * 8 + krow);
+#pragma unroll
+                    for (int a = 0; a < NG; ++a) {
+                        const uint32_t ad = sb + row * F::CODE + a * (G / 2) + t * (G / 8);
+                        if constexpr (G == 128) {
+                            const uint4 v = lds128(ad);
+                            kw[e][0] = v.x; kw[e][1] = v.y; kw[e][2] = v.z; kw[e][3] = v.w;
+                        } else {
+                            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(kw[e][2 * a]), "=r"(kw[e][2 * a + 1]) : "r"(ad));
+                        }
+                        const uint32_t pa = sb + 2 * C::CODES + row * F::PAIR + a * 4;
+                        uint32_t w;
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(pa));
+                        kp[e][a] = *reinterpret_cast<const __half2*>(&w);
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(pa + C::PAIRS));
+                        vp[blk][e][a] = *reinterpret_cast<const __half2*>(&w);
+                    }
+                }
+                float acc[NG][NT][4];
+#pragma unroll
+                for (int w = 0; w < KW; ++w) {
+                    const int a = w / (G / 32);
+                    const uint32_t a0[4] = {kw[0][w] & LO, kw[1][w] & LO, kw[0][w] & HI, kw[1][w] & HI};
+                    const uint32_t s0 = kw[0][w] >> 8, s1 = kw[1][w] >> 8;
+                    const uint32_t a1[4] = {s0 & LO, s1 & LO, s0 & HI, s1 & HI};
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        if (w % (G / 32) == 0) mma_16816_zero(acc[a][n], a0, qf[2 * w][n][0], qf[2 * w][n][1]);
+                        else mma_16816(acc[a][n], a0, qf[2 * w][n][0], qf[2 * w][n][1]);
+                        mma_16816(acc[a][n], a1, qf[2 * w + 1][n][0], qf[2 * w + 1][n][1]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            float v = __low2float(kp[e][0]) * acc[0][n][2 * e + r];
+                            v = fmaf(__high2float(kp[e][0]), qs[0][n][r], v);
+                            if constexpr (NG == 2) {
+                                v = fmaf(__low2float(kp[e][1]), acc[1][n][2 * e + r], v);
+                                v = fmaf(__high2float(kp[e][1]), qs[1][n][r], v);
+                            }
+                            x[blk][n][2 * e + r] = v;
+                        }
+            }
+            // masks: tokens that a row does not see weigh nothing, and what lies past the sequence's
+            // end (never written: any bits) must not reach a product
+            uint32_t gone = 0;                                   // bit 16 n + 8 blk + 4 .. : masked scores
+            if (!inside) {
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int tk = tok + blk * 16 + e * 8 + krow;
+                        if (tk >= h.len || tk < lo_all)
+#pragma unroll
+                            for (int a = 0; a < NG; ++a) vp[blk][e][a] = __half2half2(__ushort_as_half(0));
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r)
+                                if (tk >= hi[n][r] || tk < lo[n][r]) gone |= 1u << (8 * n + 4 * blk + 2 * e + r);
+                    }
+            }
+            float y[2][NT][4], top[NT][2];
+            auto relative = [&]() {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+                        for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float v = fmaf(x[blk][n][2 * e + r], r24[n][r], -m[n][r]);
+                                y[blk][n][2 * e + r] = (gone >> (8 * n + 4 * blk + 2 * e + r)) & 1u ? -INFINITY : v;
+                            }
+                        top[n][r] = fmaxf(fmaxf(y[0][n][r], y[0][n][2 + r]), fmaxf(y[1][n][r], y[1][n][2 + r]));
+                    }
+            };
+            relative();
+            float vmax = 0.f;
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int a = 0; a < NG; ++a) vmax = fmaxf(vmax, __low2float(vp[blk][e][a]));
+            bool move = vmax > vlim;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) move |= top[n][0] > thr[n][0] || top[n][1] > thr[n][1];
+            // The maximum moves only when a score passes it by 2^8 (weights stay below 2^8): a few
+            // times a segment, so the reductions over the warp and the rescaling are rare.
+            if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
+                float vkeep = 1.f;
+                if (vmax > vlim) {
+                    // the power of two above vmax
+                    const float lim = __uint_as_float((__float_as_uint(vmax) & 0x7F800000u) + 0x00800000u);
+                    vkeep = vlim / lim;
+                    vlim = lim;
+                    vmul = 64.f / lim;
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float keep[2];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        float d = top[n][r];
+#pragma unroll
+                        for (int k = 4; k < 32; k *= 2) d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, k));
+                        const bool fresh = thr[n][r] < 0.f;
+                        keep[r] = 1.f;
+                        if (d > (fresh ? -3.0e38f : 0.f)) {
+                            m[n][r] += d;
+                            keep[r] = fresh ? 0.f : exp2_fast(-d);
+                            thr[n][r] = 8.f;
+                        }
+                        sum[n][r] *= keep[r];
+#pragma unroll
+                        for (int a = 0; a < NG; ++a) msum[a][n][r] *= keep[r];
+                    }
+#pragma unroll
+                    for (int a = 0; a < NG; ++a) {
+                        oc[a][n][0] *= keep[0] * vkeep; oc[a][n][1] *= keep[1] * vkeep;
+                        oc[a][n][2] = oc[a][n][0]; oc[a][n][3] = oc[a][n][1];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4 * VW; ++j) {
+                        o[j][n][0] *= keep[0] * vkeep; o[j][n][1] *= keep[1] * vkeep;
+                        o[j][n][2] *= keep[0] * vkeep; o[j][n][3] *= keep[1] * vkeep;
+                    }
+                }
+                relative();
+            }
+            // weights, and their fp16 form in the layout of the product's right operand
+            uint32_t pf[2][NG][NT][2];
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float p0 = exp2_fast(y[blk][n][2 * e]), p1 = exp2_fast(y[blk][n][2 * e + 1]);
+                        sum[n][0] += p0;
+                        sum[n][1] += p1;
+#pragma unroll
+                        for (int a = 0; a < NG; ++a) {
+                            const float sv = __low2float(vp[blk][e][a]), vs = sv * vmul;
+                            const float vm = fmaf(8.f, sv, __high2float(vp[blk][e][a]));
+                            msum[a][n][0] = fmaf(p0, vm, msum[a][n][0]);
+                            msum[a][n][1] = fmaf(p1, vm, msum[a][n][1]);
+                            pf[blk][a][n][e] = movmatrix_trans(pack16(p0 * vs, p1 * vs, false));
+                        }
+                    }
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk) {
+                const uint32_t eight[4] = {0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u};   // 8 2^-24 each
+#pragma unroll
+                for (int a = 0; a < NG; ++a)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma_16816(oc[a][n], eight, pf[blk][a][n][0], pf[blk][a][n][1]);
+                uint32_t vw[4][VW];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t row = (uint32_t)(w0 + blk * 16 + 4 * k + t);
+                    const uint32_t ad = sb + C::CODES + row * F::CODE + g * (G / 16);
+                    if constexpr (G == 128) {
+                        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(vw[k][0]), "=r"(vw[k][1]) : "r"(ad));
+                    } else {
+#pragma unroll
+                        for (int a = 0; a < NG; ++a)
+                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(vw[k][a]) : "r"(ad + a * (G / 2)));
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < VW; ++w) {
+                    const int a = w / (G / 64);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t sel = half ? 0x7632u : 0x5410u;
+                        uint32_t x01 = __byte_perm(vw[0][w], vw[1][w], sel), x23 = __byte_perm(vw[2][w], vw[3][w], sel);
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const uint32_t af[4] = {x01 & LO, x01 & HI, x23 & LO, x23 & HI};
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma_16816(o[4 * w + 2 * half + q][n], af, pf[blk][a][n][0], pf[blk][a][n][1]);
+                            x01 >>= 8;
+                            x23 >>= 8;
+                        }
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty(st));
+
+        if (h.flags & 2) {
+            // ---- the end of this CTA's part: the four warps' states become one
+            const int rows = h.nq * p.shared;
+            float* mine = merge + warp * ROWS * C::LD;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int row = 2 * t + r + 8 * n;
+                    float s = sum[n][r], a0 = msum[0][n][r], a1 = NG == 2 ? msum[NG - 1][n][r] : 0.f;
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) {
+                        s += __shfl_xor_sync(0xffffffffu, s, d);
+                        a0 += __shfl_xor_sync(0xffffffffu, a0, d);
+                        if constexpr (NG == 2) a1 += __shfl_xor_sync(0xffffffffu, a1, d);
+                    }
+                    if (row < rows) {
+                        const float up24 = 16777216.f / vmul, up20 = 1048576.f / vmul;
+#pragma unroll
+                        for (int j = 0; j < 4 * VW; ++j) {
+                            const int w = j / 4, a = w / (G / 64);
+                            const int d = a * G + g * (G / 8) + (w % (G / 64)) * 8 + 2 * (j % 4);
+                            float2 v;
+                            v.x = fmaf(o[j][n][r] - oc[a][n][r], up24, a ? a1 : a0);
+                            v.y = fmaf(fmaf(-16.f, oc[a][n][r], o[j][n][2 + r]), up20, a ? a1 : a0);
+                            *reinterpret_cast<float2*>(mine + row * C::LD + d) = v;
+                        }
+                        if (g == 0) {
+                            mine[row * C::LD + D] = thr[n][r] < 0.f ? -INFINITY : m[n][r];
+                            mine[row * C::LD + D + 1] = s;
+                        }
+                    }
+                }
+            mbar_arrive(merge_bar);
+            if (!__all_sync(0xffffffffu, mbar_wait(merge_bar, merge_phase, kDevTimeoutCache))) return;
+            merge_phase ^= 1;
+            constexpr int V4 = D / 4;
+            for (int i = threadIdx.x; i < rows * V4; i += kCdWarps * 32) {
+                const int row = i / V4, d = i % V4 * 4;
+                const float* src = merge + row * C::LD;
+                float mm = -INFINITY, ss = 0.f;
+#pragma unroll
+                for (int w = 0; w < kCdWarps; ++w) mm = fmaxf(mm, src[w * ROWS * C::LD + D]);
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kCdWarps; ++w) {
+                    const float* sw = src + w * ROWS * C::LD;
+                    // a warp that saw nothing has no maximum, and sums of zero (or NaN, which must stay)
+                    const float k = sw[D] == -INFINITY ? 1.f : exp2_fast(sw[D] - mm);
+                    const float4 x4 = *reinterpret_cast<const float4*>(sw + d);
+                    v.x = fmaf(k, x4.x, v.x); v.y = fmaf(k, x4.y, v.y); v.z = fmaf(k, x4.z, v.z); v.w = fmaf(k, x4.w, v.w);
+                    ss = fmaf(k, sw[D + 1], ss);
+                }
+                if (h.flags & 4) {
+                    float* slot = reinterpret_cast<float*>(p.workspace + cd_info_bytes((int64_t)p.batch * hk)) +
+                                  (size_t)h.slot * cd_slot_floats(ROWS, D);
+                    *reinterpret_cast<float4*>(slot + row * D + d) = v;
+                    if (d == 0) {
+                        slot[ROWS * D + row] = mm;
+                        slot[ROWS * D + ROWS + row] = ss;
+                    }
+                } else {
+                    const float inv = ss == 0.f ? 0.f : 1.f / ss;
+                    const int64_t at = (int64_t)(h.q0 + row / p.shared) * (hk * p.shared) + h.head * p.shared + row % p.shared;
+                    uint2 w2;
+                    w2.x = pack16(v.x * inv, v.y * inv, p.bf16);
+                    w2.y = pack16(v.z * inv, v.w * inv, p.bf16);
+                    *reinterpret_cast<uint2*>(p.out + at * D + d) = w2;
+                    if (p.lse && d == 0) p.lse[at] = ss == 0.f ? -INFINITY : (mm + log2f(ss)) * kLn2;
+                }
+            }
+            // the buffer is free again once every warp has read it
+            mbar_arrive(merge_bar);
+            if (!__all_sync(0xffffffffu, mbar_wait(merge_bar, merge_phase, kDevTimeoutCache))) return;
+            merge_phase ^= 1;
+        }
+    }
+}
+
+// Joins the parts of the segments that several CTAs held, and writes the zeros of sequences
+// with nothing cached.  Grid (sequence x key head, row); D / 4 threads hold one row's values and
+// the block's other threads take every so many parts.
+template <int D>
+__global__ void cache_decode_combine_kernel(const __grid_constant__ AttentionParams p, int slot_rows) {
+    constexpr int V4 = D / 4;
+    __shared__ float4 part[512];
+    __shared__ float red[2][32];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int hk = p.c.kv_heads, b = blockIdx.x / hk, head = blockIdx.x % hk, row = blockIdx.y;
+    const SeqSpan s = seq_span(p, b);
+    if (row >= s.nq * p.shared) return;
+    const int64_t at = (int64_t)(s.q0 + row / p.shared) * (hk * p.shared) + head * p.shared + row % p.shared;
+    const int lane_d = threadIdx.x % V4, slice = threadIdx.x / V4, slices = blockDim.x / V4;
+    if (cd_tiles(p, s) == 0) {
+        if (slice == 0) {
+            *reinterpret_cast<uint2*>(p.out + at * D + lane_d * 4) = make_uint2(0u, 0u);
+            if (p.lse && lane_d == 0) p.lse[at] = -INFINITY;
+        }
+        return;
+    }
+    const int4 info = *(reinterpret_cast<const int4*>(p.workspace) + blockIdx.x);
+    const int n = info.y - info.x + 1;
+    if (n == 1) return;                                    // one CTA had it all and has written it
+    const float* slots = reinterpret_cast<const float*>(p.workspace + cd_info_bytes((int64_t)p.batch * hk));
+    const size_t size = cd_slot_floats(slot_rows, D);
+    auto part_of = [&](int c) { return slots + (size_t)(2 * (info.x + c) + (c == 0 ? info.z : 0)) * size; };
+    // the row's maximum over the parts
+    float mm = -INFINITY;
+    for (int c = threadIdx.x; c < n; c += blockDim.x) mm = fmaxf(mm, part_of(c)[slot_rows * D + row]);
+#pragma unroll
+    for (int d = 16; d; d /= 2) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+    if (threadIdx.x % 32 == 0) red[0][threadIdx.x / 32] = mm;
+    __syncthreads();
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) mm = fmaxf(mm, red[0][w]);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float ss = 0.f;
+#pragma unroll 4
+    for (int c = slice; c < n; c += slices) {
+        const float* x = part_of(c);
+        const float mc = x[slot_rows * D + row], sc = x[slot_rows * D + slot_rows + row];
+        const float4 y = *reinterpret_cast<const float4*>(x + row * D + lane_d * 4);
+        const float k = mc == -INFINITY ? 1.f : exp2_fast(mc - mm);      // see the merge above
+        v.x = fmaf(k, y.x, v.x); v.y = fmaf(k, y.y, v.y); v.z = fmaf(k, y.z, v.z); v.w = fmaf(k, y.w, v.w);
+        ss = fmaf(k, sc, ss);
+    }
+    part[threadIdx.x] = v;
+    if (lane_d == 0) red[1][slice] = ss;
+    __syncthreads();
+    if (slice == 0) {
+        float total = 0.f;
+        for (int j = 0; j < slices; ++j) total += red[1][j];
+        for (int j = 1; j < slices; ++j) {
+            const float4 y = part[j * V4 + lane_d];
+            v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+        }
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        uint2 w2;
+        w2.x = pack16(v.x * inv, v.y * inv, p.bf16);
+        w2.y = pack16(v.z * inv, v.w * inv, p.bf16);
+        *reinterpret_cast<uint2*>(p.out + at * D + lane_d * 4) = w2;
+        if (p.lse && lane_d == 0) p.lse[at] = total == 0.f ? -INFINITY : (mm + log2f(total)) * kLn2;
+    }
+}
+
+}  // namespace w4a16
