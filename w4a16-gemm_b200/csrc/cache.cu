@@ -9,7 +9,7 @@
 #include "cache_format.cuh"
 #include "cache_attention.cuh"
 #include "cache_decode.cuh"
-#include "cache_rows.cuh"
+#include "cache_prompt.cuh"
 
 namespace w4a16 {
 
@@ -139,8 +139,9 @@ static AttentionParams attention_params(const w4a16_cache& c, const w4a16_cache_
 
 // How an attention call is run: by rows (query heads of a key head times queries).
 struct AttentionPlan {
-    int nt;              // 8-row tiles of the decode kernel; 0: more rows than it takes
+    int nt;              // 8-row tiles of the decode kernel; 0: more rows than it takes, the prompt kernel
     int grid;
+    CpGrid prompt;
     size_t workspace;
 };
 
@@ -149,17 +150,36 @@ static AttentionPlan plan_decode_t(const w4a16_cache& c, const w4a16_cache_atten
     using C = CdCfg<D, G, NT>;
     const int64_t segments = (int64_t)a.batch * c.kv_heads;
     const int64_t tiles = ((int64_t)a.table_pages * c.page_size + kCdTile - 1) / kCdTile;
-    AttentionPlan p;
+    AttentionPlan p = {};
     p.nt = NT;
     p.grid = (int)std::max<int64_t>(1, std::min<int64_t>(segments * tiles, (int64_t)C::CTAS * dev.num_sms));
     p.workspace = cd_info_bytes(segments) + 2 * (size_t)p.grid * cd_slot_floats(C::ROWS, D) * sizeof(float);
     return p;
 }
 
+// Row blocks of 256 (128, with the halves on alternate tiles, if no sequence has more rows); a
+// block's tiles are split over CTAs when the blocks alone would leave SMs idle.
+static AttentionPlan plan_prompt(const w4a16_cache& c, const w4a16_cache_attention_args& a, const DeviceInfo& dev) {
+    const int64_t shared = a.q_heads / c.kv_heads, rows = a.max_q * shared;
+    AttentionPlan p = {};
+    p.prompt.kv2 = rows <= kCpRows;
+    const int64_t block_rows = p.prompt.kv2 ? kCpRows : 2 * kCpRows;
+    p.prompt.blocks = (int)((rows + block_rows - 1) / block_rows);
+    const int64_t busy = c.kv_heads * std::min<int64_t>((int64_t)p.prompt.blocks * a.batch,
+                                                        a.q_tokens * shared / block_rows + a.batch);
+    const int64_t tiles = ((int64_t)a.table_pages * c.page_size + kCpTile - 1) / kCpTile;
+    p.prompt.splits = (int)std::max<int64_t>(1, std::min<int64_t>(dev.num_sms / busy, tiles / 4));
+    p.prompt.parts = p.prompt.splits * (p.prompt.kv2 ? 2 : 1);
+    p.grid = (int)((int64_t)p.prompt.blocks * a.batch * c.kv_heads * p.prompt.splits);
+    if (p.prompt.parts > 1)
+        p.workspace = (size_t)p.prompt.parts * (size_t)(a.q_tokens * a.q_heads) * (size_t)(c.head_dim + 2) * sizeof(float);
+    return p;
+}
+
 static AttentionPlan plan_attention(const w4a16_cache& c, const w4a16_cache_attention_args& a, const DeviceInfo& dev) {
     const int64_t rows = (int64_t)a.max_q * (a.q_heads / c.kv_heads);
+    if (rows > 16) return plan_prompt(c, a, dev);
     AttentionPlan p = {};
-    if (rows > 16) return p;
     with_format(c, [&](auto d, auto g) {
         p = rows <= 8 ? plan_decode_t<d.value, g.value, 1>(c, a, dev) : plan_decode_t<d.value, g.value, 2>(c, a, dev);
         return cudaSuccess;
@@ -187,6 +207,19 @@ static cudaError_t launch_decode_t(const AttentionParams& ap, const AttentionPla
                   (int)C::ROWS);
 }
 
+template <int D, int G>
+static cudaError_t launch_prompt_t(const AttentionParams& ap, const AttentionPlan& plan, cudaStream_t stream, bool pdl) {
+    using C = CpCfg<D, G>;
+    auto kern = cache_prompt_kernel<D, G>;
+    cudaError_t err = ensure_max_dynamic_smem(reinterpret_cast<const void*>(kern));
+    if (err != cudaSuccess) return err;
+    err = launch(kern, dim3((unsigned)plan.grid), kCpThreads, C::SMEM, stream, pdl, ap, plan.prompt);
+    if (err != cudaSuccess || plan.prompt.parts == 1) return err;
+    const int64_t rows = (int64_t)ap.max_q * ap.shared * ap.c.kv_heads, per = 128 / (D / 4);
+    return launch(cache_prompt_combine_kernel<D>, dim3((unsigned)((rows + per - 1) / per), (unsigned)ap.batch), 128, 0, stream,
+                  pdl, ap, plan.prompt.parts);
+}
+
 cudaError_t launch_cache_attention(const w4a16_cache& c, const w4a16_cache_attention_args& a, const DeviceInfo& dev,
                                    void* workspace, cudaStream_t stream, bool pdl) {
     AttentionParams p = attention_params(c, a);
@@ -195,8 +228,7 @@ cudaError_t launch_cache_attention(const w4a16_cache& c, const w4a16_cache_atten
     return with_format(c, [&](auto d, auto g) {
         if (plan.nt == 1) return launch_decode_t<d.value, g.value, 1>(p, plan, stream, pdl);
         if (plan.nt == 2) return launch_decode_t<d.value, g.value, 2>(p, plan, stream, pdl);
-        const int64_t warps = (int64_t)a.batch * a.max_q * a.q_heads;
-        return launch(cache_attention_kernel<d.value, g.value>, dim3((unsigned)((warps + 7) / 8)), 256, 0, stream, pdl, p);
+        return launch_prompt_t<d.value, g.value>(p, plan, stream, pdl);
     });
 }
 

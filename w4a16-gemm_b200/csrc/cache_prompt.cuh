@@ -1,0 +1,553 @@
+// Attention of many rows (prompts, chunks of prompts, drafts of more than 16 rows) over the
+// 4-bit cache on the tensor cores: tcgen05 products with accumulators in TMEM.  Included by
+// cache.cu only.
+//
+// A CTA takes up to 256 rows (query heads of a key head times queries, in that order) of one
+// sequence and key head as two tiles of 128, and walks the 128-token tiles of the cache that
+// any of its rows sees:
+//     S = Q K^T   (128 x 128, TMEM)  ->  P = 2^(r S - m), fp16, over S in TMEM
+//     O += P V    (128 x D, TMEM)
+// While the tensor cores work on one half's products, the other half's softmax runs.  With 128
+// rows or fewer the halves take alternate tiles of the cache instead, for the same rows, and
+// are joined by the combine kernel like any other parts.
+//
+// Warps: 0 issues the products; 4-7 turn codes into fp16 operands in shared memory (keys
+// [token][value], values transposed [value][token], both K-major with 128-byte swizzle); 8-11
+// and 12-15 hold one half each, a thread a row: they load the queries, run the softmax and write
+// the result.
+//
+// Rounding.  A cached value code * scale + minimum is rounded once to fp16 (2^-11), as a 16-bit
+// cache would hold it.  Queries become fp16 after a power of two (exact within 2^-24 of the
+// row's largest).  Weights are fp16 up to 2^14: the maximum is followed only when a score passes
+// it by 2^8, and 2^6 is put on top, so weights down to 2^-20 of the row's largest keep all
+// bits.  Sums, maxima and accumulators are fp32.
+#pragma once
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "cache_attention.cuh"
+
+namespace w4a16 {
+
+__device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+                 :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+
+// D[tmem] (+)= A[smem desc] * B[smem desc]; kind::f16, one CTA.
+__device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
+
+constexpr int kCpRows = 128;        // rows of a half
+constexpr int kCpTile = 128;        // cached tokens of a tile
+constexpr int kCpThreads = 512;
+
+template <int D, int G>
+struct CpCfg {
+    using F = CacheFmt<D, G>;
+    static constexpr int Q_BYTES = kCpRows * D * 2;
+    static constexpr int K_BYTES = kCpTile * D * 2;
+    static constexpr int V_BYTES = D * kCpTile * 2;
+    static constexpr int ST = 2;                                   // stages of K and of V
+    static constexpr int USED = 1024 + 2 * Q_BYTES + ST * (K_BYTES + V_BYTES) + 256;
+    // more than half of the SM's shared memory: one CTA, which owns all of TMEM, on an SM
+    static constexpr int SMEM = USED > 116 * 1024 ? USED : 116 * 1024;
+    static constexpr int S_COL = 0;                                // TMEM columns: S of both halves, O of both halves
+    static constexpr int O_COL = 2 * kCpTile;
+    static constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(kCpTile >> 3) << 17) | ((uint32_t)(kCpRows >> 4) << 24);
+    static constexpr uint32_t IDESC_O = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kCpRows >> 4) << 24);
+};
+
+// What a grid of prompt CTAs does, set on the host.
+struct CpGrid {
+    int blocks;      // row blocks of the longest sequence
+    int splits;      // CTAs that share the tiles of one row block
+    int kv2;         // 128 rows or fewer: the halves take alternate tiles
+    int parts;       // results to be joined for each row: splits * (kv2 ? 2 : 1); 1: written at once
+};
+
+// Shared-memory matrix descriptor: K-major, 128-byte swizzle, 8-row groups 1024 B apart.
+__device__ __forceinline__ uint64_t cp_desc(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+           ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
+__device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+
+// Two codes as fp16 times scale plus minimum, one rounding: w holds them in the low nibbles of
+// its halves (high: in bits 4-7).  1024 + c, or 1024 + 16 c, is the half 0x6400 | bits.
+__device__ __forceinline__ uint32_t value_lo(uint32_t w, __half2 sc, __half2 mn) {
+    const __half2 c = __hadd2(as_half2((w & 0x000F000Fu) | 0x64006400u), __half2half2(__ushort_as_half(0xE400)));
+    return as_u32(__hfma2(c, sc, mn));
+}
+__device__ __forceinline__ uint32_t value_hi(uint32_t w, __half2 sc, __half2 mn) {
+    const __half2 c = __hfma2(as_half2((w & 0x00F000F0u) | 0x64006400u), __half2half2(__ushort_as_half(0x2C00)),
+                              __half2half2(__ushort_as_half(0xD400)));
+    return as_u32(__hfma2(c, sc, mn));
+}
+
+template <int D, int G>
+__global__ void __launch_bounds__(kCpThreads, 1)
+cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ CpGrid gr) {
+    using C = CpCfg<D, G>;
+    using F = CacheFmt<D, G>;
+    constexpr int ST = C::ST;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t qs = base, ks = qs + 2 * C::Q_BYTES, vs = ks + ST * C::K_BYTES, bar0 = vs + ST * C::V_BYTES;
+    auto k_full = [&](int s) { return bar0 + 8u * s; };
+    auto k_empty = [&](int s) { return bar0 + 8u * (ST + s); };
+    auto v_full = [&](int s) { return bar0 + 8u * (2 * ST + s); };
+    auto v_empty = [&](int s) { return bar0 + 8u * (3 * ST + s); };
+    auto q_full = [&](int h) { return bar0 + 8u * (4 * ST + h); };
+    auto s_full = [&](int h) { return bar0 + 8u * (4 * ST + 2 + h); };
+    auto p_full = [&](int h) { return bar0 + 8u * (4 * ST + 4 + h); };
+    auto o_done = [&](int h) { return bar0 + 8u * (4 * ST + 6 + h); };
+    const uint32_t done_bar = bar0 + 8u * (4 * ST + 8), tmem_slot = done_bar + 8;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(k_full(s), 128);
+            mbar_init(k_empty(s), 1);
+            mbar_init(v_full(s), 128);
+            mbar_init(v_empty(s), 1);
+        }
+        for (int h = 0; h < 2; ++h) {
+            mbar_init(q_full(h), 128);
+            mbar_init(s_full(h), 1);
+            mbar_init(p_full(h), 128);
+            mbar_init(o_done(h), 1);
+        }
+        mbar_init(done_bar, 1);
+        fence_mbar_init();
+    }
+    if (warp == 0) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - raw));
+    pdl_wait();
+    pdl_launch_dependents();
+
+    // ---- this CTA's rows and tiles; the row blocks that see most come first
+    const int hk = p.c.kv_heads, heads = hk * p.shared;
+    int idx = blockIdx.x;
+    const int split = idx % gr.splits; idx /= gr.splits;
+    const int head = idx % hk; idx /= hk;
+    const int b = idx % p.batch;
+    const int block = gr.blocks - 1 - idx / p.batch;
+    const SeqSpan s = seq_span(p, b);
+    const int block_rows = gr.kv2 ? kCpRows : 2 * kCpRows;
+    const int row0 = block * block_rows, rows = min(s.nq * p.shared - row0, block_rows);   // rows <= 0: nothing here
+    const int pos_first = s.len - s.nq + row0 / p.shared, pos_last = s.len - s.nq + (row0 + max(rows, 1) - 1) / p.shared;
+    const int tok_lo = seen_lo(p, pos_first), tok_hi = seen_hi(p, pos_last, s.len);
+    int t0 = tok_lo / kCpTile, n = rows > 0 ? max((tok_hi + kCpTile - 1) / kCpTile - t0, 0) : 0;
+    {
+        const int a = (int)((long long)n * split / gr.splits), e = (int)((long long)n * (split + 1) / gr.splits);
+        t0 += a;
+        n = e - a;
+    }
+    // events: a half's products with one tile, the halves in turn
+    const bool two = gr.kv2 ? n > 1 : rows > kCpRows;               // the second half has work
+    const int shift = gr.kv2 ? 0 : two ? 1 : 0;                     // tile of event e: e >> shift
+    const int events = n << shift;
+    auto half_of = [&](int e) { return two ? e & 1 : 0; };
+    auto steps_of = [&](int h) { return two ? (gr.kv2 ? (n + 1 - h) / 2 : n) : (h == 0 ? n : 0); };
+
+    if (warp < 4) {
+        reg_dec<40>();
+        if (warp == 0 && lane == 0 && events > 0) {
+            // -------------------------------------------------------- products
+            bool ok = true;
+            auto issue_s = [&](int e) {
+                const int h = half_of(e), tile = e >> shift, st = tile % ST;
+                ok = ok && mbar_wait(k_full(st), (tile / ST) & 1, kDevTimeoutCache);
+                if (!ok) return;
+                tc_fence_after();
+                const uint32_t qa = qs + (gr.kv2 ? 0 : h) * C::Q_BYTES, kb = ks + st * C::K_BYTES;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                    tc_mma_ss(tmem + C::S_COL + h * kCpTile, cp_desc(qa + (k / 4) * (kCpRows * 128) + (k % 4) * 32),
+                              cp_desc(kb + (k / 4) * (kCpTile * 128) + (k % 4) * 32), C::IDESC_S, k != 0);
+                tc_commit(s_full(h));
+                if (shift == 0 || h == 1) tc_commit(k_empty(st));
+            };
+            ok = mbar_wait(q_full(0), 0, kDevTimeoutCache) && ((gr.kv2 || !two) || mbar_wait(q_full(1), 0, kDevTimeoutCache));
+            issue_s(0);
+            if (two && events > 1) issue_s(1);
+            const int ahead = two ? 2 : 1;
+            for (int e = 0; e < events && ok; ++e) {
+                const int h = half_of(e), tile = e >> shift, st = tile % ST, step = two ? e >> 1 : e;
+                ok = mbar_wait(v_full(st), (tile / ST) & 1, kDevTimeoutCache) &&
+                     mbar_wait(p_full(h), step & 1, kDevTimeoutCache);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t vb = vs + st * C::V_BYTES, pt = tmem + C::S_COL + h * kCpTile;
+#pragma unroll
+                for (int k = 0; k < kCpTile / 16; ++k)
+                    tc_mma_ts(tmem + C::O_COL + h * D, pt + k * 8, cp_desc(vb + (k / 4) * (D * 128) + (k % 4) * 32), C::IDESC_O,
+                              (step | k) != 0);
+                tc_commit(o_done(h));
+                if (shift == 0 || h == 1) tc_commit(v_empty(st));
+                // the half's next S goes over this P: products run in the order of their issue
+                if (e + ahead < events) issue_s(e + ahead);
+            }
+            tc_commit(done_bar);            // every product retired before TMEM is released
+            mbar_wait(done_bar, 0, kDevTimeoutDrain);
+        }
+    } else if (warp < 8) {
+        // ------------------------------------------------------------ codes -> operands
+        reg_dec<104>();
+        const int w = warp - 4;
+        const int g = lane >> 2, t = lane & 3;
+        constexpr int KB = D / 8;                     // bytes of a key that a thread takes: D / 4 values
+        constexpr int KWD = KB / 4;                   // in words
+        constexpr int DV = D / 8, VWD = DV / 8;       // values of each of 8 tokens that it takes, in words
+        const int chunk = lane & 7, dg = (lane >> 3) + 4 * (w >> 1), vtok = (w & 1) * 64 + chunk * 8;
+        const uint32_t ps_mask = (1u << p.c.page_shift) - 1u;
+        const int ka = t * (D / 4) / G, va = dg * DV / G;               // groups
+        uint32_t kw[4][KWD], kp[4], vw[8][VWD], vp[8];
+        auto load_k = [&](int tile) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int tok = (t0 + tile) * kCpTile + i * 32 + w * 8 + g;
+                kp[i] = 0;
+#pragma unroll
+                for (int j = 0; j < KWD; ++j) kw[i][j] = 0;
+                if (tok >= s.len || tok < tok_lo) continue;
+                const uint8_t* blk = cache_block(p.c, page_of(p, b, tok >> p.c.page_shift), head);
+                const uint32_t row = (uint32_t)tok & ps_mask;
+                const uint8_t* src = blk + row * F::CODE + t * KB;
+                if constexpr (KWD == 4) {
+                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
+                    kw[i][0] = v.x; kw[i][1] = v.y; kw[i][2] = v.z; kw[i][3] = v.w;
+                } else {
+                    const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
+                    kw[i][0] = v.x; kw[i][1] = v.y;
+                }
+                kp[i] = __ldg(reinterpret_cast<const uint32_t*>(blk + ((2 * F::CODE) << p.c.page_shift) + row * F::PAIR + ka * 4));
+            }
+        };
+        auto load_v = [&](int tile) {
+            const int tok = (t0 + tile) * kCpTile + vtok;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                vp[k] = 0;
+#pragma unroll
+                for (int j = 0; j < VWD; ++j) vw[k][j] = 0;
+            }
+            if (tok >= s.len || tok + 8 <= tok_lo) return;
+            const uint8_t* blk = cache_block(p.c, page_of(p, b, tok >> p.c.page_shift), head);
+            const uint32_t row = (uint32_t)tok & ps_mask;
+            const uint8_t* src = blk + (F::CODE << p.c.page_shift) + row * F::CODE + dg * (DV / 2);
+            const uint8_t* pr = blk + ((2 * F::CODE + F::PAIR) << p.c.page_shift) + row * F::PAIR + va * 4;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                // a row past the end, or below what is seen, may never have been written
+                const bool here = tok + k < s.len && tok + k >= tok_lo;
+                if constexpr (VWD == 2) {
+                    const uint2 v = __ldg(reinterpret_cast<const uint2*>(src + k * F::CODE));
+                    vw[k][0] = v.x; vw[k][1] = v.y;
+                } else {
+                    vw[k][0] = __ldg(reinterpret_cast<const uint32_t*>(src + k * F::CODE));
+                }
+                const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(pr + k * F::PAIR));
+                vp[k] = here ? v : 0u;
+            }
+        };
+        bool ok = true;
+        if (n > 0) load_k(0);
+        for (int tile = 0; tile < n; ++tile) {
+            const int st = tile % ST;
+            load_v(tile);
+            ok = __all_sync(0xffffffffu, mbar_wait(k_empty(st), ((tile / ST) & 1) ^ 1, kDevTimeoutCache));
+            if (!ok) break;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = i * 32 + w * 8 + g;
+                const __half2 pr = as_half2(kp[i]);
+                const __half2 sc = __low2half2(pr), mn = __high2half2(pr);
+                uint8_t* dst = smem_raw + (ks - raw) + st * C::K_BYTES + row * 128;
+#pragma unroll
+                for (int j = 0; j < KWD; ++j) {
+                    const uint32_t x = kw[i][j], z = x >> 8;
+                    uint4 o;
+                    o.x = value_lo(x, sc, mn); o.y = value_hi(x, sc, mn);
+                    o.z = value_lo(z, sc, mn); o.w = value_hi(z, sc, mn);
+                    const int c = t * KWD + j;                           // 16-byte chunk of the token's row
+                    *reinterpret_cast<uint4*>(dst + (c / 8) * (kCpTile * 128) + (((c % 8) ^ (row & 7)) * 16)) = o;
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(k_full(st));
+            if (tile + 1 < n) load_k(tile + 1);
+            ok = __all_sync(0xffffffffu, mbar_wait(v_empty(st), ((tile / ST) & 1) ^ 1, kDevTimeoutCache));
+            if (!ok) break;
+            {
+                __half2 sc[4], mn[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    sc[k] = as_half2(__byte_perm(vp[2 * k], vp[2 * k + 1], 0x5410));
+                    mn[k] = as_half2(__byte_perm(vp[2 * k], vp[2 * k + 1], 0x7632));
+                }
+                uint8_t* dst = smem_raw + (vs - raw) + st * C::V_BYTES + (vtok / 64) * (D * 128);
+#pragma unroll
+                for (int j = 0; j < VWD; ++j)
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        uint32_t x[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) x[k] = __byte_perm(vw[2 * k][j], vw[2 * k + 1][j], hf ? 0x7632 : 0x5410);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int d = dg * DV + j * 8 + hf * 4 + q;
+                            uint32_t o[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const uint32_t y = q >= 2 ? x[k] >> 8 : x[k];
+                                o[k] = q & 1 ? value_hi(y, sc[k], mn[k]) : value_lo(y, sc[k], mn[k]);
+                            }
+                            *reinterpret_cast<uint4*>(dst + d * 128 + ((chunk ^ (d & 7)) * 16)) = make_uint4(o[0], o[1], o[2], o[3]);
+                        }
+                    }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(v_full(st));
+        }
+    } else {
+        // ------------------------------------------------------------ softmax: a thread a row
+        reg_inc<184>();
+        const int h = (warp - 8) >> 2;
+        const int r_in = (warp & 3) * 32 + lane;                       // row of the half = TMEM lane
+        const int row = row0 + (gr.kv2 ? 0 : h * kCpRows) + r_in;      // row of the (sequence, key head)
+        const bool live = row < row0 + rows;
+        const int token = live ? row / p.shared : 0, qh = live ? head * p.shared + row % p.shared : 0;
+        const int64_t at = (int64_t)(s.q0 + token) * heads + qh;       // row of out
+        const bool warp_live = row - lane < row0 + rows;               // some row of the warp is real
+        const int steps = steps_of(h);
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t s_t = tmem + lanes + C::S_COL + h * kCpTile, o_t = tmem + lanes + C::O_COL + h * D;
+        float r = 1.f;
+        if (steps > 0 && (h == 0 || !gr.kv2)) {
+            // the row's queries, scaled by a power of two: the largest comes to [2^13, 2^14).  Values of a
+            // group of eight go in the order in which the keys' nibbles come out: 0 4 1 5 2 6 3 7.
+            const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)(s.q0 + token) * p.q_token + (int64_t)qh * p.q_head);
+            uint4 v[D / 8];
+            uint32_t amax = 0;
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) v[j] = live ? __ldg(src + j) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) {
+                float x[8];
+                if (p.bf16) unpack8<true>(v[j], x);
+                else unpack8<false>(v[j], x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+            }
+            const int ex = min(max((int)(amax >> 23), 24), 250);
+            float down = __uint_as_float((uint32_t)(267 - ex) << 23);                  // 2^(140 - ex)
+            r = __uint_as_float((uint32_t)(ex - 13) << 23) * fabsf(p.scale_log2);      // 2^(ex - 140) ...
+            if (p.scale_log2 < 0.f) down = -down;
+            uint8_t* dst = smem_raw + (qs - raw) + h * C::Q_BYTES + r_in * 128;
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) {
+                float x[8];
+                if (p.bf16) unpack8<true>(v[j], x);
+                else unpack8<false>(v[j], x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] *= down;
+                const uint4 o = make_uint4(pack16(x[0], x[4], false), pack16(x[1], x[5], false), pack16(x[2], x[6], false),
+                                           pack16(x[3], x[7], false));
+                *reinterpret_cast<uint4*>(dst + (j / 8) * (kCpRows * 128) + (((j % 8) ^ (r_in & 7)) * 16)) = o;
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(q_full(h));
+        }
+        if (gr.kv2) {
+            // both halves hold the same rows: the second takes the first's factors
+            float* fac = reinterpret_cast<float*>(smem_raw + (qs - raw) + C::Q_BYTES);    // the second half's queries are not used
+            if (h == 0) fac[r_in] = r;
+            bar_sync_named(1, 256);
+            r = fac[r_in];
+        }
+        r = fmaxf(r, 1e-37f);                                          // never zero: a masked score is -inf * r
+        const int pos = s.len - s.nq + token;
+        const int hi = live ? seen_hi(p, pos, s.len) : s.len, lo = live ? seen_lo(p, pos) : 0;
+        float m = 0.f, l = 0.f;
+        bool fresh = true;                                             // no score seen yet
+        const int row_a = row - r_in, row_e = min(row_a + kCpRows, row0 + rows) - 1;
+        const int in_hi = seen_hi(p, s.len - s.nq + row_a / p.shared, s.len);      // every row of the half sees [in_lo, in_hi)
+        const int in_lo = seen_lo(p, s.len - s.nq + max(row_e, 0) / p.shared);
+        bool ok = true;
+        for (int step = 0; step < steps; ++step) {
+            const int tile = t0 + (gr.kv2 && two ? 2 * step + h : step);
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full(h), step & 1, kDevTimeoutCache));
+            if (!ok) break;
+            tc_fence_after();
+            if (warp_live) {
+                uint32_t x[kCpTile];
+#pragma unroll
+                for (int c = 0; c < kCpTile; c += 32) tmem_ld_x32(s_t + c, x + c);
+                tc_wait_ld();
+                const int k0 = tile * kCpTile;
+                if (k0 < in_lo || k0 + kCpTile > in_hi) {
+#pragma unroll
+                    for (int c = 0; c < kCpTile; ++c)
+                        if (k0 + c >= hi || k0 + c < lo) x[c] = 0xFF800000u;
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < kCpTile; c += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1])));
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * r;
+                const bool move = fresh ? top > -INFINITY : top > m + 8.f;
+                if (__any_sync(0xffffffffu, move)) {
+                    float keep = 1.f;
+                    if (move) {
+                        keep = fresh ? 0.f : exp2_fast(m - top);
+                        m = top;
+                        fresh = false;
+                    }
+                    l *= keep;
+                    if (step > 0) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(o_done(h), (step - 1) & 1, kDevTimeoutCache));
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld_x32(o_t + c, o);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tmem_st_x32(o_t + c, o);
+                        }
+                    }
+                }
+                const float off = 6.f - m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < kCpTile; c += 64) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const float p0 = exp2_fast(fmaf(__uint_as_float(x[c + 2 * e]), r, off));
+                        const float p1 = exp2_fast(fmaf(__uint_as_float(x[c + 2 * e + 1]), r, off));
+                        sum[2 * (e & 1)] += p0;
+                        sum[2 * (e & 1) + 1] += p1;
+                        pk[e] = pack16(p0, p1, false);
+                    }
+                    tmem_st_x32(s_t + c / 2, pk);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tc_wait_st();
+            }
+            tc_fence_before();
+            mbar_arrive(p_full(h));
+        }
+        if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done(h), (steps - 1) & 1, kDevTimeoutCache));
+        // ---- results
+        if (ok && warp_live && rows > 0) {
+            tc_fence_after();
+            const int part = split * (gr.kv2 ? 2 : 1) + (gr.kv2 ? h : 0);
+            const int64_t all = p.q_tokens * heads;
+            float* po = reinterpret_cast<float*>(p.workspace) + ((int64_t)part * all + at) * D;
+            float* pm = reinterpret_cast<float*>(p.workspace) + (int64_t)gr.parts * all * D + ((int64_t)part * all + at) * 2;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                if (steps > 0) {
+                    tmem_ld_x32(o_t + c, o);
+                    tc_wait_ld();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0u;
+                }
+                if (live && gr.parts == 1) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        float f[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(o[e + k]) * inv;
+                        *reinterpret_cast<uint4*>(p.out + at * D + c + e) = p.bf16 ? pack8<true>(f) : pack8<false>(f);
+                    }
+                } else if (live) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<uint4*>(po + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+            }
+            if (live && gr.parts == 1) {
+                if (p.lse) p.lse[at] = l == 0.f ? -INFINITY : (m - 6.f + log2f(l)) * kLn2;
+            } else if (live) {
+                pm[0] = fresh ? -INFINITY : m;
+                pm[1] = l;
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+// Joins the parts of each row.  Grid (rows of the longest sequence, sequence); D / 4 threads a row.
+template <int D>
+__global__ void __launch_bounds__(128) cache_prompt_combine_kernel(const __grid_constant__ AttentionParams p, int parts) {
+    constexpr int V4 = D / 4;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int heads = p.c.kv_heads * p.shared;
+    const SeqSpan s = seq_span(p, blockIdx.y);
+    const int64_t i = (int64_t)blockIdx.x * (128 / V4) + threadIdx.x / V4;
+    if (i >= (int64_t)s.nq * heads) return;
+    const int64_t all = p.q_tokens * heads, at = (int64_t)s.q0 * heads + i;
+    const int d = threadIdx.x % V4 * 4;
+    const float* po = reinterpret_cast<const float*>(p.workspace) + at * D + d;
+    const float* pm = reinterpret_cast<const float*>(p.workspace) + (int64_t)parts * all * D + at * 2;
+    float mm = -INFINITY;
+    for (int c = 0; c < parts; ++c) mm = fmaxf(mm, pm[c * all * 2]);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float ss = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < parts; ++c) {
+        const float2 ml = *reinterpret_cast<const float2*>(pm + c * all * 2);
+        const float4 y = *reinterpret_cast<const float4*>(po + c * all * D);
+        const float k = ml.x == -INFINITY ? 1.f : exp2_fast(ml.x - mm);        // nothing seen: zeros (or NaN, which must stay)
+        v.x = fmaf(k, y.x, v.x); v.y = fmaf(k, y.y, v.y); v.z = fmaf(k, y.z, v.z); v.w = fmaf(k, y.w, v.w);
+        ss = fmaf(k, ml.y, ss);
+    }
+    const float inv = ss == 0.f ? 0.f : 1.f / ss;
+    uint2 w2;
+    w2.x = pack16(v.x * inv, v.y * inv, p.bf16);
+    w2.y = pack16(v.z * inv, v.w * inv, p.bf16);
+    *reinterpret_cast<uint2*>(p.out + at * D + d) = w2;
+    if (p.lse && d == 0) p.lse[at] = ss == 0.f ? -INFINITY : (mm - 6.f + log2f(ss)) * kLn2;
+}
+
+}  // namespace w4a16

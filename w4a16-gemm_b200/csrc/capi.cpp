@@ -469,6 +469,8 @@ w4a16_status check_attention_sizes(const w4a16_cache* c, const w4a16_cache_atten
         return fail(W4A16_ERR_CACHE, "batch must be in [0, 65535] and table_pages must not be negative");
     if (a->q_tokens < 0 || a->q_tokens * a->q_heads >= (1LL << 31))
         return fail(W4A16_ERR_DIM_RANGE, "q_tokens * q_heads must fit in int32");
+    if ((int64_t)a->batch * ((int64_t)a->max_q * a->q_heads / 128 + c->kv_heads) >= (1LL << 31))
+        return fail(W4A16_ERR_DIM_RANGE, "batch * max_q * q_heads must be below 2^38");
     if (a->max_q < 0 || a->max_q > a->q_tokens) return fail(W4A16_ERR_CACHE, "max_q must be in [0, q_tokens]");
     if ((int64_t)a->table_pages * c->page_size >= (1LL << 31))
         return fail(W4A16_ERR_DIM_RANGE, "a sequence's tokens (table_pages * page_size) must fit in int32");
