@@ -33,6 +33,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "cache_attention.cuh"
 
 namespace w4a16 {
@@ -46,7 +48,8 @@ constexpr int kCdThreads = (kCdWarps + 1) * 32;
 struct __align__(16) CdStage {
     int tok0;        // first token of the unit
     int b, head;
-    int flags;       // 1: first unit of this CTA's part of the segment, 2: last, 4: the part is not all of it
+    int flags;       // 1: first unit of this CTA's part of the segment, 2: last, 4: the part is not all of it,
+                     // 8: last unit of this CTA
     int len, nq, q0;
     int slot;        // workspace slot of the part
 };
@@ -66,6 +69,10 @@ struct CdCfg {
     static constexpr int CTAS = NT == 1 ? 3 : 2;                   // resident on an SM (shared memory and registers)
 };
 
+// What the start and end of a segment cost beside its units (queries, merge), in units: ranges
+// are cut by cost, so that a CTA with many short segments is not the last to finish.
+constexpr int kCdSegmentCost = 2;
+
 // Units of one sequence and key head.
 __device__ __forceinline__ int cd_first_tile(const AttentionParams& p, const SeqSpan& s) {
     return seen_lo(p, s.len - s.nq) / kCdTile;
@@ -74,11 +81,16 @@ __device__ __forceinline__ int cd_tiles(const AttentionParams& p, const SeqSpan&
     if (s.nq == 0 || s.len == 0) return 0;
     return (s.len + kCdTile - 1) / kCdTile - cd_first_tile(p, s);
 }
+__device__ __forceinline__ int cd_cost(const AttentionParams& p, const SeqSpan& s) {
+    const int nt = cd_tiles(p, s);
+    return nt ? nt + kCdSegmentCost : 0;
+}
 
-// Workspace: per (sequence, key head) the CTAs {first, last, first one's slot, 0} that hold
-// parts of it, then 2 slots a CTA of ROWS x (D + 2) floats: sums, maxima, sums of weights.
+// Workspace: per (sequence, key head) the CTAs {first, last} that hold parts of it, then 2 slots
+// a CTA of ROWS x (D + 2) floats: sums, maxima, sums of weights.  Slot 0 is the part of a segment
+// that began in an earlier CTA, slot 1 of one that begins here.
 __host__ __device__ __forceinline__ size_t cd_info_bytes(int64_t segments) {
-    return (size_t)(segments * 16 + 255) / 256 * 256;
+    return (size_t)(segments * 8 + 255) / 256 * 256;
 }
 __host__ __device__ __forceinline__ size_t cd_slot_floats(int rows, int D) {
     return (size_t)rows * (D + 2);
@@ -86,8 +98,20 @@ __host__ __device__ __forceinline__ size_t cd_slot_floats(int rows, int D) {
 
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
     uint32_t d;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
+}
+
+// D(16x8, f32) += A(16x16, f16, row) * B(16x8, f16, col); free to be scheduled.
+__device__ __forceinline__ void hmma(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ void hmma_zero(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
 }
 
 template <int D, int G, int NT>
@@ -115,8 +139,9 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
         mbar_init(merge_bar, kCdWarps * 32);
         fence_mbar_init();
     }
+    // No early trigger: with one, the waiting combine CTAs get in the way of the next call's CTAs
+    // (64 x 8192 tokens, calls back to back: 114 us a call; without 82 us).
     pdl_wait();
-    pdl_launch_dependents();
 
     // ---- this CTA's range of units: a scan over the sequences
     const int hk = p.c.kv_heads;
@@ -125,7 +150,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
         const int per = (p.batch + kCdThreads - 1) / kCdThreads;
         const int b0 = min((int)threadIdx.x * per, p.batch), b1 = min(b0 + per, p.batch);
         long long mine = 0;
-        for (int b = b0; b < b1; ++b) mine += cd_tiles(p, seq_span(p, b));
+        for (int b = b0; b < b1; ++b) mine += cd_cost(p, seq_span(p, b));
         mine *= hk;
         long long incl = mine;
 #pragma unroll
@@ -147,7 +172,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
         if (u0 >= base && u0 < base + mine) {
             int b = b0;
             for (; b < b1; ++b) {
-                const long long n = (long long)cd_tiles(p, seq_span(p, b)) * hk;
+                const long long n = (long long)cd_cost(p, seq_span(p, b)) * hk;
                 if (u0 < base + n) break;
                 base += n;
             }
@@ -171,25 +196,32 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
         const uint32_t dst_off = (part < 2 ? part * C::CODES : 2 * C::CODES + (part - 2) * C::PAIRS) + run * run_bytes;
         const uint32_t src_part = part < 2 ? (uint32_t)(part * F::CODE) << ps_log
                                            : (uint32_t)(2 * F::CODE + (part - 2) * F::PAIR) << ps_log;
+        // u counts cost: a segment's units follow the kCdSegmentCost of its start, which are passed over
         int b = (int)found[2];
-        long long base = found[1];
         SeqSpan s = seq_span(p, b);
         int nt = cd_tiles(p, s), first = cd_first_tile(p, s);
-        int local = (int)(u0 - base);
-        int head = local / nt, tile = local % nt;
+        const int local = (int)(u0 - found[1]);
+        int head = local / (nt + kCdSegmentCost), tile = local % (nt + kCdSegmentCost) - kCdSegmentCost;
+        long long u = u0;
+        if (tile < 0) { u -= tile; tile = 0; }
         bool begins = true;
-        long long seg0 = u0 - tile;                              // first unit of the segment
-        int4* info = reinterpret_cast<int4*>(p.workspace);
-        long long it = 0;
+        long long seg0 = u - tile;                               // the segment's first unit
+        int2* info = reinterpret_cast<int2*>(p.workspace);
+        if (u >= u1 && lane == 0) {                              // a start and no unit: nothing to do
+            CdStage h = {};
+            h.flags = 8;
+            hdr[0] = h;
+            mbar_arrive(full(0));
+        }
+        int st = 0, turn = 0, issued = 0;
         bool ok = true;
-        for (long long u = u0; u < u1; ++u, ++it) {
-            const int st = (int)(it % ST);
+        while (u < u1) {
             const int tok0 = (first + tile) * kCdTile;
             const int tok = tok0 + run * rows;
             const bool valid = run * rows < kCdTile && tok < s.len && tok + rows > seen_lo(p, s.len - s.nq);
             const int64_t page = valid ? page_of(p, b, tok >> ps_log) : 0;
             const uint8_t* src = cache_block(p.c, page, head) + src_part + (uint32_t)(tok & ((1 << ps_log) - 1)) * unit_b;
-            const bool got = mbar_wait(empty(st), (uint32_t)((it / ST) & 1) ^ 1, kDevTimeoutCache);
+            const bool got = mbar_wait_sleep(empty(st), (uint32_t)turn ^ 1u, kDevTimeoutCache);
             if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
             const int runs = __popc(__ballot_sync(0xffffffffu, valid)) / 4;
             const bool ends = tile + 1 == nt || u + 1 == u1;
@@ -197,22 +229,26 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                 const bool part_of = seg0 < u0 || seg0 + nt > u1;
                 CdStage h;
                 h.tok0 = tok0; h.b = b; h.head = head;
-                h.flags = (begins ? 1 : 0) | (ends ? 2 : 0) | (part_of ? 4 : 0);
+                const bool last = u + 1 + (tile + 1 == nt ? kCdSegmentCost : 0) >= u1;
+                h.flags = (begins ? 1 : 0) | (ends ? 2 : 0) | (part_of ? 4 : 0) | (last ? 8 : 0);
                 h.len = s.len; h.nq = s.nq; h.q0 = s.q0;
-                h.slot = 2 * (int)blockIdx.x + (seg0 > u0 ? 1 : 0);
+                h.slot = 2 * (int)blockIdx.x + (seg0 >= u0 ? 1 : 0);
                 hdr[st] = h;
                 if (tile == 0)
-                    info[(int64_t)b * hk + head] = make_int4((int)blockIdx.x,
-                        (int)(((seg0 + nt) * ctas - 1) / total), seg0 > u0 ? 1 : 0, 0);
+                    info[(int64_t)b * hk + head] = make_int2((int)blockIdx.x, (int)(((seg0 + nt) * ctas - 1) / total));
                 mbar_arrive_expect_tx(full(st), (uint32_t)(runs * rows * F::TOKEN));
             }
             __syncwarp();
             if (valid) bulk_load(smem_u32(smem + st * C::STAGE) + dst_off, src, run_bytes, full(st));
+            ++issued;
+            if (++st == ST) { st = 0; turn ^= 1; }
             begins = ends;
+            ++u;
             if (++tile == nt) {
                 tile = 0;
-                seg0 = u + 1;
-                if (++head == hk && u + 1 < u1) {
+                u += kCdSegmentCost;
+                seg0 = u;
+                if (++head == hk && u < u1) {
                     head = 0;
                     do { s = seq_span(p, ++b); nt = cd_tiles(p, s); } while (nt == 0);
                     first = cd_first_tile(p, s);
@@ -221,8 +257,8 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
         }
         if (!ok) {
             // Error path: the last stages that were issued may still be landing.
-            for (long long j = it > ST ? it - ST : 0; j < it; ++j)
-                mbar_wait(full((int)(j % ST)), (uint32_t)((j / ST) & 1), kDevTimeoutDrain);
+            for (int j = max(0, issued - ST); j < issued; ++j)
+                mbar_wait(full(j % ST), (uint32_t)(j / ST) & 1u, kDevTimeoutDrain);
         }
         return;
     }
@@ -244,10 +280,10 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
     float vlim = 0.f, vmul = 1.f;                                // s_t <= vlim; w_t s_t vmul is what fp16 holds
     int lo_all = 0, lo_max = 0, hi_min = 0;
 
-    const long long n_units = u1 - u0;
-    for (long long it = 0; it < n_units; ++it) {
-        const int st = (int)(it % ST);
-        if (!__all_sync(0xffffffffu, mbar_wait(full(st), (uint32_t)((it / ST) & 1), kDevTimeoutCache))) return;
+    const int w0 = warp * kCdWarpTokens;                         // this warp's tokens of a unit
+    int st = 0, turn = 0;
+    while (true) {
+        if (!__all_sync(0xffffffffu, mbar_wait(full(st), (uint32_t)turn, kDevTimeoutCache))) return;
         const CdStage h = hdr[st];
         if (h.flags & 1) {
             // ---- a new segment: queries, masks, empty state
@@ -341,69 +377,74 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
             vmul = 1.f;
         }
 
-        const int w0 = warp * kCdWarpTokens, tok = h.tok0 + w0;  // this warp's first token
-        if (tok < h.len && tok + kCdWarpTokens > lo_all) {
-            const uint32_t sb = smem_u32(smem + st * C::STAGE);
-            const bool inside = tok >= lo_max && tok + kCdWarpTokens <= hi_min;
-            float x[2][NT][4];                                   // [block][..][token g rows 2t, 2t+1; token g+8]
-            __half2 vp[2][2][NG];                                // value pairs of this lane's tokens
+        const int tok = h.tok0 + w0;                             // this warp's first token
+        const uint8_t* sp = smem + st * C::STAGE;
+        auto step = [&](auto masked) {
+            constexpr bool MASKED = decltype(masked)::value;
+            uint32_t kw[2][2][KW];                               // [block][token g, g + 8][word]
+            __half2 kp[2][2][NG], vp[2][2][NG];                  // (scale, minimum) of this lane's tokens
 #pragma unroll
-            for (int blk = 0; blk < 2; ++blk) {
-                uint32_t kw[2][KW];
-                __half2 kp[2][NG];
+            for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const uint32_t row = (uint32_t)(w0 + blk * 16 + e * 8 + krow);
+                    const int row = w0 + krow + blk * 16 + e * 8;
 #pragma unroll
                     for (int a = 0; a < NG; ++a) {
-                        const uint32_t ad = sb + row * F::CODE + a * (G / 2) + t * (G / 8);
+                        const uint8_t* src = sp + row * F::CODE + t * (G / 8) + a * (G / 2);
                         if constexpr (G == 128) {
-                            const uint4 v = lds128(ad);
-                            kw[e][0] = v.x; kw[e][1] = v.y; kw[e][2] = v.z; kw[e][3] = v.w;
+                            const uint4 v = *reinterpret_cast<const uint4*>(src);
+                            kw[blk][e][0] = v.x; kw[blk][e][1] = v.y; kw[blk][e][2] = v.z; kw[blk][e][3] = v.w;
                         } else {
-                            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(kw[e][2 * a]), "=r"(kw[e][2 * a + 1]) : "r"(ad));
+                            const uint2 v = *reinterpret_cast<const uint2*>(src);
+                            kw[blk][e][2 * a] = v.x; kw[blk][e][2 * a + 1] = v.y;
                         }
-                        const uint32_t pa = sb + 2 * C::CODES + row * F::PAIR + a * 4;
-                        uint32_t w;
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(pa));
-                        kp[e][a] = *reinterpret_cast<const __half2*>(&w);
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(pa + C::PAIRS));
-                        vp[blk][e][a] = *reinterpret_cast<const __half2*>(&w);
+                        const uint8_t* pr = sp + 2 * C::CODES + row * F::PAIR + a * 4;
+                        kp[blk][e][a] = *reinterpret_cast<const __half2*>(pr);
+                        vp[blk][e][a] = *reinterpret_cast<const __half2*>(pr + C::PAIRS);
                     }
                 }
-                float acc[NG][NT][4];
+            // q . codes: two accumulators a group and block, so that few products wait for another
+            float acc[2][NG][NT][2][4];
 #pragma unroll
-                for (int w = 0; w < KW; ++w) {
-                    const int a = w / (G / 32);
-                    const uint32_t a0[4] = {kw[0][w] & LO, kw[1][w] & LO, kw[0][w] & HI, kw[1][w] & HI};
-                    const uint32_t s0 = kw[0][w] >> 8, s1 = kw[1][w] >> 8;
-                    const uint32_t a1[4] = {s0 & LO, s1 & LO, s0 & HI, s1 & HI};
+            for (int w = 0; w < KW; ++w) {
+                const int a = w / (G / 32);
+                const bool first = w % (G / 32) == 0;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        if (w % (G / 32) == 0) mma_16816_zero(acc[a][n], a0, qf[2 * w][n][0], qf[2 * w][n][1]);
-                        else mma_16816(acc[a][n], a0, qf[2 * w][n][0], qf[2 * w][n][1]);
-                        mma_16816(acc[a][n], a1, qf[2 * w + 1][n][0], qf[2 * w + 1][n][1]);
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int blk = 0; blk < 2; ++blk) {
+                        const uint32_t x0 = q ? kw[blk][0][w] >> 8 : kw[blk][0][w], x1 = q ? kw[blk][1][w] >> 8 : kw[blk][1][w];
+                        const uint32_t af[4] = {x0 & LO, x1 & LO, x0 & HI, x1 & HI};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            if (first) hmma_zero(acc[blk][a][n][q], af, qf[2 * w + q][n]);
+                            else hmma(acc[blk][a][n][q], af, qf[2 * w + q][n]);
+                        }
                     }
-                }
+            }
+            float x[2][NT][4];                                   // [block][..][token g rows 2t, 2t+1; token g+8]
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            float v = __low2float(kp[e][0]) * acc[0][n][2 * e + r];
-                            v = fmaf(__high2float(kp[e][0]), qs[0][n][r], v);
-                            if constexpr (NG == 2) {
-                                v = fmaf(__low2float(kp[e][1]), acc[1][n][2 * e + r], v);
-                                v = fmaf(__high2float(kp[e][1]), qs[1][n][r], v);
+                            float v = 0.f;
+#pragma unroll
+                            for (int a = 0; a < NG; ++a) {
+                                const float c = acc[blk][a][n][0][2 * e + r] + acc[blk][a][n][1][2 * e + r];
+                                const float sc = __low2float(kp[blk][e][a]), mn = __high2float(kp[blk][e][a]);
+                                v = a ? fmaf(sc, c, v) : sc * c;
+                                v = fmaf(mn, qs[a][n][r], v);
                             }
                             x[blk][n][2 * e + r] = v;
                         }
-            }
             // masks: tokens that a row does not see weigh nothing, and what lies past the sequence's
             // end (never written: any bits) must not reach a product
-            uint32_t gone = 0;                                   // bit 16 n + 8 blk + 4 .. : masked scores
-            if (!inside) {
+            uint32_t gone = 0;
+            if constexpr (MASKED) {
 #pragma unroll
                 for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
@@ -429,20 +470,23 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                         for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                const float v = fmaf(x[blk][n][2 * e + r], r24[n][r], -m[n][r]);
-                                y[blk][n][2 * e + r] = (gone >> (8 * n + 4 * blk + 2 * e + r)) & 1u ? -INFINITY : v;
+                                float v = fmaf(x[blk][n][2 * e + r], r24[n][r], -m[n][r]);
+                                if constexpr (MASKED)
+                                    if ((gone >> (8 * n + 4 * blk + 2 * e + r)) & 1u) v = -INFINITY;
+                                y[blk][n][2 * e + r] = v;
                             }
                         top[n][r] = fmaxf(fmaxf(y[0][n][r], y[0][n][2 + r]), fmaxf(y[1][n][r], y[1][n][2 + r]));
                     }
             };
             relative();
-            float vmax = 0.f;
+            __half2 vtop = __half2half2(__ushort_as_half(0));
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
-                    for (int a = 0; a < NG; ++a) vmax = fmaxf(vmax, __low2float(vp[blk][e][a]));
+                    for (int a = 0; a < NG; ++a) vtop = __hmax2(vtop, vp[blk][e][a]);
+            float vmax = __low2float(vtop);
             bool move = vmax > vlim;
 #pragma unroll
             for (int n = 0; n < NT; ++n) move |= top[n][0] > thr[n][0] || top[n][1] > thr[n][1];
@@ -496,7 +540,14 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
+                for (int e = 0; e < 2; ++e) {
+                    float vs[NG], vm[NG];
+#pragma unroll
+                    for (int a = 0; a < NG; ++a) {
+                        const float sv = __low2float(vp[blk][e][a]);
+                        vs[a] = sv * vmul;
+                        vm[a] = fmaf(8.f, sv, __high2float(vp[blk][e][a]));
+                    }
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         const float p0 = exp2_fast(y[blk][n][2 * e]), p1 = exp2_fast(y[blk][n][2 * e + 1]);
@@ -504,33 +555,31 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                         sum[n][1] += p1;
 #pragma unroll
                         for (int a = 0; a < NG; ++a) {
-                            const float sv = __low2float(vp[blk][e][a]), vs = sv * vmul;
-                            const float vm = fmaf(8.f, sv, __high2float(vp[blk][e][a]));
-                            msum[a][n][0] = fmaf(p0, vm, msum[a][n][0]);
-                            msum[a][n][1] = fmaf(p1, vm, msum[a][n][1]);
-                            pf[blk][a][n][e] = movmatrix_trans(pack16(p0 * vs, p1 * vs, false));
+                            msum[a][n][0] = fmaf(p0, vm[a], msum[a][n][0]);
+                            msum[a][n][1] = fmaf(p1, vm[a], msum[a][n][1]);
+                            pf[blk][a][n][e] = movmatrix_trans(pack16(p0 * vs[a], p1 * vs[a], false));
                         }
                     }
+                }
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) {
+                uint32_t vw[4][VW];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint8_t* src = sp + C::CODES + (w0 + t + blk * 16 + 4 * k) * F::CODE + g * (G / 16);
+                    if constexpr (G == 128) {
+                        const uint2 v = *reinterpret_cast<const uint2*>(src);
+                        vw[k][0] = v.x; vw[k][1] = v.y;
+                    } else {
+#pragma unroll
+                        for (int a = 0; a < NG; ++a) vw[k][a] = *reinterpret_cast<const uint32_t*>(src + a * (G / 2));
+                    }
+                }
                 const uint32_t eight[4] = {0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u};   // 8 2^-24 each
 #pragma unroll
                 for (int a = 0; a < NG; ++a)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_16816(oc[a][n], eight, pf[blk][a][n][0], pf[blk][a][n][1]);
-                uint32_t vw[4][VW];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t row = (uint32_t)(w0 + blk * 16 + 4 * k + t);
-                    const uint32_t ad = sb + C::CODES + row * F::CODE + g * (G / 16);
-                    if constexpr (G == 128) {
-                        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(vw[k][0]), "=r"(vw[k][1]) : "r"(ad));
-                    } else {
-#pragma unroll
-                        for (int a = 0; a < NG; ++a)
-                            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(vw[k][a]) : "r"(ad + a * (G / 2)));
-                    }
-                }
+                    for (int n = 0; n < NT; ++n) hmma(oc[a][n], eight, pf[blk][a][n]);
 #pragma unroll
                 for (int w = 0; w < VW; ++w) {
                     const int a = w / (G / 64);
@@ -542,16 +591,21 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                         for (int q = 0; q < 2; ++q) {
                             const uint32_t af[4] = {x01 & LO, x01 & HI, x23 & LO, x23 & HI};
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) mma_16816(o[4 * w + 2 * half + q][n], af, pf[blk][a][n][0], pf[blk][a][n][1]);
+                            for (int n = 0; n < NT; ++n) hmma(o[4 * w + 2 * half + q][n], af, pf[blk][a][n]);
                             x01 >>= 8;
                             x23 >>= 8;
                         }
                     }
                 }
             }
+        };
+        if (tok < h.len && tok + kCdWarpTokens > lo_all) {
+            if (tok >= lo_max && tok + kCdWarpTokens <= hi_min) step(std::false_type{});
+            else step(std::true_type{});
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(empty(st));
+        if (++st == ST) { st = 0; turn ^= 1; }
 
         if (h.flags & 2) {
             // ---- the end of this CTA's part: the four warps' states become one
@@ -629,6 +683,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
             if (!__all_sync(0xffffffffu, mbar_wait(merge_bar, merge_phase, kDevTimeoutCache))) return;
             merge_phase ^= 1;
         }
+        if (h.flags & 8) return;
     }
 }
 
@@ -654,12 +709,12 @@ __global__ void cache_decode_combine_kernel(const __grid_constant__ AttentionPar
         }
         return;
     }
-    const int4 info = *(reinterpret_cast<const int4*>(p.workspace) + blockIdx.x);
+    const int2 info = *(reinterpret_cast<const int2*>(p.workspace) + blockIdx.x);
     const int n = info.y - info.x + 1;
     if (n == 1) return;                                    // one CTA had it all and has written it
     const float* slots = reinterpret_cast<const float*>(p.workspace + cd_info_bytes((int64_t)p.batch * hk));
     const size_t size = cd_slot_floats(slot_rows, D);
-    auto part_of = [&](int c) { return slots + (size_t)(2 * (info.x + c) + (c == 0 ? info.z : 0)) * size; };
+    auto part_of = [&](int c) { return slots + (size_t)(2 * (info.x + c) + (c == 0 ? 1 : 0)) * size; };
     // the row's maximum over the parts
     float mm = -INFINITY;
     for (int c = threadIdx.x; c < n; c += blockDim.x) mm = fmaxf(mm, part_of(c)[slot_rows * D + row]);
