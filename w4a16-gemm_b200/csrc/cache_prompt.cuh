@@ -11,10 +11,19 @@
 // rows or fewer the halves take alternate tiles of the cache instead, for the same rows, and
 // are joined by the combine kernel like any other parts.
 //
-// Warps: 0 issues the products; 4-7 turn codes into fp16 operands in shared memory (keys
-// [token][value], values transposed [value][token], both K-major with 128-byte swizzle); 8-11
-// and 12-15 hold one half each, a thread a row: they load the queries, run the softmax and write
-// the result.
+// Warps: 0 issues the products; 1 fetches codes and pairs (bulk copies); 4-7 turn them into fp16
+// operands in shared memory (keys [token][value], values transposed [value][token], both K-major
+// with 128-byte swizzle); 8-11 and 12-15 hold one half each, a thread a row: they load the queries,
+// run the softmax and write the result.
+//
+// What bounds it: the chain of a half's step, some 4600 cycles for a 128-token tile of both halves
+// where the products alone take 2048 and the exponentials (16 a cycle and SM) as many: scores
+// read 180, maximum 370, weights 1800, then 1000 for PV and the next S, with 100 to 200 for each
+// hand-over; shared memory is half used.  512 queries of 64 heads over 32768 tokens: 660 us, 827
+// TFLOP/s, at 990 W of the GPU's 1000.  Measured and not kept: two threads a row (680 us), a warp of its own for
+// the products of each half (765), a PV and the next S issued in one go after all their waits
+// (758), a quarter of the exponentials as polynomials on the FMA pipe (792), a second read of the scores from
+// TMEM in place of 128 registers (1160).
 //
 // Rounding.  A cached value code * scale + minimum is rounded once to fp16 (2^-11), as a 16-bit
 // cache would hold it.  Queries become fp16 after a power of two (exact within 2^-24 of the
@@ -37,21 +46,78 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
                  :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
 
-// D[tmem] (+)= A[smem desc] * B[smem desc]; kind::f16, one CTA.
-__device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                          uint32_t accumulate) {
+// Two fp32 operations in one instruction, on register pairs.
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ void split2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float v;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+    return v;
+}
+
+// Products issued by a whole warp with its values uniform and one elected lane (677 us with a
+// branch for one lane where this takes 660).  Descriptors are given by their low words; the high
+// word is the same for every operand here: 8-row groups 1024 bytes apart, 128-byte swizzle.
+constexpr uint32_t kCpDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t cp_desc_lo(uint32_t saddr) { return ((saddr >> 4) & 0x3FFFu) | (1u << 16); }
+
+// D[tmem] (+)= A[smem] * B[smem]
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+        "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+        :: "r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kCpDescHi) : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 b, {%2, %5};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+        :: "r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kCpDescHi) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+        :: "r"(bar) : "memory");
 }
 
 template <int N>
 __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(N)); }
 template <int N>
 __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(N)); }
+
+// One arrival for a warp whose lanes have all come here.
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
 
 constexpr int kCpRows = 128;        // rows of a half
 constexpr int kCpTile = 128;        // cached tokens of a tile
@@ -64,7 +130,15 @@ struct CpCfg {
     static constexpr int K_BYTES = kCpTile * D * 2;
     static constexpr int V_BYTES = D * kCpTile * 2;
     static constexpr int ST = 2;                                   // stages of K and of V
-    static constexpr int USED = 1024 + 2 * Q_BYTES + ST * (K_BYTES + V_BYTES) + 256;
+    // Codes and pairs as they come from the cache: a slot for the keys or the values of a tile.  Values
+    // lie in chunks of 8 tokens with 16 bytes between them: a warp reads 8 chunks at once, and stores
+    // 16-byte columns of 8 tokens without conflicts either.  (Unpadded, with 8-way conflicts of the
+    // loads, 665 us in the case above; with those of the stores instead, 762 us.)
+    static constexpr int RAW_CHUNK = 8 * F::CODE, RAW_PAD = RAW_CHUNK + 16;
+    static constexpr int RAW_PAIRS = (kCpTile / 8) * RAW_PAD;      // offset of the pairs
+    static constexpr int RAW = RAW_PAIRS + kCpTile * F::PAIR;
+    static constexpr int RAWS = 3;
+    static constexpr int USED = 1024 + 2 * Q_BYTES + ST * (K_BYTES + V_BYTES) + RAWS * RAW + 256;
     // more than half of the SM's shared memory: one CTA, which owns all of TMEM, on an SM
     static constexpr int SMEM = USED > 116 * 1024 ? USED : 116 * 1024;
     static constexpr int S_COL = 0;                                // TMEM columns: S of both halves, O of both halves
@@ -80,12 +154,6 @@ struct CpGrid {
     int kv2;         // 128 rows or fewer: the halves take alternate tiles
     int parts;       // results to be joined for each row: splits * (kv2 ? 2 : 1); 1: written at once
 };
-
-// Shared-memory matrix descriptor: K-major, 128-byte swizzle, 8-row groups 1024 B apart.
-__device__ __forceinline__ uint64_t cp_desc(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-           ((uint64_t)2 << 61);
-}
 
 __device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
@@ -112,29 +180,37 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t qs = base, ks = qs + 2 * C::Q_BYTES, vs = ks + ST * C::K_BYTES, bar0 = vs + ST * C::V_BYTES;
+    const uint32_t qs = base, ks = qs + 2 * C::Q_BYTES, vs = ks + ST * C::K_BYTES, raws = vs + ST * C::V_BYTES,
+                   bar0 = raws + C::RAWS * C::RAW;
     auto k_full = [&](int s) { return bar0 + 8u * s; };
     auto k_empty = [&](int s) { return bar0 + 8u * (ST + s); };
     auto v_full = [&](int s) { return bar0 + 8u * (2 * ST + s); };
     auto v_empty = [&](int s) { return bar0 + 8u * (3 * ST + s); };
     auto q_full = [&](int h) { return bar0 + 8u * (4 * ST + h); };
     auto s_full = [&](int h) { return bar0 + 8u * (4 * ST + 2 + h); };
-    auto p_full = [&](int h) { return bar0 + 8u * (4 * ST + 4 + h); };
-    auto o_done = [&](int h) { return bar0 + 8u * (4 * ST + 6 + h); };
-    const uint32_t done_bar = bar0 + 8u * (4 * ST + 8), tmem_slot = done_bar + 8;
+    auto p_full = [&](int h, int i) { return bar0 + 8u * (4 * ST + 4 + 2 * h + i); };      // of the first and second 64 tokens
+    auto o_done = [&](int h) { return bar0 + 8u * (4 * ST + 8 + h); };
+    auto r_full = [&](int i) { return bar0 + 8u * (4 * ST + 10 + i); };
+    auto r_empty = [&](int i) { return bar0 + 8u * (4 * ST + 10 + C::RAWS + i); };
+    const uint32_t done_bar = bar0 + 8u * (4 * ST + 10 + 2 * C::RAWS), tmem_slot = done_bar + 8;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < ST; ++s) {
-            mbar_init(k_full(s), 128);
+            mbar_init(k_full(s), 4);
             mbar_init(k_empty(s), 1);
-            mbar_init(v_full(s), 128);
+            mbar_init(v_full(s), 4);
             mbar_init(v_empty(s), 1);
         }
         for (int h = 0; h < 2; ++h) {
-            mbar_init(q_full(h), 128);
+            mbar_init(q_full(h), 4);
             mbar_init(s_full(h), 1);
-            mbar_init(p_full(h), 128);
+            mbar_init(p_full(h, 0), 4);
+            mbar_init(p_full(h, 1), 4);
             mbar_init(o_done(h), 1);
+        }
+        for (int i = 0; i < C::RAWS; ++i) {
+            mbar_init(r_full(i), 1);
+            mbar_init(r_empty(i), 4);
         }
         mbar_init(done_bar, 1);
         fence_mbar_init();
@@ -177,44 +253,93 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
 
     if (warp < 4) {
         reg_dec<40>();
-        if (warp == 0 && lane == 0 && events > 0) {
+        if (warp == 0 && events > 0) {
             // -------------------------------------------------------- products
             bool ok = true;
+            auto wait = [&](uint32_t bar, int phase) {
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, (uint32_t)phase & 1u, kDevTimeoutCache));
+            };
+            const uint32_t q_lo = cp_desc_lo(qs), k_lo = cp_desc_lo(ks), v_lo = cp_desc_lo(vs);
             auto issue_s = [&](int e) {
                 const int h = half_of(e), tile = e >> shift, st = tile % ST;
-                ok = ok && mbar_wait(k_full(st), (tile / ST) & 1, kDevTimeoutCache);
+                wait(k_full(st), tile / ST);
                 if (!ok) return;
                 tc_fence_after();
-                const uint32_t qa = qs + (gr.kv2 ? 0 : h) * C::Q_BYTES, kb = ks + st * C::K_BYTES;
+                const uint32_t qa = q_lo + (gr.kv2 ? 0 : h) * (C::Q_BYTES >> 4), kb = k_lo + st * (C::K_BYTES >> 4);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    tc_mma_ss(tmem + C::S_COL + h * kCpTile, cp_desc(qa + (k / 4) * (kCpRows * 128) + (k % 4) * 32),
-                              cp_desc(kb + (k / 4) * (kCpTile * 128) + (k % 4) * 32), C::IDESC_S, k != 0);
-                tc_commit(s_full(h));
-                if (shift == 0 || h == 1) tc_commit(k_empty(st));
+                    mma_ss(tmem + C::S_COL + h * kCpTile, qa + (k / 4) * (kCpRows * 128 >> 4) + (k % 4) * 2,
+                           kb + (k / 4) * (kCpTile * 128 >> 4) + (k % 4) * 2, C::IDESC_S, k != 0);
+                mma_commit(s_full(h));
+                if (shift == 0 || h == 1) mma_commit(k_empty(st));
             };
-            ok = mbar_wait(q_full(0), 0, kDevTimeoutCache) && ((gr.kv2 || !two) || mbar_wait(q_full(1), 0, kDevTimeoutCache));
+            wait(q_full(0), 0);
+            if (two && !gr.kv2) wait(q_full(1), 0);
             issue_s(0);
             if (two && events > 1) issue_s(1);
             const int ahead = two ? 2 : 1;
             for (int e = 0; e < events && ok; ++e) {
                 const int h = half_of(e), tile = e >> shift, st = tile % ST, step = two ? e >> 1 : e;
-                ok = mbar_wait(v_full(st), (tile / ST) & 1, kDevTimeoutCache) &&
-                     mbar_wait(p_full(h), step & 1, kDevTimeoutCache);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t vb = vs + st * C::V_BYTES, pt = tmem + C::S_COL + h * kCpTile;
+                const uint32_t vb = v_lo + st * (C::V_BYTES >> 4), pt = tmem + C::S_COL + h * kCpTile;
+                wait(v_full(st), tile / ST);
 #pragma unroll
-                for (int k = 0; k < kCpTile / 16; ++k)
-                    tc_mma_ts(tmem + C::O_COL + h * D, pt + k * 8, cp_desc(vb + (k / 4) * (D * 128) + (k % 4) * 32), C::IDESC_O,
-                              (step | k) != 0);
-                tc_commit(o_done(h));
-                if (shift == 0 || h == 1) tc_commit(v_empty(st));
+                for (int i = 0; i < 2; ++i) {
+                    wait(p_full(h, i), step);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_ts(tmem + C::O_COL + h * D, pt + (4 * i + k) * 8, vb + i * (D * 128 >> 4) + k * 2, C::IDESC_O,
+                               i | k ? 1 : step);
+                }
+                if (!ok) break;
+                if (step + 1 == steps_of(h)) mma_commit(o_done(h));
+                if (shift == 0 || h == 1) mma_commit(v_empty(st));
                 // the half's next S goes over this P: products run in the order of their issue
                 if (e + ahead < events) issue_s(e + ahead);
             }
-            tc_commit(done_bar);            // every product retired before TMEM is released
+            mma_commit(done_bar);           // every product retired before TMEM is released
             mbar_wait(done_bar, 0, kDevTimeoutDrain);
+        } else if (warp == 1) {
+            // -------------------------------------------------------- codes and pairs into shared memory
+            // Lanes 0-7: the codes of the keys of a run (the part of a page that is in the tile); 8-15: its
+            // pairs; 16-31: the codes of the values of a chunk.  Few copies: issuing one takes some 40 cycles.
+            const int ps_log = p.c.page_shift, run_rows = min(1 << ps_log, kCpTile);
+            const int kind = lane < 8 ? 0 : lane < 16 ? 1 : 2;
+            const int rows_c = kind == 2 ? 8 : run_rows, unit = kind == 2 ? lane - 16 : lane & 7;
+            const uint32_t row_b = kind == 1 ? F::PAIR : F::CODE, bytes = (uint32_t)rows_c * row_b;
+            const uint32_t dst_off = kind == 0 ? unit * bytes : kind == 1 ? C::RAW_PAIRS + unit * bytes : unit * C::RAW_PAD;
+            const uint32_t src_off = kind == 0 ? 0u : kind == 1 ? (uint32_t)(2 * F::CODE) << ps_log : (uint32_t)F::CODE << ps_log;
+            auto token_of = [&](int tile) {
+                const int tok = (t0 + tile) * kCpTile + unit * rows_c;
+                return unit * rows_c < kCpTile && tok < s.len && tok + rows_c > tok_lo ? tok : -1;
+            };
+            bool ok = true;
+            int i = 0, slot = 0, turn = 1;
+            int tok = n > 0 ? token_of(0) : -1;
+            int64_t page = tok >= 0 ? page_of(p, b, tok >> ps_log) : 0;
+            for (int tile = 0; tile < n && ok; ++tile) {
+                const uint32_t valid = __ballot_sync(0xffffffffu, tok >= 0);
+                const bool mine = tok >= 0;
+                const uint8_t* src = cache_block(p.c, page, head) + src_off + (uint32_t)(tok & ((1 << ps_log) - 1)) * row_b;
+                tok = tile + 1 < n ? token_of(tile + 1) : -1;
+                page = tok >= 0 ? page_of(p, b, tok >> ps_log) : 0;
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv, ++i) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_sleep(r_empty(slot), (uint32_t)turn, kDevTimeoutCache));
+                    if (!ok) break;
+                    const uint32_t codes = kv ? __popc(valid >> 16) * 8u * F::CODE : __popc(valid & 0xFFu) * (uint32_t)run_rows * F::CODE;
+                    const uint32_t pairs = __popc(valid & 0xFF00u) * (uint32_t)run_rows * F::PAIR;
+                    if (lane == 0) mbar_arrive_expect_tx(r_full(slot), codes + pairs);
+                    __syncwarp();
+                    if (mine && kind != (kv ? 0 : 2))
+                        bulk_load(raws + slot * C::RAW + dst_off, src + (kv && kind == 1 ? (uint32_t)F::PAIR << ps_log : 0u), bytes,
+                                  r_full(slot));
+                    if (++slot == C::RAWS) { slot = 0; turn ^= 1; }
+                }
+            }
+            if (!ok)       // what was issued may still be landing
+                for (int j = max(0, i - C::RAWS); j < i; ++j) mbar_wait(r_full(j % C::RAWS), (uint32_t)(j / C::RAWS) & 1u, kDevTimeoutDrain);
         }
     } else if (warp < 8) {
         // ------------------------------------------------------------ codes -> operands
@@ -225,64 +350,28 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
         constexpr int KWD = KB / 4;                   // in words
         constexpr int DV = D / 8, VWD = DV / 8;       // values of each of 8 tokens that it takes, in words
         const int chunk = lane & 7, dg = (lane >> 3) + 4 * (w >> 1), vtok = (w & 1) * 64 + chunk * 8;
-        const uint32_t ps_mask = (1u << p.c.page_shift) - 1u;
         const int ka = t * (D / 4) / G, va = dg * DV / G;               // groups
-        uint32_t kw[4][KWD], kp[4], vw[8][VWD], vp[8];
-        auto load_k = [&](int tile) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int tok = (t0 + tile) * kCpTile + i * 32 + w * 8 + g;
-                kp[i] = 0;
-#pragma unroll
-                for (int j = 0; j < KWD; ++j) kw[i][j] = 0;
-                if (tok >= s.len || tok < tok_lo) continue;
-                const uint8_t* blk = cache_block(p.c, page_of(p, b, tok >> p.c.page_shift), head);
-                const uint32_t row = (uint32_t)tok & ps_mask;
-                const uint8_t* src = blk + row * F::CODE + t * KB;
-                if constexpr (KWD == 4) {
-                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
-                    kw[i][0] = v.x; kw[i][1] = v.y; kw[i][2] = v.z; kw[i][3] = v.w;
-                } else {
-                    const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
-                    kw[i][0] = v.x; kw[i][1] = v.y;
-                }
-                kp[i] = __ldg(reinterpret_cast<const uint32_t*>(blk + ((2 * F::CODE) << p.c.page_shift) + row * F::PAIR + ka * 4));
-            }
-        };
-        auto load_v = [&](int tile) {
-            const int tok = (t0 + tile) * kCpTile + vtok;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                vp[k] = 0;
-#pragma unroll
-                for (int j = 0; j < VWD; ++j) vw[k][j] = 0;
-            }
-            if (tok >= s.len || tok + 8 <= tok_lo) return;
-            const uint8_t* blk = cache_block(p.c, page_of(p, b, tok >> p.c.page_shift), head);
-            const uint32_t row = (uint32_t)tok & ps_mask;
-            const uint8_t* src = blk + (F::CODE << p.c.page_shift) + row * F::CODE + dg * (DV / 2);
-            const uint8_t* pr = blk + ((2 * F::CODE + F::PAIR) << p.c.page_shift) + row * F::PAIR + va * 4;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                // a row past the end, or below what is seen, may never have been written
-                const bool here = tok + k < s.len && tok + k >= tok_lo;
-                if constexpr (VWD == 2) {
-                    const uint2 v = __ldg(reinterpret_cast<const uint2*>(src + k * F::CODE));
-                    vw[k][0] = v.x; vw[k][1] = v.y;
-                } else {
-                    vw[k][0] = __ldg(reinterpret_cast<const uint32_t*>(src + k * F::CODE));
-                }
-                const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(pr + k * F::PAIR));
-                vp[k] = here ? v : 0u;
-            }
-        };
         bool ok = true;
-        if (n > 0) load_k(0);
+        int slot = 0, turn = 0;
         for (int tile = 0; tile < n; ++tile) {
             const int st = tile % ST;
-            load_v(tile);
-            ok = __all_sync(0xffffffffu, mbar_wait(k_empty(st), ((tile / ST) & 1) ^ 1, kDevTimeoutCache));
+            ok = __all_sync(0xffffffffu, mbar_wait(r_full(slot), (uint32_t)turn, kDevTimeoutCache) &&
+                                             mbar_wait(k_empty(st), ((tile / ST) & 1) ^ 1, kDevTimeoutCache));
             if (!ok) break;
+            const uint8_t* src = smem_raw + (raws - raw) + slot * C::RAW;
+            uint32_t kw[4][KWD], kp[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = i * 32 + w * 8 + g;
+                if constexpr (KWD == 4) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(src + row * F::CODE + t * KB);
+                    kw[i][0] = v.x; kw[i][1] = v.y; kw[i][2] = v.z; kw[i][3] = v.w;
+                } else {
+                    const uint2 v = *reinterpret_cast<const uint2*>(src + row * F::CODE + t * KB);
+                    kw[i][0] = v.x; kw[i][1] = v.y;
+                }
+                kp[i] = *reinterpret_cast<const uint32_t*>(src + C::RAW_PAIRS + row * F::PAIR + ka * 4);
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int row = i * 32 + w * 8 + g;
@@ -300,10 +389,46 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                 }
             }
             fence_proxy_async_smem();
-            mbar_arrive(k_full(st));
-            if (tile + 1 < n) load_k(tile + 1);
-            ok = __all_sync(0xffffffffu, mbar_wait(v_empty(st), ((tile / ST) & 1) ^ 1, kDevTimeoutCache));
+            warp_arrive(k_full(st));
+            warp_arrive(r_empty(slot));
+            if (++slot == C::RAWS) { slot = 0; turn ^= 1; }
+            ok = __all_sync(0xffffffffu, mbar_wait(r_full(slot), (uint32_t)turn, kDevTimeoutCache) &&
+                                             mbar_wait(v_empty(st), ((tile / ST) & 1) ^ 1, kDevTimeoutCache));
             if (!ok) break;
+            src = smem_raw + (raws - raw) + slot * C::RAW;
+            uint32_t vw[8][VWD], vp[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint8_t* at = src + (vtok / 8) * C::RAW_PAD + k * F::CODE + dg * (DV / 2);
+                if constexpr (VWD == 2) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(at);
+                    vw[k][0] = v.x; vw[k][1] = v.y;
+                } else {
+                    vw[k][0] = *reinterpret_cast<const uint32_t*>(at);
+                }
+            }
+            {
+                const uint4* at = reinterpret_cast<const uint4*>(src + C::RAW_PAIRS + vtok * F::PAIR);
+                if constexpr (F::NG == 1) {
+                    const uint4 v0 = at[0], v1 = at[1];
+                    vp[0] = v0.x; vp[1] = v0.y; vp[2] = v0.z; vp[3] = v0.w;
+                    vp[4] = v1.x; vp[5] = v1.y; vp[6] = v1.z; vp[7] = v1.w;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint4 v = at[k];
+                        vp[2 * k] = va ? v.y : v.x;
+                        vp[2 * k + 1] = va ? v.w : v.z;
+                    }
+                }
+            }
+            const int tok = (t0 + tile) * kCpTile + vtok;
+            if (tok < tok_lo || tok + 8 > s.len) {
+                // a row past the end, or below what is seen, may never have been written
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (tok + k >= s.len || tok + k < tok_lo) vp[k] = 0u;
+            }
             {
                 __half2 sc[4], mn[4];
 #pragma unroll
@@ -333,7 +458,9 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                     }
             }
             fence_proxy_async_smem();
-            mbar_arrive(v_full(st));
+            warp_arrive(v_full(st));
+            warp_arrive(r_empty(slot));
+            if (++slot == C::RAWS) { slot = 0; turn ^= 1; }
         }
     } else {
         // ------------------------------------------------------------ softmax: a thread a row
@@ -382,7 +509,7 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                 *reinterpret_cast<uint4*>(dst + (j / 8) * (kCpRows * 128) + (((j % 8) ^ (r_in & 7)) * 16)) = o;
             }
             fence_proxy_async_smem();
-            mbar_arrive(q_full(h));
+            warp_arrive(q_full(h));
         }
         if (gr.kv2) {
             // both halves hold the same rows: the second takes the first's factors
@@ -420,9 +547,8 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
 #pragma unroll
                 for (int c = 0; c < kCpTile; c += 8)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1])));
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * r;
+                    for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1]));
+                const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * r;
                 const bool move = fresh ? top > -INFINITY : top > m + 8.f;
                 if (__any_sync(0xffffffffu, move)) {
                     float keep = 1.f;
@@ -432,10 +558,7 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                         fresh = false;
                     }
                     l *= keep;
-                    if (step > 0) {
-                        ok = __all_sync(0xffffffffu, mbar_wait(o_done(h), (step - 1) & 1, kDevTimeoutCache));
-                        if (!ok) break;
-                        tc_fence_after();
+                    if (step > 0) {             // this S was issued after the last step's PV: O is at rest
 #pragma unroll 1
                         for (int c = 0; c < D; c += 32) {
                             uint32_t o[32];
@@ -447,28 +570,37 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                         }
                     }
                 }
-                const float off = 6.f - m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const uint64_t r2 = pair2(r, r), off2 = pair2(6.f - m, 6.f - m);
+                uint64_t sum2[2] = {pair2(0.f, 0.f), pair2(0.f, 0.f)};
 #pragma unroll
-                for (int c = 0; c < kCpTile; c += 64) {
-                    uint32_t pk[32];
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t pk[16];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const float p0 = exp2_fast(fmaf(__uint_as_float(x[c + 2 * e]), r, off));
-                        const float p1 = exp2_fast(fmaf(__uint_as_float(x[c + 2 * e + 1]), r, off));
-                        sum[2 * (e & 1)] += p0;
-                        sum[2 * (e & 1) + 1] += p1;
+                    for (int e = 0; e < 16; ++e) {
+                        float p0, p1;
+                        split2(fma2(pair2(__uint_as_float(x[32 * c + 2 * e]), __uint_as_float(x[32 * c + 2 * e + 1])), r2, off2), p0, p1);
+                        p0 = exp2_fast(p0);
+                        p1 = exp2_fast(p1);
+                        sum2[e & 1] = add2(sum2[e & 1], pair2(p0, p1));
                         pk[e] = pack16(p0, p1, false);
                     }
-                    tmem_st_x32(s_t + c / 2, pk);
+                    tmem_st_x16(s_t + 16 * c, pk);
+                    if (c & 1) {
+                        tc_wait_st();
+                        tc_fence_before();
+                        warp_arrive(p_full(h, c >> 1));
+                    }
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tc_wait_st();
+                float a0, a1, b0, b1;
+                split2(sum2[0], a0, a1);
+                split2(sum2[1], b0, b1);
+                l += (a0 + a1) + (b0 + b1);
+            } else {
+                warp_arrive(p_full(h, 0));
+                warp_arrive(p_full(h, 1));
             }
-            tc_fence_before();
-            mbar_arrive(p_full(h));
         }
-        if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done(h), (steps - 1) & 1, kDevTimeoutCache));
+        if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done(h), 0, kDevTimeoutCache));
         // ---- results
         if (ok && warp_live && rows > 0) {
             tc_fence_after();
