@@ -139,19 +139,20 @@ static AttentionParams attention_params(const w4a16_cache& c, const w4a16_cache_
 
 // How an attention call is run: by rows (query heads of a key head times queries).
 struct AttentionPlan {
-    int nt;              // 8-row tiles of the decode kernel; 0: more rows than it takes, the prompt kernel
+    int row_blocks;      // blocks of 8 rows of the decode kernel; 0: the prompt kernel
     int grid;
     CpGrid prompt;
     size_t workspace;
 };
 
-template <int D, int G, int NT>
+template <int D, int G>
 static AttentionPlan plan_decode_t(const w4a16_cache& c, const w4a16_cache_attention_args& a, const DeviceInfo& dev) {
-    using C = CdCfg<D, G, NT>;
-    const int64_t segments = (int64_t)a.batch * c.kv_heads;
+    using C = CdCfg<D, G>;
+    const int64_t rows = (int64_t)a.max_q * (a.q_heads / c.kv_heads);
+    const int64_t blocks = (rows + C::ROWS - 1) / C::ROWS, segments = (int64_t)a.batch * c.kv_heads * blocks;
     const int64_t tiles = ((int64_t)a.table_pages * c.page_size + kCdTile - 1) / kCdTile;
     AttentionPlan p = {};
-    p.nt = NT;
+    p.row_blocks = (int)blocks;
     p.grid = (int)std::max<int64_t>(1, std::min<int64_t>(segments * tiles, (int64_t)C::CTAS * dev.num_sms));
     p.workspace = cd_info_bytes(segments) + 2 * (size_t)p.grid * cd_slot_floats(C::ROWS, D) * sizeof(float);
     return p;
@@ -176,12 +177,19 @@ static AttentionPlan plan_prompt(const w4a16_cache& c, const w4a16_cache_attenti
     return p;
 }
 
+// Up to 32 rows a (sequence, key head) go to the decode kernel, which streams the codes once for
+// each 8 of them; more to the prompt kernel, whose 128-row products cost the same for few rows.
+// Measured with 4 rows a query (decode / prompt kernel, us): 16 sequences of up to 4096 tokens, 5
+// queries 41 / 73, 8 queries 52 / 74, 12 queries 77 / 81; 64 of up to 512, 8 queries 63 / 67, 12
+// queries 88 / 70; 2 of 16384, 8 queries 43 / 53, 12 queries 60 / 54.
+constexpr int64_t kDecodeRows = 32;
+
 static AttentionPlan plan_attention(const w4a16_cache& c, const w4a16_cache_attention_args& a, const DeviceInfo& dev) {
     const int64_t rows = (int64_t)a.max_q * (a.q_heads / c.kv_heads);
-    if (rows > 16) return plan_prompt(c, a, dev);
+    if (rows > kDecodeRows) return plan_prompt(c, a, dev);
     AttentionPlan p = {};
     with_format(c, [&](auto d, auto g) {
-        p = rows <= 8 ? plan_decode_t<d.value, g.value, 1>(c, a, dev) : plan_decode_t<d.value, g.value, 2>(c, a, dev);
+        p = plan_decode_t<d.value, g.value>(c, a, dev);
         return cudaSuccess;
     });
     return p;
@@ -191,16 +199,16 @@ size_t cache_attention_workspace(const w4a16_cache& c, const w4a16_cache_attenti
     return plan_attention(c, a, dev).workspace;
 }
 
-template <int D, int G, int NT>
+template <int D, int G>
 static cudaError_t launch_decode_t(const AttentionParams& ap, const AttentionPlan& plan, cudaStream_t stream, bool pdl) {
-    using C = CdCfg<D, G, NT>;
-    auto kern = cache_decode_kernel<D, G, NT>;
+    using C = CdCfg<D, G>;
+    auto kern = cache_decode_kernel<D, G>;
     cudaError_t err = ensure_max_dynamic_smem(reinterpret_cast<const void*>(kern));
     if (err != cudaSuccess) return err;
     err = launch(kern, dim3(plan.grid), kCdThreads, C::SMEM, stream, pdl, ap);
     if (err != cudaSuccess) return err;
     // threads of a combine block: enough slices of the parts that a segment may have
-    const int64_t segments = (int64_t)ap.batch * ap.c.kv_heads;
+    const int64_t segments = (int64_t)ap.batch * ap.c.kv_heads * ap.row_blocks;
     const int threads = plan.grid / segments >= 64 ? 512 : 128;
     const int rows = std::min(C::ROWS, ap.max_q * ap.shared);
     return launch(cache_decode_combine_kernel<D>, dim3((unsigned)segments, (unsigned)rows), threads, 0, stream, pdl, ap,
@@ -225,9 +233,9 @@ cudaError_t launch_cache_attention(const w4a16_cache& c, const w4a16_cache_atten
     AttentionParams p = attention_params(c, a);
     p.workspace = static_cast<char*>(workspace);
     const AttentionPlan plan = plan_attention(c, a, dev);
+    p.row_blocks = plan.row_blocks;
     return with_format(c, [&](auto d, auto g) {
-        if (plan.nt == 1) return launch_decode_t<d.value, g.value, 1>(p, plan, stream, pdl);
-        if (plan.nt == 2) return launch_decode_t<d.value, g.value, 2>(p, plan, stream, pdl);
+        if (plan.row_blocks > 0) return launch_decode_t<d.value, g.value>(p, plan, stream, pdl);
         return launch_prompt_t<d.value, g.value>(p, plan, stream, pdl);
     });
 }

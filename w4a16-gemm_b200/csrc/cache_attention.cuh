@@ -31,6 +31,7 @@ struct AttentionParams {
     int32_t table_pages, batch, max_q;
     int32_t shared;              // query heads of a key head
     int32_t window;
+    int32_t row_blocks;          // decode kernel: blocks of rows of the sequence with most queries
     bool causal, bf16;
     char* workspace;
 };

@@ -1,11 +1,12 @@
-// Attention of few rows (query heads of a key head times queries of a sequence, at most 16)
-// over the 4-bit cache: one pass over the codes, bound by memory.  Included by cache.cu only.
+// Attention of few rows (query heads of a key head times queries of a sequence) over the 4-bit
+// cache: rows in blocks of 8, one pass over the codes a block.  Included by cache.cu only.
 //
-// Work.  A unit is 128 cached tokens of one (sequence, key head).  All units of the call,
-// sequence by sequence and head by head, are cut into equal contiguous ranges, one a CTA, so
-// that ragged batches load every SM alike whatever the lengths; lengths are read on the device.
-// A range holds whole segments (a (sequence, head) pair), whose results are written at once,
-// and at most two parts of segments, whose sums go to the workspace for combine_kernel.
+// Work.  A segment is a (sequence, key head, block of rows), a unit 128 cached tokens of one.  All
+// units of the call, segment by segment (a head's blocks after one another: from the second on
+// the codes come from L2), are cut into equal contiguous ranges, one a CTA, so that ragged batches
+// load every SM alike whatever the lengths; lengths are read on the device.  A range holds whole
+// segments, whose results are written at once, and at most two parts of segments, whose sums go
+// to the workspace for cache_decode_combine_kernel.
 //
 // A CTA is one producer warp, which walks the page table and fills a ring of stages with bulk
 // copies (the runs of key codes, value codes and pairs of each page), and four consumer warps,
@@ -40,6 +41,7 @@
 namespace w4a16 {
 
 constexpr int kCdTile = 128;        // tokens of a unit
+constexpr int kCdRows = 8;          // rows of a block: the right side of an m16n8k16 product
 constexpr int kCdWarps = 4;         // consumer warps
 constexpr int kCdWarpTokens = kCdTile / kCdWarps;
 constexpr int kCdThreads = (kCdWarps + 1) * 32;
@@ -47,26 +49,26 @@ constexpr int kCdThreads = (kCdWarps + 1) * 32;
 // What the producer tells the consumers about a stage.
 struct __align__(16) CdStage {
     int tok0;        // first token of the unit
-    int b, head;
+    int row0, head;  // first row of the block, key head
     int flags;       // 1: first unit of this CTA's part of the segment, 2: last, 4: the part is not all of it,
                      // 8: last unit of this CTA
     int len, nq, q0;
     int slot;        // workspace slot of the part
 };
 
-template <int D, int G, int NT>
+template <int D, int G>
 struct CdCfg {
     using F = CacheFmt<D, G>;
     static constexpr int CODES = kCdTile * F::CODE;
     static constexpr int PAIRS = kCdTile * F::PAIR;
     static constexpr int STAGE = 2 * (CODES + PAIRS);
-    static constexpr int ROWS = 8 * NT;
+    static constexpr int ROWS = kCdRows;
     static constexpr int STAGES = D == 64 ? 5 : 3;
     static constexpr int LD = D + 4;                               // floats of a row in the merge buffer
     static constexpr int MERGE = kCdWarps * ROWS * LD * 4;         // [warp][row][LD]: sums, then maximum and sum of weights
     static constexpr int HDR = STAGES * (int)sizeof(CdStage);
     static constexpr int SMEM = STAGES * STAGE + MERGE + HDR + 256;
-    static constexpr int CTAS = NT == 1 ? 3 : 2;                   // resident on an SM (shared memory and registers)
+    static constexpr int CTAS = 3;                                 // resident on an SM (shared memory, 128 registers a thread)
 };
 
 // What the start and end of a segment cost beside its units (queries, merge), in units: ranges
@@ -81,12 +83,18 @@ __device__ __forceinline__ int cd_tiles(const AttentionParams& p, const SeqSpan&
     if (s.nq == 0 || s.len == 0) return 0;
     return (s.len + kCdTile - 1) / kCdTile - cd_first_tile(p, s);
 }
-__device__ __forceinline__ int cd_cost(const AttentionParams& p, const SeqSpan& s) {
+// Blocks of rows of a sequence, and what all its segments cost.
+template <int ROWS>
+__device__ __forceinline__ int cd_blocks(const AttentionParams& p, const SeqSpan& s) {
+    return (s.nq * p.shared + ROWS - 1) / ROWS;
+}
+template <int ROWS>
+__device__ __forceinline__ long long cd_cost(const AttentionParams& p, const SeqSpan& s) {
     const int nt = cd_tiles(p, s);
-    return nt ? nt + kCdSegmentCost : 0;
+    return nt ? (long long)(nt + kCdSegmentCost) * (p.c.kv_heads * cd_blocks<ROWS>(p, s)) : 0;
 }
 
-// Workspace: per (sequence, key head) the CTAs {first, last} that hold parts of it, then 2 slots
+// Workspace: per segment the CTAs {first, last} that hold parts of it, then 2 slots
 // a CTA of ROWS x (D + 2) floats: sums, maxima, sums of weights.  Slot 0 is the part of a segment
 // that began in an earlier CTA, slot 1 of one that begins here.
 __host__ __device__ __forceinline__ size_t cd_info_bytes(int64_t segments) {
@@ -114,10 +122,10 @@ __device__ __forceinline__ void hmma_zero(float (&d)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
 }
 
-template <int D, int G, int NT>
-__global__ void __launch_bounds__(kCdThreads, CdCfg<D, G, NT>::CTAS)
+template <int D, int G>
+__global__ void __launch_bounds__(kCdThreads, CdCfg<D, G>::CTAS)
 cache_decode_kernel(const __grid_constant__ AttentionParams p) {
-    using C = CdCfg<D, G, NT>;
+    using C = CdCfg<D, G>;
     using F = CacheFmt<D, G>;
     constexpr int NG = F::NG, ST = C::STAGES, ROWS = C::ROWS;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -150,8 +158,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
         const int per = (p.batch + kCdThreads - 1) / kCdThreads;
         const int b0 = min((int)threadIdx.x * per, p.batch), b1 = min(b0 + per, p.batch);
         long long mine = 0;
-        for (int b = b0; b < b1; ++b) mine += cd_cost(p, seq_span(p, b));
-        mine *= hk;
+        for (int b = b0; b < b1; ++b) mine += cd_cost<ROWS>(p, seq_span(p, b));
         long long incl = mine;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
@@ -172,7 +179,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
         if (u0 >= base && u0 < base + mine) {
             int b = b0;
             for (; b < b1; ++b) {
-                const long long n = (long long)cd_cost(p, seq_span(p, b)) * hk;
+                const long long n = cd_cost<ROWS>(p, seq_span(p, b));
                 if (u0 < base + n) break;
                 base += n;
             }
@@ -200,8 +207,9 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
         int b = (int)found[2];
         SeqSpan s = seq_span(p, b);
         int nt = cd_tiles(p, s), first = cd_first_tile(p, s);
-        const int local = (int)(u0 - found[1]);
-        int head = local / (nt + kCdSegmentCost), tile = local % (nt + kCdSegmentCost) - kCdSegmentCost;
+        int blocks = cd_blocks<ROWS>(p, s);
+        const long long local = u0 - found[1];
+        int seg = (int)(local / (nt + kCdSegmentCost)), tile = (int)(local % (nt + kCdSegmentCost)) - kCdSegmentCost;   // of the sequence
         long long u = u0;
         if (tile < 0) { u -= tile; tile = 0; }
         bool begins = true;
@@ -220,7 +228,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
             const int tok = tok0 + run * rows;
             const bool valid = run * rows < kCdTile && tok < s.len && tok + rows > seen_lo(p, s.len - s.nq);
             const int64_t page = valid ? page_of(p, b, tok >> ps_log) : 0;
-            const uint8_t* src = cache_block(p.c, page, head) + src_part + (uint32_t)(tok & ((1 << ps_log) - 1)) * unit_b;
+            const uint8_t* src = cache_block(p.c, page, seg / blocks) + src_part + (uint32_t)(tok & ((1 << ps_log) - 1)) * unit_b;
             const bool got = mbar_wait_sleep(empty(st), (uint32_t)turn ^ 1u, kDevTimeoutCache);
             if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
             const int runs = __popc(__ballot_sync(0xffffffffu, valid)) / 4;
@@ -228,14 +236,14 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
             if (lane == 0) {
                 const bool part_of = seg0 < u0 || seg0 + nt > u1;
                 CdStage h;
-                h.tok0 = tok0; h.b = b; h.head = head;
+                h.tok0 = tok0; h.row0 = seg % blocks * ROWS; h.head = seg / blocks;
                 const bool last = u + 1 + (tile + 1 == nt ? kCdSegmentCost : 0) >= u1;
                 h.flags = (begins ? 1 : 0) | (ends ? 2 : 0) | (part_of ? 4 : 0) | (last ? 8 : 0);
                 h.len = s.len; h.nq = s.nq; h.q0 = s.q0;
                 h.slot = 2 * (int)blockIdx.x + (seg0 >= u0 ? 1 : 0);
                 hdr[st] = h;
                 if (tile == 0)
-                    info[(int64_t)b * hk + head] = make_int2((int)blockIdx.x, (int)(((seg0 + nt) * ctas - 1) / total));
+                    info[((int64_t)b * hk + h.head) * p.row_blocks + seg % blocks] = make_int2((int)blockIdx.x, (int)(((seg0 + nt) * ctas - 1) / total));
                 mbar_arrive_expect_tx(full(st), (uint32_t)(runs * rows * F::TOKEN));
             }
             __syncwarp();
@@ -248,10 +256,11 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                 tile = 0;
                 u += kCdSegmentCost;
                 seg0 = u;
-                if (++head == hk && u < u1) {
-                    head = 0;
+                if (++seg == hk * blocks && u < u1) {
+                    seg = 0;
                     do { s = seq_span(p, ++b); nt = cd_tiles(p, s); } while (nt == 0);
                     first = cd_first_tile(p, s);
+                    blocks = cd_blocks<ROWS>(p, s);
                 }
             }
         }
@@ -271,12 +280,12 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
     float* merge = reinterpret_cast<float*>(merge_p);
     uint32_t merge_phase = 0;
 
-    uint32_t qf[2 * KW][NT][2];                                  // query fragments, contraction steps of 16
-    float o[4 * VW][NT][4];                                      // sums: (value 2j, rows 2t, 2t+1), (value 2j+1, ...)
-    float oc[NG][NT][4];                                         // the same weights times 8
-    float m[NT][2], thr[NT][2], sum[NT][2], msum[NG][NT][2];
-    float r24[NT][2], qs[NG][NT][2];                             // score = r24 (s (q'.c) + m qs)
-    int lo[NT][2], hi[NT][2];
+    uint32_t qf[2 * KW][2];                                  // query fragments, contraction steps of 16
+    float o[4 * VW][4];                                      // sums: (value 2j, rows 2t, 2t+1), (value 2j+1, ...)
+    float oc[NG][4];                                         // the same weights times 8
+    float m[2], thr[2], sum[2], msum[NG][2];
+    float r24[2], qs[NG][2];                             // score = r24 (s (q'.c) + m qs)
+    int lo[2], hi[2];
     float vlim = 0.f, vmul = 1.f;                                // s_t <= vlim; w_t s_t vmul is what fp16 holds
     int lo_all = 0, lo_max = 0, hi_min = 0;
 
@@ -287,92 +296,89 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
         const CdStage h = hdr[st];
         if (h.flags & 1) {
             // ---- a new segment: queries, masks, empty state
-            const int rows = h.nq * p.shared;
-            const int pos0 = h.len - h.nq;
-            lo_all = seen_lo(p, pos0);
-            lo_max = seen_lo(p, h.len - 1);
-            hi_min = seen_hi(p, pos0, h.len);
+            const int rows = min(h.nq * p.shared - h.row0, ROWS);
+            const int pos0 = h.len - h.nq, pos_first = pos0 + h.row0 / p.shared;
+            lo_all = seen_lo(p, pos_first);
+            lo_max = seen_lo(p, pos0 + (h.row0 + rows - 1) / p.shared);
+            hi_min = seen_hi(p, pos_first, h.len);
+            const int row = g;
+            uint4 raw[NG][G / 32];
+            uint32_t amax = 0;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int row = g + 8 * n;
-                uint4 raw[NG][G / 32];
-                uint32_t amax = 0;
+            for (int a = 0; a < NG; ++a)
 #pragma unroll
-                for (int a = 0; a < NG; ++a)
+                for (int j = 0; j < G / 32; ++j) {
+                    raw[a][j] = make_uint4(0, 0, 0, 0);
+                    if (row < rows)
+                        raw[a][j] = __ldg(reinterpret_cast<const uint4*>(
+                            p.q + (int64_t)(h.q0 + (h.row0 + row) / p.shared) * p.q_token +
+                            (int64_t)(h.head * p.shared + (h.row0 + row) % p.shared) * p.q_head + a * G + t * (G / 4)) + j);
+                }
+            float f[NG][G / 4];
 #pragma unroll
-                    for (int j = 0; j < G / 32; ++j) {
-                        raw[a][j] = make_uint4(0, 0, 0, 0);
-                        if (row < rows)
-                            raw[a][j] = __ldg(reinterpret_cast<const uint4*>(
-                                p.q + (int64_t)(h.q0 + row / p.shared) * p.q_token +
-                                (int64_t)(h.head * p.shared + row % p.shared) * p.q_head + a * G + t * (G / 4)) + j);
-                    }
-                float f[NG][G / 4];
+            for (int a = 0; a < NG; ++a)
 #pragma unroll
-                for (int a = 0; a < NG; ++a)
+                for (int j = 0; j < G / 32; ++j) {
+                    float x[8];
+                    if (p.bf16) unpack8<true>(raw[a][j], x);
+                    else unpack8<false>(raw[a][j], x);
 #pragma unroll
-                    for (int j = 0; j < G / 32; ++j) {
-                        float x[8];
-                        if (p.bf16) unpack8<true>(raw[a][j], x);
-                        else unpack8<false>(raw[a][j], x);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            f[a][8 * j + e] = x[e];
-                            amax = max(amax, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-                        }
-                    }
-                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                // the row's power of two: its largest value comes to [2^13, 2^14)
-                const int ex = min(max((int)(amax >> 23), 24), 250);
-                const float down = __uint_as_float((uint32_t)(267 - ex) << 23 & 0x7F800000u);   // 2^(140 - ex)
-                const float back = __uint_as_float((uint32_t)(ex - 13) << 23);                  // 2^(ex - 140)
-                float total_q[NG];
-#pragma unroll
-                for (int a = 0; a < NG; ++a) {
-                    total_q[a] = 0.f;
-#pragma unroll
-                    for (int e = 0; e < G / 4; ++e) {
-                        f[a][e] *= down;
-                        total_q[a] += __half2float(__float2half_rn(f[a][e]));
-                    }
-                    total_q[a] += __shfl_xor_sync(0xffffffffu, total_q[a], 1);
-                    total_q[a] += __shfl_xor_sync(0xffffffffu, total_q[a], 2);
-#pragma unroll
-                    for (int w = 0; w < G / 32; ++w) {
-                        const float* x = &f[a][8 * w];
-                        const int c = 2 * (a * (G / 32) + w);
-                        qf[c][n][0] = pack16(x[0], x[4], false);
-                        qf[c][n][1] = pack16(x[1] * 0.0625f, x[5] * 0.0625f, false);
-                        qf[c + 1][n][0] = pack16(x[2], x[6], false);
-                        qf[c + 1][n][1] = pack16(x[3] * 0.0625f, x[7] * 0.0625f, false);
+                    for (int e = 0; e < 8; ++e) {
+                        f[a][8 * j + e] = x[e];
+                        amax = max(amax, __float_as_uint(x[e]) & 0x7FFFFFFFu);
                     }
                 }
-                const float r = back * p.scale_log2 * 16777216.f;
+            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            // the row's power of two: its largest value comes to [2^13, 2^14)
+            const int ex = min(max((int)(amax >> 23), 24), 250);
+            const float down = __uint_as_float((uint32_t)(267 - ex) << 23 & 0x7F800000u);   // 2^(140 - ex)
+            const float back = __uint_as_float((uint32_t)(ex - 13) << 23);                  // 2^(ex - 140)
+            float total_q[NG];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int from = 8 * t + 4 * e, mine = 2 * t + e + 8 * n;
-                    r24[n][e] = __shfl_sync(0xffffffffu, r, from);
+            for (int a = 0; a < NG; ++a) {
+                total_q[a] = 0.f;
 #pragma unroll
-                    for (int a = 0; a < NG; ++a) qs[a][n][e] = __shfl_sync(0xffffffffu, total_q[a], from) * 5.9604644775390625e-8f;
-                    const int pos = pos0 + mine / p.shared;
-                    hi[n][e] = mine < rows ? seen_hi(p, pos, h.len) : h.len;
-                    lo[n][e] = mine < rows ? seen_lo(p, pos) : 0;
-                    m[n][e] = 0.f;
-                    thr[n][e] = -3.0e38f;                        // nothing seen yet: any score sets the maximum
-                    sum[n][e] = 0.f;
-#pragma unroll
-                    for (int a = 0; a < NG; ++a) msum[a][n][e] = 0.f;
+                for (int e = 0; e < G / 4; ++e) {
+                    f[a][e] *= down;
+                    total_q[a] += __half2float(__float2half_rn(f[a][e]));
                 }
+                total_q[a] += __shfl_xor_sync(0xffffffffu, total_q[a], 1);
+                total_q[a] += __shfl_xor_sync(0xffffffffu, total_q[a], 2);
 #pragma unroll
-                for (int j = 0; j < 4 * VW; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[j][n][e] = 0.f;
-#pragma unroll
-                for (int a = 0; a < NG; ++a)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) oc[a][n][e] = 0.f;
+                for (int w = 0; w < G / 32; ++w) {
+                    const float* x = &f[a][8 * w];
+                    const int c = 2 * (a * (G / 32) + w);
+                    qf[c][0] = pack16(x[0], x[4], false);
+                    qf[c][1] = pack16(x[1] * 0.0625f, x[5] * 0.0625f, false);
+                    qf[c + 1][0] = pack16(x[2], x[6], false);
+                    qf[c + 1][1] = pack16(x[3] * 0.0625f, x[7] * 0.0625f, false);
+                }
             }
+            const float r = back * p.scale_log2 * 16777216.f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int from = 8 * t + 4 * e, mine = 2 * t + e;
+                r24[e] = __shfl_sync(0xffffffffu, r, from);
+#pragma unroll
+                for (int a = 0; a < NG; ++a) qs[a][e] = __shfl_sync(0xffffffffu, total_q[a], from) * 5.9604644775390625e-8f;
+                const int pos = pos0 + (h.row0 + mine) / p.shared;
+                hi[e] = mine < rows ? seen_hi(p, pos, h.len) : h.len;
+                lo[e] = mine < rows ? seen_lo(p, pos) : 0;
+                m[e] = 0.f;
+                thr[e] = -3.0e38f;                        // nothing seen yet: any score sets the maximum
+                sum[e] = 0.f;
+#pragma unroll
+                for (int a = 0; a < NG; ++a) msum[a][e] = 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 4 * VW; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+#pragma unroll
+            for (int a = 0; a < NG; ++a)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) oc[a][e] = 0.f;
             vlim = 0.f;
             vmul = 1.f;
         }
@@ -403,43 +409,38 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                         vp[blk][e][a] = *reinterpret_cast<const __half2*>(pr + C::PAIRS);
                     }
                 }
-            // q . codes: two accumulators a group and block, so that few products wait for another
-            float acc[2][NG][NT][2][4];
+            // q . codes: four accumulators (two a block, by group or by step), so that few products wait for another
+            constexpr int NA = 2 / NG;
+            float acc[2][NG][NA][4];
 #pragma unroll
             for (int w = 0; w < KW; ++w) {
                 const int a = w / (G / 32);
-                const bool first = w % (G / 32) == 0;
 #pragma unroll
                 for (int q = 0; q < 2; ++q)
 #pragma unroll
                     for (int blk = 0; blk < 2; ++blk) {
                         const uint32_t x0 = q ? kw[blk][0][w] >> 8 : kw[blk][0][w], x1 = q ? kw[blk][1][w] >> 8 : kw[blk][1][w];
                         const uint32_t af[4] = {x0 & LO, x1 & LO, x0 & HI, x1 & HI};
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            if (first) hmma_zero(acc[blk][a][n][q], af, qf[2 * w + q][n]);
-                            else hmma(acc[blk][a][n][q], af, qf[2 * w + q][n]);
-                        }
+                        if (2 * (w % (G / 32)) + q < NA) hmma_zero(acc[blk][a][q % NA], af, qf[2 * w + q]);
+                        else hmma(acc[blk][a][q % NA], af, qf[2 * w + q]);
                     }
             }
-            float x[2][NT][4];                                   // [block][..][token g rows 2t, 2t+1; token g+8]
+            float x[2][4];                                   // [block][..][token g rows 2t, 2t+1; token g+8]
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
                         for (int r = 0; r < 2; ++r) {
                             float v = 0.f;
 #pragma unroll
                             for (int a = 0; a < NG; ++a) {
-                                const float c = acc[blk][a][n][0][2 * e + r] + acc[blk][a][n][1][2 * e + r];
+                                const float c = NA == 2 ? acc[blk][a][0][2 * e + r] + acc[blk][a][NA - 1][2 * e + r] : acc[blk][a][0][2 * e + r];
                                 const float sc = __low2float(kp[blk][e][a]), mn = __high2float(kp[blk][e][a]);
                                 v = a ? fmaf(sc, c, v) : sc * c;
-                                v = fmaf(mn, qs[a][n][r], v);
+                                v = fmaf(mn, qs[a][r], v);
                             }
-                            x[blk][n][2 * e + r] = v;
+                            x[blk][2 * e + r] = v;
                         }
             // masks: tokens that a row does not see weigh nothing, and what lies past the sequence's
             // end (never written: any bits) must not reach a product
@@ -454,28 +455,24 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
 #pragma unroll
                             for (int a = 0; a < NG; ++a) vp[blk][e][a] = __half2half2(__ushort_as_half(0));
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
                             for (int r = 0; r < 2; ++r)
-                                if (tk >= hi[n][r] || tk < lo[n][r]) gone |= 1u << (8 * n + 4 * blk + 2 * e + r);
+                                if (tk >= hi[r] || tk < lo[r]) gone |= 1u << (4 * blk + 2 * e + r);
                     }
             }
-            float y[2][NT][4], top[NT][2];
+            float y[2][4], top[2];
             auto relative = [&]() {
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
 #pragma unroll
                         for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                float v = fmaf(x[blk][n][2 * e + r], r24[n][r], -m[n][r]);
+                                float v = fmaf(x[blk][2 * e + r], r24[r], -m[r]);
                                 if constexpr (MASKED)
-                                    if ((gone >> (8 * n + 4 * blk + 2 * e + r)) & 1u) v = -INFINITY;
-                                y[blk][n][2 * e + r] = v;
+                                    if ((gone >> (4 * blk + 2 * e + r)) & 1u) v = -INFINITY;
+                                y[blk][2 * e + r] = v;
                             }
-                        top[n][r] = fmaxf(fmaxf(y[0][n][r], y[0][n][2 + r]), fmaxf(y[1][n][r], y[1][n][2 + r]));
+                        top[r] = fmaxf(fmaxf(y[0][r], y[0][2 + r]), fmaxf(y[1][r], y[1][2 + r]));
                     }
             };
             relative();
@@ -488,8 +485,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                     for (int a = 0; a < NG; ++a) vtop = __hmax2(vtop, vp[blk][e][a]);
             float vmax = __low2float(vtop);
             bool move = vmax > vlim;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) move |= top[n][0] > thr[n][0] || top[n][1] > thr[n][1];
+            move |= top[0] > thr[0] || top[1] > thr[1];
             // The maximum moves only when a score passes it by 2^8 (weights stay below 2^8): a few
             // times a segment, so the reductions over the warp and the rescaling are rare.
             if (__any_sync(0xffffffffu, move)) {
@@ -503,40 +499,37 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                     vlim = lim;
                     vmul = 64.f / lim;
                 }
+                float keep[2];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float keep[2];
+                for (int r = 0; r < 2; ++r) {
+                    float d = top[r];
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        float d = top[n][r];
-#pragma unroll
-                        for (int k = 4; k < 32; k *= 2) d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, k));
-                        const bool fresh = thr[n][r] < 0.f;
-                        keep[r] = 1.f;
-                        if (d > (fresh ? -3.0e38f : 0.f)) {
-                            m[n][r] += d;
-                            keep[r] = fresh ? 0.f : exp2_fast(-d);
-                            thr[n][r] = 8.f;
-                        }
-                        sum[n][r] *= keep[r];
-#pragma unroll
-                        for (int a = 0; a < NG; ++a) msum[a][n][r] *= keep[r];
+                    for (int k = 4; k < 32; k *= 2) d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, k));
+                    const bool fresh = thr[r] < 0.f;
+                    keep[r] = 1.f;
+                    if (d > (fresh ? -3.0e38f : 0.f)) {
+                        m[r] += d;
+                        keep[r] = fresh ? 0.f : exp2_fast(-d);
+                        thr[r] = 8.f;
                     }
+                    sum[r] *= keep[r];
 #pragma unroll
-                    for (int a = 0; a < NG; ++a) {
-                        oc[a][n][0] *= keep[0] * vkeep; oc[a][n][1] *= keep[1] * vkeep;
-                        oc[a][n][2] = oc[a][n][0]; oc[a][n][3] = oc[a][n][1];
-                    }
+                    for (int a = 0; a < NG; ++a) msum[a][r] *= keep[r];
+                }
 #pragma unroll
-                    for (int j = 0; j < 4 * VW; ++j) {
-                        o[j][n][0] *= keep[0] * vkeep; o[j][n][1] *= keep[1] * vkeep;
-                        o[j][n][2] *= keep[0] * vkeep; o[j][n][3] *= keep[1] * vkeep;
-                    }
+                for (int a = 0; a < NG; ++a) {
+                    oc[a][0] *= keep[0] * vkeep; oc[a][1] *= keep[1] * vkeep;
+                    oc[a][2] = oc[a][0]; oc[a][3] = oc[a][1];
+                }
+#pragma unroll
+                for (int j = 0; j < 4 * VW; ++j) {
+                    o[j][0] *= keep[0] * vkeep; o[j][1] *= keep[1] * vkeep;
+                    o[j][2] *= keep[0] * vkeep; o[j][3] *= keep[1] * vkeep;
                 }
                 relative();
             }
             // weights, and their fp16 form in the layout of the product's right operand
-            uint32_t pf[2][NG][NT][2];
+            uint32_t pf[2][NG][2];
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
@@ -548,17 +541,14 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                         vs[a] = sv * vmul;
                         vm[a] = fmaf(8.f, sv, __high2float(vp[blk][e][a]));
                     }
+                    const float p0 = exp2_fast(y[blk][2 * e]), p1 = exp2_fast(y[blk][2 * e + 1]);
+                    sum[0] += p0;
+                    sum[1] += p1;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const float p0 = exp2_fast(y[blk][n][2 * e]), p1 = exp2_fast(y[blk][n][2 * e + 1]);
-                        sum[n][0] += p0;
-                        sum[n][1] += p1;
-#pragma unroll
-                        for (int a = 0; a < NG; ++a) {
-                            msum[a][n][0] = fmaf(p0, vm[a], msum[a][n][0]);
-                            msum[a][n][1] = fmaf(p1, vm[a], msum[a][n][1]);
-                            pf[blk][a][n][e] = movmatrix_trans(pack16(p0 * vs[a], p1 * vs[a], false));
-                        }
+                    for (int a = 0; a < NG; ++a) {
+                        msum[a][0] = fmaf(p0, vm[a], msum[a][0]);
+                        msum[a][1] = fmaf(p1, vm[a], msum[a][1]);
+                        pf[blk][a][e] = movmatrix_trans(pack16(p0 * vs[a], p1 * vs[a], false));
                     }
                 }
 #pragma unroll
@@ -578,8 +568,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                 const uint32_t eight[4] = {0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u};   // 8 2^-24 each
 #pragma unroll
                 for (int a = 0; a < NG; ++a)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) hmma(oc[a][n], eight, pf[blk][a][n]);
+                    hmma(oc[a], eight, pf[blk][a]);
 #pragma unroll
                 for (int w = 0; w < VW; ++w) {
                     const int a = w / (G / 64);
@@ -590,8 +579,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
                             const uint32_t af[4] = {x01 & LO, x01 & HI, x23 & LO, x23 & HI};
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) hmma(o[4 * w + 2 * half + q][n], af, pf[blk][a][n]);
+                            hmma(o[4 * w + 2 * half + q], af, pf[blk][a]);
                             x01 >>= 8;
                             x23 >>= 8;
                         }
@@ -609,14 +597,12 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
 
         if (h.flags & 2) {
             // ---- the end of this CTA's part: the four warps' states become one
-            const int rows = h.nq * p.shared;
+            const int rows = min(h.nq * p.shared - h.row0, ROWS);
             float* mine = merge + warp * ROWS * C::LD;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const int row = 2 * t + r + 8 * n;
-                    float s = sum[n][r], a0 = msum[0][n][r], a1 = NG == 2 ? msum[NG - 1][n][r] : 0.f;
+                    const int row = 2 * t + r;
+                    float s = sum[r], a0 = msum[0][r], a1 = NG == 2 ? msum[NG - 1][r] : 0.f;
 #pragma unroll
                     for (int d = 4; d < 32; d *= 2) {
                         s += __shfl_xor_sync(0xffffffffu, s, d);
@@ -630,12 +616,12 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                             const int w = j / 4, a = w / (G / 64);
                             const int d = a * G + g * (G / 8) + (w % (G / 64)) * 8 + 2 * (j % 4);
                             float2 v;
-                            v.x = fmaf(o[j][n][r] - oc[a][n][r], up24, a ? a1 : a0);
-                            v.y = fmaf(fmaf(-16.f, oc[a][n][r], o[j][n][2 + r]), up20, a ? a1 : a0);
+                            v.x = fmaf(o[j][r] - oc[a][r], up24, a ? a1 : a0);
+                            v.y = fmaf(fmaf(-16.f, oc[a][r], o[j][2 + r]), up20, a ? a1 : a0);
                             *reinterpret_cast<float2*>(mine + row * C::LD + d) = v;
                         }
                         if (g == 0) {
-                            mine[row * C::LD + D] = thr[n][r] < 0.f ? -INFINITY : m[n][r];
+                            mine[row * C::LD + D] = thr[r] < 0.f ? -INFINITY : m[r];
                             mine[row * C::LD + D + 1] = s;
                         }
                     }
@@ -661,7 +647,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                     ss = fmaf(k, sw[D + 1], ss);
                 }
                 if (h.flags & 4) {
-                    float* slot = reinterpret_cast<float*>(p.workspace + cd_info_bytes((int64_t)p.batch * hk)) +
+                    float* slot = reinterpret_cast<float*>(p.workspace + cd_info_bytes((int64_t)p.batch * hk * p.row_blocks)) +
                                   (size_t)h.slot * cd_slot_floats(ROWS, D);
                     *reinterpret_cast<float4*>(slot + row * D + d) = v;
                     if (d == 0) {
@@ -670,7 +656,8 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                     }
                 } else {
                     const float inv = ss == 0.f ? 0.f : 1.f / ss;
-                    const int64_t at = (int64_t)(h.q0 + row / p.shared) * (hk * p.shared) + h.head * p.shared + row % p.shared;
+                    const int64_t at = (int64_t)(h.q0 + (h.row0 + row) / p.shared) * (hk * p.shared) + h.head * p.shared +
+                                       (h.row0 + row) % p.shared;
                     uint2 w2;
                     w2.x = pack16(v.x * inv, v.y * inv, p.bf16);
                     w2.y = pack16(v.z * inv, v.w * inv, p.bf16);
@@ -688,7 +675,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
 }
 
 // Joins the parts of the segments that several CTAs held, and writes the zeros of sequences
-// with nothing cached.  Grid (sequence x key head, row); D / 4 threads hold one row's values and
+// with nothing cached.  Grid (sequence x key head x block, row); D / 4 threads hold one row's values and
 // the block's other threads take every so many parts.
 template <int D>
 __global__ void cache_decode_combine_kernel(const __grid_constant__ AttentionParams p, int slot_rows) {
@@ -697,10 +684,12 @@ __global__ void cache_decode_combine_kernel(const __grid_constant__ AttentionPar
     __shared__ float red[2][32];
     pdl_wait();
     pdl_launch_dependents();
-    const int hk = p.c.kv_heads, b = blockIdx.x / hk, head = blockIdx.x % hk, row = blockIdx.y;
+    const int hk = p.c.kv_heads, row = blockIdx.y;
+    const int block = blockIdx.x % p.row_blocks, bh = blockIdx.x / p.row_blocks, b = bh / hk, head = bh % hk;
     const SeqSpan s = seq_span(p, b);
-    if (row >= s.nq * p.shared) return;
-    const int64_t at = (int64_t)(s.q0 + row / p.shared) * (hk * p.shared) + head * p.shared + row % p.shared;
+    const int whole = block * slot_rows + row;                // the row among all of the sequence and head
+    if (whole >= s.nq * p.shared) return;
+    const int64_t at = (int64_t)(s.q0 + whole / p.shared) * (hk * p.shared) + head * p.shared + whole % p.shared;
     const int lane_d = threadIdx.x % V4, slice = threadIdx.x / V4, slices = blockDim.x / V4;
     if (cd_tiles(p, s) == 0) {
         if (slice == 0) {
@@ -712,7 +701,7 @@ __global__ void cache_decode_combine_kernel(const __grid_constant__ AttentionPar
     const int2 info = *(reinterpret_cast<const int2*>(p.workspace) + blockIdx.x);
     const int n = info.y - info.x + 1;
     if (n == 1) return;                                    // one CTA had it all and has written it
-    const float* slots = reinterpret_cast<const float*>(p.workspace + cd_info_bytes((int64_t)p.batch * hk));
+    const float* slots = reinterpret_cast<const float*>(p.workspace + cd_info_bytes((int64_t)p.batch * hk * p.row_blocks));
     const size_t size = cd_slot_floats(slot_rows, D);
     auto part_of = [&](int c) { return slots + (size_t)(2 * (info.x + c) + (c == 0 ? 1 : 0)) * size; };
     // the row's maximum over the parts
