@@ -429,3 +429,66 @@ def test_a_query_that_is_not_finite_spoils_its_own_row_only():
         assert torch.isnan(got[0, 1]).all()
         got[0, 1] = want[0, 1]
         assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------------------ refusals of the binding
+
+def test_attention_refuses_what_it_cannot_take():
+    import w4a16_opt as w
+    p = Problem([50, 60], [1, 1], 4, 2, 128, 128, 64)
+    ok = dict(q=p.q, cache=p.cache, page_table=p.table, seq_lens=p.seq_lens)
+
+    def refused(match, **kw):
+        with pytest.raises(RuntimeError, match=match):
+            w.cache_attention(**{**ok, **kw})
+
+    refused("fp16 or bf16", q=p.q.float())
+    refused("last dimension", q=torch.randn(2, 128, 4, device="cuda").half().transpose(1, 2))
+    refused("multiples of 8", q=torch.zeros(2, 4, 132, device="cuda").half()[:, :, :128].as_strided((2, 4, 128), (516, 129, 1)))
+    refused("16-byte aligned", q=torch.zeros(2 * 4 * 128 + 8, device="cuda").half()[4:4 + 1024].view(2, 4, 128))
+    refused("multiple of kv_heads", q=torch.zeros(2, 3, 128, device="cuda").half())
+    refused("must be", q=torch.zeros(2, 4, 64, device="cuda").half())
+    refused("one token for each sequence", q=torch.zeros(3, 4, 128, device="cuda").half())
+    refused("page_table must be int32", page_table=p.table.long())
+    refused("seq_lens must be int32", seq_lens=p.seq_lens[:1])
+    refused("cu_q must be int32", cu_q=p.cu.long(), max_q=1)
+    refused("CUDA|device", seq_lens=p.seq_lens.cpu())
+    refused("window", window=-3)
+    refused("out must be", out=torch.empty(2, 4, 128, device="cuda"))
+    refused("workspace too small", workspace=torch.empty(256, dtype=torch.uint8, device="cuda"))
+    big = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
+    refused("256-byte aligned", workspace=big[16:])
+    assert torch.equal(w.cache_attention(**ok, workspace=big), p.run())
+
+
+def test_append_and_read_refuse_what_they_cannot_take():
+    import w4a16_opt as w
+    cache = w.Int4KVCache(4, 2, 128, 64)
+    k = torch.zeros(3, 2, 128, device="cuda").half()
+    slots = torch.arange(3, device="cuda")
+    cs = torch.zeros(8, 128, device="cuda")
+    pos = torch.zeros(3, dtype=torch.long, device="cuda")
+
+    def refused(match, **kw):
+        a = dict(cache=cache, k=k, v=k, slots=slots)
+        a.update(kw)
+        with pytest.raises(RuntimeError, match=match):
+            w.cache_append(**a)
+
+    refused("fp16 or bf16", k=k.float(), v=k.float())
+    refused("one dtype", v=k.bfloat16())
+    refused("k must be", k=k[:2])
+    refused("v must be", v=k[:, :1])
+    refused("slots must be", slots=slots.int())
+    refused("go together", positions=pos)
+    refused("need positions", q=k)
+    refused("positions must be", positions=pos.int(), cos_sin=cs)
+    refused("cos_sin must be", positions=pos, cos_sin=cs.half())
+    refused("rotary_dim must be", positions=pos, cos_sin=cs[:, :96].contiguous())
+    refused("need sections", positions=pos.expand(3, 3).contiguous(), cos_sin=cs)
+    refused("one entry for each axis", positions=pos.expand(3, 3).contiguous(), cos_sin=cs, sections=(32, 32))
+    refused("add up", positions=pos.expand(3, 3).contiguous(), cos_sin=cs, sections=(32, 32, 32))
+    refused("q must be", positions=pos, cos_sin=cs, q=k.float())
+    with pytest.raises(RuntimeError, match="slots must be"):
+        w.cache_read(cache, slots.cpu())
+    assert not cache.data.any()

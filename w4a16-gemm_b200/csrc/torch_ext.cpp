@@ -321,8 +321,8 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> cache_attention_py(
     } else {
         TORCH_CHECK(q.size(0) == batch, "without cu_q, q must hold one token for each sequence");
     }
-    TORCH_CHECK(q.size(1) <= INT_MAX && batch <= INT_MAX && page_table.size(1) <= INT_MAX && max_q >= 0 && max_q <= INT_MAX &&
-                    window >= 0 && window <= INT_MAX, "sizes must fit in int32 and must not be negative");
+    TORCH_CHECK(q.size(1) <= INT_MAX && batch <= INT_MAX && page_table.size(1) <= INT_MAX && max_q <= INT_MAX,
+                "dimensions must fit in int32");
     const at::cuda::CUDAGuard guard(data.device());
     w4a16_cache_attention_args a = {};
     a.dtype = act_dtype(q.scalar_type(), "q");
@@ -351,9 +351,9 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> cache_attention_py(
     a.q_heads = (int32_t)q.size(1);
     a.batch = (int32_t)batch;
     a.table_pages = (int32_t)page_table.size(1);
-    a.max_q = (int32_t)max_q;
+    a.max_q = (int32_t)std::max<int64_t>(max_q, -1);
     a.causal = causal;
-    a.window = (int32_t)window;
+    a.window = (int32_t)std::min<int64_t>(std::max<int64_t>(window, -1), INT_MAX);   // negative: refused below the ABI
     cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
     uint64_t ws_bytes = 0;
     torch::Tensor ws;
