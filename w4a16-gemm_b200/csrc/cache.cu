@@ -211,12 +211,16 @@ static cudaError_t launch_decode_t(const AttentionParams& ap, const AttentionPla
     if (err != cudaSuccess) return err;
     err = launch(kern, dim3(plan.grid), kCdThreads, C::SMEM, stream, pdl, ap);
     if (err != cudaSuccess) return err;
-    // threads of a combine block: enough slices of the parts that a segment may have
+    // slices of a row's parts: by how many CTAs a segment may be spread over
     const int64_t segments = (int64_t)ap.batch * ap.c.kv_heads * ap.row_blocks;
-    const int threads = plan.grid / segments >= 64 ? 512 : 128;
-    const int rows = std::min(C::ROWS, ap.max_q * ap.shared);
-    return launch(cache_decode_combine_kernel<D>, dim3((unsigned)segments, (unsigned)rows), threads, 0, stream, pdl, ap,
-                  (int)C::ROWS);
+    const int64_t spread = plan.grid / segments;
+    const int seg_rows = std::min(C::ROWS, ap.max_q * ap.shared);
+    const int64_t rows = segments * seg_rows, per = 128 / (D / 4);
+    if (spread < 8)
+        return launch(cache_decode_combine_kernel<D, 1>, dim3((unsigned)((rows + per - 1) / per)), 128, 0, stream, pdl, ap, seg_rows, rows);
+    if (spread < 64)
+        return launch(cache_decode_combine_kernel<D, 4>, dim3((unsigned)rows), D, 0, stream, pdl, ap, seg_rows, rows);
+    return launch(cache_decode_combine_kernel<D, 16>, dim3((unsigned)rows), 4 * D, 0, stream, pdl, ap, seg_rows, rows);
 }
 
 template <int D, int G>

@@ -104,6 +104,13 @@ __host__ __device__ __forceinline__ size_t cd_slot_floats(int rows, int D) {
     return (size_t)rows * (D + 2);
 }
 
+// floor(a * b / c) and floor(a / c) of non-negative numbers; 32-bit divisions where they do (a 64-bit one
+// takes some 400 cycles, and a short call has several of them in a row).
+__device__ __forceinline__ long long mul_div(long long a, long long b, long long c) {
+    const unsigned long long ab = (unsigned long long)a * (unsigned long long)b;
+    return (ab | (unsigned long long)c) >> 32 ? (long long)(ab / (unsigned long long)c) : (long long)((uint32_t)ab / (uint32_t)c);
+}
+
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
     uint32_t d;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -173,7 +180,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
             if (w < warp) before += warp_sum[w];
             total += warp_sum[w];
         }
-        const long long u0 = total * blockIdx.x / max(min((long long)gridDim.x, total), 1LL);
+        const long long u0 = mul_div(total, blockIdx.x, max(min((long long)gridDim.x, total), 1LL));
         long long base = before + incl - mine;
         if (threadIdx.x == 0) found[0] = total;
         if (u0 >= base && u0 < base + mine) {
@@ -191,7 +198,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
     const long long total = found[0];
     const long long ctas = min((long long)gridDim.x, total);      // those with work: a unit at least
     if (blockIdx.x >= ctas) return;
-    const long long u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
+    const long long u0 = mul_div(total, blockIdx.x, ctas), u1 = mul_div(total, blockIdx.x + 1, ctas);
 
     if (warp == kCdWarps) {
         // ------------------------------------------------------------ producer
@@ -209,10 +216,16 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
         int nt = cd_tiles(p, s), first = cd_first_tile(p, s);
         int blocks = cd_blocks<ROWS>(p, s);
         const long long local = u0 - found[1];
-        int seg = (int)(local / (nt + kCdSegmentCost)), tile = (int)(local % (nt + kCdSegmentCost)) - kCdSegmentCost;   // of the sequence
+        int seg = (int)mul_div(local, 1, nt + kCdSegmentCost);   // of the sequence
+        int tile = (int)(local - (long long)seg * (nt + kCdSegmentCost)) - kCdSegmentCost;
         long long u = u0;
         if (tile < 0) { u -= tile; tile = 0; }
         bool begins = true;
+        // the CTA that holds the unit before `end`: floor((end * ctas - 1) / total)
+        auto cta_of = [&](long long end) {
+            const unsigned long long x = (unsigned long long)end * (unsigned long long)ctas - 1ull;
+            return (x | (unsigned long long)total) >> 32 ? (long long)(x / (unsigned long long)total) : (long long)((uint32_t)x / (uint32_t)total);
+        };
         long long seg0 = u - tile;                               // the segment's first unit
         int2* info = reinterpret_cast<int2*>(p.workspace);
         if (u >= u1 && lane == 0) {                              // a start and no unit: nothing to do
@@ -243,7 +256,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                 h.slot = 2 * (int)blockIdx.x + (seg0 >= u0 ? 1 : 0);
                 hdr[st] = h;
                 if (tile == 0)
-                    info[((int64_t)b * hk + h.head) * p.row_blocks + seg % blocks] = make_int2((int)blockIdx.x, (int)(((seg0 + nt) * ctas - 1) / total));
+                    info[((int64_t)b * hk + h.head) * p.row_blocks + seg % blocks] = make_int2((int)blockIdx.x, (int)cta_of(seg0 + nt));
                 mbar_arrive_expect_tx(full(st), (uint32_t)(runs * rows * F::TOKEN));
             }
             __syncwarp();
@@ -675,22 +688,27 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
 }
 
 // Joins the parts of the segments that several CTAs held, and writes the zeros of sequences
-// with nothing cached.  Grid (sequence x key head x block, row); D / 4 threads hold one row's values and
-// the block's other threads take every so many parts.
-template <int D>
-__global__ void cache_decode_combine_kernel(const __grid_constant__ AttentionParams p, int slot_rows) {
+// with nothing cached.  SLICES groups of D / 4 threads hold a row's values and take every SLICES-th
+// part; a block has several rows where few slices do (16 x 5 x 4096 with a block a row: 5.4 us of
+// the call's 39).  `seg_rows`: rows of a segment that any sequence has.
+template <int D, int SLICES>
+__global__ void __launch_bounds__(SLICES == 1 ? 128 : D / 4 * SLICES)
+cache_decode_combine_kernel(const __grid_constant__ AttentionParams p, int seg_rows, int64_t rows) {
     constexpr int V4 = D / 4;
-    __shared__ float4 part[512];
-    __shared__ float red[2][32];
     pdl_wait();
     pdl_launch_dependents();
-    const int hk = p.c.kv_heads, row = blockIdx.y;
-    const int block = blockIdx.x % p.row_blocks, bh = blockIdx.x / p.row_blocks, b = bh / hk, head = bh % hk;
+    const int lane_d = threadIdx.x % V4, slice = SLICES == 1 ? 0 : threadIdx.x / V4;
+    const int64_t r = SLICES == 1 ? (int64_t)blockIdx.x * (128 / V4) + threadIdx.x / V4 : (int64_t)blockIdx.x;
+    if (r >= rows) return;
+    const int64_t seg = r / seg_rows;
+    const int row = (int)(r % seg_rows);
+    const int hk = p.c.kv_heads, block = (int)(seg % p.row_blocks), bh = (int)(seg / p.row_blocks), b = bh / hk, head = bh % hk;
+    // read along with the lengths: what it says of a segment without units is not used
+    const int2 info = *(reinterpret_cast<const int2*>(p.workspace) + seg);
     const SeqSpan s = seq_span(p, b);
-    const int whole = block * slot_rows + row;                // the row among all of the sequence and head
+    const int whole = block * kCdRows + row;                  // the row among all of the sequence and head
     if (whole >= s.nq * p.shared) return;
     const int64_t at = (int64_t)(s.q0 + whole / p.shared) * (hk * p.shared) + head * p.shared + whole % p.shared;
-    const int lane_d = threadIdx.x % V4, slice = threadIdx.x / V4, slices = blockDim.x / V4;
     if (cd_tiles(p, s) == 0) {
         if (slice == 0) {
             *reinterpret_cast<uint2*>(p.out + at * D + lane_d * 4) = make_uint2(0u, 0u);
@@ -698,48 +716,47 @@ __global__ void cache_decode_combine_kernel(const __grid_constant__ AttentionPar
         }
         return;
     }
-    const int2 info = *(reinterpret_cast<const int2*>(p.workspace) + blockIdx.x);
     const int n = info.y - info.x + 1;
     if (n == 1) return;                                    // one CTA had it all and has written it
     const float* slots = reinterpret_cast<const float*>(p.workspace + cd_info_bytes((int64_t)p.batch * hk * p.row_blocks));
-    const size_t size = cd_slot_floats(slot_rows, D);
+    constexpr size_t size = (size_t)kCdRows * (D + 2);
     auto part_of = [&](int c) { return slots + (size_t)(2 * (info.x + c) + (c == 0 ? 1 : 0)) * size; };
     // the row's maximum over the parts
+    const uint32_t row_lanes = V4 == 32 ? 0xFFFFFFFFu : 0xFFFFu << (threadIdx.x & 16);
     float mm = -INFINITY;
-    for (int c = threadIdx.x; c < n; c += blockDim.x) mm = fmaxf(mm, part_of(c)[slot_rows * D + row]);
+    for (int c = lane_d; c < n; c += V4) mm = fmaxf(mm, part_of(c)[kCdRows * D + row]);
 #pragma unroll
-    for (int d = 16; d; d /= 2) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-    if (threadIdx.x % 32 == 0) red[0][threadIdx.x / 32] = mm;
-    __syncthreads();
-    for (int w = 0; w < (int)blockDim.x / 32; ++w) mm = fmaxf(mm, red[0][w]);
+    for (int d = V4 / 2; d; d /= 2) mm = fmaxf(mm, __shfl_xor_sync(row_lanes, mm, d));
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     float ss = 0.f;
 #pragma unroll 4
-    for (int c = slice; c < n; c += slices) {
+    for (int c = slice; c < n; c += SLICES) {
         const float* x = part_of(c);
-        const float mc = x[slot_rows * D + row], sc = x[slot_rows * D + slot_rows + row];
+        const float mc = x[kCdRows * D + row], sc = x[kCdRows * D + kCdRows + row];
         const float4 y = *reinterpret_cast<const float4*>(x + row * D + lane_d * 4);
         const float k = mc == -INFINITY ? 1.f : exp2_fast(mc - mm);      // see the merge above
         v.x = fmaf(k, y.x, v.x); v.y = fmaf(k, y.y, v.y); v.z = fmaf(k, y.z, v.z); v.w = fmaf(k, y.w, v.w);
         ss = fmaf(k, sc, ss);
     }
-    part[threadIdx.x] = v;
-    if (lane_d == 0) red[1][slice] = ss;
-    __syncthreads();
-    if (slice == 0) {
-        float total = 0.f;
-        for (int j = 0; j < slices; ++j) total += red[1][j];
-        for (int j = 1; j < slices; ++j) {
+    if constexpr (SLICES > 1) {
+        __shared__ float4 part[V4 * SLICES];
+        __shared__ float sums[SLICES];
+        part[threadIdx.x] = v;
+        if (lane_d == 0) sums[slice] = ss;
+        __syncthreads();
+        if (slice > 0) return;
+        for (int j = 1; j < SLICES; ++j) {
             const float4 y = part[j * V4 + lane_d];
             v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+            ss += sums[j];
         }
-        const float inv = total == 0.f ? 0.f : 1.f / total;
-        uint2 w2;
-        w2.x = pack16(v.x * inv, v.y * inv, p.bf16);
-        w2.y = pack16(v.z * inv, v.w * inv, p.bf16);
-        *reinterpret_cast<uint2*>(p.out + at * D + lane_d * 4) = w2;
-        if (p.lse && lane_d == 0) p.lse[at] = total == 0.f ? -INFINITY : (mm + log2f(total)) * kLn2;
     }
+    const float inv = ss == 0.f ? 0.f : 1.f / ss;
+    uint2 w2;
+    w2.x = pack16(v.x * inv, v.y * inv, p.bf16);
+    w2.y = pack16(v.z * inv, v.w * inv, p.bf16);
+    *reinterpret_cast<uint2*>(p.out + at * D + lane_d * 4) = w2;
+    if (p.lse && lane_d == 0) p.lse[at] = ss == 0.f ? -INFINITY : (mm + log2f(ss)) * kLn2;
 }
 
 }  // namespace w4a16
