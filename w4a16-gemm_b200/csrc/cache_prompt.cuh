@@ -18,12 +18,14 @@
 //
 // What bounds it: the chain of a half's step, some 4600 cycles for a 128-token tile of both halves
 // where the products alone take 2048 and the exponentials (16 a cycle and SM) as many: scores
-// read 180, maximum 370, weights 1800, then 1000 for PV and the next S, with 100 to 200 for each
-// hand-over; shared memory is half used.  512 queries of 64 heads over 32768 tokens: 660 us, 827
-// TFLOP/s, at 990 W of the GPU's 1000.  Measured and not kept: two threads a row (680 us), a warp of its own for
-// the products of each half (765), a PV and the next S issued in one go after all their waits
-// (758), a quarter of the exponentials as polynomials on the FMA pipe (792), a second read of the scores from
-// TMEM in place of 128 registers (1160).
+// read 180, maximum 370, weights 1800, then 1800 for PV, the next S and the hand-overs between
+// warps (100 to 200 each); shared memory is half used.  512 queries of 64 heads over 32768 tokens:
+// 670 us, 815 TFLOP/s, at 990 W of the GPU's 1000.  Measured there and not kept: two threads a row
+// (680 us), a warp of its own for the products of each half (765), a PV and the next S issued in one
+// go after all their waits (758), a quarter of the exponentials as polynomials on the FMA pipe (792),
+// a second read of the scores from TMEM in place of 128 registers (1160); and with no difference:
+// weights handed over in two parts, a third S buffer with 64-wide heads, queries and results moved
+// in coalesced rows.
 //
 // Rounding.  A cached value code * scale + minimum is rounded once to fp16 (2^-11), as a 16-bit
 // cache would hold it.  Queries become fp16 after a power of two (exact within 2^-24 of the
@@ -33,6 +35,8 @@
 #pragma once
 #include <cuda_fp16.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "cache_attention.cuh"
 
@@ -188,11 +192,11 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
     auto v_empty = [&](int s) { return bar0 + 8u * (3 * ST + s); };
     auto q_full = [&](int h) { return bar0 + 8u * (4 * ST + h); };
     auto s_full = [&](int h) { return bar0 + 8u * (4 * ST + 2 + h); };
-    auto p_full = [&](int h, int i) { return bar0 + 8u * (4 * ST + 4 + 2 * h + i); };      // of the first and second 64 tokens
-    auto o_done = [&](int h) { return bar0 + 8u * (4 * ST + 8 + h); };
-    auto r_full = [&](int i) { return bar0 + 8u * (4 * ST + 10 + i); };
-    auto r_empty = [&](int i) { return bar0 + 8u * (4 * ST + 10 + C::RAWS + i); };
-    const uint32_t done_bar = bar0 + 8u * (4 * ST + 10 + 2 * C::RAWS), tmem_slot = done_bar + 8;
+    auto p_full = [&](int h) { return bar0 + 8u * (4 * ST + 4 + h); };
+    auto o_done = [&](int h) { return bar0 + 8u * (4 * ST + 6 + h); };
+    auto r_full = [&](int i) { return bar0 + 8u * (4 * ST + 8 + i); };
+    auto r_empty = [&](int i) { return bar0 + 8u * (4 * ST + 8 + C::RAWS + i); };
+    const uint32_t done_bar = bar0 + 8u * (4 * ST + 8 + 2 * C::RAWS), tmem_slot = done_bar + 8;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < ST; ++s) {
@@ -204,8 +208,7 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
         for (int h = 0; h < 2; ++h) {
             mbar_init(q_full(h), 4);
             mbar_init(s_full(h), 1);
-            mbar_init(p_full(h, 0), 4);
-            mbar_init(p_full(h, 1), 4);
+            mbar_init(p_full(h), 4);
             mbar_init(o_done(h), 1);
         }
         for (int i = 0; i < C::RAWS; ++i) {
@@ -282,17 +285,12 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                 const int h = half_of(e), tile = e >> shift, st = tile % ST, step = two ? e >> 1 : e;
                 const uint32_t vb = v_lo + st * (C::V_BYTES >> 4), pt = tmem + C::S_COL + h * kCpTile;
                 wait(v_full(st), tile / ST);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    wait(p_full(h, i), step);
-                    if (!ok) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        mma_ts(tmem + C::O_COL + h * D, pt + (4 * i + k) * 8, vb + i * (D * 128 >> 4) + k * 2, C::IDESC_O,
-                               i | k ? 1 : step);
-                }
+                wait(p_full(h), step);
                 if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < kCpTile / 16; ++k)
+                    mma_ts(tmem + C::O_COL + h * D, pt + k * 8, vb + (k / 4) * (D * 128 >> 4) + (k % 4) * 2, C::IDESC_O, k ? 1 : step);
                 if (step + 1 == steps_of(h)) mma_commit(o_done(h));
                 if (shift == 0 || h == 1) mma_commit(v_empty(st));
                 // the half's next S goes over this P: products run in the order of their issue
@@ -532,16 +530,26 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
             ok = __all_sync(0xffffffffu, mbar_wait(s_full(h), step & 1, kDevTimeoutCache));
             if (!ok) break;
             tc_fence_after();
-            if (warp_live) {
+            const int k0 = tile * kCpTile;
+            auto weights = [&](auto masked) {
                 uint32_t x[kCpTile];
 #pragma unroll
                 for (int c = 0; c < kCpTile; c += 32) tmem_ld_x32(s_t + c, x + c);
                 tc_wait_ld();
-                const int k0 = tile * kCpTile;
-                if (k0 < in_lo || k0 + kCpTile > in_hi) {
+                if constexpr (decltype(masked)::value) {
+                    // One comparison a score and side that needs one (12 heads, window 700, with both sides
+                    // compared in every tile at an end: 61 us against 57).
+                    const int from = lo - k0, to = hi - k0;
+                    if (k0 + kCpTile > in_hi) {
 #pragma unroll
-                    for (int c = 0; c < kCpTile; ++c)
-                        if (k0 + c >= hi || k0 + c < lo) x[c] = 0xFF800000u;
+                        for (int c = 0; c < kCpTile; ++c)
+                            if (c >= to) x[c] = 0xFF800000u;
+                    }
+                    if (k0 < in_lo) {
+#pragma unroll
+                        for (int c = 0; c < kCpTile; ++c)
+                            if (c < from) x[c] = 0xFF800000u;
+                    }
                 }
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -585,19 +593,20 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                         pk[e] = pack16(p0, p1, false);
                     }
                     tmem_st_x16(s_t + 16 * c, pk);
-                    if (c & 1) {
-                        tc_wait_st();
-                        tc_fence_before();
-                        warp_arrive(p_full(h, c >> 1));
-                    }
                 }
+                tc_wait_st();
+                tc_fence_before();
+                warp_arrive(p_full(h));
                 float a0, a1, b0, b1;
                 split2(sum2[0], a0, a1);
                 split2(sum2[1], b0, b1);
                 l += (a0 + a1) + (b0 + b1);
+            };
+            if (warp_live) {
+                if (k0 < in_lo || k0 + kCpTile > in_hi) weights(std::true_type{});
+                else weights(std::false_type{});
             } else {
-                warp_arrive(p_full(h, 0));
-                warp_arrive(p_full(h, 1));
+                warp_arrive(p_full(h));
             }
         }
         if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done(h), 0, kDevTimeoutCache));
