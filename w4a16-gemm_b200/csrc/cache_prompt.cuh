@@ -20,8 +20,8 @@
 // where the products alone take 2048 and the exponentials (16 a cycle and SM) as many: scores
 // read 180, maximum 370, weights 1800, then 1800 for PV, the next S and the hand-overs between
 // warps (100 to 200 each); shared memory is half used.  512 queries of 64 heads over 32768 tokens:
-// 670 us, 815 TFLOP/s, at 990 W of the GPU's 1000.  Measured there and not kept: two threads a row
-// (680 us), a warp of its own for the products of each half (765), a PV and the next S issued in one
+// 625 us, 870 TFLOP/s, at 990 W of the GPU's 1000.  Measured there and not kept: two threads a row
+// (680 us where this kernel then took 660), a warp of its own for the products of each half (765), a PV and the next S issued in one
 // go after all their waits (758), a quarter of the exponentials as polynomials on the FMA pipe (792),
 // a second read of the scores from TMEM in place of 128 registers (1160); and with no difference:
 // weights handed over in two parts, a third S buffer with 64-wide heads, queries and results moved
@@ -255,7 +255,7 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
     auto steps_of = [&](int h) { return two ? (gr.kv2 ? (n + 1 - h) / 2 : n) : (h == 0 ? n : 0); };
 
     if (warp < 4) {
-        reg_dec<40>();
+        reg_dec<48>();
         if (warp == 0 && events > 0) {
             // -------------------------------------------------------- products
             bool ok = true;
@@ -341,7 +341,7 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
         }
     } else if (warp < 8) {
         // ------------------------------------------------------------ codes -> operands
-        reg_dec<104>();
+        reg_dec<96>();
         const int w = warp - 4;
         const int g = lane >> 2, t = lane & 3;
         constexpr int KB = D / 8;                     // bytes of a key that a thread takes: D / 4 values
