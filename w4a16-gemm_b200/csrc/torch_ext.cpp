@@ -5,6 +5,7 @@
 // order and with the same messages (src/vectorized/kernel.cu:219-223); every
 // other check and the launch happen behind the C ABI.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -215,6 +216,12 @@ int32_t act_dtype(torch::ScalarType t, const char* what) {
     return t == torch::kHalf ? W4A16_ACT_F16 : W4A16_ACT_BF16;
 }
 
+// A fresh tensor beside `like`, straight from the caching allocator: these calls are short enough for
+// the dispatcher's share of torch::empty to show.
+torch::Tensor fresh(at::IntArrayRef sizes, torch::ScalarType type, const torch::Tensor& like) {
+    return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
+
 // [tokens, heads, head_dim] activations with a dense last dimension, on the cache's device.
 void check_act(const torch::Tensor& x, const torch::Tensor& data, int64_t tokens, int64_t heads, int64_t dim,
                const char* what) {
@@ -274,7 +281,7 @@ c10::optional<torch::Tensor> cache_append_py(torch::Tensor data, int64_t head_di
             TORCH_CHECK(q->dim() == 3 && q->scalar_type() == k.scalar_type(), "q must be [tokens, q_heads, head_dim] of k's dtype");
             check_act(*q, data, tokens, q->size(1), head_dim, "q");
             TORCH_CHECK(q->size(1) >= 1 && q->size(1) <= INT_MAX, "q_heads must be at least 1");
-            q_out = torch::empty({tokens, q->size(1), head_dim}, q->options());
+            q_out = fresh({tokens, q->size(1), head_dim}, q->scalar_type(), data);
             r.q = q->data_ptr();
             r.q_out = q_out.data_ptr();
             r.q_token_stride = q->stride(0);
@@ -294,9 +301,9 @@ std::tuple<torch::Tensor, torch::Tensor> cache_read_py(torch::Tensor data, int64
     const w4a16_cache c = cache_of(data, head_dim, page_size, group_size);
     check_slots(slots, data);
     const at::cuda::CUDAGuard guard(data.device());
-    const auto opts = data.options().dtype(bf16 ? torch::kBFloat16 : torch::kHalf);
-    auto k = torch::empty({slots.size(0), c.kv_heads, head_dim}, opts);
-    auto v = torch::empty({slots.size(0), c.kv_heads, head_dim}, opts);
+    const auto type = bf16 ? torch::kBFloat16 : torch::kHalf;
+    auto k = fresh({slots.size(0), c.kv_heads, head_dim}, type, data);
+    auto v = fresh({slots.size(0), c.kv_heads, head_dim}, type, data);
     check(w4a16_cache_read(&c, slots.data_ptr<int64_t>(), slots.size(0), k.data_ptr(), v.data_ptr(),
                            bf16 ? W4A16_ACT_BF16 : W4A16_ACT_F16, at::cuda::getCurrentCUDAStream().stream()));
     return {k, v};
@@ -332,10 +339,10 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> cache_attention_py(
         TORCH_CHECK(y.is_cuda() && y.device() == q.device() && y.scalar_type() == q.scalar_type() && y.sizes() == q.sizes() &&
                         y.is_contiguous(), "out must be a contiguous tensor of q's shape, dtype and device");
     } else {
-        y = torch::empty(q.sizes(), q.options());
+        y = fresh(q.sizes(), q.scalar_type(), data);
     }
     if (return_lse) {
-        lse = torch::empty({q.size(0), q.size(1)}, q.options().dtype(torch::kFloat));
+        lse = fresh({q.size(0), q.size(1)}, torch::kFloat, data);
         a.lse = lse.data_ptr<float>();
     }
     a.q = q.data_ptr();
