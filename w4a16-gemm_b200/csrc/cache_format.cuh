@@ -100,6 +100,8 @@ struct AppendParams {
     int32_t log_par;         // log2 of the lane groups that share a token's vectors
 };
 
+// Neither kernel here lets the next one start early: its waiting CTAs take the place of CTAs that
+// have work (reads of 8192 tokens of 8 heads back to back: 8.8 us a call with a trigger, 7.7 without).
 constexpr int kAppendThreads = 256;
 
 // 8 values -> 8 codes (one word), with the group's (scale, minimum).
@@ -163,7 +165,6 @@ __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const __gr
     constexpr int L = D / 8;
     using F = CacheFmt<D, G>;
     pdl_wait();
-    pdl_launch_dependents();
     const int64_t group = ((int64_t)blockIdx.x * kAppendThreads + threadIdx.x) / L;
     const int l = threadIdx.x % L, par = 1 << p.log_par;
     const int64_t token_raw = group >> p.log_par;
@@ -335,7 +336,6 @@ cache_read_kernel(const __grid_constant__ CacheView c, const int64_t* __restrict
     constexpr int L = D / 8, PER = kReadThreads / L;             // vectors that a CTA reads at a time
     using F = CacheFmt<D, G>;
     pdl_wait();
-    pdl_launch_dependents();
     const int l = threadIdx.x % L;
     const int64_t first = (int64_t)blockIdx.x * (PER * kReadVecs) + threadIdx.x / L;
     uint32_t w[kReadVecs][2], pair[kReadVecs][2];
