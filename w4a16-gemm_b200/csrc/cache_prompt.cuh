@@ -20,8 +20,8 @@
 // where the products alone take 2048 and the exponentials (16 a cycle and SM) as many: scores
 // read 180, maximum 370, weights 1800, then 1800 for PV, the next S and the hand-overs between
 // warps (100 to 200 each); shared memory is half used.  512 queries of 64 heads over 32768 tokens:
-// 625 us, 870 TFLOP/s, at 990 W of the GPU's 1000.  Measured there and not kept: two threads a row
-// (680 us where this kernel then took 660), a warp of its own for the products of each half (765), a PV and the next S issued in one
+// 611 us, 892 TFLOP/s, at 990 W of the GPU's 1000.  Measured there and not kept: two threads a row
+// (680 us where this kernel then took 660; the figures that follow are of that time too), a warp of its own for the products of each half (765), a PV and the next S issued in one
 // go after all their waits (758), a quarter of the exponentials as polynomials on the FMA pipe (792),
 // a second read of the scores from TMEM in place of 128 registers (1160); and with no difference:
 // weights handed over in two parts, a third S buffer with 64-wide heads, queries and results moved
