@@ -5,7 +5,7 @@
 // A CTA takes up to 256 rows (query heads of a key head times queries, in that order) of one
 // sequence and key head as two tiles of 128, and walks the 128-token tiles of the cache that
 // any of its rows sees:
-//     S = Q K^T   (128 x 128, TMEM)  ->  P = 2^(r S - m), fp16, over S in TMEM
+//     S = Q K^T   (128 x 128, TMEM)  ->  P = 2^(r S - m), fp16, TMEM
 //     O += P V    (128 x D, TMEM)
 // While the tensor cores work on one half's products, the other half's softmax runs.  With 128
 // rows or fewer the halves take alternate tiles of the cache instead, for the same rows, and
@@ -20,7 +20,7 @@
 // where the products alone take 2048 and the exponentials (16 a cycle and SM) as many: scores
 // read 180, maximum 370, weights 1800, then 1800 for PV, the next S and the hand-overs between
 // warps (100 to 200 each); shared memory is half used.  512 queries of 64 heads over 32768 tokens:
-// 611 us, 892 TFLOP/s, at 990 W of the GPU's 1000.  Measured there and not kept: two threads a row
+// 650 us, 840 TFLOP/s.  Measured there and not kept: two threads a row
 // (680 us where this kernel then took 660; the figures that follow are of that time too), a warp of its own for the products of each half (765), a PV and the next S issued in one
 // go after all their waits (758), a quarter of the exponentials as polynomials on the FMA pipe (792),
 // a second read of the scores from TMEM in place of 128 registers (1160); and with no difference:
@@ -39,6 +39,7 @@
 #include <type_traits>
 
 #include "cache_attention.cuh"
+#include "cache_schedule.h"
 
 namespace w4a16 {
 
@@ -123,8 +124,6 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar) {
     if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
-constexpr int kCpRows = 128;        // rows of a half
-constexpr int kCpTile = 128;        // cached tokens of a tile
 constexpr int kCpThreads = 512;
 
 template <int D, int G>
@@ -133,7 +132,7 @@ struct CpCfg {
     static constexpr int Q_BYTES = kCpRows * D * 2;
     static constexpr int K_BYTES = kCpTile * D * 2;
     static constexpr int V_BYTES = D * kCpTile * 2;
-    static constexpr int ST = 2;                                   // stages of K and of V
+    static constexpr int ST = kCpStages;
     // Codes and pairs as they come from the cache: a slot for the keys or the values of a tile.  Values
     // lie in chunks of 8 tokens with 16 bytes between them: a warp reads 8 chunks at once, and stores
     // 16-byte columns of 8 tokens without conflicts either.  (Unpadded, with 8-way conflicts of the
@@ -145,10 +144,63 @@ struct CpCfg {
     static constexpr int USED = 1024 + 2 * Q_BYTES + ST * (K_BYTES + V_BYTES) + RAWS * RAW + 256;
     // more than half of the SM's shared memory: one CTA, which owns all of TMEM, on an SM
     static constexpr int SMEM = USED > 116 * 1024 ? USED : 116 * 1024;
-    static constexpr int S_COL = 0;                                // TMEM columns: S of both halves, O of both halves
-    static constexpr int O_COL = 2 * kCpTile;
     static constexpr uint32_t IDESC_S = (1u << 4) | ((uint32_t)(kCpTile >> 3) << 17) | ((uint32_t)(kCpRows >> 4) << 24);
     static constexpr uint32_t IDESC_O = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kCpRows >> 4) << 24);
+};
+
+// The CTA's barriers, 8 bytes each from `base` on, then the word for TMEM's address.
+template <int RAWS>
+struct CpBars {
+    uint32_t base;
+    static constexpr int ST = kCpStages;
+    __device__ __forceinline__ uint32_t k_full(int s) const { return base + 8u * s; }
+    __device__ __forceinline__ uint32_t k_empty(int s) const { return base + 8u * (ST + s); }
+    __device__ __forceinline__ uint32_t v_full(int s) const { return base + 8u * (2 * ST + s); }
+    __device__ __forceinline__ uint32_t v_empty(int s) const { return base + 8u * (3 * ST + s); }
+    __device__ __forceinline__ uint32_t q_full(int h) const { return base + 8u * (4 * ST + h); }
+    __device__ __forceinline__ uint32_t s_full(int h) const { return base + 8u * (4 * ST + 2 + h); }
+    __device__ __forceinline__ uint32_t p_full(int h) const { return base + 8u * (4 * ST + 4 + h); }
+    __device__ __forceinline__ uint32_t o_done(int h) const { return base + 8u * (4 * ST + 6 + h); }
+    __device__ __forceinline__ uint32_t r_full(int i) const { return base + 8u * (4 * ST + 8 + i); }
+    __device__ __forceinline__ uint32_t r_empty(int i) const { return base + 8u * (4 * ST + 8 + RAWS + i); }
+    __device__ __forceinline__ uint32_t done() const { return base + 8u * (4 * ST + 8 + 2 * RAWS); }
+    __device__ __forceinline__ uint32_t tmem_slot() const { return done() + 8; }
+};
+
+// What cp_products asks for, by a whole warp.
+template <int D, int G>
+struct CpIssue {
+    using C = CpCfg<D, G>;
+    const CpBars<C::RAWS> bar;
+    const uint32_t tmem, q_lo, k_lo, v_lo;       // operands as descriptors' low words
+    const bool kv2;
+    __device__ __forceinline__ bool wait(uint32_t b, int turn) const {
+        return __all_sync(0xffffffffu, mbar_wait(b, (uint32_t)turn & 1u, kDevTimeoutCache));
+    }
+    __device__ __forceinline__ bool wait_q(int h) const { return wait(bar.q_full(h), 0); }
+    __device__ __forceinline__ bool wait_k(int st, int turn) const { return wait(bar.k_full(st), turn); }
+    __device__ __forceinline__ bool wait_v(int st, int turn) const { return wait(bar.v_full(st), turn); }
+    __device__ __forceinline__ bool wait_p(int h, int step) const { return wait(bar.p_full(h), step); }
+    __device__ __forceinline__ bool wait_o(int h, int step) const { return wait(bar.o_done(h), step); }
+    __device__ __forceinline__ void scores(int h, int st) const {
+        tc_fence_after();
+        const uint32_t qa = q_lo + (kv2 ? 0 : h) * (C::Q_BYTES >> 4), kb = k_lo + st * (C::K_BYTES >> 4);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+            mma_ss(tmem + CpTmem<D>::S(h), qa + (k / 4) * (kCpRows * 128 >> 4) + (k % 4) * 2,
+                   kb + (k / 4) * (kCpTile * 128 >> 4) + (k % 4) * 2, C::IDESC_S, k != 0);
+    }
+    __device__ __forceinline__ void values(int h, int st, int step) const {
+        tc_fence_after();
+        const uint32_t vb = v_lo + st * (C::V_BYTES >> 4), pt = tmem + CpTmem<D>::P(h);
+#pragma unroll
+        for (int k = 0; k < kCpTile / 16; ++k)
+            mma_ts(tmem + CpTmem<D>::O(h), pt + k * 8, vb + (k / 4) * (D * 128 >> 4) + (k % 4) * 2, C::IDESC_O, k ? 1 : step);
+    }
+    __device__ __forceinline__ void commit_s(int h) const { mma_commit(bar.s_full(h)); }
+    __device__ __forceinline__ void commit_o(int h) const { mma_commit(bar.o_done(h)); }
+    __device__ __forceinline__ void commit_k(int st) const { mma_commit(bar.k_empty(st)); }
+    __device__ __forceinline__ void commit_v(int st) const { mma_commit(bar.v_empty(st)); }
 };
 
 // What a grid of prompt CTAs does, set on the host.
@@ -186,46 +238,36 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t qs = base, ks = qs + 2 * C::Q_BYTES, vs = ks + ST * C::K_BYTES, raws = vs + ST * C::V_BYTES,
                    bar0 = raws + C::RAWS * C::RAW;
-    auto k_full = [&](int s) { return bar0 + 8u * s; };
-    auto k_empty = [&](int s) { return bar0 + 8u * (ST + s); };
-    auto v_full = [&](int s) { return bar0 + 8u * (2 * ST + s); };
-    auto v_empty = [&](int s) { return bar0 + 8u * (3 * ST + s); };
-    auto q_full = [&](int h) { return bar0 + 8u * (4 * ST + h); };
-    auto s_full = [&](int h) { return bar0 + 8u * (4 * ST + 2 + h); };
-    auto p_full = [&](int h) { return bar0 + 8u * (4 * ST + 4 + h); };
-    auto o_done = [&](int h) { return bar0 + 8u * (4 * ST + 6 + h); };
-    auto r_full = [&](int i) { return bar0 + 8u * (4 * ST + 8 + i); };
-    auto r_empty = [&](int i) { return bar0 + 8u * (4 * ST + 8 + C::RAWS + i); };
-    const uint32_t done_bar = bar0 + 8u * (4 * ST + 8 + 2 * C::RAWS), tmem_slot = done_bar + 8;
+    const CpBars<C::RAWS> bar{bar0};
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < ST; ++s) {
-            mbar_init(k_full(s), 4);
-            mbar_init(k_empty(s), 1);
-            mbar_init(v_full(s), 4);
-            mbar_init(v_empty(s), 1);
+            mbar_init(bar.k_full(s), 4);
+            mbar_init(bar.k_empty(s), 1);
+            mbar_init(bar.v_full(s), 4);
+            mbar_init(bar.v_empty(s), 1);
         }
         for (int h = 0; h < 2; ++h) {
-            mbar_init(q_full(h), 4);
-            mbar_init(s_full(h), 1);
-            mbar_init(p_full(h), 4);
-            mbar_init(o_done(h), 1);
+            mbar_init(bar.q_full(h), 4);
+            mbar_init(bar.s_full(h), 1);
+            mbar_init(bar.p_full(h), 4);
+            mbar_init(bar.o_done(h), 1);
         }
         for (int i = 0; i < C::RAWS; ++i) {
-            mbar_init(r_full(i), 1);
-            mbar_init(r_empty(i), 4);
+            mbar_init(bar.r_full(i), 1);
+            mbar_init(bar.r_empty(i), 4);
         }
-        mbar_init(done_bar, 1);
+        mbar_init(bar.done(), 1);
         fence_mbar_init();
     }
     if (warp == 0) {
-        tmem_alloc(tmem_slot, 512);
+        tmem_alloc(bar.tmem_slot(), 512);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - raw));
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + (bar.tmem_slot() - raw));
     // No early trigger: the next kernel's waiting CTAs slow this one's down (prompt 4096, calls back to
     // back: 188 us with it, 183 without).
     pdl_wait();
@@ -248,57 +290,16 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
         t0 += a;
         n = e - a;
     }
-    // events: a half's products with one tile, the halves in turn
-    const bool two = gr.kv2 ? n > 1 : rows > kCpRows;               // the second half has work
-    const int shift = gr.kv2 ? 0 : two ? 1 : 0;                     // tile of event e: e >> shift
-    const int events = n << shift;
-    auto half_of = [&](int e) { return two ? e & 1 : 0; };
-    auto steps_of = [&](int h) { return two ? (gr.kv2 ? (n + 1 - h) / 2 : n) : (h == 0 ? n : 0); };
+    const CpWalk walk{n, gr.kv2 ? n > 1 : rows > kCpRows, gr.kv2 != 0};
 
     if (warp < 4) {
         reg_dec<48>();
-        if (warp == 0 && events > 0) {
+        if (warp == 0 && n > 0) {
             // -------------------------------------------------------- products
-            bool ok = true;
-            auto wait = [&](uint32_t bar, int phase) {
-                ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, (uint32_t)phase & 1u, kDevTimeoutCache));
-            };
-            const uint32_t q_lo = cp_desc_lo(qs), k_lo = cp_desc_lo(ks), v_lo = cp_desc_lo(vs);
-            auto issue_s = [&](int e) {
-                const int h = half_of(e), tile = e >> shift, st = tile % ST;
-                wait(k_full(st), tile / ST);
-                if (!ok) return;
-                tc_fence_after();
-                const uint32_t qa = q_lo + (gr.kv2 ? 0 : h) * (C::Q_BYTES >> 4), kb = k_lo + st * (C::K_BYTES >> 4);
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k)
-                    mma_ss(tmem + C::S_COL + h * kCpTile, qa + (k / 4) * (kCpRows * 128 >> 4) + (k % 4) * 2,
-                           kb + (k / 4) * (kCpTile * 128 >> 4) + (k % 4) * 2, C::IDESC_S, k != 0);
-                mma_commit(s_full(h));
-                if (shift == 0 || h == 1) mma_commit(k_empty(st));
-            };
-            wait(q_full(0), 0);
-            if (two && !gr.kv2) wait(q_full(1), 0);
-            issue_s(0);
-            if (two && events > 1) issue_s(1);
-            const int ahead = two ? 2 : 1;
-            for (int e = 0; e < events && ok; ++e) {
-                const int h = half_of(e), tile = e >> shift, st = tile % ST, step = two ? e >> 1 : e;
-                const uint32_t vb = v_lo + st * (C::V_BYTES >> 4), pt = tmem + C::S_COL + h * kCpTile;
-                wait(v_full(st), tile / ST);
-                wait(p_full(h), step);
-                if (!ok) break;
-                tc_fence_after();
-#pragma unroll
-                for (int k = 0; k < kCpTile / 16; ++k)
-                    mma_ts(tmem + C::O_COL + h * D, pt + k * 8, vb + (k / 4) * (D * 128 >> 4) + (k % 4) * 2, C::IDESC_O, k ? 1 : step);
-                if (step + 1 == steps_of(h)) mma_commit(o_done(h));
-                if (shift == 0 || h == 1) mma_commit(v_empty(st));
-                // the half's next S goes over this P: products run in the order of their issue
-                if (e + ahead < events) issue_s(e + ahead);
-            }
-            mma_commit(done_bar);           // every product retired before TMEM is released
-            mbar_wait(done_bar, 0, kDevTimeoutDrain);
+            CpIssue<D, G> issue{bar, tmem, cp_desc_lo(qs), cp_desc_lo(ks), cp_desc_lo(vs), gr.kv2 != 0};
+            cp_products<D>(walk, issue);
+            mma_commit(bar.done());         // every product retired before TMEM is released
+            mbar_wait(bar.done(), 0, kDevTimeoutDrain);
         } else if (warp == 1) {
             // -------------------------------------------------------- codes and pairs into shared memory
             // Lanes 0-7: the codes of the keys of a run (the part of a page that is in the tile); 8-15: its
@@ -325,20 +326,20 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                 page = tok >= 0 ? page_of(p, b, tok >> ps_log) : 0;
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv, ++i) {
-                    ok = __all_sync(0xffffffffu, mbar_wait_sleep(r_empty(slot), (uint32_t)turn, kDevTimeoutCache));
+                    ok = __all_sync(0xffffffffu, mbar_wait_sleep(bar.r_empty(slot), (uint32_t)turn, kDevTimeoutCache));
                     if (!ok) break;
                     const uint32_t codes = kv ? __popc(valid >> 16) * 8u * F::CODE : __popc(valid & 0xFFu) * (uint32_t)run_rows * F::CODE;
                     const uint32_t pairs = __popc(valid & 0xFF00u) * (uint32_t)run_rows * F::PAIR;
-                    if (lane == 0) mbar_arrive_expect_tx(r_full(slot), codes + pairs);
+                    if (lane == 0) mbar_arrive_expect_tx(bar.r_full(slot), codes + pairs);
                     __syncwarp();
                     if (mine && kind != (kv ? 0 : 2))
                         bulk_load(raws + slot * C::RAW + dst_off, src + (kv && kind == 1 ? (uint32_t)F::PAIR << ps_log : 0u), bytes,
-                                  r_full(slot));
+                                  bar.r_full(slot));
                     if (++slot == C::RAWS) { slot = 0; turn ^= 1; }
                 }
             }
             if (!ok)       // what was issued may still be landing
-                for (int j = max(0, i - C::RAWS); j < i; ++j) mbar_wait(r_full(j % C::RAWS), (uint32_t)(j / C::RAWS) & 1u, kDevTimeoutDrain);
+                for (int j = max(0, i - C::RAWS); j < i; ++j) mbar_wait(bar.r_full(j % C::RAWS), (uint32_t)(j / C::RAWS) & 1u, kDevTimeoutDrain);
         }
     } else if (warp < 8) {
         // ------------------------------------------------------------ codes -> operands
@@ -354,8 +355,8 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
         int slot = 0, turn = 0;
         for (int tile = 0; tile < n; ++tile) {
             const int st = tile % ST;
-            ok = __all_sync(0xffffffffu, mbar_wait(r_full(slot), (uint32_t)turn, kDevTimeoutCache) &&
-                                             mbar_wait(k_empty(st), ((tile / ST) & 1) ^ 1, kDevTimeoutCache));
+            ok = __all_sync(0xffffffffu, mbar_wait(bar.r_full(slot), (uint32_t)turn, kDevTimeoutCache) &&
+                                             mbar_wait(bar.k_empty(st), ((tile / ST) & 1) ^ 1, kDevTimeoutCache));
             if (!ok) break;
             const uint8_t* src = smem_raw + (raws - raw) + slot * C::RAW;
             uint32_t kw[4][KWD], kp[4];
@@ -388,11 +389,11 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                 }
             }
             fence_proxy_async_smem();
-            warp_arrive(k_full(st));
-            warp_arrive(r_empty(slot));
+            warp_arrive(bar.k_full(st));
+            warp_arrive(bar.r_empty(slot));
             if (++slot == C::RAWS) { slot = 0; turn ^= 1; }
-            ok = __all_sync(0xffffffffu, mbar_wait(r_full(slot), (uint32_t)turn, kDevTimeoutCache) &&
-                                             mbar_wait(v_empty(st), ((tile / ST) & 1) ^ 1, kDevTimeoutCache));
+            ok = __all_sync(0xffffffffu, mbar_wait(bar.r_full(slot), (uint32_t)turn, kDevTimeoutCache) &&
+                                             mbar_wait(bar.v_empty(st), ((tile / ST) & 1) ^ 1, kDevTimeoutCache));
             if (!ok) break;
             src = smem_raw + (raws - raw) + slot * C::RAW;
             uint32_t vw[8][VWD], vp[8];
@@ -457,8 +458,8 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                     }
             }
             fence_proxy_async_smem();
-            warp_arrive(v_full(st));
-            warp_arrive(r_empty(slot));
+            warp_arrive(bar.v_full(st));
+            warp_arrive(bar.r_empty(slot));
             if (++slot == C::RAWS) { slot = 0; turn ^= 1; }
         }
     } else {
@@ -471,9 +472,9 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
         const int token = live ? row / p.shared : 0, qh = live ? head * p.shared + row % p.shared : 0;
         const int64_t at = (int64_t)(s.q0 + token) * heads + qh;       // row of out
         const bool warp_live = row - lane < row0 + rows;               // some row of the warp is real
-        const int steps = steps_of(h);
+        const int steps = walk.steps(h);
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t s_t = tmem + lanes + C::S_COL + h * kCpTile, o_t = tmem + lanes + C::O_COL + h * D;
+        const uint32_t s_t = tmem + lanes + CpTmem<D>::S(h), p_t = tmem + lanes + CpTmem<D>::P(h), o_t = tmem + lanes + CpTmem<D>::O(h);
         float r = 1.f;
         if (steps > 0 && (h == 0 || !gr.kv2)) {
             // the row's queries, scaled by a power of two: the largest comes to [2^13, 2^14).  Values of a
@@ -508,7 +509,7 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                 *reinterpret_cast<uint4*>(dst + (j / 8) * (kCpRows * 128) + (((j % 8) ^ (r_in & 7)) * 16)) = o;
             }
             fence_proxy_async_smem();
-            warp_arrive(q_full(h));
+            warp_arrive(bar.q_full(h));
         }
         if (gr.kv2) {
             // both halves hold the same rows: the second takes the first's factors
@@ -527,8 +528,8 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
         const int in_lo = seen_lo(p, s.len - s.nq + max(row_e, 0) / p.shared);
         bool ok = true;
         for (int step = 0; step < steps; ++step) {
-            const int tile = t0 + (gr.kv2 && two ? 2 * step + h : step);
-            ok = __all_sync(0xffffffffu, mbar_wait(s_full(h), step & 1, kDevTimeoutCache));
+            const int tile = t0 + (gr.kv2 && walk.two ? 2 * step + h : step);
+            ok = __all_sync(0xffffffffu, mbar_wait(bar.s_full(h), step & 1, kDevTimeoutCache));
             if (!ok) break;
             tc_fence_after();
             const int k0 = tile * kCpTile;
@@ -567,7 +568,7 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                         fresh = false;
                     }
                     l *= keep;
-                    if (step > 0) {             // this S was issued after the last step's PV: O is at rest
+                    if (step > 0) {             // this S was committed after the last step's PV: O is at rest
 #pragma unroll 1
                         for (int c = 0; c < D; c += 32) {
                             uint32_t o[32];
@@ -593,11 +594,11 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                         sum2[e & 1] = add2(sum2[e & 1], pair2(p0, p1));
                         pk[e] = pack16(p0, p1, false);
                     }
-                    tmem_st_x16(s_t + 16 * c, pk);
+                    tmem_st_x16(p_t + 16 * c, pk);
                 }
                 tc_wait_st();
                 tc_fence_before();
-                warp_arrive(p_full(h));
+                warp_arrive(bar.p_full(h));
                 float a0, a1, b0, b1;
                 split2(sum2[0], a0, a1);
                 split2(sum2[1], b0, b1);
@@ -607,10 +608,10 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                 if (k0 < in_lo || k0 + kCpTile > in_hi) weights(std::true_type{});
                 else weights(std::false_type{});
             } else {
-                warp_arrive(p_full(h));
+                warp_arrive(bar.p_full(h));
             }
         }
-        if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done(h), 0, kDevTimeoutCache));
+        if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar.o_done(h), walk.last_o<D>(h) & 1, kDevTimeoutCache));
         // ---- results
         if (ok && warp_live && rows > 0) {
             tc_fence_after();
