@@ -41,8 +41,9 @@ constexpr float kLn2 = 0.6931471805599453f;
 // One sequence's queries and cached tokens, clamped to what the arrays hold.
 struct SeqSpan {
     int32_t q0;      // first query's token
-    int32_t nq;      // queries
+    int32_t nq;      // queries that are answered: at most max_q
     int32_t len;     // cached tokens
+    int32_t pos0;    // first query's position: by all of the sequence's queries, answered or not
 };
 
 __device__ __forceinline__ SeqSpan seq_span(const AttentionParams& p, int b) {
@@ -53,10 +54,13 @@ __device__ __forceinline__ SeqSpan seq_span(const AttentionParams& p, int b) {
         const int64_t a = min((int64_t)max(__ldg(p.cu_q + b), 0), p.q_tokens);
         const int64_t e = min((int64_t)max(__ldg(p.cu_q + b + 1), 0), p.q_tokens);
         s.q0 = (int32_t)a;
-        s.nq = (int32_t)min(max(e - a, (int64_t)0), (int64_t)p.max_q);
+        const int32_t all = (int32_t)max(e - a, (int64_t)0);
+        s.nq = min(all, p.max_q);
+        s.pos0 = s.len - all;
     } else {
         s.q0 = b;
         s.nq = b < p.q_tokens ? 1 : 0;
+        s.pos0 = s.len - 1;
     }
     return s;
 }

@@ -58,8 +58,9 @@ struct __align__(16) CdStage {
     int tok0;        // first token of the unit
     int row0, head;  // first row of the block, key head
     int flags;       // 1: first unit of this CTA's part of the segment, 2: last, 4: the part is not all of it,
-                     // 8: last unit of this CTA
-    int len, nq, q0;
+                     // 8: last unit of this CTA; from bit 8 on: rows of the block
+    int len, q0;
+    int pos0;        // position of the sequence's first query
     int slot;        // workspace slot of the part
 };
 
@@ -84,7 +85,7 @@ constexpr int kCdSegmentCost = 2;
 
 // Units of one sequence and key head.
 __device__ __forceinline__ int cd_first_tile(const AttentionParams& p, const SeqSpan& s) {
-    return seen_lo(p, s.len - s.nq) / kCdTile;
+    return seen_lo(p, s.pos0) / kCdTile;
 }
 __device__ __forceinline__ int cd_tiles(const AttentionParams& p, const SeqSpan& s) {
     if (s.nq == 0 || s.len == 0) return 0;
@@ -246,7 +247,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
         while (u < u1) {
             const int tok0 = (first + tile) * kCdTile;
             const int tok = tok0 + run * rows;
-            const bool valid = run * rows < kCdTile && tok < s.len && tok + rows > seen_lo(p, s.len - s.nq);
+            const bool valid = run * rows < kCdTile && tok < s.len && tok + rows > seen_lo(p, s.pos0);
             const int64_t page = valid ? page_of(p, b, tok >> ps_log) : 0;
             const uint8_t* src = cache_block(p.c, page, seg / blocks) + src_part + (uint32_t)(tok & ((1 << ps_log) - 1)) * unit_b;
             const bool got = mbar_wait_sleep(empty(st), (uint32_t)turn ^ 1u, kDevTimeoutCache);
@@ -257,9 +258,10 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                 const bool part_of = seg0 < u0 || seg0 + nt > u1;
                 CdStage h;
                 h.tok0 = tok0; h.row0 = seg % blocks * ROWS; h.head = seg / blocks;
+                const int block_rows = min(s.nq * p.shared - h.row0, ROWS);
                 const bool last = u + 1 + (tile + 1 == nt ? kCdSegmentCost : 0) >= u1;
-                h.flags = (begins ? 1 : 0) | (ends ? 2 : 0) | (part_of ? 4 : 0) | (last ? 8 : 0);
-                h.len = s.len; h.nq = s.nq; h.q0 = s.q0;
+                h.flags = (begins ? 1 : 0) | (ends ? 2 : 0) | (part_of ? 4 : 0) | (last ? 8 : 0) | block_rows << 8;
+                h.len = s.len; h.pos0 = s.pos0; h.q0 = s.q0;
                 h.slot = 2 * (int)blockIdx.x + (seg0 >= u0 ? 1 : 0);
                 hdr[st] = h;
                 if (tile == 0)
@@ -316,8 +318,8 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
         const CdStage h = hdr[st];
         if (h.flags & 1) {
             // ---- a new segment: queries, masks, empty state
-            const int rows = min(h.nq * p.shared - h.row0, ROWS);
-            const int pos0 = h.len - h.nq, pos_first = pos0 + h.row0 / p.shared;
+            const int rows = h.flags >> 8;
+            const int pos0 = h.pos0, pos_first = pos0 + h.row0 / p.shared;
             lo_all = seen_lo(p, pos_first);
             lo_max = seen_lo(p, pos0 + (h.row0 + rows - 1) / p.shared);
             hi_min = seen_hi(p, pos_first, h.len);
@@ -617,7 +619,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
 
         if (h.flags & 2) {
             // ---- the end of this CTA's part: the four warps' states become one
-            const int rows = min(h.nq * p.shared - h.row0, ROWS);
+            const int rows = h.flags >> 8;
             float* mine = merge + warp * ROWS * C::LD;
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {

@@ -282,7 +282,7 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
     const SeqSpan s = seq_span(p, b);
     const int block_rows = gr.kv2 ? kCpRows : 2 * kCpRows;
     const int row0 = block * block_rows, rows = min(s.nq * p.shared - row0, block_rows);   // rows <= 0: nothing here
-    const int pos_first = s.len - s.nq + row0 / p.shared, pos_last = s.len - s.nq + (row0 + max(rows, 1) - 1) / p.shared;
+    const int pos_first = s.pos0 + row0 / p.shared, pos_last = s.pos0 + (row0 + max(rows, 1) - 1) / p.shared;
     const int tok_lo = seen_lo(p, pos_first), tok_hi = seen_hi(p, pos_last, s.len);
     int t0 = tok_lo / kCpTile, n = rows > 0 ? max((tok_hi + kCpTile - 1) / kCpTile - t0, 0) : 0;
     {
@@ -519,13 +519,13 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
             r = fac[r_in];
         }
         r = fmaxf(r, 1e-37f);                                          // never zero: a masked score is -inf * r
-        const int pos = s.len - s.nq + token;
+        const int pos = s.pos0 + token;
         const int hi = live ? seen_hi(p, pos, s.len) : s.len, lo = live ? seen_lo(p, pos) : 0;
         float m = 0.f, l = 0.f;
         bool fresh = true;                                             // no score seen yet
         const int row_a = row - r_in, row_e = min(row_a + kCpRows, row0 + rows) - 1;
-        const int in_hi = seen_hi(p, s.len - s.nq + row_a / p.shared, s.len);      // every row of the half sees [in_lo, in_hi)
-        const int in_lo = seen_lo(p, s.len - s.nq + max(row_e, 0) / p.shared);
+        const int in_hi = seen_hi(p, s.pos0 + row_a / p.shared, s.len);      // every row of the half sees [in_lo, in_hi)
+        const int in_lo = seen_lo(p, s.pos0 + max(row_e, 0) / p.shared);
         bool ok = true;
         for (int step = 0; step < steps; ++step) {
             const int tile = t0 + (gr.kv2 && walk.two ? 2 * step + h : step);
