@@ -20,7 +20,7 @@
 // where the products alone take 2048 and the exponentials (16 a cycle and SM) as many: scores
 // read 180, maximum 370, weights 1800, then 1800 for PV, the next S and the hand-overs between
 // warps (100 to 200 each); shared memory is half used.  512 queries of 64 heads over 32768 tokens:
-// 650 us, 840 TFLOP/s.  Measured there and not kept: two threads a row
+// 640 us, 853 TFLOP/s.  Measured there and not kept: two threads a row
 // (680 us where this kernel then took 660; the figures that follow are of that time too), a warp of its own for the products of each half (765), a PV and the next S issued in one
 // go after all their waits (758), a quarter of the exponentials as polynomials on the FMA pipe (792),
 // a second read of the scores from TMEM in place of 128 registers (1160); and with no difference:
@@ -343,7 +343,7 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
         }
     } else if (warp < 8) {
         // ------------------------------------------------------------ codes -> operands
-        reg_dec<96>();
+        reg_dec<80>();
         const int w = warp - 4;
         const int g = lane >> 2, t = lane & 3;
         constexpr int KB = D / 8;                     // bytes of a key that a thread takes: D / 4 values
@@ -464,7 +464,7 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
         }
     } else {
         // ------------------------------------------------------------ softmax: a thread a row
-        reg_inc<184>();
+        reg_inc<192>();
         const int h = (warp - 8) >> 2;
         const int r_in = (warp & 3) * 32 + lane;                       // row of the half = TMEM lane
         const int row = row0 + (gr.kv2 ? 0 : h * kCpRows) + r_in;      // row of the (sequence, key head)
