@@ -337,7 +337,7 @@ typedef struct w4a16_cache_attention_args {
     int32_t q_heads;         /* a multiple of kv_heads */
     int32_t batch;
     int32_t table_pages;
-    int32_t max_q;           /* no sequence has more queries (1 if cu_q is NULL) */
+    int32_t max_q;           /* no sequence has more queries (1 if cu_q is NULL); see below */
     int32_t causal;          /* 0: a query sees every cached token of its sequence */
     int32_t window;          /* > 0: a query at position p sees tokens above p - window only */
 } w4a16_cache_attention_args;
@@ -361,7 +361,9 @@ w4a16_status w4a16_cache_read(const w4a16_cache* cache, const int64_t* slots, in
  * of a sequence of L cached tokens has position L - T + i; with `causal` it sees tokens up to
  * its position.  A query that sees no token gives zeros and lse -inf.  q_heads / kv_heads
  * query heads share a key head (head h reads key head h / (q_heads / kv_heads)).  Entries of
- * the page table past a sequence's end are not used; lengths are clamped to the table. */
+ * the page table past a sequence's end are not used; lengths are clamped to the table.  Rows of
+ * q that belong to no sequence (before cu_q[0], or from cu_q[batch] on), and the queries of a sequence past
+ * its first max_q, give zeros and lse -inf.  A call whose batch, q_tokens or max_q is 0 writes nothing. */
 w4a16_status w4a16_cache_attention(const w4a16_cache* cache, const w4a16_cache_attention_args* args, void* workspace,
                                    uint64_t workspace_bytes, void* stream);
 

@@ -60,9 +60,43 @@ __device__ __forceinline__ SeqSpan seq_span(const AttentionParams& p, int b) {
     } else {
         s.q0 = b;
         s.nq = b < p.q_tokens ? 1 : 0;
-        s.pos0 = s.len - 1;
+        s.pos0 = s.len - s.nq;
     }
     return s;
+}
+
+// Zeros, and -inf in lse, for the rows of tokens [from, to); every worker takes some of them.
+template <int D>
+__device__ __forceinline__ void clear_rows(const AttentionParams& p, int64_t from, int64_t to, int64_t worker, int64_t workers) {
+    const int heads = p.c.kv_heads * p.shared;
+    uint4* const end = reinterpret_cast<uint4*>(p.out + to * heads * D);
+#pragma unroll 1
+    for (uint4* o = reinterpret_cast<uint4*>(p.out + from * heads * D) + worker; o < end; o += workers) *o = make_uint4(0, 0, 0, 0);
+    if (p.lse) {
+        float* const lse_end = p.lse + to * heads;
+#pragma unroll 1
+        for (float* l = p.lse + from * heads + worker; l < lse_end; l += workers) *l = -INFINITY;
+    }
+}
+
+// Rows that belong to no sequence: before the first one's queries and after the last one's, as in a call
+// of fixed size that serves fewer queries.
+template <int D>
+__device__ __forceinline__ void clear_outside(const AttentionParams& p, int64_t worker, int64_t workers) {
+    int64_t first = 0, last = p.batch;
+    if (p.cu_q) {
+        first = min((int64_t)max(__ldg(p.cu_q), 0), p.q_tokens);
+        last = max(__ldg(p.cu_q + p.batch), 0);
+    }
+    if (first > 0) clear_rows<D>(p, 0, first, worker, workers);
+    if (last < p.q_tokens) clear_rows<D>(p, last, p.q_tokens, worker, workers);
+}
+
+// Queries of a sequence past the max_q that are answered.
+template <int D>
+__device__ __forceinline__ void clear_past_max(const AttentionParams& p, const SeqSpan& s, int worker, int workers) {
+    const int all = s.len - s.pos0;
+    if (all > s.nq) clear_rows<D>(p, (int64_t)s.q0 + s.nq, (int64_t)s.q0 + all, worker, workers);
 }
 
 // The tokens [lo, hi) that a query at position pos sees.

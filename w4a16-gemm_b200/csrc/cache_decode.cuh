@@ -697,7 +697,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
 }
 
 // Joins the parts of the segments that several CTAs held, and writes the zeros of sequences
-// with nothing cached.  SLICES groups of D / 4 threads hold a row's values and take every SLICES-th
+// with nothing cached and of rows that are not answered.  SLICES groups of D / 4 threads hold a row's values and take every SLICES-th
 // part; a block has several rows where few slices do (16 x 5 x 4096 with a block a row: 5.4 us of
 // the call's 39).  `seg_rows`: rows of a segment that any sequence has.
 template <int D, int SLICES>
@@ -706,6 +706,7 @@ cache_decode_combine_kernel(const __grid_constant__ AttentionParams p, int seg_r
     constexpr int V4 = D / 4;
     pdl_wait();
     pdl_launch_dependents();
+    clear_outside<D>(p, (int64_t)blockIdx.x * blockDim.x + threadIdx.x, (int64_t)gridDim.x * blockDim.x);
     const int lane_d = threadIdx.x % V4, slice = SLICES == 1 ? 0 : threadIdx.x / V4;
     const int64_t r = SLICES == 1 ? (int64_t)blockIdx.x * (128 / V4) + threadIdx.x / V4 : (int64_t)blockIdx.x;
     if (r >= rows) return;
@@ -716,6 +717,7 @@ cache_decode_combine_kernel(const __grid_constant__ AttentionParams p, int seg_r
     const int2 info = *(reinterpret_cast<const int2*>(p.workspace) + seg);
     const SeqSpan s = seq_span(p, b);
     const int whole = block * kCdRows + row;                  // the row among all of the sequence and head
+    if (whole == 0 && head == 0) clear_past_max<D>(p, s, slice * V4 + lane_d, SLICES * V4);
     if (whole >= s.nq * p.shared) return;
     const int64_t at = (int64_t)(s.q0 + whole / p.shared) * (hk * p.shared) + head * p.shared + whole % p.shared;
     if (cd_tiles(p, s) == 0) {

@@ -11,7 +11,7 @@
 // rows or fewer the halves take alternate tiles of the cache instead, for the same rows, and
 // are joined by the combine kernel like any other parts.
 //
-// Warps: 0 issues the products; 1 fetches codes and pairs (bulk copies); 4-7 turn them into fp16
+// Warps: 0 issues the products; 1 fetches codes and pairs (bulk copies); 2 clears rows that are not answered; 4-7 turn them into fp16
 // operands in shared memory (keys [token][value], values transposed [value][token], both K-major
 // with 128-byte swizzle); 8-11 and 12-15 hold one half each, a thread a row: they load the queries,
 // run the softmax and write the result.
@@ -340,6 +340,10 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
             }
             if (!ok)       // what was issued may still be landing
                 for (int j = max(0, i - C::RAWS); j < i; ++j) mbar_wait(bar.r_full(j % C::RAWS), (uint32_t)(j / C::RAWS) & 1u, kDevTimeoutDrain);
+        } else if (warp == 2) {
+            // -------------------------------------------------------- rows that are not answered
+            clear_outside<D>(p, (int64_t)blockIdx.x * 32 + lane, (int64_t)gridDim.x * 32);
+            if (block == 0 && head == 0 && split == 0) clear_past_max<D>(p, s, lane, 32);
         }
     } else if (warp < 8) {
         // ------------------------------------------------------------ codes -> operands

@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <limits>
 #include <map>
 #include <vector>
 #include <mutex>
@@ -372,6 +373,10 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> cache_attention_py(
     } else {
         check(w4a16_cache_attention_workspace(&c, &a, &ws_bytes));
         ws = workspace_for(data, ws_bytes, stream);
+    }
+    if (batch == 0 || a.max_q == 0) {       // checked and left alone below the ABI: no row is answered
+        y.zero_();
+        if (return_lse) lse.fill_(-std::numeric_limits<float>::infinity());
     }
     check(w4a16_cache_attention(&c, &a, ws.defined() ? ws.data_ptr() : nullptr, ws_bytes, stream));
     return {y, return_lse ? c10::optional<torch::Tensor>(lse) : c10::nullopt};

@@ -103,7 +103,9 @@ def cache_attention(q: torch.Tensor, cache: Int4KVCache, page_table: torch.Tenso
     int32 [batch, pages] lists each sequence's pages in order (entries past its end are not used),
     ``seq_lens`` int32 [batch] its cached tokens, those of the queries included.  ``cu_q`` int32
     [batch + 1] says where each sequence's queries start in ``q`` and ``max_q`` how many the
-    longest has (any number above it will do too); without ``cu_q`` there is one for each.
+    longest has (any number above it will do too); without ``cu_q`` there is one for each.  Rows
+    that belong to no sequence, as in a captured step of fixed size, and queries of a sequence past
+    its first ``max_q`` give zeros (and -inf, below).
 
     Query i of the T of a sequence of L tokens has position L - T + i.  It sees every token of
     the sequence, with ``causal`` those up to its position, with ``window`` > 0 those above its
