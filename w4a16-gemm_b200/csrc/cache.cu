@@ -180,7 +180,7 @@ static AttentionPlan plan_prompt(const w4a16_cache& c, const w4a16_cache_attenti
     const int64_t busy = c.kv_heads * std::min<int64_t>((int64_t)p.prompt.blocks * a.batch,
                                                         a.q_tokens * shared / block_rows + a.batch);
     const int64_t tiles = ((int64_t)a.table_pages * c.page_size + kCpTile - 1) / kCpTile;
-    const size_t part_bytes = (size_t)(p.prompt.kv2 ? 2 : 1) * (size_t)(a.q_tokens * a.q_heads) * (size_t)(c.head_dim + 2) * sizeof(float);
+    const size_t part_bytes = (size_t)(a.q_tokens * a.q_heads) * (size_t)(c.head_dim + 2) * sizeof(float);
     const double block_tiles = (double)block_rows / (double)shared / kCpTile;          // that a block's tokens make
     const double most = a.window > 0 ? std::min((double)tiles, (double)a.window / kCpTile + block_tiles + 1.0) : (double)tiles;
     const double least = a.causal ? std::min(most, std::max(1.0, (double)tiles - (p.prompt.blocks - 1) * block_tiles)) : most;
@@ -193,18 +193,16 @@ static AttentionPlan plan_prompt(const w4a16_cache& c, const w4a16_cache_attenti
         if (s == 1 || t < 0.95 * best) { best = t; p.prompt.splits = (int)s; }
         if (waves >= 8.0) break;
     }
-    p.prompt.parts = p.prompt.splits * (p.prompt.kv2 ? 2 : 1);
     p.grid = (int)((int64_t)p.prompt.blocks * a.batch * c.kv_heads * p.prompt.splits);
-    if (p.prompt.parts > 1)
-        p.workspace = (size_t)p.prompt.parts * (size_t)(a.q_tokens * a.q_heads) * (size_t)(c.head_dim + 2) * sizeof(float);
+    if (p.prompt.splits > 1) p.workspace = (size_t)p.prompt.splits * part_bytes;
     return p;
 }
 
 // Up to 32 rows a (sequence, key head) go to the decode kernel, which streams the codes once for
 // each 8 of them; more to the prompt kernel, whose 128-row products cost the same for few rows.
 // Measured with 4 rows a query (decode / prompt kernel, us): 16 sequences of up to 4096 tokens, 5
-// queries 41 / 73, 8 queries 52 / 74, 12 queries 77 / 81; 64 of up to 512, 8 queries 63 / 67, 12
-// queries 88 / 70; 2 of 16384, 8 queries 43 / 53, 12 queries 60 / 54.
+// queries 43 / 65, 8 queries 53 / 65, 9 queries 64 / 65, 12 queries 75 / 65; 64 of up to 512, 8 queries
+// 54 / 52, 9 queries 65 / 53; 2 of up to 16384, 8 queries 33 / 40, 9 queries 37 / 41, 12 queries 41 / 41.
 constexpr int64_t kDecodeRows = 32;
 
 static AttentionPlan plan_attention(const w4a16_cache& c, const w4a16_cache_attention_args& a, const DeviceInfo& dev) {
@@ -249,10 +247,10 @@ static cudaError_t launch_prompt_t(const AttentionParams& ap, const AttentionPla
     cudaError_t err = ensure_max_dynamic_smem(reinterpret_cast<const void*>(kern));
     if (err != cudaSuccess) return err;
     err = launch(kern, dim3((unsigned)plan.grid), kCpThreads, C::SMEM, stream, pdl, ap, plan.prompt);
-    if (err != cudaSuccess || plan.prompt.parts == 1) return err;
+    if (err != cudaSuccess || plan.prompt.splits == 1) return err;
     const int64_t rows = (int64_t)ap.max_q * ap.shared * ap.c.kv_heads, per = 128 / (D / 4);
     return launch(cache_prompt_combine_kernel<D>, dim3((unsigned)((rows + per - 1) / per), (unsigned)ap.batch), 128, 0, stream,
-                  pdl, ap, plan.prompt.parts);
+                  pdl, ap, plan.prompt.splits);
 }
 
 cudaError_t launch_cache_attention(const w4a16_cache& c, const w4a16_cache_attention_args& a, const DeviceInfo& dev,

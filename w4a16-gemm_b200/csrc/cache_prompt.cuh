@@ -8,8 +8,8 @@
 //     S = Q K^T   (128 x 128, TMEM)  ->  P = 2^(r S - m), fp16, TMEM
 //     O += P V    (128 x D, TMEM)
 // While the tensor cores work on one half's products, the other half's softmax runs.  With 128
-// rows or fewer the halves take alternate tiles of the cache instead, for the same rows, and
-// are joined by the combine kernel like any other parts.
+// rows or fewer the halves take alternate tiles of the cache instead, for the same rows; the first
+// one's warps join the two results from TMEM.
 //
 // Warps: 0 issues the products; 1 fetches codes and pairs (bulk copies); 2 clears rows that are not answered; 4-7 turn them into fp16
 // operands in shared memory (keys [token][value], values transposed [value][token], both K-major
@@ -206,9 +206,8 @@ struct CpIssue {
 // What a grid of prompt CTAs does, set on the host.
 struct CpGrid {
     int blocks;      // row blocks of the longest sequence
-    int splits;      // CTAs that share the tiles of one row block
+    int splits;      // CTAs that share the tiles of one row block: 1, results are written at once; else joined
     int kv2;         // 128 rows or fewer: the halves take alternate tiles
-    int parts;       // results to be joined for each row: splits * (kv2 ? 2 : 1); 1: written at once
 };
 
 __device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
@@ -617,13 +616,29 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
         }
         if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar.o_done(h), walk.last_o<D>(h) & 1, kDevTimeoutCache));
         // ---- results
-        if (ok && warp_live && rows > 0) {
+        float keep = 1.f, other = 0.f;                                 // factors of this half's result and of the second's
+        if (gr.kv2) {
+            float* ml = reinterpret_cast<float*>(smem_raw + (qs - raw) + C::Q_BYTES) + kCpRows;    // behind the factors
+            if (h == 1) { ml[r_in] = fresh ? -INFINITY : m; ml[kCpRows + r_in] = l; }
+            bar_sync_named(1, 256);
+            if (h == 0 && walk.steps(1) > 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait(bar.o_done(1), walk.last_o<D>(1) & 1, kDevTimeoutCache)) && ok;
+                const float m1 = ml[r_in], top = fresh ? m1 : fmaxf(m, m1);
+                // a half that saw nothing has sums of zero (or NaN, which must stay)
+                keep = fresh ? 1.f : exp2_fast(m - top);
+                other = m1 == -INFINITY ? 1.f : exp2_fast(m1 - top);
+                l = fmaf(l, keep, ml[kCpRows + r_in] * other);
+                fresh = top == -INFINITY;
+                m = top;
+            }
+        }
+        if (ok && warp_live && rows > 0 && !(gr.kv2 && h == 1)) {
             tc_fence_after();
-            const int part = split * (gr.kv2 ? 2 : 1) + (gr.kv2 ? h : 0);
             const int64_t all = p.q_tokens * heads;
-            float* po = reinterpret_cast<float*>(p.workspace) + ((int64_t)part * all + at) * D;
-            float* pm = reinterpret_cast<float*>(p.workspace) + (int64_t)gr.parts * all * D + ((int64_t)part * all + at) * 2;
+            float* po = reinterpret_cast<float*>(p.workspace) + ((int64_t)split * all + at) * D;
+            float* pm = reinterpret_cast<float*>(p.workspace) + (int64_t)gr.splits * all * D + ((int64_t)split * all + at) * 2;
             const float inv = l == 0.f ? 0.f : 1.f / l;
+            const bool joined = gr.kv2 && walk.steps(1) > 0;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
@@ -634,7 +649,15 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = 0u;
                 }
-                if (live && gr.parts == 1) {
+                if (joined) {
+                    uint32_t o1[32];
+                    tmem_ld_x32(tmem + lanes + CpTmem<D>::O(1) + c, o1);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        o[e] = __float_as_uint(fmaf(__uint_as_float(o[e]), keep, __uint_as_float(o1[e]) * other));
+                }
+                if (live && gr.splits == 1) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
                         float f[8];
@@ -648,7 +671,7 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                         *reinterpret_cast<uint4*>(po + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 }
             }
-            if (live && gr.parts == 1) {
+            if (live && gr.splits == 1) {
                 if (p.lse) p.lse[at] = l == 0.f ? -INFINITY : (m - 6.f + log2f(l)) * kLn2;
             } else if (live) {
                 pm[0] = fresh ? -INFINITY : m;
