@@ -27,9 +27,17 @@ def rotary_table(max_pos: int, rotary_dim: int, theta: float = 500000.0, device=
 
 
 def slots_of(page_table: torch.Tensor, sequence: torch.Tensor, positions: torch.Tensor, page_size: int) -> torch.Tensor:
-    """Cache slots (int64) of tokens, by their sequence and position (int64 tensors of one shape)."""
-    page = page_table[sequence, positions // page_size].long()
-    return page * page_size + positions % page_size
+    """Cache slots (int64) of tokens, by their sequence and position (int64 tensors of one shape).
+
+    A position that the table has no column for gets slot -1, which an append skips.
+    """
+    width = page_table.shape[1]
+    if width == 0:
+        return torch.full_like(positions, -1)
+    column = positions // page_size
+    inside = column.clamp(0, width - 1)
+    slot = torch.add(positions % page_size, page_table[sequence, inside], alpha=page_size)
+    return slot.masked_fill_(column != inside, -1)
 
 
 class AttentionBlock:
@@ -49,16 +57,30 @@ class AttentionBlock:
 
 
 class DecodeLoop:
-    """One-token steps of a batch from a captured graph: lengths, positions and slots live on the device."""
+    """One-token steps of a batch from a captured graph: lengths, positions and slots live on the device.
+
+    The loop keeps the caller's ``page_table`` and ``seq_lens`` and counts the latter up in place, one a step;
+    the caller may change both between steps (a finished sequence's place given to another).  A step for
+    which some sequence's table has no column is refused.
+    """
 
     def __init__(self, block: AttentionBlock, x: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor):
         self.block, self.x, self.page_table, self.seq_lens = block, x.clone(), page_table, seq_lens
+        self._left = self._room()
         self._sequence = torch.arange(x.shape[0], device=x.device)
         self._step()                                        # set-up calls happen outside the capture
         self.seq_lens -= 1
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self.out = self._step()
+
+    def _room(self) -> int:
+        """Steps until the longest sequence fills its table, at least one (waits for the device)."""
+        most = self.page_table.shape[1] * self.block.cache.page_size
+        room = most - int(self.seq_lens.max()) if self.seq_lens.numel() else most
+        if room <= 0:
+            raise RuntimeError(f"no step is left: a sequence fills its page table ({most} tokens)")
+        return room
 
     def _step(self):
         positions = self.seq_lens.long()
@@ -68,6 +90,9 @@ class DecodeLoop:
 
     def step(self, x: torch.Tensor) -> torch.Tensor:
         """Appends one token a sequence and returns the block's output (valid until the next step)."""
+        if self._left == 0:                                 # or fewer sequences than there were: look again
+            self._left = self._room()
+        self._left -= 1
         self.x.copy_(x)
         self.graph.replay()
         return self.out
