@@ -336,7 +336,7 @@ typedef struct w4a16_cache_attention_args {
     int32_t dtype;           /* w4a16_act_dtype of q and out */
     int32_t q_heads;         /* a multiple of kv_heads */
     int32_t batch;
-    int32_t table_pages;
+    int32_t table_pages;     /* of page_size tokens each: at most 2^31 - 1024 tokens */
     int32_t max_q;           /* no sequence has more queries (1 if cu_q is NULL); see below */
     int32_t causal;          /* 0: a query sees every cached token of its sequence */
     int32_t window;          /* > 0: a query at position p sees tokens above p - window only */

@@ -472,8 +472,9 @@ w4a16_status check_attention_sizes(const w4a16_cache* c, const w4a16_cache_atten
     if ((int64_t)a->batch * ((int64_t)a->max_q * a->q_heads / 128 + c->kv_heads) >= (1LL << 31))
         return fail(W4A16_ERR_DIM_RANGE, "batch * max_q * q_heads must be below 2^38");
     if (a->max_q < 0 || a->max_q > a->q_tokens) return fail(W4A16_ERR_CACHE, "max_q must be in [0, q_tokens]");
-    if ((int64_t)a->table_pages * c->page_size >= (1LL << 31))
-        return fail(W4A16_ERR_DIM_RANGE, "a sequence's tokens (table_pages * page_size) must fit in int32");
+    // the kernels round token indexes up to tiles, and step up to eight runs of 128 past a tile's start, in int32
+    if ((int64_t)a->table_pages * c->page_size > (1LL << 31) - 1024)
+        return fail(W4A16_ERR_DIM_RANGE, "a sequence's tokens (table_pages * page_size) must be at most 2^31 - 1024");
     if (a->window < 0) return fail(W4A16_ERR_CACHE, "window must not be negative (0: none)");
     if (!(a->scale == a->scale)) return fail(W4A16_ERR_CACHE, "scale must be a number");
     return ok();
