@@ -455,6 +455,11 @@ w4a16_status check_act_dtype(int32_t dtype) {
     return ok();
 }
 
+// A count of any size times at most 2^32 heads.
+bool product_fits_int32(int64_t count, int64_t heads) {
+    return count >= 0 && count < (1LL << 31) && count * heads < (1LL << 31);
+}
+
 bool strides8(int64_t a, int64_t b) { return a % 8 == 0 && b % 8 == 0; }
 
 // Everything of an attention call but its pointers.
@@ -467,7 +472,7 @@ w4a16_status check_attention_sizes(const w4a16_cache* c, const w4a16_cache_atten
         return fail(W4A16_ERR_CACHE, "q_heads must be a multiple of kv_heads");
     if (a->batch < 0 || a->batch > 65535 || a->table_pages < 0)
         return fail(W4A16_ERR_CACHE, "batch must be in [0, 65535] and table_pages must not be negative");
-    if (a->q_tokens < 0 || a->q_tokens * a->q_heads >= (1LL << 31))
+    if (!product_fits_int32(a->q_tokens, a->q_heads))
         return fail(W4A16_ERR_DIM_RANGE, "q_tokens * q_heads must fit in int32");
     if ((int64_t)a->batch * ((int64_t)a->max_q * a->q_heads / 128 + c->kv_heads) >= (1LL << 31))
         return fail(W4A16_ERR_DIM_RANGE, "batch * max_q * q_heads must be below 2^38");
@@ -497,7 +502,7 @@ w4a16_status w4a16_cache_append(const w4a16_cache* cache, const void* k, const v
     if (s != W4A16_OK) return s;
     if ((s = check_act_dtype(dtype)) != W4A16_OK) return s;
     const int64_t q_heads = rotary && rotary->q ? rotary->q_heads : 0;
-    if (tokens < 0 || tokens * (cache->kv_heads + q_heads) >= (1LL << 31))
+    if (!product_fits_int32(tokens, cache->kv_heads + q_heads))
         return fail(W4A16_ERR_DIM_RANGE, "tokens * heads must fit in int32");
     if (rotary) {
         const w4a16_rotary& r = *rotary;
@@ -555,7 +560,7 @@ w4a16_status w4a16_cache_read(const w4a16_cache* cache, const int64_t* slots, in
     w4a16_status s = check_cache(cache);
     if (s != W4A16_OK) return s;
     if ((s = check_act_dtype(dtype)) != W4A16_OK) return s;
-    if (tokens < 0 || tokens * cache->kv_heads >= (1LL << 31))
+    if (!product_fits_int32(tokens, cache->kv_heads))
         return fail(W4A16_ERR_DIM_RANGE, "tokens * heads must fit in int32");
     if (tokens == 0) return ok();
     if (!cache->data || !slots || !k_out || !v_out)
