@@ -376,11 +376,13 @@ w4a16_status w4a16_cache_attention_workspace(const w4a16_cache* cache, const w4a
  * ran out (0 = none).  Synchronises the device.  reset != 0 clears it. */
 w4a16_status w4a16_device_status(int32_t* code, int32_t reset);
 
-/* Diagnostic of the bounded-wait policy: launches two one-thread kernels that each wait for
+/* Diagnostic of the bounded-wait policy: launches one-thread kernels that each wait for
  * an mbarrier phase nothing completes, with the busy-polling and the sleeping wait the GEMM
  * kernels use.  Each wait gives up after its limit (about 2 s), records its code in the
  * device status word (4, then 1) and returns; codes[0..1] receive the status word read after
- * each kernel, which is then cleared.  Synchronises the device; takes about 4 s. */
+ * each kernel, which is then cleared.  A third kernel does the same for the cache kernels' wait and their
+ * part of the status word (8); the call fails if that does not come back.  Synchronises the
+ * device; takes about 6 s. */
 w4a16_status w4a16_check_wait_limits(int32_t* codes);
 
 /* Short name of a status code. */

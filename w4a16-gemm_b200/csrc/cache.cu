@@ -21,6 +21,12 @@ cudaError_t read_cache_device_status(int* code, bool reset) {
     return cudaMemcpyToSymbol(w4a16_device_status, &zero, sizeof(int));
 }
 
+cudaError_t run_cache_wait_limit_check() {
+    wait_limit_kernel<<<1, 32>>>(1, kDevTimeoutCache);
+    const cudaError_t err = cudaGetLastError();
+    return err != cudaSuccess ? err : cudaDeviceSynchronize();
+}
+
 static CacheView cache_view(const w4a16_cache& c) {
     CacheView v;
     v.data = static_cast<uint8_t*>(c.data);

@@ -637,7 +637,11 @@ w4a16_status w4a16_check_wait_limits(int32_t* codes) {
         if (err == cudaSuccess) err = w4a16::read_device_status(&c, true);
         codes[i] = c;
     }
+    if (err == cudaSuccess) err = w4a16::run_cache_wait_limit_check();
+    if (err == cudaSuccess) err = w4a16::read_device_status(&c, true);
     if (err != cudaSuccess) return fail(W4A16_ERR_CUDA, std::string("CUDA error: ") + cudaGetErrorString(err));
+    if (c != 8)
+        return fail(W4A16_ERR_DEVICE_TIMEOUT, "a wait of the cache kernels ran out and the device status was " + std::to_string(c) + ", not 8");
     return ok();
 }
 

@@ -125,6 +125,8 @@ cudaError_t launch_cache_attention(const w4a16_cache& c, const w4a16_cache_atten
                                    void* workspace, cudaStream_t stream, bool pdl);
 // read_device_status for cache.cu's status word (no synchronisation of its own).
 cudaError_t read_cache_device_status(int* code, bool reset);
+// run_wait_limit_check in cache.cu: records kDevTimeoutCache in its status word.
+cudaError_t run_cache_wait_limit_check();
 
 // ---------------------------------------------------------------- debug dequant
 cudaError_t launch_dequant(const void* wp, const void* scales, void* out, int N, int K, int G,

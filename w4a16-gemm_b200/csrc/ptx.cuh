@@ -125,6 +125,19 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int cod
     }
 }
 
+// One thread waits for phase 0 of an mbarrier that nothing arrives at, with the wait the
+// kernels use (busy polls, or polls that sleep between tries): after the wait limit it
+// records `code` in this translation unit's status word and returns.
+static __global__ void wait_limit_kernel(int sleeping, int code) {
+    __shared__ __align__(8) uint64_t bar;
+    if (threadIdx.x == 0) {
+        mbar_init(smem_u32(&bar), 1);
+        fence_mbar_init();
+        if (sleeping) mbar_wait_sleep(smem_u32(&bar), 0, code);
+        else mbar_wait(smem_u32(&bar), 0, code);
+    }
+}
+
 // Tiled tensor copies (TMA), no multicast.
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tmap, int c0, int c1, uint32_t bar) {
     asm volatile(
