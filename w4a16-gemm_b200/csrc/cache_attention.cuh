@@ -11,6 +11,7 @@
 #include <stdint.h>
 
 #include "cache_format.cuh"
+#include "cache_partition.h"
 #include "internal.h"
 #include "ptx.cuh"
 
@@ -104,7 +105,7 @@ __device__ __forceinline__ int seen_hi(const AttentionParams& p, int pos, int le
     return p.causal ? min(max(pos + 1, 0), len) : len;
 }
 __device__ __forceinline__ int seen_lo(const AttentionParams& p, int pos) {
-    return p.window ? max(0, max(pos + 1, 0) - p.window) : 0;
+    return seen_from(p.window, pos);
 }
 
 // A page of a sequence; what the table should not hold is led back into the cache.

@@ -44,11 +44,10 @@
 #include <type_traits>
 
 #include "cache_attention.cuh"
+#include "cache_partition.h"
 
 namespace w4a16 {
 
-constexpr int kCdTile = 128;        // tokens of a unit
-constexpr int kCdRows = 8;          // rows of a block: the right side of an m16n8k16 product
 constexpr int kCdWarps = 4;         // consumer warps
 constexpr int kCdWarpTokens = kCdTile / kCdWarps;
 constexpr int kCdThreads = (kCdWarps + 1) * 32;
@@ -76,47 +75,12 @@ struct CdCfg {
     static constexpr int MERGE = kCdWarps * ROWS * LD * 4;         // [warp][row][LD]: sums, then maximum and sum of weights
     static constexpr int HDR = STAGES * (int)sizeof(CdStage);
     static constexpr int SMEM = STAGES * STAGE + MERGE + HDR + 256;
-    static constexpr int CTAS = 3;                                 // resident on an SM (shared memory, 128 registers a thread)
+    static constexpr int CTAS = kCdCtas;
 };
 
-// What the start and end of a segment cost beside its units (queries, merge), in units: ranges
-// are cut by cost, so that a CTA with many short segments is not the last to finish.
-constexpr int kCdSegmentCost = 2;
-
-// Units of one sequence and key head.
-__device__ __forceinline__ int cd_first_tile(const AttentionParams& p, const SeqSpan& s) {
-    return seen_lo(p, s.pos0) / kCdTile;
-}
-__device__ __forceinline__ int cd_tiles(const AttentionParams& p, const SeqSpan& s) {
-    if (s.nq == 0 || s.len == 0) return 0;
-    return (s.len + kCdTile - 1) / kCdTile - cd_first_tile(p, s);
-}
-// Blocks of rows of a sequence, and what all its segments cost.
-template <int ROWS>
-__device__ __forceinline__ int cd_blocks(const AttentionParams& p, const SeqSpan& s) {
-    return (s.nq * p.shared + ROWS - 1) / ROWS;
-}
-template <int ROWS>
-__device__ __forceinline__ long long cd_cost(const AttentionParams& p, const SeqSpan& s) {
-    const int nt = cd_tiles(p, s);
-    return nt ? (long long)(nt + kCdSegmentCost) * (p.c.kv_heads * cd_blocks<ROWS>(p, s)) : 0;
-}
-
-// Workspace: per segment the CTAs {first, last} that hold parts of it, then 2 slots
-// a CTA of ROWS x (D + 2) floats: sums, maxima, sums of weights.  Slot 0 is the part of a segment
-// that began in an earlier CTA, slot 1 of one that begins here.
-__host__ __device__ __forceinline__ size_t cd_info_bytes(int64_t segments) {
-    return (size_t)(segments * 8 + 255) / 256 * 256;
-}
-__host__ __device__ __forceinline__ size_t cd_slot_floats(int rows, int D) {
-    return (size_t)rows * (D + 2);
-}
-
-// floor(a * b / c) and floor(a / c) of non-negative numbers; 32-bit divisions where they do (a 64-bit one
-// takes some 400 cycles, and a short call has several of them in a row).
-__device__ __forceinline__ long long mul_div(long long a, long long b, long long c) {
-    const unsigned long long ab = (unsigned long long)a * (unsigned long long)b;
-    return (ab | (unsigned long long)c) >> 32 ? (long long)(ab / (unsigned long long)c) : (long long)((uint32_t)ab / (uint32_t)c);
+// The segments of one sequence.
+__device__ __forceinline__ CdShape cd_shape(const AttentionParams& p, const SeqSpan& s) {
+    return cd_shape(s.nq, p.shared, s.len, s.pos0, p.window);
 }
 
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
@@ -173,7 +137,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
         const int per = (p.batch + kCdThreads - 1) / kCdThreads;
         const int b0 = min((int)threadIdx.x * per, p.batch), b1 = min(b0 + per, p.batch);
         long long mine = 0;
-        for (int b = b0; b < b1; ++b) mine += cd_cost<ROWS>(p, seq_span(p, b));
+        for (int b = b0; b < b1; ++b) mine += cd_shape(p, seq_span(p, b)).cost(hk);
         long long incl = mine;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
@@ -188,13 +152,13 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
             if (w < warp) before += warp_sum[w];
             total += warp_sum[w];
         }
-        const long long u0 = mul_div(total, blockIdx.x, max(min((long long)gridDim.x, total), 1LL));
+        const long long u0 = CdCut(total, (int)gridDim.x).begin(blockIdx.x);
         long long base = before + incl - mine;
         if (threadIdx.x == 0) found[0] = total;
         if (u0 >= base && u0 < base + mine) {
             int b = b0;
             for (; b < b1; ++b) {
-                const long long n = cd_cost<ROWS>(p, seq_span(p, b));
+                const long long n = cd_shape(p, seq_span(p, b)).cost(hk);
                 if (u0 < base + n) break;
                 base += n;
             }
@@ -203,10 +167,8 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
         }
         __syncthreads();
     }
-    const long long total = found[0];
-    const long long ctas = min((long long)gridDim.x, total);      // those with work: a unit at least
-    if (blockIdx.x >= ctas) return;
-    const long long u0 = mul_div(total, blockIdx.x, ctas), u1 = mul_div(total, blockIdx.x + 1, ctas);
+    const CdCut cut(found[0], (int)gridDim.x);
+    if (blockIdx.x >= cut.ctas) return;
 
     if (warp == kCdWarps) {
         // ------------------------------------------------------------ producer
@@ -218,25 +180,12 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
         const uint32_t dst_off = (part < 2 ? part * C::CODES : 2 * C::CODES + (part - 2) * C::PAIRS) + run * run_bytes;
         const uint32_t src_part = part < 2 ? (uint32_t)(part * F::CODE) << ps_log
                                            : (uint32_t)(2 * F::CODE + (part - 2) * F::PAIR) << ps_log;
-        // u counts cost: a segment's units follow the kCdSegmentCost of its start, which are passed over
         int b = (int)found[2];
         SeqSpan s = seq_span(p, b);
-        int nt = cd_tiles(p, s), first = cd_first_tile(p, s);
-        int blocks = cd_blocks<ROWS>(p, s);
-        const long long local = u0 - found[1];
-        int seg = (int)mul_div(local, 1, nt + kCdSegmentCost);   // of the sequence
-        int tile = (int)(local - (long long)seg * (nt + kCdSegmentCost)) - kCdSegmentCost;
-        long long u = u0;
-        if (tile < 0) { u -= tile; tile = 0; }
+        CdWalk w(cut, blockIdx.x, found[1], cd_shape(p, s));
         bool begins = true;
-        // the CTA that holds the unit before `end`: floor((end * ctas - 1) / total)
-        auto cta_of = [&](long long end) {
-            const unsigned long long x = (unsigned long long)end * (unsigned long long)ctas - 1ull;
-            return (x | (unsigned long long)total) >> 32 ? (long long)(x / (unsigned long long)total) : (long long)((uint32_t)x / (uint32_t)total);
-        };
-        long long seg0 = u - tile;                               // the segment's first unit
         int2* info = reinterpret_cast<int2*>(p.workspace);
-        if (u >= u1 && lane == 0) {                              // a start and no unit: nothing to do
+        if (!w.more() && lane == 0) {                            // a start and no unit: nothing to do
             CdStage h = {};
             h.flags = 8;
             hdr[0] = h;
@@ -244,28 +193,26 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
         }
         int st = 0, turn = 0, issued = 0;
         bool ok = true;
-        while (u < u1) {
-            const int tok0 = (first + tile) * kCdTile;
+        while (w.more()) {
+            const int tok0 = (w.sh.first + w.tile) * kCdTile;
             const int tok = tok0 + run * rows;
             const bool valid = run * rows < kCdTile && tok < s.len && tok + rows > seen_lo(p, s.pos0);
             const int64_t page = valid ? page_of(p, b, tok >> ps_log) : 0;
-            const uint8_t* src = cache_block(p.c, page, seg / blocks) + src_part + (uint32_t)(tok & ((1 << ps_log) - 1)) * unit_b;
+            const uint8_t* src = cache_block(p.c, page, w.head()) + src_part + (uint32_t)(tok & ((1 << ps_log) - 1)) * unit_b;
             const bool got = mbar_wait_sleep(empty(st), (uint32_t)turn ^ 1u, kDevTimeoutCache);
             if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
             const int runs = __popc(__ballot_sync(0xffffffffu, valid)) / 4;
-            const bool ends = tile + 1 == nt || u + 1 == u1;
+            const bool ends = w.ends();
             if (lane == 0) {
-                const bool part_of = seg0 < u0 || seg0 + nt > u1;
                 CdStage h;
-                h.tok0 = tok0; h.row0 = seg % blocks * ROWS; h.head = seg / blocks;
+                h.tok0 = tok0; h.row0 = w.block() * ROWS; h.head = w.head();
                 const int block_rows = min(s.nq * p.shared - h.row0, ROWS);
-                const bool last = u + 1 + (tile + 1 == nt ? kCdSegmentCost : 0) >= u1;
-                h.flags = (begins ? 1 : 0) | (ends ? 2 : 0) | (part_of ? 4 : 0) | (last ? 8 : 0) | block_rows << 8;
+                h.flags = (begins ? 1 : 0) | (ends ? 2 : 0) | (w.part() ? 4 : 0) | (w.last() ? 8 : 0) | block_rows << 8;
                 h.len = s.len; h.pos0 = s.pos0; h.q0 = s.q0;
-                h.slot = 2 * (int)blockIdx.x + (seg0 >= u0 ? 1 : 0);
+                h.slot = w.slot((int)blockIdx.x);
                 hdr[st] = h;
-                if (tile == 0)
-                    info[((int64_t)b * hk + h.head) * p.row_blocks + seg % blocks] = make_int2((int)blockIdx.x, (int)cta_of(seg0 + nt));
+                if (w.tile == 0)
+                    info[((int64_t)b * hk + h.head) * p.row_blocks + w.block()] = make_int2((int)blockIdx.x, cut.cta_before(w.seg0 + w.sh.tiles));
                 mbar_arrive_expect_tx(full(st), (uint32_t)(runs * rows * F::TOKEN));
             }
             __syncwarp();
@@ -273,17 +220,10 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
             ++issued;
             if (++st == ST) { st = 0; turn ^= 1; }
             begins = ends;
-            ++u;
-            if (++tile == nt) {
-                tile = 0;
-                u += kCdSegmentCost;
-                seg0 = u;
-                if (++seg == hk * blocks && u < u1) {
-                    seg = 0;
-                    do { s = seq_span(p, ++b); nt = cd_tiles(p, s); } while (nt == 0);
-                    first = cd_first_tile(p, s);
-                    blocks = cd_blocks<ROWS>(p, s);
-                }
+            if (w.advance(hk)) {
+                CdShape next;
+                do { s = seq_span(p, ++b); next = cd_shape(p, s); } while (next.tiles == 0);
+                w.follow(next);
             }
         }
         if (!ok) {
@@ -670,7 +610,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                 }
                 if (h.flags & 4) {
                     float* slot = reinterpret_cast<float*>(p.workspace + cd_info_bytes((int64_t)p.batch * hk * p.row_blocks)) +
-                                  (size_t)h.slot * cd_slot_floats(ROWS, D);
+                                  (size_t)h.slot * cd_slot_floats(D);
                     *reinterpret_cast<float4*>(slot + row * D + d) = v;
                     if (d == 0) {
                         slot[ROWS * D + row] = mm;
@@ -720,7 +660,7 @@ cache_decode_combine_kernel(const __grid_constant__ AttentionParams p, int seg_r
     if (whole == 0 && head == 0) clear_past_max<D>(p, s, slice * V4 + lane_d, SLICES * V4);
     if (whole >= s.nq * p.shared) return;
     const int64_t at = (int64_t)(s.q0 + whole / p.shared) * (hk * p.shared) + head * p.shared + whole % p.shared;
-    if (cd_tiles(p, s) == 0) {
+    if (cd_shape(p, s).tiles == 0) {
         if (slice == 0) {
             *reinterpret_cast<uint2*>(p.out + at * D + lane_d * 4) = make_uint2(0u, 0u);
             if (p.lse && lane_d == 0) p.lse[at] = -INFINITY;
@@ -730,8 +670,7 @@ cache_decode_combine_kernel(const __grid_constant__ AttentionParams p, int seg_r
     const int n = info.y - info.x + 1;
     if (n == 1) return;                                    // one CTA had it all and has written it
     const float* slots = reinterpret_cast<const float*>(p.workspace + cd_info_bytes((int64_t)p.batch * hk * p.row_blocks));
-    constexpr size_t size = (size_t)kCdRows * (D + 2);
-    auto part_of = [&](int c) { return slots + (size_t)(2 * (info.x + c) + (c == 0 ? 1 : 0)) * size; };
+    auto part_of = [&](int c) { return slots + (size_t)cd_part_slot(info.x, c) * cd_slot_floats(D); };
     // the row's maximum over the parts
     const uint32_t row_lanes = V4 == 32 ? 0xFFFFFFFFu : 0xFFFFu << (threadIdx.x & 16);
     float mm = -INFINITY;

@@ -39,6 +39,7 @@
 #include <type_traits>
 
 #include "cache_attention.cuh"
+#include "cache_plan.h"
 #include "cache_schedule.h"
 
 namespace w4a16 {
@@ -201,13 +202,6 @@ struct CpIssue {
     __device__ __forceinline__ void commit_o(int h) const { mma_commit(bar.o_done(h)); }
     __device__ __forceinline__ void commit_k(int st) const { mma_commit(bar.k_empty(st)); }
     __device__ __forceinline__ void commit_v(int st) const { mma_commit(bar.v_empty(st)); }
-};
-
-// What a grid of prompt CTAs does, set on the host.
-struct CpGrid {
-    int blocks;      // row blocks of the longest sequence
-    int splits;      // CTAs that share the tiles of one row block: 1, results are written at once; else joined
-    int kv2;         // 128 rows or fewer: the halves take alternate tiles
 };
 
 __device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
