@@ -245,11 +245,12 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
     uint32_t qf[2 * KW][2];                                  // query fragments, contraction steps of 16
     float o[4 * VW][4];                                      // sums: (value 2j, rows 2t, 2t+1), (value 2j+1, ...)
     float oc[NG][4];                                         // the same weights times 8
-    float m[2], thr[2], sum[2], msum[NG][2];
+    float m[2], thr[2], sum[2], msum[NG][2];                 // maximum followed, score above which it moves
     float r24[2], qs[NG][2];                             // score = r24 (s (q'.c) + m qs)
     int lo[2], hi[2];
     float vlim = 0.f, vmul = 1.f;                                // s_t <= vlim; w_t s_t vmul is what fp16 holds
     int lo_all = 0, lo_max = 0, hi_min = 0;
+    bool wide = false;                                           // some row of the block has huge queries
 
     const int w0 = warp * kCdWarpTokens;                         // this warp's tokens of a unit
     int st = 0, turn = 0;
@@ -293,7 +294,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
             amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             // the row's power of two: its largest value comes to [2^13, 2^14)
-            const int ex = min(max((int)(amax >> 23), 24), 250);
+            const int ex = min(max((int)(amax >> 23), 24), 253);
             const float down = __uint_as_float((uint32_t)(267 - ex) << 23 & 0x7F800000u);   // 2^(140 - ex)
             const float back = __uint_as_float((uint32_t)(ex - 13) << 23);                  // 2^(ex - 140)
             float total_q[NG];
@@ -317,7 +318,9 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                     qf[c + 1][1] = pack16(x[3] * 0.0625f, x[7] * 0.0625f, false);
                 }
             }
-            const float r = back * p.scale_log2 * 16777216.f;
+            // with queries of 2^94 and more 2^16 of the factor goes to the scores first: all of it may pass fp32
+            wide = __any_sync(0xffffffffu, ex > 220);
+            const float r = back * p.scale_log2 * (wide ? 256.f : 16777216.f);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int from = 8 * t + 4 * e, mine = 2 * t + e;
@@ -328,7 +331,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                 hi[e] = mine < rows ? seen_hi(p, pos, h.len) : h.len;
                 lo[e] = mine < rows ? seen_lo(p, pos) : 0;
                 m[e] = 0.f;
-                thr[e] = -3.0e38f;                        // nothing seen yet: any score sets the maximum
+                thr[e] = -INFINITY;                       // nothing seen yet: any score sets the maximum
                 sum[e] = 0.f;
 #pragma unroll
                 for (int a = 0; a < NG; ++a) msum[a][e] = 0.f;
@@ -421,23 +424,28 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                                 if (tk >= hi[r] || tk < lo[r]) gone |= 1u << (4 * blk + 2 * e + r);
                     }
             }
+            if (wide) {
+#pragma unroll
+                for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[blk][e] *= 65536.f;
+            }
+            // Scores, rounded to fp32 before the maximum is taken off: the maximum's own difference is then zero at any
+            // size (fused, it is what the rounding left, 2^-25 of the score).
             float y[2][4], top[2];
-            auto relative = [&]() {
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < 2; ++r) {
 #pragma unroll
-                        for (int blk = 0; blk < 2; ++blk)
+                for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                float v = fmaf(x[blk][2 * e + r], r24[r], -m[r]);
-                                if constexpr (MASKED)
-                                    if ((gone >> (4 * blk + 2 * e + r)) & 1u) v = -INFINITY;
-                                y[blk][2 * e + r] = v;
-                            }
-                        top[r] = fmaxf(fmaxf(y[0][r], y[0][2 + r]), fmaxf(y[1][r], y[1][2 + r]));
+                    for (int e = 0; e < 2; ++e) {
+                        float v = __fmul_rn(x[blk][2 * e + r], r24[r]);
+                        if constexpr (MASKED)
+                            if ((gone >> (4 * blk + 2 * e + r)) & 1u) v = -INFINITY;
+                        y[blk][2 * e + r] = v;
                     }
-            };
-            relative();
+                top[r] = fmaxf(fmaxf(y[0][r], y[0][2 + r]), fmaxf(y[1][r], y[1][2 + r]));
+            }
             __half2 vtop = __half2half2(__ushort_as_half(0));
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk)
@@ -467,12 +475,12 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                     float d = top[r];
 #pragma unroll
                     for (int k = 4; k < 32; k *= 2) d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, k));
-                    const bool fresh = thr[r] < 0.f;
+                    const bool fresh = thr[r] == -INFINITY;
                     keep[r] = 1.f;
-                    if (d > (fresh ? -3.0e38f : 0.f)) {
-                        m[r] += d;
-                        keep[r] = fresh ? 0.f : exp2_fast(-d);
-                        thr[r] = 8.f;
+                    if (d > (fresh ? -INFINITY : m[r])) {
+                        keep[r] = fresh ? 0.f : exp2_fast(m[r] - d);
+                        m[r] = d;
+                        thr[r] = __fadd_rd(d, 8.f);
                     }
                     sum[r] *= keep[r];
 #pragma unroll
@@ -488,7 +496,6 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                     o[j][0] *= keep[0] * vkeep; o[j][1] *= keep[1] * vkeep;
                     o[j][2] *= keep[0] * vkeep; o[j][3] *= keep[1] * vkeep;
                 }
-                relative();
             }
             // weights, and their fp16 form in the layout of the product's right operand
             uint32_t pf[2][NG][2];
@@ -503,7 +510,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                         vs[a] = sv * vmul;
                         vm[a] = fmaf(8.f, sv, __high2float(vp[blk][e][a]));
                     }
-                    const float p0 = exp2_fast(y[blk][2 * e]), p1 = exp2_fast(y[blk][2 * e + 1]);
+                    const float p0 = exp2_fast(__fsub_rn(y[blk][2 * e], m[0])), p1 = exp2_fast(__fsub_rn(y[blk][2 * e + 1], m[1]));
                     sum[0] += p0;
                     sum[1] += p1;
 #pragma unroll
@@ -583,7 +590,7 @@ cache_decode_kernel(const __grid_constant__ AttentionParams p) {
                             *reinterpret_cast<float2*>(mine + row * C::LD + d) = v;
                         }
                         if (g == 0) {
-                            mine[row * C::LD + D] = thr[r] < 0.f ? -INFINITY : m[r];
+                            mine[row * C::LD + D] = thr[r] == -INFINITY ? -INFINITY : m[r];
                             mine[row * C::LD + D + 1] = s;
                         }
                     }

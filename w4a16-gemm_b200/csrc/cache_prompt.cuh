@@ -489,7 +489,7 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
 #pragma unroll
                 for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(x[e]) & 0x7FFFFFFFu);
             }
-            const int ex = min(max((int)(amax >> 23), 24), 250);
+            const int ex = min(max((int)(amax >> 23), 24), 253);
             float down = __uint_as_float((uint32_t)(267 - ex) << 23);                  // 2^(140 - ex)
             r = __uint_as_float((uint32_t)(ex - 13) << 23) * fabsf(p.scale_log2);      // 2^(ex - 140) ...
             if (p.scale_log2 < 0.f) down = -down;
@@ -520,6 +520,7 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
         const int hi = live ? seen_hi(p, pos, s.len) : s.len, lo = live ? seen_lo(p, pos) : 0;
         float m = 0.f, l = 0.f;
         bool fresh = true;                                             // no score seen yet
+        bool large = false;                                            // some row's maximum of the warp is
         const int row_a = row - r_in, row_e = min(row_a + kCpRows, row0 + rows) - 1;
         const int in_hi = seen_hi(p, s.pos0 + row_a / p.shared, s.len);      // every row of the half sees [in_lo, in_hi)
         const int in_lo = seen_lo(p, s.pos0 + max(row_e, 0) / p.shared);
@@ -530,12 +531,14 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
             if (!ok) break;
             tc_fence_after();
             const int k0 = tile * kCpTile;
-            auto weights = [&](auto masked) {
+            // The tile's weights; false, with nothing changed, where the plain form does not do.
+            auto weights = [&](auto careful) {
+                constexpr bool CAREFUL = decltype(careful)::value;         // masks, and scores of any size
                 uint32_t x[kCpTile];
 #pragma unroll
                 for (int c = 0; c < kCpTile; c += 32) tmem_ld_x32(s_t + c, x + c);
                 tc_wait_ld();
-                if constexpr (decltype(masked)::value) {
+                if constexpr (CAREFUL) {
                     // One comparison a score and side that needs one (12 heads, window 700, with both sides
                     // compared in every tile at an end: 61 us against 57).
                     const int from = lo - k0, to = hi - k0;
@@ -555,9 +558,12 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                 for (int c = 0; c < kCpTile; c += 8)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1]));
-                const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * r;
-                const bool move = fresh ? top > -INFINITY : top > m + 8.f;
+                const float top = __fmul_rn(fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]), r);
+                const bool move = fresh ? top > -INFINITY : top > __fadd_rd(m, 8.f);
                 if (__any_sync(0xffffffffu, move)) {
+                    // a large maximum: see below
+                    large = __any_sync(0xffffffffu, fabsf(move ? top : m) > 1048576.f);
+                    if (!CAREFUL && large) return false;
                     float keep = 1.f;
                     if (move) {
                         keep = fresh ? 0.f : exp2_fast(m - top);
@@ -577,7 +583,15 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                         }
                     }
                 }
-                const uint64_t r2 = pair2(r, r), off2 = pair2(6.f - m, 6.f - m);
+                uint64_t r2 = pair2(r, r), off2 = pair2(6.f - m, 6.f - m);
+                if (CAREFUL && large) {
+                    // Scores are rounded before the maximum is taken off, as the maximum was: fused, the maximum's own difference
+                    // is what the rounding left, 2^-25 of the score.
+#pragma unroll
+                    for (int c = 0; c < kCpTile; ++c) x[c] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(x[c]), r), m));
+                    r2 = pair2(1.f, 1.f);
+                    off2 = pair2(6.f, 6.f);
+                }
                 uint64_t sum2[2] = {pair2(0.f, 0.f), pair2(0.f, 0.f)};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
@@ -600,10 +614,10 @@ cache_prompt_kernel(const __grid_constant__ AttentionParams p, const __grid_cons
                 split2(sum2[0], a0, a1);
                 split2(sum2[1], b0, b1);
                 l += (a0 + a1) + (b0 + b1);
+                return true;
             };
             if (warp_live) {
-                if (k0 < in_lo || k0 + kCpTile > in_hi) weights(std::true_type{});
-                else weights(std::false_type{});
+                if (large || k0 < in_lo || k0 + kCpTile > in_hi || !weights(std::false_type{})) weights(std::true_type{});
             } else {
                 warp_arrive(bar.p_full(h));
             }
