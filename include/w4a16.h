@@ -346,7 +346,8 @@ typedef struct w4a16_cache_attention_args {
 w4a16_status w4a16_cache_page_bytes(int32_t page_size, int32_t head_dim, int32_t group_size, uint64_t* bytes);
 
 /* Quantises k and v ([tokens][kv_heads][head_dim]) into the slots (int64 [tokens]; a slot
- * outside the cache is skipped; of equal slots one, unspecified, is kept per value).
+ * outside the cache is skipped; what equal slots of one call leave is unspecified: codes of one
+ * token may meet scales of another).
  * rotary (may be NULL): keys are turned before they are quantised, and queries into q_out. */
 w4a16_status w4a16_cache_append(const w4a16_cache* cache, const void* k, const void* v, int64_t k_token_stride,
                                 int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, int32_t dtype,

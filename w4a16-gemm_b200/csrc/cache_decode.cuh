@@ -1,7 +1,7 @@
 // Attention of few rows (query heads of a key head times queries of a sequence) over the 4-bit
 // cache: rows in blocks of 8, one pass over the codes a block.  Included by cache.cu only.
 //
-// Work.  A segment is a (sequence, key head, block of rows), a unit 128 cached tokens of one.  All
+// Work (cache_partition.h).  A segment is a (sequence, key head, block of rows), a unit 128 cached tokens of one.  All
 // units of the call, segment by segment (a head's blocks after one another: from the second on
 // the codes come from L2), are cut into equal contiguous ranges, one a CTA, so that ragged batches
 // load every SM alike whatever the lengths; lengths are read on the device.  A range holds whole
@@ -14,8 +14,9 @@
 // end of a segment.
 //
 // What bounds it: the products' instructions.  64 sequences of up to 8192 tokens, 8 key heads of 128
-// with 4 query heads each: 83 us, 3.9 TB/s; 79 with every read from L2, 60 without the products;
-// masks and byte permutes keep the ALU at 51 %, HMMA is at 25 %.  Measured there and not kept: 16 consumer
+// with 4 query heads each: 82 us, 4.0 TB/s; 79 with every read from L2, 60 without the products;
+// masks and byte permutes keep the ALU at 51 %, HMMA is at 25 %.  With two groups a key, 128 registers are
+// a few short (32 bytes of spills).  Measured there and not kept: 16 consumer
 // warps an SM in place of 12 (each with a ring of its own 93 us; with 96 registers 90; with the
 // queries in shared memory 85), the codes' shifts on the multiplier (90), blocks of 16 rows (a fifth
 // slower from 16 rows on).

@@ -41,10 +41,14 @@ inline AttentionPlan plan_decode(const w4a16_cache& c, const w4a16_cache_attenti
 // block's tiles are split over as many CTAs as an estimate says is shortest: a tile 2.4 us, a CTA's
 // start and end 7 us (measured); the work spread over the SMs, and for the last wave, as far as it is not
 // full, a CTA of the block with fewest tiles (heavy blocks come first); and the parts written and
-// joined.  Lengths are not known here:
-// the page table's width stands for them.  Measured, 32/8 heads, unsplit / as chosen: 800 queries over
-// 16384 tokens (104 blocks) 305 / 269 us, 1200 (152) 543 / 429; a prompt of 1500 (192, unsplit) 43.
-// Results of split blocks pass through the workspace, which is kept below 256 MB.
+// joined.  Measured, 32/8 heads, unsplit / as chosen: 800 queries over 16384 tokens (104 blocks) 292 / 285 us,
+// 1200 (152) 556 / 443, 2 x 12 over up to 16384 204 / 42; a prompt of 1500 (192, unsplit) 43.
+// Results of split blocks pass through the workspace, which is kept at 256 MB or below.
+//
+// Lengths are not known here: the page table's width stands for them, so that a table far wider than its
+// sequences splits blocks that have nothing to split.  A prompt of 1500: 43 us with a table of its
+// size, 108 with one of 32768 tokens; of 4096: 177 and 301.  A caller who knows the lengths passes a view of the
+// columns in use.
 inline AttentionPlan plan_prompt(const w4a16_cache& c, const w4a16_cache_attention_args& a, int num_sms) {
     const int64_t shared = a.q_heads / c.kv_heads, rows = a.max_q * shared;
     AttentionPlan p = {};

@@ -1,4 +1,4 @@
-// Attention of many rows (prompts, chunks of prompts, drafts of more than 16 rows) over the
+// Attention of many rows (more than 32 a sequence and key head: prompts, chunks of prompts, long drafts) over the
 // 4-bit cache on the tensor cores: tcgen05 products with accumulators in TMEM.  Included by
 // cache.cu only.
 //
@@ -11,25 +11,33 @@
 // rows or fewer the halves take alternate tiles of the cache instead, for the same rows; the first
 // one's warps join the two results from TMEM.
 //
-// Warps: 0 issues the products; 1 fetches codes and pairs (bulk copies); 2 clears rows that are not answered; 4-7 turn them into fp16
-// operands in shared memory (keys [token][value], values transposed [value][token], both K-major
-// with 128-byte swizzle); 8-11 and 12-15 hold one half each, a thread a row: they load the queries,
-// run the softmax and write the result.
+// Warps: 0 issues the products; 1 fetches codes and pairs (bulk copies); 2 clears rows that are not
+// answered; 4-7 turn codes and pairs into fp16 operands in shared memory (keys [token][value], values
+// transposed [value][token], both K-major with 128-byte swizzle); 8-11 and 12-15 hold one half each, a
+// thread a row: they load the queries, run the softmax and write the result.
 //
-// What bounds it: the chain of a half's step, some 4600 cycles for a 128-token tile of both halves
+// What bounds it: the chain of a half's step, some 4800 cycles for a 128-token tile of both halves
 // where the products alone take 2048 and the exponentials (16 a cycle and SM) as many: scores
 // read 180, maximum 370, weights 1800, then 1800 for PV, the next S and the hand-overs between
-// warps (100 to 200 each); shared memory is half used.  512 queries of 64 heads over 32768 tokens:
-// 640 us, 853 TFLOP/s.  Measured there and not kept: two threads a row
-// (680 us where this kernel then took 660; the figures that follow are of that time too), a warp of its own for the products of each half (765), a PV and the next S issued in one
-// go after all their waits (758), a quarter of the exponentials as polynomials on the FMA pipe (792),
-// a second read of the scores from TMEM in place of 128 registers (1160); and with no difference:
-// weights handed over in two parts, a third S buffer with 64-wide heads, queries and results moved
-// in coalesced rows.
+// warps (100 to 200 each), and the wait for PV before that S (128-wide heads).  512 queries of 64 heads
+// over 32768 tokens: 630 to 660 us, 840 TFLOP/s, at the GPU's power limit; a prompt of 4096 (32/8 heads) 189 us.
+//
+// Measured on those 512 queries and not kept, when this kernel took 660 us: two threads a row (680), a warp
+// of its own for the products of each half (765), a PV and the next S issued in one go after all their
+// waits (758), a quarter of the exponentials as polynomials on the FMA pipe (792), a second read of the
+// scores from TMEM in place of 128 registers (1160); and with no difference: weights handed over in two
+// parts, a third S buffer with 64-wide heads, queries and results moved in coalesced rows.
 //
 // Rounding.  A cached value code * scale + minimum is rounded once to fp16 (2^-11), as a 16-bit
-// cache would hold it.  Queries become fp16 after a power of two (exact within 2^-24 of the
-// row's largest).  Weights are fp16 up to 2^14: the maximum is followed only when a score passes
+// cache would hold it, which for keys moves a score by some 2^-12 of what its largest channels add.  With
+// fp16 outputs and outlier channels the result is 5.5e-4 from 64 bits (1e-3 on other inputs), where the
+// decode kernel's is 2.5e-4 and the output's own rounding 2.1e-4; with bf16 outputs 1.8e-3 to 2.0e-3, of
+// which their rounding is 1.7e-3.  Measured and not kept: codes as operands, with scales and minima in fp32
+// on the scores, give 3.3e-4 but take 223 us where this took 188 (a prompt of 4096), and 951 where it took
+// 640 with two groups a key (their scores in two parts); the scores in fragment order, for fewer loads of
+// the scales, 232 and 1316.
+//
+// Queries become fp16 after a power of two (exact within 2^-24 of the row's largest).  Weights are fp16 up to 2^14: the maximum is followed only when a score passes
 // it by 2^8, and 2^6 is put on top, so weights down to 2^-20 of the row's largest keep all
 // bits.  Sums, maxima and accumulators are fp32.
 #pragma once

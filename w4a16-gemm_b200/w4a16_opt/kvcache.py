@@ -68,7 +68,8 @@ def cache_append(cache: Int4KVCache, k: torch.Tensor, v: torch.Tensor, slots: to
                  cos_sin: torch.Tensor | None = None, sections=None, interleaved: bool = False):
     """Quantises ``k`` and ``v`` [tokens, kv_heads, head_dim] into ``slots`` (int64 [tokens]).
 
-    A slot outside the cache (-1, say) is skipped.  Values are clamped to +-57344 and NaN becomes
+    A slot outside the cache (-1, say) is skipped; what equal slots of one call leave is
+    unspecified (codes of one token may meet scales of another).  Values are clamped to +-57344 and NaN becomes
     0, so that whatever is read back is finite.
 
     ``positions`` (int64 [tokens], or [axes, tokens] with up to three axes) and ``cos_sin`` (fp32
@@ -111,6 +112,11 @@ def cache_attention(q: torch.Tensor, cache: Int4KVCache, page_table: torch.Tenso
     the sequence, with ``causal`` those up to its position, with ``window`` > 0 those above its
     position - window.  A query that sees none gives zeros, and -inf in the log of the sum of
     exponentials (fp32 [tokens, q_heads]) that comes second with ``return_lse``.
+
+    The lengths stay on the device, and the call is planned by the sizes of its arguments.  A table of
+    far more columns than the sequences use makes prompts slower: a view of the columns in use will
+    do.  More than 32 rows (``max_q`` times the query heads that share a key head) send the whole
+    call to the kernel for prompts, where single tokens are slow: give them a call of their own.
 
     ``scale`` defaults to 1 / sqrt(head_dim).  ``workspace``: optional scratch CUDA buffer
     (256-byte aligned); without it the binding keeps one per (device, stream).
