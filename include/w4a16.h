@@ -75,7 +75,11 @@ typedef enum w4a16_status {
     W4A16_ERR_FLAGS = 17,            /* flags holds bits that are not w4a16_flags values */
     W4A16_ERR_TP_GROUP = 18,         /* a w4a16_tp_group or an exchange's sizes are not usable */
     W4A16_ERR_CACHE = 19,            /* a w4a16_cache, or the sizes of a call on it, are not usable */
-    W4A16_ERR_ACT_DTYPE = 20         /* dtype is not a w4a16_act_dtype value */
+    W4A16_ERR_ACT_DTYPE = 20,        /* dtype is not a w4a16_act_dtype value */
+    W4A16_ERR_ACTIVATION = 21,       /* activation is not a w4a16_activation value */
+    W4A16_ERR_OVERLAP = 22,          /* an output overlaps an input that is read meanwhile */
+    W4A16_ERR_NORM = 23,             /* the sizes of a norm are not usable */
+    W4A16_ERR_MOE = 24               /* the sizes of a router's or an expert layer's call are not usable */
 } w4a16_status;
 
 typedef enum w4a16_flags {
@@ -166,6 +170,33 @@ w4a16_status w4a16_gemm_ex(const int32_t* Wp, const void* x, const void* scales,
 w4a16_status w4a16_gemm_noalloc(const int32_t* Wp, const void* x, const void* scales, void* y,
                                 int64_t M, int64_t N, int64_t K, int64_t groups, int64_t wp_words,
                                 int32_t variant, int32_t out_dtype, void* stream);
+
+/* Activations of w4a16_linear and w4a16_moe_experts: z; max(z, 0); z / (1 + e^-z); z Phi(z) with the
+ * normal distribution's Phi; z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2. */
+typedef enum w4a16_activation {
+    W4A16_ACTIVATION_NONE = 0,
+    W4A16_ACTIVATION_RELU = 1,
+    W4A16_ACTIVATION_SILU = 2,
+    W4A16_ACTIVATION_GELU = 3,
+    W4A16_ACTIVATION_GELU_TANH = 4
+} w4a16_activation;
+
+typedef struct w4a16_epilogue {
+    const void* bias;        /* fp16 [N] in the order of the weight's rows, or NULL */
+    const void* residual;    /* fp16, y's shape, dense, or NULL; may be y itself */
+    int32_t activation;      /* w4a16_activation */
+    int32_t gated;           /* rows 16i .. 16i + 7 of W are the gate's, the eight after them the other factor's */
+} w4a16_epilogue;
+
+/* A GEMM with its epilogue.  With z = x @ W^T + bias in fp32,
+ *     y[M, N]     = act(z) + residual                                     (gated == 0)
+ *     y[M, N / 2] : y_j = act(z_g) * z_u + residual_j, g = 16 (j / 8) + j % 8, u = g + 8   (gated != 0)
+ * rounded to fp16 once.  W is the dequantised weight of w4a16_gemm (fp16), whose kernels, variants, flags, workspace
+ * (w4a16_workspace_bytes) and stream order these are.  y may be the residual; it must not overlap x, bias, the
+ * weights or the scales.  y is 4-byte aligned. */
+w4a16_status w4a16_linear(const int32_t* Wp, const void* x, const void* scales, void* y, int64_t M, int64_t N,
+                          int64_t K, int64_t groups, int64_t wp_words, const w4a16_epilogue* epilogue, int32_t variant,
+                          uint32_t flags, void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* The launch w4a16_gemm would make for this call (kernel choice, tiles, grid).
  * Mirrors the reference's routing (kernel.cu:242-249) and prefill config
@@ -372,6 +403,46 @@ w4a16_status w4a16_cache_attention(const w4a16_cache* cache, const w4a16_cache_a
  * initialisation, 256-byte aligned, one per concurrent call. */
 w4a16_status w4a16_cache_attention_workspace(const w4a16_cache* cache, const w4a16_cache_attention_args* args,
                                              uint64_t* bytes);
+
+/* ------------------------------------------------------------------------------
+ * What stands around the products of a decoder layer.  No counterpart in the reference. */
+
+typedef struct w4a16_norm_args {
+    const void* x;           /* [tokens][heads][dim] */
+    const void* weight;      /* [dim], x's dtype */
+    const void* residual;    /* x's shape, or NULL */
+    void* y;                 /* x's shape and dtype; may be x or the residual, with the same strides and type */
+    void* residual_out;      /* x + residual in the residual's type (with a residual); may be the residual or x likewise */
+    int64_t x_token_stride, x_head_stride;                       /* strides in elements, multiples of 8 */
+    int64_t residual_token_stride, residual_head_stride;
+    int64_t y_token_stride, y_head_stride;
+    int64_t residual_out_token_stride, residual_out_head_stride;
+    int64_t tokens;
+    int32_t heads;           /* 1 for rows [tokens][dim] */
+    int32_t dim;             /* a multiple of 8, at most 32768 */
+    int32_t dtype;           /* w4a16_act_dtype of x, weight and y */
+    int32_t residual_f32;    /* the residual and residual_out are fp32 instead of dtype */
+    float eps;
+} w4a16_norm_args;
+
+/* Root-mean-square norm of rows: with h = x + residual (fp32), y = h * weight / sqrt(mean(h^2) + eps), and
+ * residual_out = h; each rounded once (y from the unrounded h).  Pointers are 16-byte aligned, strides not
+ * negative; the rows of an output must not overlap one another. */
+w4a16_status w4a16_rms_norm(const w4a16_norm_args* args, void* stream);
+
+typedef enum w4a16_logits_dtype {
+    W4A16_LOGITS_F16 = 0,
+    W4A16_LOGITS_BF16 = 1,
+    W4A16_LOGITS_F32 = 2
+} w4a16_logits_dtype;
+
+/* The router of a mixture of experts.  logits [tokens][num_experts] with rows row_stride elements apart -> the k
+ * experts of largest logit in falling order (equal ones by index), experts int32 and weights fp32 [tokens][k]
+ * dense: weights exp(l - max) / sum, the sum over all experts or, with renormalize, over the chosen ones.  A logit
+ * of -inf or NaN is never chosen: where too few remain the rest is expert -1 with weight 0.  num_experts is in [1,
+ * 1024], k in [1, min(32, num_experts)]. */
+w4a16_status w4a16_moe_route(const void* logits, int32_t dtype, int64_t row_stride, int64_t tokens, int32_t num_experts,
+                             int32_t k, int32_t renormalize, float* weights, int32_t* experts, void* stream);
 
 /* Reads the current device's status word, set by a kernel whose bounded wait
  * ran out (0 = none).  Synchronises the device.  reset != 0 clears it. */

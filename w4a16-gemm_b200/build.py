@@ -30,7 +30,7 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3"]
 
-LIB_SOURCES = ["kernels.cu", "cache.cu", "capi.cpp"]
+LIB_SOURCES = ["kernels.cu", "cache.cu", "layer.cu", "capi.cpp"]
 LIB_PATH = os.path.join(OUT_DIR, "libw4a16.so")
 EXT_PATH = os.path.join(OUT_DIR, "_C" + sysconfig.get_config_var("EXT_SUFFIX"))
 
@@ -60,7 +60,7 @@ def build_library(force=False):
     if not force and not _stale(LIB_PATH, deps):
         return LIB_PATH
     tmp = LIB_PATH + ".tmp"
-    _run([NVCC, *ARCH_FLAGS, *NVCC_FLAGS, "--threads", "2", "-shared", "-I", INCLUDE,
+    _run([NVCC, *ARCH_FLAGS, *NVCC_FLAGS, "--threads", "4", "-shared", "-I", INCLUDE,
           *[os.path.join(CSRC, f) for f in LIB_SOURCES], "-o", tmp])
     os.replace(tmp, LIB_PATH)
     return LIB_PATH

@@ -6,6 +6,7 @@
 #include <cmath>
 
 #include "internal.h"
+#include "launch.cuh"
 #include "ptx.cuh"
 #include "cache_format.cuh"
 #include "cache_plan.h"
@@ -51,22 +52,6 @@ static cudaError_t with_format(const w4a16_cache& c, Fn&& f) {
 template <typename Fn>
 static cudaError_t with_bool(bool b, Fn&& f) {
     return b ? f(std::integral_constant<bool, true>{}) : f(std::integral_constant<bool, false>{});
-}
-
-template <typename... KArgs, typename... Args>
-static cudaError_t launch(void (*kern)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t stream, bool pdl,
-                          Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads, 1, 1);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
 cudaError_t launch_cache_append(const CacheAppendArgs& a) {

@@ -130,6 +130,50 @@ w4a16_status w4a16_validate(const void* Wp, const void* x, const void* scales, i
     return ok();
 }
 
+namespace {
+
+// What w4a16_gemm_ex and w4a16_linear do after their checks of arguments.
+w4a16_status launch_gemm(w4a16::GemmArgs a, int32_t variant) {
+    w4a16::DeviceInfo d;
+    w4a16_status s = check_device(&d);
+    if (s != W4A16_OK) return s;
+    const Route r = make_route(a.M, a.N, a.K, a.G, variant, d);
+    const size_t need = route_workspace(r);
+    if (need > 0) {
+        if (!a.workspace) return fail(W4A16_ERR_WORKSPACE, "this call needs a workspace of " + std::to_string(need) + " bytes");
+        if (a.workspace_bytes < need)
+            return fail(W4A16_ERR_WORKSPACE, "workspace too small: " + std::to_string(a.workspace_bytes) + " < " +
+                                                 std::to_string(need) + " bytes");
+        if (reinterpret_cast<uintptr_t>(a.workspace) % 256) return fail(W4A16_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+    }
+    trace_route(r, a.M, a.N, a.K, a.G);
+    cudaError_t err = r.decode ? w4a16::launch_decode(a, r.dp) : w4a16::launch_prefill(a, r.pp);
+    if (err == cudaSuccess) err = cudaGetLastError();
+    if (err != cudaSuccess) return fail(W4A16_ERR_CUDA, std::string("kernel launch failed: ") + cudaGetErrorString(err));
+    return ok();
+}
+
+constexpr uint32_t kKnownFlags = W4A16_FLAG_WEIGHTS_RESIDENT | W4A16_FLAG_FP32_SCALE;
+
+w4a16_status check_flags(uint32_t flags) {
+    if (flags & ~kKnownFlags) return fail(W4A16_ERR_FLAGS, "unknown flag bits " + std::to_string(flags & ~kKnownFlags));
+    return ok();
+}
+
+w4a16_status check_activation(int32_t activation) {
+    if (activation < W4A16_ACTIVATION_NONE || activation > W4A16_ACTIVATION_GELU_TANH)
+        return fail(W4A16_ERR_ACTIVATION, "activation must be 0 (none), 1 (relu), 2 (silu), 3 (gelu) or 4 (gelu_tanh)");
+    return ok();
+}
+
+// Whether [a, a + a_bytes) and [b, b + b_bytes) share a byte (a NULL pointer shares none).
+bool overlap(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
+    const uint64_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
+}
+
+}  // namespace
+
 w4a16_status w4a16_gemm_ex(const int32_t* Wp, const void* x, const void* scales, void* y, int64_t M, int64_t N,
                            int64_t K, int64_t groups, int64_t wp_words, int32_t variant, int32_t out_dtype,
                            uint32_t flags, void* workspace, uint64_t workspace_bytes, void* stream) {
@@ -138,28 +182,38 @@ w4a16_status w4a16_gemm_ex(const int32_t* Wp, const void* x, const void* scales,
     if (!Wp || !x || !scales || !y) return fail(W4A16_ERR_NULL_POINTER, "Wp, x, scales and y must be non-null");
     if (out_dtype != W4A16_OUT_F16 && out_dtype != W4A16_OUT_F32)
         return fail(W4A16_ERR_OUT_DTYPE, "out_dtype must be 0 (fp16) or 1 (fp32)");
-    constexpr uint32_t kKnownFlags = W4A16_FLAG_WEIGHTS_RESIDENT | W4A16_FLAG_FP32_SCALE;
-    if (flags & ~kKnownFlags) return fail(W4A16_ERR_FLAGS, "unknown flag bits " + std::to_string(flags & ~kKnownFlags));
-    w4a16::DeviceInfo d;
-    if ((s = check_device(&d)) != W4A16_OK) return s;
-    const int G = (int)(K / groups);
-    w4a16::GemmArgs a{Wp, x, scales, y, (int)M, (int)N, (int)K, G, out_dtype == W4A16_OUT_F32,
-                      static_cast<cudaStream_t>(stream), pdl_enabled(), (flags & W4A16_FLAG_WEIGHTS_RESIDENT) != 0,
-                      (flags & W4A16_FLAG_FP32_SCALE) != 0, workspace, (size_t)workspace_bytes};
-    const Route r = make_route(a.M, a.N, a.K, G, variant, d);
-    const size_t need = route_workspace(r);
-    if (need > 0) {
-        if (!workspace) return fail(W4A16_ERR_WORKSPACE, "this call needs a workspace of " + std::to_string(need) + " bytes");
-        if (workspace_bytes < need)
-            return fail(W4A16_ERR_WORKSPACE, "workspace too small: " + std::to_string(workspace_bytes) + " < " +
-                                                 std::to_string(need) + " bytes");
-        if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(W4A16_ERR_WORKSPACE, "workspace must be 256-byte aligned");
-    }
-    trace_route(r, a.M, a.N, a.K, G);
-    cudaError_t err = r.decode ? w4a16::launch_decode(a, r.dp) : w4a16::launch_prefill(a, r.pp);
-    if (err == cudaSuccess) err = cudaGetLastError();
-    if (err != cudaSuccess) return fail(W4A16_ERR_CUDA, std::string("kernel launch failed: ") + cudaGetErrorString(err));
-    return ok();
+    if ((s = check_flags(flags)) != W4A16_OK) return s;
+    return launch_gemm({Wp, x, scales, y, (int)M, (int)N, (int)K, (int)(K / groups), out_dtype == W4A16_OUT_F32,
+                        static_cast<cudaStream_t>(stream), pdl_enabled(), (flags & W4A16_FLAG_WEIGHTS_RESIDENT) != 0,
+                        (flags & W4A16_FLAG_FP32_SCALE) != 0, workspace, (size_t)workspace_bytes, w4a16::kEpiNone, {}},
+                       variant);
+}
+
+w4a16_status w4a16_linear(const int32_t* Wp, const void* x, const void* scales, void* y, int64_t M, int64_t N, int64_t K,
+                          int64_t groups, int64_t wp_words, const w4a16_epilogue* epilogue, int32_t variant,
+                          uint32_t flags, void* workspace, uint64_t workspace_bytes, void* stream) {
+    w4a16_status s = w4a16_validate(Wp, x, scales, M, N, K, groups, wp_words, variant);
+    if (s != W4A16_OK) return s;
+    if (N == 0) return fail(W4A16_ERR_N_MULTIPLE, "N must be at least 16");
+    if (!Wp || !x || !scales || !y || !epilogue)
+        return fail(W4A16_ERR_NULL_POINTER, "Wp, x, scales, y and epilogue must be non-null");
+    const w4a16_epilogue& e = *epilogue;
+    if ((s = check_activation(e.activation)) != W4A16_OK) return s;
+    if ((s = check_flags(flags)) != W4A16_OK) return s;
+    if (reinterpret_cast<uintptr_t>(y) % 4 || reinterpret_cast<uintptr_t>(e.bias) % 2 || reinterpret_cast<uintptr_t>(e.residual) % 2)
+        return fail(W4A16_ERR_ALIGNMENT, "y must be 4-byte aligned, bias and residual 2-byte");
+    const uint64_t y_bytes = (uint64_t)M * (uint64_t)(e.gated ? N / 2 : N) * 2;
+    if (overlap(y, y_bytes, x, (uint64_t)M * (uint64_t)K * 2) || overlap(y, y_bytes, Wp, (uint64_t)wp_words * 4) ||
+        overlap(y, y_bytes, scales, (uint64_t)groups * (uint64_t)N * 2) || overlap(y, y_bytes, e.bias, (uint64_t)N * 2) ||
+        (e.residual != y && overlap(y, y_bytes, e.residual, y_bytes)))
+        return fail(W4A16_ERR_OVERLAP, "y must not overlap x, the weights, the scales, the bias or a part of the residual");
+    const bool plain = !e.gated && !e.bias && !e.residual && e.activation == W4A16_ACTIVATION_NONE;
+    return launch_gemm({Wp, x, scales, y, (int)M, (int)N, (int)K, (int)(K / groups), false,
+                        static_cast<cudaStream_t>(stream), pdl_enabled(), (flags & W4A16_FLAG_WEIGHTS_RESIDENT) != 0,
+                        (flags & W4A16_FLAG_FP32_SCALE) != 0, workspace, (size_t)workspace_bytes,
+                        plain ? w4a16::kEpiNone : e.gated ? w4a16::kEpiGated : w4a16::kEpiPlain,
+                        {e.bias, e.residual, e.activation}},
+                       variant);
 }
 
 w4a16_status w4a16_gemm(const int32_t* Wp, const void* x, const void* scales, void* y, int64_t M, int64_t N,
@@ -614,6 +668,98 @@ w4a16_status w4a16_cache_attention(const w4a16_cache* cache, const w4a16_cache_a
     return err == cudaSuccess ? ok() : cuda_fail(err);
 }
 
+// ------------------------------------------------------------------ norm, router
+namespace {
+
+// A [tokens][heads][dim] view in memory.
+struct View {
+    const void* p;
+    int64_t token, head;
+    int32_t size;          // bytes of an element
+    bool operator==(const View& o) const { return p == o.p && token == o.token && head == o.head && size == o.size; }
+};
+
+uint64_t span_bytes(const View& v, int64_t tokens, int64_t heads, int64_t dim) {
+    return (uint64_t)((tokens - 1) * v.token + (heads - 1) * v.head + dim) * (uint64_t)v.size;
+}
+
+// Whether no element of a view has two places in it: either dimension inside the other.
+bool rows_apart(const View& v, int64_t tokens, int64_t heads, int64_t dim) {
+    const bool head_ok = heads == 1 || v.head >= dim, token_ok = tokens == 1 || v.token >= dim;
+    if (!head_ok || !token_ok) return false;
+    return heads == 1 || tokens == 1 || v.token >= (heads - 1) * v.head + dim || v.head >= (tokens - 1) * v.token + dim;
+}
+
+}  // namespace
+
+w4a16_status w4a16_rms_norm(const w4a16_norm_args* args, void* stream) {
+    if (!args) return fail(W4A16_ERR_NULL_POINTER, "args must be non-null");
+    const w4a16_norm_args& n = *args;
+    w4a16_status s = check_act_dtype(n.dtype);
+    if (s != W4A16_OK) return s;
+    if (n.dim < 8 || n.dim % 8 || n.dim > w4a16::kNormMaxDim)
+        return fail(W4A16_ERR_NORM, "dim must be a multiple of 8 in [8, " + std::to_string(w4a16::kNormMaxDim) + "]");
+    if (n.heads < 1) return fail(W4A16_ERR_NORM, "heads must be at least 1");
+    if (!product_fits_int32(n.tokens, n.heads)) return fail(W4A16_ERR_DIM_RANGE, "tokens * heads must fit in int32");
+    if (!(n.eps >= 0.f) || n.eps > 3e38f) return fail(W4A16_ERR_NORM, "eps must be a number and not negative");
+    if (n.tokens == 0) return ok();
+    if (!n.x || !n.weight || !n.y || (n.residual && !n.residual_out))
+        return fail(W4A16_ERR_NULL_POINTER, "x, weight and y must be non-null, and residual_out with a residual");
+    const int32_t extra = n.residual_f32 ? 4 : 2;
+    const View x{n.x, n.x_token_stride, n.x_head_stride, 2}, y{n.y, n.y_token_stride, n.y_head_stride, 2};
+    const View r{n.residual, n.residual_token_stride, n.residual_head_stride, extra};
+    const View h{n.residual ? n.residual_out : nullptr, n.residual_out_token_stride, n.residual_out_head_stride, extra};
+    constexpr int64_t kMostStride = 1LL << 31;      // spans stay far inside 64 bits
+    const View* const views[4] = {&x, &y, &r, &h};
+    for (const View* v : views) {
+        if (!v->p) continue;
+        if (!aligned16(v->p) || !strides8(v->token, v->head))
+            return fail(W4A16_ERR_ALIGNMENT, "x, residual and outputs must be 16-byte aligned, their strides multiples of 8 elements");
+        if (v->token < 0 || v->head < 0 || v->token > kMostStride || v->head > kMostStride)
+            return fail(W4A16_ERR_NORM, "strides must be in [0, 2^31]");
+    }
+    if (!aligned16(n.weight)) return fail(W4A16_ERR_ALIGNMENT, "weight must be 16-byte aligned");
+    const auto span = [&](const View& v) { return span_bytes(v, n.tokens, n.heads, n.dim); };
+    const auto clash = [&](const View& a, const View& b) { return overlap(a.p, span(a), b.p, span(b)); };
+    if (!rows_apart(y, n.tokens, n.heads, n.dim) || (h.p && !rows_apart(h, n.tokens, n.heads, n.dim)))
+        return fail(W4A16_ERR_OVERLAP, "the rows of an output must not overlap one another");
+    const uint64_t w_bytes = (uint64_t)n.dim * 2;
+    // an output may take an input's very place (a row is read before it is written), nothing in between
+    if ((!(y == x) && clash(y, x)) || (!(y == r) && clash(y, r)) || (!(h == x) && clash(h, x)) || (!(h == r) && clash(h, r)) ||
+        clash(y, h) || overlap(y.p, span(y), n.weight, w_bytes) || overlap(h.p, h.p ? span(h) : 0, n.weight, w_bytes))
+        return fail(W4A16_ERR_OVERLAP, "an output must be an input's very view or apart from every input and output");
+    w4a16::DeviceInfo d;
+    if ((s = check_device(&d)) != W4A16_OK) return s;
+    const cudaError_t err = w4a16::launch_rms_norm(n, static_cast<cudaStream_t>(stream), pdl_enabled());
+    return err == cudaSuccess ? ok() : cuda_fail(err);
+}
+
+w4a16_status w4a16_moe_route(const void* logits, int32_t dtype, int64_t row_stride, int64_t tokens, int32_t num_experts,
+                             int32_t k, int32_t renormalize, float* weights, int32_t* experts, void* stream) {
+    if (dtype < W4A16_LOGITS_F16 || dtype > W4A16_LOGITS_F32)
+        return fail(W4A16_ERR_ACT_DTYPE, "dtype of the logits must be 0 (fp16), 1 (bf16) or 2 (fp32)");
+    if (num_experts < 1 || num_experts > w4a16::kRouteMaxExperts)
+        return fail(W4A16_ERR_MOE, "num_experts must be in [1, " + std::to_string(w4a16::kRouteMaxExperts) + "]");
+    if (k < 1 || k > w4a16::kRouteMaxK || k > num_experts)
+        return fail(W4A16_ERR_MOE, "k must be in [1, min(" + std::to_string(w4a16::kRouteMaxK) + ", num_experts)]");
+    if (!product_fits_int32(tokens, num_experts)) return fail(W4A16_ERR_DIM_RANGE, "tokens * num_experts must fit in int32");
+    if (row_stride < 0 || row_stride > (1LL << 31)) return fail(W4A16_ERR_MOE, "row_stride must be in [0, 2^31]");
+    if (tokens == 0) return ok();
+    if (!logits || !weights || !experts) return fail(W4A16_ERR_NULL_POINTER, "logits, weights and experts must be non-null");
+    const int32_t size = dtype == W4A16_LOGITS_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(logits) % size || reinterpret_cast<uintptr_t>(weights) % 4 || reinterpret_cast<uintptr_t>(experts) % 4)
+        return fail(W4A16_ERR_ALIGNMENT, "logits, weights and experts must be aligned to their elements");
+    const uint64_t in = (uint64_t)((tokens - 1) * row_stride + num_experts) * (uint64_t)size, out = (uint64_t)(tokens * k) * 4;
+    if (overlap(logits, in, weights, out) || overlap(logits, in, experts, out) || overlap(weights, out, experts, out))
+        return fail(W4A16_ERR_OVERLAP, "logits, weights and experts must not overlap");
+    w4a16::DeviceInfo d;
+    w4a16_status s = check_device(&d);
+    if (s != W4A16_OK) return s;
+    const cudaError_t err = w4a16::launch_moe_route(logits, dtype, row_stride, tokens, num_experts, k, renormalize != 0,
+                                                    weights, experts, static_cast<cudaStream_t>(stream), pdl_enabled());
+    return err == cudaSuccess ? ok() : cuda_fail(err);
+}
+
 w4a16_status w4a16_device_status(int32_t* code, int32_t reset) {
     if (!code) return fail(W4A16_ERR_NULL_POINTER, "code must be non-null");
     int c = 0;
@@ -668,6 +814,10 @@ const char* w4a16_status_string(w4a16_status status) {
         case W4A16_ERR_TP_GROUP: return "W4A16_ERR_TP_GROUP";
         case W4A16_ERR_CACHE: return "W4A16_ERR_CACHE";
         case W4A16_ERR_ACT_DTYPE: return "W4A16_ERR_ACT_DTYPE";
+        case W4A16_ERR_ACTIVATION: return "W4A16_ERR_ACTIVATION";
+        case W4A16_ERR_OVERLAP: return "W4A16_ERR_OVERLAP";
+        case W4A16_ERR_NORM: return "W4A16_ERR_NORM";
+        case W4A16_ERR_MOE: return "W4A16_ERR_MOE";
     }
     return "W4A16_ERR_UNKNOWN";
 }

@@ -48,6 +48,7 @@
 
 #include "decode_partition.h"
 #include "dequant.cuh"
+#include "epilogue.cuh"
 #include "internal.h"
 #include "ptx.cuh"
 
@@ -91,11 +92,11 @@ inline DcPartition dc_partition(int N, int K, int num_sms) {
     return cache[key] = dc_cut(N, K, num_sms);
 }
 
-template <int G, int MP, bool OUT_F32, bool FP32_SCALE>
+template <int G, int MP, bool OUT_F32, bool FP32_SCALE, int EPI>
 __global__ void __launch_bounds__(kDcThreads, 1)
 decode_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
               const __grid_constant__ CUtensorMap ts, void* __restrict__ yv, int M, int N, int box_blocks,
-              int box_chunks, DcPartition part, float* __restrict__ partials, int pre_stages)
+              int box_chunks, DcPartition part, float* __restrict__ partials, int pre_stages, Epilogue epi)
 {
     using C = DcCfg<MP>;
     constexpr int ST = C::ST;
@@ -331,27 +332,42 @@ decode_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CU
                 const int nb = g * kDcBlocks + warp * BPW + bb;
                 const int colb = (warp * BPW + bb) * 16 + g8;           // column inside the group
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int mt = 0; mt < MT; ++mt) {
+                    float v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        v[i] = 0.f;
+#pragma unroll
+                        for (int ch = 0; ch < CH; ++ch) {
+                            v[i] += acc[bb][ch][mt][i];
+                            acc[bb][ch][mt][i] = 0.f;
+                        }
+                    }
+                    if (EPI != kEpiNone && whole) {
+#pragma unroll
+                        for (int i = 0; i < (EPI == kEpiGated ? 2 : 4); ++i) {
+                            const int tok = mt * 8 + 2 * t4 + (i & 1);
+                            if (nb < NB && tok < M)
+                                store_epilogue<EPI>(static_cast<__half*>(yv), epi, tok, N, g * kDcCols + colb + 8 * (i >> 1),
+                                                    v[i], EPI == kEpiGated ? v[i + 2] : 0.f);
+                        }
+                        continue;
+                    }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int tok = mt * 8 + 2 * t4 + (i & 1);
-                        float v = 0.f;
-#pragma unroll
-                        for (int ch = 0; ch < CH; ++ch) {
-                            v += acc[bb][ch][mt][i];
-                            acc[bb][ch][mt][i] = 0.f;
-                        }
                         if (nb < NB && tok < M) {
                             const int dc = 8 * (i >> 1);
                             if (whole) {
                                 const size_t o = (size_t)tok * N + g * kDcCols + colb + dc;
-                                if (OUT_F32) static_cast<float*>(yv)[o] = v;
-                                else static_cast<__half*>(yv)[o] = __float2half_rn(v);
+                                if (OUT_F32) static_cast<float*>(yv)[o] = v[i];
+                                else static_cast<__half*>(yv)[o] = __float2half_rn(v[i]);
                             } else {
-                                __stcg(my + tok * kDcCols + colb + dc, v);
+                                __stcg(my + tok * kDcCols + colb + dc, v[i]);
                             }
                         }
                     }
+                }
             }
             gkc0 = 0;
         }
@@ -364,32 +380,40 @@ decode_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CU
 // resident early and griddepcontrol.wait releases it once decode_kernel's writes are
 // complete and visible.  Sums the partials in CTA order (deterministic); the loads of
 // 8 partials are issued together so the sum is not one serial chain of L2 trips.
-template <bool OUT_F32>
+template <bool OUT_F32, int EPI>
 __global__ void __launch_bounds__(kDcCols) decode_combine_kernel(void* __restrict__ yv, int N, DcPartition part,
-                                                                 const float* __restrict__ partials) {
+                                                                 const float* __restrict__ partials, Epilogue epi) {
     const int g = blockIdx.x, tok = blockIdx.y;
     const int cf = part.first_cta(g), cl = part.last_cta(g);
     pdl_launch_dependents();
     if (cf == cl) return;
     pdl_wait();
-    const int col = g * kDcCols + threadIdx.x;
+    // a gated result's thread sums both of its factors' columns, eight apart
+    const int t = threadIdx.x, local = EPI == kEpiGated ? t + (t & ~7) : t;
+    const int col = g * kDcCols + local;
     if (col >= N) return;
     // CTA cf may have started in an earlier group (its second slot); every later CTA
     // of the group starts inside it (its first slot, 2 * cc).
-    const float* const p = partials + tok * kDcCols + threadIdx.x;
+    const float* const p = partials + tok * kDcCols + local;
     const int slot_f = part.slot(cf, g);
-    float sum = 0.f;
+    float sum = 0.f, sum_u = 0.f;
     for (int cc = cf; cc <= cl; cc += 8) {
-        float v[8];
+        float v[8], u[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int c = cc + i;
-            v[i] = c <= cl ? __ldcg(p + (size_t)(c == cf ? slot_f : 2 * c) * kDcSlotFloats) : 0.f;
+            const float* const q = p + (size_t)(c == cf ? slot_f : 2 * c) * kDcSlotFloats;
+            v[i] = c <= cl ? __ldcg(q) : 0.f;
+            if (EPI == kEpiGated) u[i] = c <= cl ? __ldcg(q + 8) : 0.f;
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += v[i];
+        for (int i = 0; i < 8; ++i) {
+            sum += v[i];
+            if (EPI == kEpiGated) sum_u += u[i];
+        }
     }
-    if (OUT_F32) static_cast<float*>(yv)[(size_t)tok * N + col] = sum;
+    if (EPI != kEpiNone) store_epilogue<EPI>(static_cast<__half*>(yv), epi, tok, N, col, sum, sum_u);
+    else if (OUT_F32) static_cast<float*>(yv)[(size_t)tok * N + col] = sum;
     else static_cast<__half*>(yv)[(size_t)tok * N + col] = __float2half_rn(sum);
 }
 
@@ -419,10 +443,10 @@ size_t decode_workspace_bytes(int N, int K, const DeviceInfo& dev) {
 cudaError_t make_decode_tensor_maps(const GemmArgs& a, int box_blocks, int box_chunks, int mp, CUtensorMap* tw,
                                     CUtensorMap* tx, CUtensorMap* ts);
 
-template <int G, int MP, bool F32, bool FS>
+template <int G, int MP, bool F32, bool FS, int EPI>
 static cudaError_t launch_decode_t(const GemmArgs& a, const DecodePlan& p) {
     (void)p;
-    auto kern = decode_kernel<G, MP, F32, FS>;
+    auto kern = decode_kernel<G, MP, F32, FS, EPI>;
     cudaError_t err = ensure_max_dynamic_smem(reinterpret_cast<const void*>(kern));
     if (err != cudaSuccess) return err;
     DeviceInfo dev;
@@ -444,36 +468,39 @@ static cudaError_t launch_decode_t(const GemmArgs& a, const DecodePlan& p) {
     cfg.attrs = &attr;
     cfg.numAttrs = a.pdl ? 1 : 0;
     const int pre = a.pdl && a.weights_resident ? kDcPreStages : 0;
-    err = cudaLaunchKernelEx(&cfg, kern, tw, tx, ts, a.y, a.M, a.N, box_blocks, box_chunks, part, partials, pre);
+    err = cudaLaunchKernelEx(&cfg, kern, tw, tx, ts, a.y, a.M, a.N, box_blocks, box_chunks, part, partials, pre,
+                             a.epi);
     if (err != cudaSuccess || !part.split) return err;
     // combine split groups; always launched programmatically dependent on decode_kernel
     cudaLaunchConfig_t fc = {};
     fc.gridDim = dim3(part.groups, a.M, 1);
-    fc.blockDim = dim3(kDcCols, 1, 1);
+    fc.blockDim = dim3(EPI == kEpiGated ? kDcCols / 2 : kDcCols, 1, 1);
     fc.stream = a.stream;
     cudaLaunchAttribute fattr;
     fattr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     fattr.val.programmaticStreamSerializationAllowed = 1;
     fc.attrs = &fattr;
     fc.numAttrs = 1;
-    return cudaLaunchKernelEx(&fc, decode_combine_kernel<F32>, a.y, a.N, part, static_cast<const float*>(partials));
+    return cudaLaunchKernelEx(&fc, decode_combine_kernel<F32, EPI>, a.y, a.N, part, static_cast<const float*>(partials), a.epi);
 }
 
-template <int G, int MP, bool F32>
+template <int G, int MP, bool F32, int EPI>
 static cudaError_t launch_decode_fs(const GemmArgs& a, const DecodePlan& p) {
     // the fp32-scale form exists for M <= 8 only (MP = 8)
-    if (MP == 8 && a.fp32_scale) return launch_decode_t<G, MP, F32, MP == 8>(a, p);
-    return launch_decode_t<G, MP, F32, false>(a, p);
+    if (MP == 8 && a.fp32_scale) return launch_decode_t<G, MP, F32, MP == 8, EPI>(a, p);
+    return launch_decode_t<G, MP, F32, false, EPI>(a, p);
+}
+
+template <int G, int MP>
+static cudaError_t launch_decode_e(const GemmArgs& a, const DecodePlan& p) {
+    if (a.form == kEpiGated) return launch_decode_fs<G, MP, false, kEpiGated>(a, p);
+    if (a.form == kEpiPlain) return launch_decode_fs<G, MP, false, kEpiPlain>(a, p);
+    return a.out_f32 ? launch_decode_fs<G, MP, true, kEpiNone>(a, p) : launch_decode_fs<G, MP, false, kEpiNone>(a, p);
 }
 
 cudaError_t launch_decode(const GemmArgs& a, const DecodePlan& p) {
-    const bool f32 = a.out_f32;
-    if (a.G == 64) {
-        if (p.mt == 1) return f32 ? launch_decode_fs<64, 8, true>(a, p) : launch_decode_fs<64, 8, false>(a, p);
-        return f32 ? launch_decode_fs<64, 16, true>(a, p) : launch_decode_fs<64, 16, false>(a, p);
-    }
-    if (p.mt == 1) return f32 ? launch_decode_fs<128, 8, true>(a, p) : launch_decode_fs<128, 8, false>(a, p);
-    return f32 ? launch_decode_fs<128, 16, true>(a, p) : launch_decode_fs<128, 16, false>(a, p);
+    if (a.G == 64) return p.mt == 1 ? launch_decode_e<64, 8>(a, p) : launch_decode_e<64, 16>(a, p);
+    return p.mt == 1 ? launch_decode_e<128, 8>(a, p) : launch_decode_e<128, 16>(a, p);
 }
 
 }  // namespace w4a16

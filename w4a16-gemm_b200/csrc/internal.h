@@ -8,6 +8,15 @@
 
 namespace w4a16 {
 
+// What w4a16_linear adds to a GEMM, and the form of a kernel's epilogue: the plain store, act(z + bias) +
+// residual, or that with a gate.
+struct Epilogue {
+    const void* bias;        // fp16 [N] or NULL, in the order of the weight's rows
+    const void* residual;    // fp16 [M, columns of y] or NULL; may be y itself
+    int32_t activation;      // w4a16_activation
+};
+constexpr int kEpiNone = 0, kEpiPlain = 1, kEpiGated = 2;
+
 // One validated GEMM call: y[M, N] = x[M, K] @ W^T, W from packed nibbles + fp16 scales.
 struct GemmArgs {
     const void* wp;       // int32 [N*K/8] packed nibbles (fragment order)
@@ -23,6 +32,8 @@ struct GemmArgs {
     bool fp32_scale;      // decode, M <= 8: scales applied in fp32 after the MMA (W4A16_FLAG_FP32_SCALE)
     void* workspace;      // decode scratch (split-group partials); no initial contents needed
     size_t workspace_bytes;
+    int form;             // kEpiNone, kEpiPlain or kEpiGated; y is fp16 with the latter two
+    Epilogue epi;
 };
 
 struct DeviceInfo {
@@ -127,6 +138,13 @@ cudaError_t launch_cache_attention(const w4a16_cache& c, const w4a16_cache_atten
 cudaError_t read_cache_device_status(int* code, bool reset);
 // run_wait_limit_check in cache.cu: records kDevTimeoutCache in its status word.
 cudaError_t run_cache_wait_limit_check();
+
+// ---------------------------------------------------------------- norm and router (layer.cu)
+cudaError_t launch_rms_norm(const w4a16_norm_args& a, cudaStream_t stream, bool pdl);
+cudaError_t launch_moe_route(const void* logits, int32_t dtype, int64_t row_stride, int64_t tokens, int32_t num_experts,
+                             int32_t k, bool renormalize, float* weights, int32_t* experts, cudaStream_t stream, bool pdl);
+constexpr int kNormMaxDim = 32768;
+constexpr int kRouteMaxExperts = 1024, kRouteMaxK = 32;
 
 // ---------------------------------------------------------------- debug dequant
 cudaError_t launch_dequant(const void* wp, const void* scales, void* out, int N, int K, int G,

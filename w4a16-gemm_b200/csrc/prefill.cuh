@@ -37,6 +37,7 @@
 #include <cmath>
 
 #include "dequant.cuh"
+#include "epilogue.cuh"
 #include "internal.h"
 #include "ptx.cuh"
 
@@ -118,10 +119,80 @@ __device__ __forceinline__ uint64_t pf_sw128_desc(uint32_t saddr) {
          | ((uint64_t)2 << 61);              // SWIZZLE_128B
 }
 
-template <int G, int TOK, bool OUT_F32>
+// Epilogue of one lane: output channel n (a row of the weight) for CW tokens from tok0 on.  Plain: hv[i]
+// holds tokens 2i and 2i + 1 of channel n.  Gated: lanes l and l + 8 of a half warp hold the two
+// factors of one result each; per pair of tokens the gate's lane makes the first one's result and
+// the other lane the second one's, so hv[i] holds tokens 4i + s and 4i + 2 + s, s = lane / 8 % 2.  The residual of
+// exactly those values is fetched into hv while the sums are still being made: 16 packed bits
+// each, since CW fp32 values would not fit beside the 78 registers that 832 threads leave a lane.
+template <int EPI, int CW>
+__device__ __forceinline__ void load_residual(uint32_t* hv, const Epilogue& e, int tok0, int M, int n, int N) {
+    constexpr int STEP = EPI == kEpiGated ? 2 : 1, PAIRS = CW / (2 * STEP);
+    if (!e.residual) {
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) hv[i] = 0u;
+        return;
+    }
+    const int cols = EPI == kEpiGated ? N / 2 : N;
+    const int col = EPI == kEpiGated ? 8 * (n / 16) + n % 8 : n;
+    const int first = tok0 + (EPI == kEpiGated ? (n >> 3 & 1) : 0);
+    const uint16_t* const r = static_cast<const uint16_t*>(e.residual) + (size_t)first * cols + col;
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+        const int t0 = 2 * i * STEP, t1 = t0 + STEP;
+        const uint32_t lo = n < N && first + t0 < M ? r[(size_t)t0 * cols] : 0u;
+        const uint32_t hi = n < N && first + t1 < M ? r[(size_t)t1 * cols] : 0u;
+        hv[i] = lo | hi << 16;
+    }
+}
+
+__device__ __forceinline__ uint32_t add_rounded(uint32_t residual, float a, float b) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&residual));
+    const __half2 v = __floats2half2_rn(a + f.x, b + f.y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// EC accumulator columns of a lane's channel: bias, activation, gate, residual (already in hv), one rounding.
+template <int EPI, int EC>
+__device__ __forceinline__ void finish_columns(const uint32_t (&r)[EC], uint32_t* hv, int activation, float bias) {
+    if constexpr (EPI == kEpiPlain) {
+#pragma unroll
+        for (int j = 0; j < EC; j += 2)
+            hv[j / 2] = add_rounded(hv[j / 2], activate(__uint_as_float(r[j]) + bias, activation),
+                                    activate(__uint_as_float(r[j + 1]) + bias, activation));
+    } else {
+        const bool up = threadIdx.x >> 3 & 1;
+        float v[EC / 2];
+#pragma unroll
+        for (int j = 0; j < EC; j += 2) {
+            const float z0 = __uint_as_float(r[j]) + bias, z1 = __uint_as_float(r[j + 1]) + bias;
+            const float got = __shfl_xor_sync(0xffffffffu, up ? z0 : z1, 8);
+            v[j / 2] = activate(up ? got : z0, activation) * (up ? z1 : got);
+        }
+#pragma unroll
+        for (int i = 0; i < EC / 4; ++i) hv[i] = add_rounded(hv[i], v[2 * i], v[2 * i + 1]);
+    }
+}
+
+// Gated results: lanes 2i and 2i + 1 trade halves as below, so that each stores pairs of channels.
+template <int CW>
+__device__ __forceinline__ void store_gated(const uint32_t* hv, __half* y, int tok0, int M, int n, int N) {
+    const int p = n & 1, cols = N / 2;
+    const int first = tok0 + (n >> 3 & 1) + 2 * p;
+    uint32_t* const y32 = reinterpret_cast<uint32_t*>(y + (size_t)first * cols + 8 * (n / 16) + n % 8 - p);
+#pragma unroll
+    for (int i = 0; i < CW / 4; ++i) {
+        const uint32_t w = hv[i];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, p ? w : (w >> 16), 1);
+        const uint32_t out = p ? __byte_perm(got, w, 0x7610) : __byte_perm(w, got, 0x5410);
+        if (n < N && first + 4 * i < M) y32[(size_t)i * 2 * cols] = out;
+    }
+}
+
+template <int G, int TOK, bool OUT_F32, int EPI>
 __global__ void __launch_bounds__(kPfThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
-               const __grid_constant__ CUtensorMap tm_s, void* __restrict__ yv, int M, int N, int K)
+               const __grid_constant__ CUtensorMap tm_s, void* __restrict__ yv, int M, int N, int K, Epilogue epi)
 {
     using C = PfCfg<TOK>;
     constexpr int ST = C::STAGES, NA = C::A_STAGES, NACC = C::ACCS;
@@ -298,10 +369,17 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
         for (int tile = blockIdx.x; tile < total; tile += gridDim.x, ++tc) {
             const int tt = tile / n_tiles, tn = tile % n_tiles;
             const int b = tc % NACC;
-            if (!__all_sync(0xffffffffu, mbar_wait(accfull(b), (tc / NACC) & 1, kDevTimeoutPipeline))) break;
-            tc_fence_after();
             const int n = tn * kPfRows + 32 * q + lane;
             const int tok0 = tt * TOK + h * CW;
+            // what is added to the sums: fetched before the wait for them
+            float bias = 0.f;
+            uint32_t hv[EPI == kEpiGated ? CW / 4 : CW / 2];
+            if constexpr (EPI != kEpiNone) {
+                if (epi.bias && n < N) bias = half_at(epi.bias, n);
+                load_residual<EPI, CW>(hv, epi, tok0, M, n, N);
+            }
+            if (!__all_sync(0xffffffffu, mbar_wait(accfull(b), (tc / NACC) & 1, kDevTimeoutPipeline))) break;
+            tc_fence_after();
             const uint32_t tcol = tmem + lane_field + (uint32_t)(b * TOK + h * CW);
             if (OUT_F32) {
 #pragma unroll 1
@@ -322,23 +400,28 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
             } else {
                 // all of this warp's columns into registers as fp16 pairs, release the
                 // accumulator, then store
-                uint32_t hv[CW / 2];
 #pragma unroll
                 for (int c0 = 0; c0 < CW; c0 += EC) {
                     uint32_t r[EC];
                     tmem_ld_cols<EC>(tcol + (uint32_t)c0, r);
                     tc_wait_ld();
+                    if constexpr (EPI != kEpiNone) {
+                        finish_columns<EPI, EC>(r, hv + c0 / (EPI == kEpiGated ? 4 : 2), epi.activation, bias);
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < EC; j += 2) {
-                        const __half2 v = __floats2half2_rn(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
-                        hv[(c0 + j) / 2] = *reinterpret_cast<const uint32_t*>(&v);
+                        for (int j = 0; j < EC; j += 2) {
+                            const __half2 v = __floats2half2_rn(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+                            hv[(c0 + j) / 2] = *reinterpret_cast<const uint32_t*>(&v);
+                        }
                     }
                 }
                 tc_fence_before();
                 mbar_arrive(accempty(b));
                 // lanes 2i and 2i+1 (channels n0, n0 + 1) trade halves so that the even lane
                 // stores tokens j and the odd lane tokens j + 1 as fp16 pairs of both channels
-                {
+                if constexpr (EPI == kEpiGated) {
+                    store_gated<CW>(hv, static_cast<__half*>(yv), tok0, M, n, N);
+                } else {
                     const int p = lane & 1;
                     const int n0 = n - p;
                     uint32_t* y32 = reinterpret_cast<uint32_t*>(static_cast<__half*>(yv) + (size_t)(tok0 + p) * N + n0);
@@ -409,12 +492,12 @@ PrefillPlan plan_prefill(int M, int N, int K, int G, int config, const DeviceInf
 // Scales: [K/G, N] fp16, box {128, 1}.  Out-of-range boxes read as zero.
 cudaError_t make_prefill_tensor_maps(const GemmArgs& a, int tok, CUtensorMap* tx, CUtensorMap* tw, CUtensorMap* ts);
 
-template <int G, int TOK, bool F32>
+template <int G, int TOK, bool F32, int EPI>
 static cudaError_t launch_prefill_t(const GemmArgs& a, const PrefillPlan& p) {
     CUtensorMap tx, tw, ts;
     cudaError_t err = make_prefill_tensor_maps(a, TOK, &tx, &tw, &ts);
     if (err != cudaSuccess) return err;
-    auto kern = prefill_kernel<G, TOK, F32>;
+    auto kern = prefill_kernel<G, TOK, F32, EPI>;
     err = ensure_max_dynamic_smem(reinterpret_cast<const void*>(kern));
     if (err != cudaSuccess) return err;
     cudaLaunchConfig_t cfg = {};
@@ -427,22 +510,28 @@ static cudaError_t launch_prefill_t(const GemmArgs& a, const PrefillPlan& p) {
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = a.pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, tx, tw, ts, a.y, a.M, a.N, a.K);
+    return cudaLaunchKernelEx(&cfg, kern, tx, tw, ts, a.y, a.M, a.N, a.K, a.epi);
 }
 
-template <int G, bool F32>
+template <int G, bool F32, int EPI>
 static cudaError_t launch_prefill_g(const GemmArgs& a, const PrefillPlan& p) {
     switch (p.tok) {
-        case 32:  return launch_prefill_t<G, 32, F32>(a, p);
-        case 64:  return launch_prefill_t<G, 64, F32>(a, p);
-        case 128: return launch_prefill_t<G, 128, F32>(a, p);
-        default:  return launch_prefill_t<G, 256, F32>(a, p);
+        case 32:  return launch_prefill_t<G, 32, F32, EPI>(a, p);
+        case 64:  return launch_prefill_t<G, 64, F32, EPI>(a, p);
+        case 128: return launch_prefill_t<G, 128, F32, EPI>(a, p);
+        default:  return launch_prefill_t<G, 256, F32, EPI>(a, p);
     }
 }
 
+template <int G>
+static cudaError_t launch_prefill_e(const GemmArgs& a, const PrefillPlan& p) {
+    if (a.form == kEpiGated) return launch_prefill_g<G, false, kEpiGated>(a, p);
+    if (a.form == kEpiPlain) return launch_prefill_g<G, false, kEpiPlain>(a, p);
+    return a.out_f32 ? launch_prefill_g<G, true, kEpiNone>(a, p) : launch_prefill_g<G, false, kEpiNone>(a, p);
+}
+
 cudaError_t launch_prefill(const GemmArgs& a, const PrefillPlan& p) {
-    if (a.G == 64) return a.out_f32 ? launch_prefill_g<64, true>(a, p) : launch_prefill_g<64, false>(a, p);
-    return a.out_f32 ? launch_prefill_g<128, true>(a, p) : launch_prefill_g<128, false>(a, p);
+    return a.G == 64 ? launch_prefill_e<64>(a, p) : launch_prefill_e<128>(a, p);
 }
 
 }  // namespace w4a16

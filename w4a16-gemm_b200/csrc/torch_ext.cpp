@@ -390,6 +390,140 @@ int64_t cache_page_bytes_py(int64_t page_size, int64_t head_dim, int64_t group_s
     return (int64_t)bytes;
 }
 
+// ------------------------------------------------------------------ around a decoder layer's products
+torch::Tensor linear_py(torch::Tensor Wp, torch::Tensor x, torch::Tensor scales, c10::optional<torch::Tensor> bias,
+                        int64_t activation, bool gated, c10::optional<torch::Tensor> residual, c10::optional<torch::Tensor> out,
+                        int64_t variant, c10::optional<torch::Tensor> workspace, bool weights_resident, bool fp32_scale) {
+    check_tensors(Wp, x, scales);
+    const int32_t v = clamp_variant(variant);
+    const int64_t M = x.size(0), N = scales.size(1), cols = gated ? N / 2 : N;
+    check(w4a16_validate(Wp.data_ptr(), x.data_ptr(), scales.data_ptr(), M, N, x.size(1), scales.size(0), Wp.numel(), v));
+    auto on_device = [&](const torch::Tensor& t) { return t.is_cuda() && t.device() == x.device() && t.dtype() == torch::kHalf && t.is_contiguous(); };
+    w4a16_epilogue e = {};
+    if (bias.has_value()) {
+        TORCH_CHECK(on_device(*bias) && bias->dim() == 1 && bias->size(0) == N, "bias must be a contiguous fp16 [N] tensor on x's device");
+        e.bias = bias->data_ptr();
+    }
+    if (residual.has_value()) {
+        TORCH_CHECK(on_device(*residual) && residual->dim() == 2 && residual->size(0) == M && residual->size(1) == cols,
+                    "residual must be a contiguous fp16 [M, ", cols, "] tensor on x's device");
+        e.residual = residual->data_ptr();
+    }
+    e.activation = (int32_t)activation;
+    e.gated = gated;
+    const at::cuda::CUDAGuard guard(x.device());
+    torch::Tensor y;
+    if (out.has_value()) {
+        y = *out;
+        TORCH_CHECK(on_device(y) && y.dim() == 2 && y.size(0) == M && y.size(1) == cols,
+                    "out must be a contiguous fp16 [M, ", cols, "] tensor on x's device");
+    } else {
+        y = fresh({M, cols}, torch::kHalf, x);
+    }
+    cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
+    uint64_t ws_bytes = 0;
+    torch::Tensor ws;
+    if (workspace.has_value()) {
+        ws = *workspace;
+        TORCH_CHECK(ws.is_cuda() && ws.device() == x.device() && ws.is_contiguous(),
+                    "workspace must be a contiguous CUDA tensor on x's device");
+        ws_bytes = (uint64_t)ws.numel() * ws.element_size();
+    } else {
+        check(w4a16_workspace_bytes(M, N, x.size(1), scales.size(0), v, &ws_bytes));
+        ws = workspace_for(x, ws_bytes, stream);
+    }
+    check(w4a16_linear(Wp.data_ptr<int32_t>(), x.data_ptr(), scales.data_ptr(), y.data_ptr(), M, N, x.size(1), scales.size(0),
+                       Wp.numel(), &e, v,
+                       (weights_resident ? (uint32_t)W4A16_FLAG_WEIGHTS_RESIDENT : 0u) | (fp32_scale ? (uint32_t)W4A16_FLAG_FP32_SCALE : 0u),
+                       ws.defined() ? ws.data_ptr() : nullptr, ws_bytes, stream));
+    return y;
+}
+
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rms_norm_py(torch::Tensor x, torch::Tensor weight, double eps,
+                                                                    c10::optional<torch::Tensor> residual,
+                                                                    c10::optional<torch::Tensor> out,
+                                                                    c10::optional<torch::Tensor> residual_out) {
+    TORCH_CHECK(x.is_cuda() && x.dim() >= 1 && x.dim() <= 3, "x must be a CUDA tensor of one to three dimensions");
+    const int64_t rank = x.dim(), dim = x.size(rank - 1);
+    w4a16_norm_args a = {};
+    a.dtype = act_dtype(x.scalar_type(), "x");
+    TORCH_CHECK(weight.is_cuda() && weight.device() == x.device() && weight.scalar_type() == x.scalar_type() && weight.dim() == 1 &&
+                    weight.size(0) == dim && weight.is_contiguous(),
+                "weight must be a contiguous [", dim, "] tensor of x's dtype and device");
+    TORCH_CHECK(dim <= INT_MAX && (rank < 3 || x.size(1) <= INT_MAX), "dimensions must fit in int32");
+    TORCH_CHECK(residual.has_value() || !residual_out.has_value(), "residual_out needs a residual");
+    auto like_x = [&](const torch::Tensor& t, const char* what) {
+        TORCH_CHECK(t.is_cuda() && t.device() == x.device() && t.sizes() == x.sizes(), what, " must be a CUDA tensor of x's shape on x's device");
+        TORCH_CHECK(dim == 1 || t.stride(rank - 1) == 1, what, "'s last dimension must be contiguous");
+    };
+    // strides count where there is something to stride over
+    auto token_stride = [&](const torch::Tensor& t) { return rank >= 2 && x.size(0) > 1 ? t.stride(0) : 0; };
+    auto head_stride = [&](const torch::Tensor& t) { return rank == 3 && x.size(1) > 1 ? t.stride(1) : 0; };
+    like_x(x, "x");
+    const at::cuda::CUDAGuard guard(x.device());
+    torch::Tensor y, h;
+    if (out.has_value()) {
+        y = *out;
+        like_x(y, "out");
+        TORCH_CHECK(y.scalar_type() == x.scalar_type(), "out must have x's dtype");
+    } else {
+        y = fresh(x.sizes(), x.scalar_type(), x);
+    }
+    if (residual.has_value()) {
+        const torch::Tensor& r = *residual;
+        like_x(r, "residual");
+        TORCH_CHECK(r.scalar_type() == x.scalar_type() || r.scalar_type() == torch::kFloat, "residual must be of x's dtype or fp32");
+        if (residual_out.has_value()) {
+            h = *residual_out;
+            like_x(h, "residual_out");
+            TORCH_CHECK(h.scalar_type() == r.scalar_type(), "residual_out must have the residual's dtype");
+        } else {
+            h = fresh(x.sizes(), r.scalar_type(), x);
+        }
+        a.residual = r.data_ptr();
+        a.residual_out = h.data_ptr();
+        a.residual_f32 = r.scalar_type() == torch::kFloat;
+        a.residual_token_stride = token_stride(r);
+        a.residual_head_stride = head_stride(r);
+        a.residual_out_token_stride = token_stride(h);
+        a.residual_out_head_stride = head_stride(h);
+    }
+    a.x = x.data_ptr();
+    a.weight = weight.data_ptr();
+    a.y = y.data_ptr();
+    a.x_token_stride = token_stride(x);
+    a.x_head_stride = head_stride(x);
+    a.y_token_stride = token_stride(y);
+    a.y_head_stride = head_stride(y);
+    a.tokens = rank >= 2 ? x.size(0) : 1;
+    a.heads = rank == 3 ? (int32_t)x.size(1) : 1;
+    a.dim = (int32_t)dim;
+    a.eps = (float)eps;
+    if (rank == 3 && x.size(1) == 0) {       // no rows
+        a.tokens = 0;
+        a.heads = 1;
+    }
+    check(w4a16_rms_norm(&a, at::cuda::getCurrentCUDAStream().stream()));
+    return {y, residual.has_value() ? c10::optional<torch::Tensor>(h) : c10::nullopt};
+}
+
+std::tuple<torch::Tensor, torch::Tensor> moe_route_py(torch::Tensor logits, int64_t k, bool renormalize) {
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, "logits must be a CUDA [tokens, experts] tensor");
+    const auto type = logits.scalar_type();
+    TORCH_CHECK(type == torch::kHalf || type == torch::kBFloat16 || type == torch::kFloat, "logits must be fp16, bf16 or fp32");
+    TORCH_CHECK(logits.size(1) < 2 || logits.stride(1) == 1, "logits' last dimension must be contiguous");
+    TORCH_CHECK(logits.size(1) >= 1 && logits.size(1) <= INT_MAX && k >= 1 && k <= logits.size(1), "k must be in [1, experts]");
+    const at::cuda::CUDAGuard guard(logits.device());
+    auto weights = fresh({logits.size(0), k}, torch::kFloat, logits);
+    auto experts = fresh({logits.size(0), k}, torch::kInt32, logits);
+    check(w4a16_moe_route(logits.data_ptr(),
+                          type == torch::kFloat ? W4A16_LOGITS_F32 : type == torch::kHalf ? W4A16_LOGITS_F16 : W4A16_LOGITS_BF16,
+                          logits.size(0) > 1 ? logits.stride(0) : 0, logits.size(0), (int32_t)logits.size(1), (int32_t)k,
+                          renormalize, weights.data_ptr<float>(), experts.data_ptr<int32_t>(),
+                          at::cuda::getCurrentCUDAStream().stream()));
+    return {weights, experts};
+}
+
 int64_t device_status_py(bool reset) {
     int32_t code = 0;
     w4a16_status s = w4a16_device_status(&code, reset ? 1 : 0);
@@ -421,5 +555,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("cache_append", &cache_append_py, "quantise keys and values into a 4-bit cache, with rotary positions");
     m.def("cache_read", &cache_read_py, "read slots of a 4-bit cache back");
     m.def("cache_attention", &cache_attention_py, "attention over a 4-bit cache");
+    m.def("linear", &linear_py, "W4A16 GEMM with bias, activation, gate and residual");
+    m.def("rms_norm", &rms_norm_py, "root-mean-square norm, with the residual's addition");
+    m.def("moe_route", &moe_route_py, "softmax over experts, the k largest");
     m.attr("ABI_VERSION") = w4a16_abi_version();
 }

@@ -25,6 +25,7 @@ STATUS_NAMES = {
     11: "W4A16_ERR_DECODE_SHAPE", 12: "W4A16_ERR_OUT_DTYPE", 13: "W4A16_ERR_DEVICE", 14: "W4A16_ERR_CUDA",
     15: "W4A16_ERR_DEVICE_TIMEOUT", 16: "W4A16_ERR_WORKSPACE", 17: "W4A16_ERR_FLAGS", 18: "W4A16_ERR_TP_GROUP",
     19: "W4A16_ERR_CACHE", 20: "W4A16_ERR_ACT_DTYPE",
+    21: "W4A16_ERR_ACTIVATION", 22: "W4A16_ERR_OVERLAP", 23: "W4A16_ERR_NORM", 24: "W4A16_ERR_MOE",
 }
 TP_MAX_RANKS = 8
 TP_CTRL_BYTES = 8192
@@ -70,6 +71,19 @@ class CacheAttentionArgs(ctypes.Structure):
                 ("max_q", _i32), ("causal", _i32), ("window", _i32)]
 
 
+class Epilogue(ctypes.Structure):
+    """w4a16_epilogue: what w4a16_linear does with a product's sums."""
+    _fields_ = [("bias", _vp), ("residual", _vp), ("activation", _i32), ("gated", _i32)]
+
+
+class NormArgs(ctypes.Structure):
+    """w4a16_norm_args: one w4a16_rms_norm call."""
+    _fields_ = [("x", _vp), ("weight", _vp), ("residual", _vp), ("y", _vp), ("residual_out", _vp)] + \
+               [(f"{name}_{axis}_stride", _i64) for name in ("x", "residual", "y", "residual_out") for axis in ("token", "head")] + \
+               [("tokens", _i64), ("heads", _i32), ("dim", _i32), ("dtype", _i32), ("residual_f32", _i32),
+                ("eps", ctypes.c_float)]
+
+
 # name -> (restype, argtypes), one entry per declaration in include/w4a16.h
 EXPORTS = {
     "w4a16_abi_version": (_i32, []),
@@ -97,6 +111,10 @@ EXPORTS = {
     "w4a16_cache_attention": (_i32, [ctypes.POINTER(Cache), ctypes.POINTER(CacheAttentionArgs), _vp, _u64, _vp]),
     "w4a16_cache_attention_workspace": (_i32, [ctypes.POINTER(Cache), ctypes.POINTER(CacheAttentionArgs),
                                                ctypes.POINTER(_u64)]),
+    "w4a16_linear": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(Epilogue), _i32,
+                            ctypes.c_uint32, _vp, _u64, _vp]),
+    "w4a16_rms_norm": (_i32, [ctypes.POINTER(NormArgs), _vp]),
+    "w4a16_moe_route": (_i32, [_vp, _i32, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp]),
     "w4a16_device_status": (_i32, [ctypes.POINTER(_i32), _i32]),
     "w4a16_check_wait_limits": (_i32, [ctypes.POINTER(_i32)]),
     "w4a16_status_string": (ctypes.c_char_p, [_i32]),
