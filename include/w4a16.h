@@ -444,6 +444,34 @@ typedef enum w4a16_logits_dtype {
 w4a16_status w4a16_moe_route(const void* logits, int32_t dtype, int64_t row_stride, int64_t tokens, int32_t num_experts,
                              int32_t k, int32_t renormalize, float* weights, int32_t* experts, void* stream);
 
+typedef struct w4a16_moe_args {
+    const void* x;                   /* fp16 [tokens][hidden], dense */
+    const int32_t* gate_up_wp;       /* [num_experts][2 * inner * hidden / 8]: each expert's packed W [2 * inner, hidden], rows gated */
+    const void* gate_up_scales;      /* fp16 [num_experts][hidden / gate_up_group][2 * inner] */
+    const int32_t* down_wp;          /* [num_experts][hidden * inner / 8]: packed W [hidden, inner] */
+    const void* down_scales;         /* fp16 [num_experts][inner / down_group][hidden] */
+    const int32_t* experts;          /* [tokens][k]; an expert outside [0, num_experts) adds nothing */
+    const float* weights;            /* [tokens][k] */
+    const void* residual;            /* fp16 [tokens][hidden] or NULL; may be y */
+    void* y;                         /* fp16 [tokens][hidden]; may be x */
+    int64_t tokens;
+    int32_t num_experts;             /* 1 .. 1024 */
+    int32_t k;                       /* choices of a token, 1 .. 32; the same expert twice counts twice */
+    int32_t hidden, inner;           /* multiples of 64 and of their group size */
+    int32_t gate_up_group, down_group;   /* 64 or 128 */
+    int32_t activation;              /* w4a16_activation, of the gate */
+} w4a16_moe_args;
+
+/* A mixture-of-experts layer: with e = experts[t][j],
+ *     h_tj = act(x_t Wg_e^T) * (x_t Wu_e^T),   y_t = residual_t + sum_j weights[t][j] (h_tj Wd_e^T).
+ * Rows of the gated weights alternate as in w4a16_epilogue; a weight is (q - 8) * scale.  Sums are fp32; h is
+ * rounded to fp16, y once.  Pointers are 16-byte aligned (experts and weights 4-byte).  The workspace is scratch, 256-byte
+ * aligned, one per concurrent call. */
+w4a16_status w4a16_moe_experts(const w4a16_moe_args* args, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of a call with these sizes (pointers in args are not read). */
+w4a16_status w4a16_moe_workspace(const w4a16_moe_args* args, uint64_t* bytes);
+
 /* Reads the current device's status word, set by a kernel whose bounded wait
  * ran out (0 = none).  Synchronises the device.  reset != 0 clears it. */
 w4a16_status w4a16_device_status(int32_t* code, int32_t reset);
@@ -453,8 +481,8 @@ w4a16_status w4a16_device_status(int32_t* code, int32_t reset);
  * kernels use.  Each wait gives up after its limit (about 2 s), records its code in the
  * device status word (4, then 1) and returns; codes[0..1] receive the status word read after
  * each kernel, which is then cleared.  A third kernel does the same for the cache kernels' wait and their
- * part of the status word (8); the call fails if that does not come back.  Synchronises the
- * device; takes about 6 s. */
+ * part of the status word (8), a fourth for the expert layer's (9); the call fails if those do not come back.
+ * Synchronises the device; takes about 8 s. */
 w4a16_status w4a16_check_wait_limits(int32_t* codes);
 
 /* Short name of a status code. */

@@ -30,7 +30,7 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3"]
 
-LIB_SOURCES = ["kernels.cu", "cache.cu", "layer.cu", "capi.cpp"]
+LIB_SOURCES = ["kernels.cu", "cache.cu", "layer.cu", "moe.cu", "capi.cpp"]
 LIB_PATH = os.path.join(OUT_DIR, "libw4a16.so")
 EXT_PATH = os.path.join(OUT_DIR, "_C" + sysconfig.get_config_var("EXT_SUFFIX"))
 

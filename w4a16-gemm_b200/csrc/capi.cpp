@@ -14,6 +14,7 @@
 
 #include "../../include/w4a16.h"
 #include "internal.h"
+#include "moe_plan.h"
 
 namespace {
 
@@ -760,6 +761,76 @@ w4a16_status w4a16_moe_route(const void* logits, int32_t dtype, int64_t row_stri
     return err == cudaSuccess ? ok() : cuda_fail(err);
 }
 
+// ------------------------------------------------------------------ expert layer
+namespace {
+
+// Everything of a call but its pointers.
+w4a16_status check_moe_sizes(const w4a16_moe_args* args) {
+    if (!args) return fail(W4A16_ERR_NULL_POINTER, "args must be non-null");
+    const w4a16_moe_args& a = *args;
+    if (a.num_experts < 1 || a.num_experts > w4a16::kMoeMaxExperts)
+        return fail(W4A16_ERR_MOE, "num_experts must be in [1, " + std::to_string(w4a16::kMoeMaxExperts) + "]");
+    if (a.k < 1 || a.k > w4a16::kRouteMaxK) return fail(W4A16_ERR_MOE, "k must be in [1, " + std::to_string(w4a16::kRouteMaxK) + "]");
+    if (a.hidden < 64 || a.inner < 64 || a.hidden % 64 || a.inner % 64)
+        return fail(W4A16_ERR_K_MULTIPLE, "hidden and inner must be multiples of 64");
+    if ((a.gate_up_group != 64 && a.gate_up_group != 128) || (a.down_group != 64 && a.down_group != 128))
+        return fail(W4A16_ERR_GROUP_SIZE, "unsupported group size, supported: 64, 128");
+    if (a.hidden % a.gate_up_group || a.inner % a.down_group)
+        return fail(W4A16_ERR_GROUPS, "hidden and inner must be multiples of their group sizes");
+    if (a.hidden > (1 << 20) || a.inner > (1 << 20)) return fail(W4A16_ERR_DIM_RANGE, "hidden and inner must be at most 2^20");
+    w4a16_status s = check_activation(a.activation);
+    if (s != W4A16_OK) return s;
+    // work items: a tile for each entry at most, its column blocks, up to four ranges of K
+    const int64_t blocks = (a.inner / 8 > a.hidden / 4) ? a.inner / 8 : a.hidden / 4;
+    if (!product_fits_int32(a.tokens, a.k) || a.tokens * a.k * blocks >= (1LL << 31))
+        return fail(W4A16_ERR_DIM_RANGE, "tokens * k * max(inner / 8, hidden / 4) must be below 2^31");
+    return ok();
+}
+
+}  // namespace
+
+w4a16_status w4a16_moe_workspace(const w4a16_moe_args* args, uint64_t* bytes) {
+    w4a16_status s = check_moe_sizes(args);
+    if (s != W4A16_OK) return s;
+    if (!bytes) return fail(W4A16_ERR_NULL_POINTER, "bytes must be non-null");
+    *bytes = 0;
+    if (args->tokens == 0) return ok();
+    w4a16::DeviceInfo d;
+    if ((s = check_device(&d)) != W4A16_OK) return s;
+    *bytes = w4a16::moe_workspace(*args, d);
+    return ok();
+}
+
+w4a16_status w4a16_moe_experts(const w4a16_moe_args* args, void* workspace, uint64_t workspace_bytes, void* stream) {
+    w4a16_status s = check_moe_sizes(args);
+    if (s != W4A16_OK) return s;
+    const w4a16_moe_args& a = *args;
+    if (a.tokens == 0) return ok();
+    if (!a.x || !a.gate_up_wp || !a.gate_up_scales || !a.down_wp || !a.down_scales || !a.experts || !a.weights || !a.y)
+        return fail(W4A16_ERR_NULL_POINTER, "x, both products' words and scales, experts, weights and y must be non-null");
+    if (!aligned16(a.x) || !aligned16(a.gate_up_wp) || !aligned16(a.gate_up_scales) || !aligned16(a.down_wp) ||
+        !aligned16(a.down_scales) || !aligned16(a.residual) || !aligned16(a.y) || reinterpret_cast<uintptr_t>(a.experts) % 4 ||
+        reinterpret_cast<uintptr_t>(a.weights) % 4)
+        return fail(W4A16_ERR_ALIGNMENT, "x, words, scales, residual and y must be 16-byte aligned, experts and weights 4-byte");
+    const uint64_t row_bytes = (uint64_t)a.tokens * (uint64_t)a.hidden * 2, entry_bytes = (uint64_t)a.tokens * (uint64_t)a.k * 4;
+    const uint64_t values = (uint64_t)a.num_experts * (uint64_t)a.hidden * (uint64_t)a.inner;
+    if ((a.y != a.x && overlap(a.y, row_bytes, a.x, row_bytes)) || (a.y != a.residual && overlap(a.y, row_bytes, a.residual, row_bytes)) ||
+        overlap(a.y, row_bytes, a.experts, entry_bytes) || overlap(a.y, row_bytes, a.weights, entry_bytes) ||
+        overlap(a.y, row_bytes, a.gate_up_wp, values) || overlap(a.y, row_bytes, a.down_wp, values / 2) ||
+        overlap(a.y, row_bytes, a.gate_up_scales, values * 4 / (uint64_t)a.gate_up_group) ||
+        overlap(a.y, row_bytes, a.down_scales, values * 2 / (uint64_t)a.down_group))
+        return fail(W4A16_ERR_OVERLAP, "y must be x or the residual itself or apart from every input");
+    w4a16::DeviceInfo d;
+    if ((s = check_device(&d)) != W4A16_OK) return s;
+    const size_t need = w4a16::moe_workspace(a, d);
+    if (!workspace) return fail(W4A16_ERR_WORKSPACE, "this call needs a workspace of " + std::to_string(need) + " bytes");
+    if (workspace_bytes < need)
+        return fail(W4A16_ERR_WORKSPACE, "workspace too small: " + std::to_string(workspace_bytes) + " < " + std::to_string(need) + " bytes");
+    if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(W4A16_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+    const cudaError_t err = w4a16::launch_moe_experts(a, d, workspace, static_cast<cudaStream_t>(stream), pdl_enabled());
+    return err == cudaSuccess ? ok() : cuda_fail(err);
+}
+
 w4a16_status w4a16_device_status(int32_t* code, int32_t reset) {
     if (!code) return fail(W4A16_ERR_NULL_POINTER, "code must be non-null");
     int c = 0;
@@ -788,6 +859,11 @@ w4a16_status w4a16_check_wait_limits(int32_t* codes) {
     if (err != cudaSuccess) return fail(W4A16_ERR_CUDA, std::string("CUDA error: ") + cudaGetErrorString(err));
     if (c != 8)
         return fail(W4A16_ERR_DEVICE_TIMEOUT, "a wait of the cache kernels ran out and the device status was " + std::to_string(c) + ", not 8");
+    err = w4a16::run_moe_wait_limit_check();
+    if (err == cudaSuccess) err = w4a16::read_device_status(&c, true);
+    if (err != cudaSuccess) return fail(W4A16_ERR_CUDA, std::string("CUDA error: ") + cudaGetErrorString(err));
+    if (c != 9)
+        return fail(W4A16_ERR_DEVICE_TIMEOUT, "a wait of the expert layer ran out and the device status was " + std::to_string(c) + ", not 9");
     return ok();
 }
 

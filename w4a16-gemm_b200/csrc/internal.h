@@ -146,6 +146,13 @@ cudaError_t launch_moe_route(const void* logits, int32_t dtype, int64_t row_stri
 constexpr int kNormMaxDim = 32768;
 constexpr int kRouteMaxExperts = 1024, kRouteMaxK = 32;
 
+// ---------------------------------------------------------------- expert layer (moe.cu)
+size_t moe_workspace(const w4a16_moe_args& a, const DeviceInfo& dev);
+// One validated call (tokens > 0).
+cudaError_t launch_moe_experts(const w4a16_moe_args& a, const DeviceInfo& dev, void* workspace, cudaStream_t stream, bool pdl);
+cudaError_t read_moe_device_status(int* code, bool reset);
+cudaError_t run_moe_wait_limit_check();
+
 // ---------------------------------------------------------------- debug dequant
 cudaError_t launch_dequant(const void* wp, const void* scales, void* out, int N, int K, int G,
                            cudaStream_t stream);

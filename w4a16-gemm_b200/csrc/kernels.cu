@@ -67,14 +67,16 @@ cudaError_t ensure_max_dynamic_smem(const void* func) {
 cudaError_t read_device_status(int* code, bool reset) {
     cudaError_t err = cudaDeviceSynchronize();
     if (err != cudaSuccess) return err;
-    int cache_code = 0;
+    int cache_code = 0, moe_code = 0;
     if ((err = read_cache_device_status(&cache_code, reset)) != cudaSuccess) return err;
+    if ((err = read_moe_device_status(&moe_code, reset)) != cudaSuccess) return err;
     err = cudaMemcpyFromSymbol(code, w4a16_device_status, sizeof(int));
     if (err == cudaSuccess && reset) {
         const int zero = 0;
         err = cudaMemcpyToSymbol(w4a16_device_status, &zero, sizeof(int));
     }
     if (*code == 0) *code = cache_code;
+    if (*code == 0) *code = moe_code;
     return err;
 }
 

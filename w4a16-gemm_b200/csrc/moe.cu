@@ -1,0 +1,69 @@
+// Device code of the expert layer.
+#include <cuda_runtime.h>
+
+#include "internal.h"
+#include "launch.cuh"
+#include "moe_experts.cuh"
+
+namespace w4a16 {
+
+cudaError_t read_moe_device_status(int* code, bool reset) {
+    cudaError_t err = cudaMemcpyFromSymbol(code, w4a16_device_status, sizeof(int));
+    if (err != cudaSuccess || !reset) return err;
+    const int zero = 0;
+    return cudaMemcpyToSymbol(w4a16_device_status, &zero, sizeof(int));
+}
+
+cudaError_t run_moe_wait_limit_check() {
+    wait_limit_kernel<<<1, 32>>>(1, kDevTimeoutExperts);
+    const cudaError_t err = cudaGetLastError();
+    return err != cudaSuccess ? err : cudaDeviceSynchronize();
+}
+
+size_t moe_workspace(const w4a16_moe_args& a, const DeviceInfo& dev) {
+    return moe_plan(a.tokens, a.k, a.num_experts, a.hidden, a.inner, dev.num_sms).bytes;
+}
+
+template <int G, int MT, bool GATED>
+static cudaError_t launch_product_t(const MoeParams& p, int grid, cudaStream_t stream, bool pdl) {
+    auto kern = moe_product_kernel<G, MT, GATED>;
+    const cudaError_t err = ensure_max_dynamic_smem(reinterpret_cast<const void*>(kern));
+    if (err != cudaSuccess) return err;
+    return launch(kern, dim3(grid), kMoeThreads, MoeCfg<MT>::SMEM, stream, pdl, p);
+}
+
+template <bool GATED>
+static cudaError_t launch_product(const MoeParams& p, int G, int grid, cudaStream_t stream, bool pdl) {
+    if (p.plan.rows == 8)
+        return G == 64 ? launch_product_t<64, 1, GATED>(p, grid, stream, pdl) : launch_product_t<128, 1, GATED>(p, grid, stream, pdl);
+    return G == 64 ? launch_product_t<64, 2, GATED>(p, grid, stream, pdl) : launch_product_t<128, 2, GATED>(p, grid, stream, pdl);
+}
+
+cudaError_t launch_moe_experts(const w4a16_moe_args& a, const DeviceInfo& dev, void* workspace, cudaStream_t stream, bool pdl) {
+    MoeParams p = {};
+    p.x = static_cast<const __half*>(a.x);
+    p.words[0] = a.gate_up_wp;
+    p.words[1] = a.down_wp;
+    p.scales[0] = static_cast<const __half*>(a.gate_up_scales);
+    p.scales[1] = static_cast<const __half*>(a.down_scales);
+    p.experts = a.experts;
+    p.weights = a.weights;
+    p.residual = static_cast<const __half*>(a.residual);
+    p.y = static_cast<__half*>(a.y);
+    p.workspace = static_cast<char*>(workspace);
+    p.plan = moe_plan(a.tokens, a.k, a.num_experts, a.hidden, a.inner, dev.num_sms);
+    p.entries = (int32_t)(a.tokens * a.k);
+    p.k = a.k;
+    p.num_experts = a.num_experts;
+    p.hidden = a.hidden;
+    p.inner = a.inner;
+    p.activation = a.activation;
+    cudaError_t err = launch(moe_plan_kernel, dim3(1), kMoePlanThreads, 0, stream, pdl, p);
+    if (err == cudaSuccess) err = launch_product<true>(p, a.gate_up_group, dev.num_sms, stream, pdl);
+    if (err == cudaSuccess) err = launch_product<false>(p, a.down_group, dev.num_sms, stream, pdl);
+    if (err != cudaSuccess) return err;
+    const int cols = 4 * kMoeFinishThreads;
+    return launch(moe_finish_kernel, dim3((unsigned)a.tokens, (unsigned)((a.hidden + cols - 1) / cols)), kMoeFinishThreads, 0, stream, pdl, p);
+}
+
+}  // namespace w4a16

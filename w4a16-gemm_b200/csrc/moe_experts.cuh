@@ -1,0 +1,366 @@
+// A mixture-of-experts layer from 4-bit experts:
+//
+//     h_tj = act(x_t Wg_e^T) * (x_t Wu_e^T),   e = experts[t][j]
+//     y_t  = residual_t + sum_j weights[t][j] (h_tj Wd_e^T)
+//
+// Four kernels, each launched behind the one before with programmatic dependent launch: the plan (entries
+// sorted by expert, tiles), the gated product, the second product, the weighted sum.  The products
+// stream the weights of the experts that were chosen, each once a tile.
+//
+// One CTA an SM takes a range of the (tile, n16 block of output channels) sequence and walks it in batches
+// of up to 8 blocks of one tile.  A batch runs over K in stages of 8 chunks of 64: one warp issues all of a
+// stage as bulk copies (a block's 8 chunks are one run of 4 KB; the chunks' scales; 1 KB of each of
+// the tile's rows) onto one mbarrier.  16 consumer warps: warp w takes chunk w % 8 of the stage for half of
+// the batch's blocks, so that K is summed over 8 warps, through shared memory, once a batch: sums are
+// whole where they are made, and the gate needs no second pass.
+//
+// The weights enter mma.m16n8k16 as the integers q - 8 (exact in fp16) and a chunk's sums are multiplied by its
+// scale in fp32: the weight (q - 8) * s is never rounded.  The gated product's results are rounded to fp16 once, being
+// operands of the second product; its results stay fp32 until the weighted sum.
+#pragma once
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "dequant.cuh"
+#include "epilogue.cuh"
+#include "internal.h"
+#include "moe_plan.h"
+#include "ptx.cuh"
+
+namespace w4a16 {
+
+constexpr int kMoeConsumers = 16;                         // warps: 8 chunks x 2 halves of the blocks
+constexpr int kMoeThreads = (kMoeConsumers + 1) * 32;
+constexpr int kMoeHalf = kMoeBlocks / 2;                  // blocks of a consumer warp
+constexpr int kMoePlanThreads = 1024;
+
+template <int MT>
+struct MoeCfg {
+    static constexpr int ROWS = 8 * MT;
+    static constexpr int X_PITCH = kMoeChunks * 128 + 16;             // rows 16 bytes apart in banks: ldmatrix without conflicts
+    static constexpr int W_BYTES = kMoeBlocks * kMoeChunks * 512;     // [block][chunk][32 lanes x 16 B]
+    static constexpr int X_BYTES = ROWS * X_PITCH;
+    static constexpr int S_ROW = kMoeBlocks * 32;                     // scales of one group of K: [block][16]
+    static constexpr int S_BYTES = kMoeChunks * S_ROW;
+    static constexpr int STAGE = W_BYTES + X_BYTES + S_BYTES;
+    static constexpr int STAGES = MT == 1 ? 4 : 3;
+    static constexpr int RED_BYTES = kMoeBlocks * kMoeChunks * MT * 512;   // [block][chunk warp][mt][lane] float4
+    static constexpr int BARS = STAGES * STAGE + RED_BYTES;
+    static constexpr int SMEM = 128 + BARS + 2 * STAGES * 8;
+    static_assert(STAGE % 16 == 0 && SMEM <= 227 * 1024, "shared memory");
+};
+
+struct MoeParams {
+    const __half* x;             // [tokens][hidden]
+    const int32_t* words[2];     // of the two products: [experts][n * k / 8]
+    const __half* scales[2];     // [experts][k / G][n]
+    const int32_t* experts;      // [tokens][k]
+    const float* weights;        // [tokens][k]
+    const __half* residual;      // [tokens][hidden] or NULL
+    __half* y;
+    char* workspace;
+    MoePlan plan;
+    int32_t entries, k, num_experts, hidden, inner, activation;
+};
+
+__device__ __forceinline__ MoeHead* moe_head(const MoeParams& p) { return reinterpret_cast<MoeHead*>(p.workspace); }
+__device__ __forceinline__ int4* moe_tiles(const MoeParams& p) { return reinterpret_cast<int4*>(p.workspace + p.plan.tiles_at); }
+__device__ __forceinline__ int32_t* moe_order(const MoeParams& p) { return reinterpret_cast<int32_t*>(p.workspace + p.plan.order_at); }
+__device__ __forceinline__ __half* moe_inner(const MoeParams& p) { return reinterpret_cast<__half*>(p.workspace + p.plan.inner_at); }
+__device__ __forceinline__ float* moe_out(const MoeParams& p) { return reinterpret_cast<float*>(p.workspace + p.plan.out_at); }
+
+// Inclusive sum over the CTA's threads, in their order.
+__device__ __forceinline__ int scan_threads(int v, int* shared) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+    }
+    if (lane == 31) shared[warp] = v;
+    __syncthreads();
+    if (warp == 0) {
+        int w = shared[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += u;
+        }
+        shared[lane] = w;
+    }
+    __syncthreads();
+    if (warp > 0) v += shared[warp - 1];
+    __syncthreads();
+    return v;
+}
+
+// One CTA: counts the experts' entries, lays their tiles out, sorts the entries.  The order of one expert's entries is
+// the order in which they arrive; no result depends on it, since every entry's row is summed by itself.
+static __global__ void __launch_bounds__(kMoePlanThreads) moe_plan_kernel(const __grid_constant__ MoeParams p) {
+    __shared__ int count[kMoeMaxExperts], cursor[kMoeMaxExperts], warps[32];
+    const int t = threadIdx.x;
+    pdl_launch_dependents();
+    count[t] = 0;
+    pdl_wait();
+    __syncthreads();
+    for (int i = t; i < p.entries; i += kMoePlanThreads) {
+        const int e = __ldg(p.experts + i);
+        if (e >= 0 && e < p.num_experts) atomicAdd(&count[e], 1);
+    }
+    __syncthreads();
+    const int mine = count[t], rows = p.plan.rows, tiles = (mine + rows - 1) / rows;
+    const int end = scan_threads(mine, warps), tile_end = scan_threads(tiles, warps);
+    cursor[t] = end - mine;
+    int4* const out = moe_tiles(p) + (tile_end - tiles);
+    for (int i = 0; i < tiles; ++i) out[i] = make_int4(t, end - mine + i * rows, min(rows, mine - i * rows), 0);
+    if (t == kMoePlanThreads - 1) {
+        moe_head(p)->tiles = tile_end;
+        moe_head(p)->entries = end;
+    }
+    __syncthreads();
+    int32_t* const order = moe_order(p);
+    for (int i = t; i < p.entries; i += kMoePlanThreads) {
+        const int e = __ldg(p.experts + i);
+        if (e >= 0 && e < p.num_experts) order[atomicAdd(&cursor[e], 1)] = i;
+    }
+}
+
+// Untiled bulk copy into this CTA's shared memory (16-byte aligned addresses and size).
+__device__ __forceinline__ void moe_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// A CTA's walk: batches of up to 8 blocks of one (tile, K range), over its range of units.  Unit u is block u % blocks
+// of K range u / blocks % splits of tile u / blocks / splits.
+struct MoeWalk {
+    int unit, end, blocks, splits;
+    int tile, split, block, n;         // of the current batch
+    __device__ __forceinline__ bool next() {
+        unit += n;
+        if (unit >= end) return false;
+        const int line = unit / blocks;
+        block = unit - line * blocks;
+        tile = line / splits;
+        split = line - tile * splits;
+        n = min(min(kMoeBlocks, blocks - block), end - unit);
+        return true;
+    }
+};
+
+// GATED: the first product (rows of x, gated, into the workspace in sorted order); else the second (rows of the
+// first's results, into the workspace by entry and K range).
+template <int G, int MT, bool GATED>
+static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(const __grid_constant__ MoeParams p) {
+    using C = MoeCfg<MT>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 127u) & ~127u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto stage = [&](int s) { return base + (uint32_t)(s * C::STAGE); };
+    auto full = [&](int s) { return base + (uint32_t)(C::BARS + s * 8); };
+    auto empty = [&](int s) { return base + (uint32_t)(C::BARS + (C::STAGES + s) * 8); };
+    const uint32_t red = base + C::STAGES * C::STAGE;
+
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), kMoeConsumers);
+        }
+        fence_mbar_init();
+    }
+    __syncthreads();
+    pdl_wait();
+
+    const int K = GATED ? p.hidden : p.inner, N = GATED ? 2 * p.inner : p.hidden;
+    const int chunks = K >> 6, all_stages = (chunks + kMoeChunks - 1) / kMoeChunks;
+    MoeWalk walk;
+    walk.blocks = N >> 4;
+    walk.splits = GATED ? 1 : p.plan.splits;
+    const long long units = (long long)__ldcg(&moe_head(p)->tiles) * walk.splits * walk.blocks;
+    walk.unit = (int)(units * blockIdx.x / gridDim.x);
+    walk.end = (int)(units * (blockIdx.x + 1) / gridDim.x);
+    walk.n = 0;
+    int it = 0;
+
+    if (warp == kMoeConsumers) {
+        // ------------------------------------------------ producer: one copy a lane
+        // lanes 0-7 the blocks' packed words, 8-15 the groups' scales, 16-31 the tile's rows
+        const int role = lane < 8 ? 0 : lane < 16 ? 1 : 2, which = role == 2 ? lane - 16 : lane & 7;
+        bool ok = true;
+        while (ok && walk.next()) {
+            const int4 tile = __ldcg(moe_tiles(p) + walk.tile);
+            const char* src = nullptr;
+            uint32_t dst = 0, step = 0;
+            int have = 0;
+            if (role == 0) {
+                src = reinterpret_cast<const char*>(p.words[GATED ? 0 : 1]) +
+                      ((int64_t)tile.x * walk.blocks + walk.block + which) * chunks * 512;
+                dst = which * (kMoeChunks * 512);
+                step = 512;
+                have = walk.n;
+            } else if (role == 1) {
+                src = reinterpret_cast<const char*>(p.scales[GATED ? 0 : 1] + (int64_t)tile.x * (K / G) * N + walk.block * 16);
+                dst = C::W_BYTES + C::X_BYTES + which * C::S_ROW;
+            } else {
+                if (which < tile.z) {
+                    const int at = tile.y + which;
+                    src = reinterpret_cast<const char*>(GATED ? p.x + (int64_t)(__ldcg(moe_order(p) + at) / p.k) * K
+                                                              : moe_inner(p) + (int64_t)at * K);
+                }
+                dst = C::W_BYTES + which * C::X_PITCH;
+                step = 128;
+                have = tile.z;
+            }
+            const int s1 = all_stages * (walk.split + 1) / walk.splits;
+            for (int st = all_stages * walk.split / walk.splits; st < s1; ++st, ++it) {
+                const int s = it % C::STAGES, c0 = st * kMoeChunks, n = min(kMoeChunks, chunks - c0);
+                if (it >= C::STAGES) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_sleep(empty(s), (it / C::STAGES - 1) & 1, kDevTimeoutExperts));
+                    if (!ok) break;
+                }
+                const int groups = (n * 64 + G - 1) / G;
+                if (lane == 0)
+                    mbar_arrive_expect_tx(full(s), (uint32_t)(walk.n * n * 512 + tile.z * n * 128 + groups * walk.n * 32));
+                __syncwarp();
+                if (role == 1) {
+                    if (which < groups) moe_copy(stage(s) + dst, src + (int64_t)(c0 * 64 / G + which) * N * 2, walk.n * 32, full(s));
+                } else if (which < have) {
+                    moe_copy(stage(s) + dst, src + (int64_t)c0 * step, n * step, full(s));
+                }
+            }
+        }
+        // copies still in flight must land before the CTA may exit (they have, unless a wait ran out)
+        for (int j = it - 1; j >= 0 && j >= it - C::STAGES; --j) mbar_wait(full(j % C::STAGES), (j / C::STAGES) & 1, kDevTimeoutExperts);
+        return;
+    }
+
+    // ---------------------------------------------------- consumers
+    // After a wait that ran out a warp computes nothing more but keeps every barrier, so that none waits for it.
+    const int chunk = warp & (kMoeChunks - 1), half = warp / kMoeChunks;
+    const int g8 = lane >> 2, t4 = lane & 3;
+    const uint32_t x_lane = C::W_BYTES + (lane & 7) * C::X_PITCH + chunk * 128 + (lane >> 3) * 16;
+    const uint32_t w_lane = (half * kMoeHalf * kMoeChunks + chunk) * 512 + lane * 16;
+    const uint32_t s_lane = C::W_BYTES + C::X_BYTES + (chunk * 64 / G) * C::S_ROW + half * kMoeHalf * 32 + g8 * 2;
+    bool ok = true;
+    while (walk.next()) {
+        float acc[kMoeHalf][MT][4];
+#pragma unroll
+        for (int b = 0; b < kMoeHalf; ++b)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[b][mt][i] = 0.f;
+        const int mine = walk.n - half * kMoeHalf;       // blocks of this warp (may be 0 or less)
+        const int s1 = all_stages * (walk.split + 1) / walk.splits;
+        for (int st = all_stages * walk.split / walk.splits; st < s1; ++st, ++it) {
+            const int s = it % C::STAGES, n = min(kMoeChunks, chunks - st * kMoeChunks);
+            ok = ok && __all_sync(0xffffffffu, mbar_wait_sleep(full(s), (it / C::STAGES) & 1, kDevTimeoutExperts));
+            if (ok && chunk < n && mine > 0) {
+                const uint32_t sb = stage(s);
+                uint32_t b[MT][8];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    ldmatrix_x4(*reinterpret_cast<uint32_t(*)[4]>(&b[mt][0]), sb + x_lane + mt * 8 * C::X_PITCH);
+                    ldmatrix_x4(*reinterpret_cast<uint32_t(*)[4]>(&b[mt][4]), sb + x_lane + mt * 8 * C::X_PITCH + 64);
+                }
+#pragma unroll
+                for (int blk = 0; blk < kMoeHalf; ++blk) {
+                    if (blk >= mine) break;
+                    const uint4 w4 = lds128(sb + w_lane + blk * (kMoeChunks * 512));
+                    const float lo = __half2float(__ushort_as_half(lds_u16(sb + s_lane + blk * 32)));
+                    const float hi = __half2float(__ushort_as_half(lds_u16(sb + s_lane + blk * 32 + 16)));
+                    float c[MT][4];
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+                        uint32_t a[4];
+                        unscaled_word(ks == 0 ? w4.x : ks == 1 ? w4.y : ks == 2 ? w4.z : w4.w, a);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            if (ks == 0) mma_16816_zero(c[mt], a, b[mt][0], b[mt][1]);
+                            else mma_16816(c[mt], a, b[mt][2 * ks], b[mt][2 * ks + 1]);
+                        }
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[blk][mt][i] = fmaf(i < 2 ? lo : hi, c[mt][i], acc[blk][mt][i]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty(s));
+        }
+        // the 8 warps' sums of each block, in their order
+        bar_sync_named(1, kMoeConsumers * 32);           // the last batch's sums have been read
+#pragma unroll
+        for (int blk = 0; blk < kMoeHalf; ++blk)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+                sts128(red + ((((half * kMoeHalf + blk) * kMoeChunks + chunk) * MT + mt) * 32 + lane) * 16,
+                       make_float4(acc[blk][mt][0], acc[blk][mt][1], acc[blk][mt][2], acc[blk][mt][3]));
+        bar_sync_named(2, kMoeConsumers * 32);
+        const int4 tile = __ldcg(moe_tiles(p) + walk.tile);
+        for (int i = warp; i < walk.n * MT; i += kMoeConsumers) {
+            const int blk = i / MT, mt = i % MT;
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < kMoeChunks; ++c) {
+                const float4 f = lds128f(red + (((blk * kMoeChunks + c) * MT + mt) * 32 + lane) * 16);
+                v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
+            }
+            // elements 0, 1: row g8 of the block for rows 2 t4, 2 t4 + 1 of the tile; 2, 3: row g8 + 8
+            const int nb = walk.block + blk;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int row = mt * 8 + 2 * t4 + j;
+                if (row >= tile.z) continue;
+                if (GATED) {
+                    moe_inner(p)[(int64_t)(tile.y + row) * p.inner + nb * 8 + g8] =
+                        __float2half_rn(activate(v[j], p.activation) * v[2 + j]);
+                } else {
+                    const int64_t entry = __ldcg(moe_order(p) + tile.y + row);
+                    float* const o = moe_out(p) + ((int64_t)walk.split * p.entries + entry) * p.hidden + nb * 16 + g8;
+                    __stcg(o, v[j]);
+                    __stcg(o + 8, v[2 + j]);
+                }
+            }
+        }
+    }
+}
+
+constexpr int kMoeFinishThreads = 256;
+
+// y = residual + the entries' results, weighted, in the order of the choices (K ranges first): four columns a thread.
+static __global__ void __launch_bounds__(kMoeFinishThreads) moe_finish_kernel(const __grid_constant__ MoeParams p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t token = blockIdx.x;
+    const int col = (blockIdx.y * kMoeFinishThreads + threadIdx.x) * 4;
+    if (col >= p.hidden) return;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (p.residual) {
+        const uint2 r = *reinterpret_cast<const uint2*>(p.residual + token * p.hidden + col);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
+        v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+    }
+    for (int j = 0; j < p.k; ++j) {
+        const int64_t entry = token * p.k + j;
+        const int e = __ldg(p.experts + entry);
+        if (e < 0 || e >= p.num_experts) continue;
+        const float w = __ldg(p.weights + entry);
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < p.plan.splits; ++i) {
+            const float4 d = __ldcg(reinterpret_cast<const float4*>(moe_out(p) + ((int64_t)i * p.entries + entry) * p.hidden + col));
+            s.x += d.x; s.y += d.y; s.z += d.z; s.w += d.w;
+        }
+        v[0] = fmaf(w, s.x, v[0]);
+        v[1] = fmaf(w, s.y, v[1]);
+        v[2] = fmaf(w, s.z, v[2]);
+        v[3] = fmaf(w, s.w, v[3]);
+    }
+    const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(p.y + token * p.hidden + col) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+}  // namespace w4a16

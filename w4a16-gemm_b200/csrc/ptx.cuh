@@ -26,9 +26,10 @@ enum DeviceError : int {
     kDevTimeoutDrain = 5,        // error path: in-flight copies did not land in time
     kDevTimeoutPeer = 7,         // tensor-parallel exchange: a peer rank never arrived
     kDevTimeoutCache = 8,        // cache attention: a pipeline barrier never completed
+    kDevTimeoutExperts = 9,      // expert layer: a pipeline barrier never completed
 };
 
-// Per-device status word of this translation unit (kernels.cu and cache.cu have one each;
+// Per-device status word of this translation unit (kernels.cu, cache.cu and moe.cu have one each;
 // the entry point that reads them reports the first that is set).
 static __device__ int w4a16_device_status = 0;
 

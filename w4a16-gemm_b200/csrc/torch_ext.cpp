@@ -524,6 +524,76 @@ std::tuple<torch::Tensor, torch::Tensor> moe_route_py(torch::Tensor logits, int6
     return {weights, experts};
 }
 
+torch::Tensor moe_experts_py(torch::Tensor x, torch::Tensor gate_up_wp, torch::Tensor gate_up_scales, torch::Tensor down_wp,
+                             torch::Tensor down_scales, torch::Tensor experts, torch::Tensor weights, int64_t activation,
+                             c10::optional<torch::Tensor> residual, c10::optional<torch::Tensor> out,
+                             c10::optional<torch::Tensor> workspace) {
+    auto is = [&](const torch::Tensor& t, torch::ScalarType type, int64_t dim) {
+        return t.is_cuda() && t.device() == x.device() && t.scalar_type() == type && t.dim() == dim && t.is_contiguous();
+    };
+    TORCH_CHECK(is(x, torch::kHalf, 2), "x must be a contiguous CUDA fp16 [tokens, hidden] tensor");
+    const int64_t tokens = x.size(0), hidden = x.size(1);
+    TORCH_CHECK(is(gate_up_scales, torch::kHalf, 3) && is(down_scales, torch::kHalf, 3),
+                "scales must be contiguous fp16 [experts, K/G, N] tensors on x's device");
+    const int64_t num = gate_up_scales.size(0), inner = gate_up_scales.size(2) / 2;
+    TORCH_CHECK(gate_up_scales.size(2) % 16 == 0 && inner > 0 && num > 0, "the gated scales must be [experts, hidden/G, 2 * inner]");
+    TORCH_CHECK(down_scales.size(0) == num && down_scales.size(2) == hidden, "the second product's scales must be [experts, inner/G, hidden]");
+    TORCH_CHECK(gate_up_scales.size(1) > 0 && hidden % gate_up_scales.size(1) == 0 && down_scales.size(1) > 0 &&
+                    inner % down_scales.size(1) == 0, "hidden and inner must be divisible by their numbers of groups");
+    TORCH_CHECK(num <= 1024 && hidden <= (1 << 20) && inner <= (1 << 20), "at most 1024 experts, hidden and inner at most 2^20");
+    TORCH_CHECK(is(gate_up_wp, torch::kInt32, 2) && gate_up_wp.size(0) == num && gate_up_wp.size(1) == hidden * inner / 4,
+                "the gated words must be a contiguous int32 [experts, 2 * inner * hidden / 8] tensor on x's device");
+    TORCH_CHECK(is(down_wp, torch::kInt32, 2) && down_wp.size(0) == num && down_wp.size(1) == hidden * inner / 8,
+                "the second product's words must be a contiguous int32 [experts, hidden * inner / 8] tensor on x's device");
+    TORCH_CHECK(is(experts, torch::kInt32, 2) && experts.size(0) == tokens && experts.size(1) <= INT_MAX,
+                "experts must be a contiguous int32 [tokens, k] tensor on x's device");
+    TORCH_CHECK(is(weights, torch::kFloat, 2) && weights.sizes() == experts.sizes(),
+                "weights must be a contiguous fp32 [tokens, k] tensor on x's device");
+    const at::cuda::CUDAGuard guard(x.device());
+    w4a16_moe_args a = {};
+    if (residual.has_value()) {
+        TORCH_CHECK(is(*residual, torch::kHalf, 2) && residual->sizes() == x.sizes(), "residual must be a contiguous fp16 tensor of x's shape");
+        a.residual = residual->data_ptr();
+    }
+    torch::Tensor y;
+    if (out.has_value()) {
+        y = *out;
+        TORCH_CHECK(is(y, torch::kHalf, 2) && y.sizes() == x.sizes(), "out must be a contiguous fp16 tensor of x's shape");
+    } else {
+        y = fresh(x.sizes(), torch::kHalf, x);
+    }
+    a.x = x.data_ptr();
+    a.gate_up_wp = gate_up_wp.data_ptr<int32_t>();
+    a.gate_up_scales = gate_up_scales.data_ptr();
+    a.down_wp = down_wp.data_ptr<int32_t>();
+    a.down_scales = down_scales.data_ptr();
+    a.experts = experts.data_ptr<int32_t>();
+    a.weights = weights.data_ptr<float>();
+    a.y = y.data_ptr();
+    a.tokens = tokens;
+    a.num_experts = (int32_t)num;
+    a.k = (int32_t)experts.size(1);
+    a.hidden = (int32_t)hidden;
+    a.inner = (int32_t)inner;
+    a.gate_up_group = (int32_t)(hidden / gate_up_scales.size(1));
+    a.down_group = (int32_t)(inner / down_scales.size(1));
+    a.activation = (int32_t)activation;
+    cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
+    uint64_t ws_bytes = 0;
+    torch::Tensor ws;
+    if (workspace.has_value()) {
+        ws = *workspace;
+        TORCH_CHECK(ws.is_cuda() && ws.device() == x.device() && ws.is_contiguous(),
+                    "workspace must be a contiguous CUDA tensor on x's device");
+        ws_bytes = (uint64_t)ws.numel() * ws.element_size();
+    } else {
+        check(w4a16_moe_workspace(&a, &ws_bytes));
+        ws = workspace_for(x, ws_bytes, stream);
+    }
+    check(w4a16_moe_experts(&a, ws.defined() ? ws.data_ptr() : nullptr, ws_bytes, stream));
+    return y;
+}
+
 int64_t device_status_py(bool reset) {
     int32_t code = 0;
     w4a16_status s = w4a16_device_status(&code, reset ? 1 : 0);
@@ -558,5 +628,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("linear", &linear_py, "W4A16 GEMM with bias, activation, gate and residual");
     m.def("rms_norm", &rms_norm_py, "root-mean-square norm, with the residual's addition");
     m.def("moe_route", &moe_route_py, "softmax over experts, the k largest");
+    m.def("moe_experts", &moe_experts_py, "mixture-of-experts layer from 4-bit experts");
     m.attr("ABI_VERSION") = w4a16_abi_version();
 }

@@ -32,7 +32,7 @@ except ImportError as exc:  # pragma: no cover - exercised only when unbuilt
 from .format import dequantize_w4, pack_int4, quantize_pack, quantize_w4, unpack_int4  # noqa: E402
 from .kvcache import Int4KVCache, cache_append, cache_attention, cache_read  # noqa: E402
 from .layer import interleave_gate_up, rms_norm, w4a16_linear  # noqa: E402
-from .moe import moe_route  # noqa: E402
+from .moe import moe_experts, moe_route  # noqa: E402
 
 LIBRARY_PATH = os.path.join(_HERE, "libw4a16.so")
 ABI_VERSION = _C.ABI_VERSION
@@ -101,6 +101,6 @@ __all__ = [
     "workspace_bytes", "make_workspace",
     "pack_int4", "unpack_int4", "quantize_w4", "quantize_pack", "dequantize_w4",
     "Int4KVCache", "cache_append", "cache_read", "cache_attention",
-    "w4a16_linear", "interleave_gate_up", "rms_norm", "moe_route",
+    "w4a16_linear", "interleave_gate_up", "rms_norm", "moe_route", "moe_experts",
     "LIBRARY_PATH", "ABI_VERSION", "PREFILL_VARIANTS",
 ]

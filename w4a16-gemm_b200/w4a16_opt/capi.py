@@ -84,6 +84,13 @@ class NormArgs(ctypes.Structure):
                 ("eps", ctypes.c_float)]
 
 
+class MoeArgs(ctypes.Structure):
+    """w4a16_moe_args: one w4a16_moe_experts call."""
+    _fields_ = [(name, _vp) for name in ("x", "gate_up_wp", "gate_up_scales", "down_wp", "down_scales", "experts", "weights",
+                                         "residual", "y")] + [("tokens", _i64)] + \
+               [(name, _i32) for name in ("num_experts", "k", "hidden", "inner", "gate_up_group", "down_group", "activation")]
+
+
 # name -> (restype, argtypes), one entry per declaration in include/w4a16.h
 EXPORTS = {
     "w4a16_abi_version": (_i32, []),
@@ -115,6 +122,8 @@ EXPORTS = {
                             ctypes.c_uint32, _vp, _u64, _vp]),
     "w4a16_rms_norm": (_i32, [ctypes.POINTER(NormArgs), _vp]),
     "w4a16_moe_route": (_i32, [_vp, _i32, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "w4a16_moe_experts": (_i32, [ctypes.POINTER(MoeArgs), _vp, _u64, _vp]),
+    "w4a16_moe_workspace": (_i32, [ctypes.POINTER(MoeArgs), ctypes.POINTER(_u64)]),
     "w4a16_device_status": (_i32, [ctypes.POINTER(_i32), _i32]),
     "w4a16_check_wait_limits": (_i32, [ctypes.POINTER(_i32)]),
     "w4a16_status_string": (ctypes.c_char_p, [_i32]),

@@ -1,6 +1,7 @@
-"""A mixture of experts: its router.
+"""A mixture of experts from 4-bit weights: its router, its experts.
 
-    weights, experts = moe_route(logits, k)
+    weights, experts = moe_route(h @ router, k)
+    x = moe_experts(h, gate_up, down, experts, weights, residual=x, out=x)
 
 The reference has no counterpart.  Every function runs on the current CUDA stream, and raises
 RuntimeError on bad input.
@@ -10,6 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _C
+from .layer import activation_code
 
 
 def moe_route(logits: torch.Tensor, k: int, *, renormalize: bool = True):
@@ -21,3 +23,21 @@ def moe_route(logits: torch.Tensor, k: int, *, renormalize: bool = True):
     left, the rest of the row is expert -1 with weight 0.
     """
     return _C.moe_route(logits, k, renormalize)
+
+
+def moe_experts(x: torch.Tensor, gate_up, down, experts: torch.Tensor, weights: torch.Tensor, *,
+                activation: str | None = "silu", residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """y_t = residual_t + sum_j weights[t, j] * down_e(act(gate_e(x_t)) * up_e(x_t)), e = experts[t, j]; fp16 [tokens, hidden].
+
+    ``x`` fp16 [tokens, hidden].  ``gate_up`` and ``down`` are (packed words, scales) of all experts, stacked: int32
+    [experts, 2 * inner * hidden / 8] and fp16 [experts, hidden/G, 2 * inner], rows laid by ``interleave_gate_up``;
+    int32 [experts, hidden * inner / 8] and fp16 [experts, inner/G, hidden].  hidden and inner are multiples of 64 and of their
+    group size (64 or 128); at most 1024 experts.  ``experts`` int32 and ``weights`` fp32 [tokens, k], as ``moe_route``
+    gives them; an expert outside [0, experts) adds nothing (another device's, say), the same one twice counts twice.
+
+    Sums are fp32; the inner results are rounded to fp16, y once.  ``out`` may be ``residual`` or ``x``.
+    ``workspace``: optional scratch CUDA buffer (256-byte aligned); without it the binding keeps one per (device, stream).
+    """
+    return _C.moe_experts(x, gate_up[0], gate_up[1], down[0], down[1], experts, weights, activation_code(activation),
+                          residual, out, workspace)
