@@ -58,7 +58,7 @@ cudaError_t launch_moe_experts(const w4a16_moe_args& a, const DeviceInfo& dev, v
     p.hidden = a.hidden;
     p.inner = a.inner;
     p.activation = a.activation;
-    cudaError_t err = launch(moe_plan_kernel, dim3(1), kMoePlanThreads, 0, stream, pdl, p);
+    cudaError_t err = p.plan.few ? cudaSuccess : launch(moe_plan_kernel, dim3(1), kMoePlanThreads, 0, stream, pdl, p);
     if (err == cudaSuccess) err = launch_product<true>(p, a.gate_up_group, dev.num_sms, stream, pdl);
     if (err == cudaSuccess) err = launch_product<false>(p, a.down_group, dev.num_sms, stream, pdl);
     if (err != cudaSuccess) return err;

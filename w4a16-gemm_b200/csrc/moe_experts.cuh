@@ -3,25 +3,34 @@
 //     h_tj = act(x_t Wg_e^T) * (x_t Wu_e^T),   e = experts[t][j]
 //     y_t  = residual_t + sum_j weights[t][j] (h_tj Wd_e^T)
 //
-// Four kernels, each launched behind the one before with programmatic dependent launch: the plan (entries
-// sorted by expert, tiles), the gated product, the second product, the weighted sum.  The products
-// stream the weights of the experts that were chosen, each once a tile.
+// Three kernels, each launched behind the one before with programmatic dependent launch: the gated product,
+// the second product, the weighted sum.  The products stream the weights of the experts that were chosen, each once a
+// tile.  Which entries make which tile every CTA works out for itself, from up to 1024 entries (about 1 us, where a
+// kernel in front takes 4); above that a kernel does it once, in front.
+//
+// The second product's CTAs start where the first one's leave, and fetch their first weights before the first
+// one has ended: what that reads was written before the call, or by the kernel in front, and the gated product lets
+// its successor start only after its own wait for whatever ran before it.
 //
 // One CTA an SM takes a range of the (tile, n16 block of output channels) sequence and walks it in batches
-// of up to 8 blocks of one tile.  A batch runs over K in stages of 8 chunks of 64: one warp issues all of a
-// stage as bulk copies (a block's 8 chunks are one run of 4 KB; the chunks' scales; 1 KB of each of
-// the tile's rows) onto one mbarrier.  16 consumer warps: warp w takes chunk w % 8 of the stage for half of
+// of up to 8 blocks of one tile.  A batch runs over K in stages of 8 chunks of 64, filled by bulk copies onto
+// one mbarrier: a block's 8 chunks are one run of 4 KB; the chunks' scales; 1 KB of each of the tile's rows.
+// Issuing a bulk copy takes about 30 ns and a producer's turn 0.3 us more, whatever their size, so the three kinds have
+// a warp each: 8 copies a turn bring 32 KB in 0.5 us, where an SM's share of the memory needs 0.7.  16 consumer warps: warp w takes chunk w % 8 of the stage for half of
 // the batch's blocks, so that K is summed over 8 warps, through shared memory, once a batch: sums are
 // whole where they are made, and the gate needs no second pass.
 //
-// The weights enter mma.m16n8k16 as the integers q - 8 (exact in fp16) and a chunk's sums are multiplied by its
-// scale in fp32: the weight (q - 8) * s is never rounded.  The gated product's results are rounded to fp16 once, being
+// The codes enter mma.m16n8k16 where they lie in their words, masked: four bits at the bottom of a half are the fp16
+// subnormal q 2^-24, the next four q 2^-20 (the first are rows 0-7 of a block, the others rows 8-15).  That
+// takes 5 instructions a word where making the fp16 numbers q - 8 takes 9.  The 8 is taken off a chunk's sums
+// with the sum of its x (a product with ones, shared by the blocks), the powers of two when a batch's sums are
+// joined.  A chunk's sums are multiplied by its scale in fp32:
+// the weight (q - 8) * s is never rounded.  The gated product's results are rounded to fp16 once, being
 // operands of the second product; its results stay fp32 until the weighted sum.
 #pragma once
 #include <cuda_fp16.h>
 #include <stdint.h>
 
-#include "dequant.cuh"
 #include "epilogue.cuh"
 #include "internal.h"
 #include "moe_plan.h"
@@ -30,7 +39,8 @@
 namespace w4a16 {
 
 constexpr int kMoeConsumers = 16;                         // warps: 8 chunks x 2 halves of the blocks
-constexpr int kMoeThreads = (kMoeConsumers + 1) * 32;
+constexpr int kMoeProducers = 3;                          // warps: packed words, scales, rows
+constexpr int kMoeThreads = (kMoeConsumers + kMoeProducers) * 32;
 constexpr int kMoeHalf = kMoeBlocks / 2;                  // blocks of a consumer warp
 constexpr int kMoePlanThreads = 1024;
 
@@ -46,7 +56,9 @@ struct MoeCfg {
     static constexpr int STAGES = MT == 1 ? 4 : 3;
     static constexpr int RED_BYTES = kMoeBlocks * kMoeChunks * MT * 512;   // [block][chunk warp][mt][lane] float4
     static constexpr int BARS = STAGES * STAGE + RED_BYTES;
-    static constexpr int SMEM = 128 + BARS + 2 * STAGES * 8;
+    static constexpr int PLAN = BARS + 2 * STAGES * 8;                     // tiles of few entries, their order
+    static constexpr int SMEM = 128 + PLAN + kMoeFewEntries * (8 + 2);
+    static_assert(RED_BYTES >= kMoeMaxExperts * 8 + kMoeFewEntries * 6, "the sort's scratch");
     static_assert(STAGE % 16 == 0 && SMEM <= 227 * 1024, "shared memory");
 };
 
@@ -125,10 +137,101 @@ static __global__ void __launch_bounds__(kMoePlanThreads) moe_plan_kernel(const 
     }
 }
 
+// One tile, packed: its expert and count, its first sorted entry.
+struct MoeSmallTile {
+    uint16_t expert, count;
+    uint32_t start;
+};
+
+// The same for up to kMoeFewEntries entries, by every CTA in its shared memory, in one order: expert by expert, the
+// entries of one as they are numbered.  scratch: two words an expert, six bytes an entry.  Returns the number of tiles.
+template <int THREADS>
+__device__ __forceinline__ int moe_sort_few(const MoeParams& p, MoeSmallTile* tiles, uint16_t* order, char* scratch) {
+    static_assert(2 * THREADS >= kMoeMaxExperts, "two experts a thread");
+    constexpr int WARPS = THREADS / 32;
+    __shared__ uint32_t sums[32];
+    int32_t* const count = reinterpret_cast<int32_t*>(scratch);
+    int32_t* const first = count + kMoeMaxExperts;
+    int32_t* const expert = first + kMoeMaxExperts;
+    uint16_t* const rank = reinterpret_cast<uint16_t*>(expert + kMoeFewEntries);
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    for (int i = t; i < kMoeMaxExperts; i += THREADS) count[i] = 0;
+    for (int i = t; i < p.entries; i += THREADS) {
+        const int e = __ldg(p.experts + i);
+        expert[i] = e >= 0 && e < p.num_experts ? e : -1;
+    }
+    __syncthreads();
+    if (warp == 0) {                     // ranks among the entries of one expert, 32 entries at a time
+        for (int i0 = 0; i0 < p.entries; i0 += 32) {
+            const int i = i0 + lane, e = i < p.entries ? expert[i] : -1;
+            const uint32_t same = __match_any_sync(0xffffffffu, e);
+            const int before = __popc(same & ((1u << lane) - 1));
+            if (e >= 0) {
+                const int r = count[e] + before;
+                rank[i] = (uint16_t)r;
+            }
+            __syncwarp();
+            if (e >= 0 && before == 0) count[e] += __popc(same);
+            __syncwarp();
+        }
+    }
+    __syncthreads();
+    // entries and tiles before each expert, 16 bits each, two experts a thread
+    uint32_t mine[2], v = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int e = 2 * t + j, n = e < kMoeMaxExperts ? count[e] : 0;
+        mine[j] = (uint32_t)n | (uint32_t)((n + p.plan.rows - 1) / p.plan.rows) << 16;
+        v += mine[j];
+    }
+    uint32_t end = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += u;
+    }
+    if (lane == 31) sums[warp] = end;
+    __syncthreads();
+    uint32_t before = end - v, all = 0;
+    for (int w = 0; w < WARPS; ++w) {
+        before += w < warp ? sums[w] : 0u;
+        all += sums[w];
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int n = mine[j] & 0xffff, start = before & 0xffff, tile = before >> 16, e = 2 * t + j;
+        if (e < kMoeMaxExperts) first[e] = start;
+        for (int i = 0; i * p.plan.rows < n; ++i)
+            tiles[tile + i] = {(uint16_t)e, (uint16_t)min(p.plan.rows, n - i * p.plan.rows), (uint32_t)(start + i * p.plan.rows)};
+        before += mine[j];
+    }
+    __syncthreads();
+    for (int i = t; i < p.entries; i += THREADS)
+        if (expert[i] >= 0) order[first[expert[i]] + rank[i]] = (uint16_t)i;
+    __syncthreads();
+    return (int)(all >> 16);
+}
+
 // Untiled bulk copy into this CTA's shared memory (16-byte aligned addresses and size).
 __device__ __forceinline__ void moe_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// The codes of one packed word as an A fragment of subnormals: rows g at 2^-24, rows g + 8 at 2^-20.
+__device__ __forceinline__ void code_word(uint32_t q, uint32_t (&a)[4]) {
+    const uint32_t q8 = q >> 8;
+    a[0] = q & 0x000F000Fu;
+    a[1] = q & 0x00F000F0u;
+    a[2] = q8 & 0x000F000Fu;
+    a[3] = q8 & 0x00F000F0u;
+}
+
+// c += a * b.  Not volatile: chains of different blocks may be put between one another.
+__device__ __forceinline__ void moe_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // A CTA's walk: batches of up to 8 blocks of one (tile, K range), over its range of units.  Unit u is block u % blocks
@@ -161,56 +264,74 @@ static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(cons
     auto empty = [&](int s) { return base + (uint32_t)(C::BARS + (C::STAGES + s) * 8); };
     const uint32_t red = base + C::STAGES * C::STAGE;
 
-    pdl_launch_dependents();
+    if (GATED) {
+        pdl_wait();
+        pdl_launch_dependents();
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) {
-            mbar_init(full(s), 1);
+            mbar_init(full(s), kMoeProducers);
             mbar_init(empty(s), kMoeConsumers);
         }
         fence_mbar_init();
     }
-    __syncthreads();
-    pdl_wait();
+    char* const smem = reinterpret_cast<char*>(smem_raw) + (base - smem_u32(smem_raw));
+    MoeSmallTile* const small = reinterpret_cast<MoeSmallTile*>(smem + C::PLAN);
+    uint16_t* const small_order = reinterpret_cast<uint16_t*>(small + kMoeFewEntries);
+    int tiles;
+    if (p.plan.few) {
+        tiles = moe_sort_few<kMoeThreads>(p, small, small_order, smem + C::STAGES * C::STAGE);
+    } else {
+        __syncthreads();
+        tiles = __ldcg(&moe_head(p)->tiles);
+    }
+    const auto tile_at = [&](int i) {
+        if (!p.plan.few) return __ldcg(moe_tiles(p) + i);
+        const MoeSmallTile t = small[i];
+        return make_int4(t.expert, (int)t.start, t.count, 0);
+    };
+    const auto entry_at = [&](int i) { return p.plan.few ? (int)small_order[i] : __ldcg(moe_order(p) + i); };
 
     const int K = GATED ? p.hidden : p.inner, N = GATED ? 2 * p.inner : p.hidden;
     const int chunks = K >> 6, all_stages = (chunks + kMoeChunks - 1) / kMoeChunks;
     MoeWalk walk;
     walk.blocks = N >> 4;
     walk.splits = GATED ? 1 : p.plan.splits;
-    const long long units = (long long)__ldcg(&moe_head(p)->tiles) * walk.splits * walk.blocks;
+    const long long units = (long long)tiles * walk.splits * walk.blocks;
     walk.unit = (int)(units * blockIdx.x / gridDim.x);
     walk.end = (int)(units * (blockIdx.x + 1) / gridDim.x);
     walk.n = 0;
     int it = 0;
 
-    if (warp == kMoeConsumers) {
-        // ------------------------------------------------ producer: one copy a lane
-        // lanes 0-7 the blocks' packed words, 8-15 the groups' scales, 16-31 the tile's rows
-        const int role = lane < 8 ? 0 : lane < 16 ? 1 : 2, which = role == 2 ? lane - 16 : lane & 7;
+    if (warp >= kMoeConsumers) {
+        // ------------------------------------------------ producers: one copy a lane
+        const int role = warp - kMoeConsumers;           // 0 the blocks' packed words, 1 the groups' scales, 2 the tile's rows
         bool ok = true;
+        if (!GATED && role == 2) pdl_wait();             // the rows are the first product's results
         while (ok && walk.next()) {
-            const int4 tile = __ldcg(moe_tiles(p) + walk.tile);
-            const char* src = nullptr;
-            uint32_t dst = 0, step = 0;
-            int have = 0;
+            const int4 tile = tile_at(walk.tile);
+            const char* src;                             // of this lane at chunk 0
+            uint32_t dst;
+            int64_t step;                                // bytes from chunk to chunk (scales: from group to group)
+            int have;                                    // lanes with a copy (scales: by the stage)
             if (role == 0) {
                 src = reinterpret_cast<const char*>(p.words[GATED ? 0 : 1]) +
-                      ((int64_t)tile.x * walk.blocks + walk.block + which) * chunks * 512;
-                dst = which * (kMoeChunks * 512);
+                      ((int64_t)tile.x * walk.blocks + walk.block + lane) * chunks * 512;
+                dst = lane * (kMoeChunks * 512);
                 step = 512;
                 have = walk.n;
             } else if (role == 1) {
-                src = reinterpret_cast<const char*>(p.scales[GATED ? 0 : 1] + (int64_t)tile.x * (K / G) * N + walk.block * 16);
-                dst = C::W_BYTES + C::X_BYTES + which * C::S_ROW;
+                src = reinterpret_cast<const char*>(p.scales[GATED ? 0 : 1] + ((int64_t)tile.x * (K / G) + lane) * N + walk.block * 16);
+                dst = C::W_BYTES + C::X_BYTES + lane * C::S_ROW;
+                step = (int64_t)N * 2;
+                have = 0;
             } else {
-                if (which < tile.z) {
-                    const int at = tile.y + which;
-                    src = reinterpret_cast<const char*>(GATED ? p.x + (int64_t)(__ldcg(moe_order(p) + at) / p.k) * K
-                                                              : moe_inner(p) + (int64_t)at * K);
-                }
-                dst = C::W_BYTES + which * C::X_PITCH;
-                step = 128;
                 have = tile.z;
+                const int at = tile.y + min(lane, have - 1);
+                src = reinterpret_cast<const char*>(GATED ? p.x + (int64_t)(entry_at(at) / p.k) * K
+                                                          : moe_inner(p) + (int64_t)at * K);
+                dst = C::W_BYTES + lane * C::X_PITCH;
+                step = 128;
             }
             const int s1 = all_stages * (walk.split + 1) / walk.splits;
             for (int st = all_stages * walk.split / walk.splits; st < s1; ++st, ++it) {
@@ -219,15 +340,11 @@ static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(cons
                     ok = __all_sync(0xffffffffu, mbar_wait_sleep(empty(s), (it / C::STAGES - 1) & 1, kDevTimeoutExperts));
                     if (!ok) break;
                 }
-                const int groups = (n * 64 + G - 1) / G;
-                if (lane == 0)
-                    mbar_arrive_expect_tx(full(s), (uint32_t)(walk.n * n * 512 + tile.z * n * 128 + groups * walk.n * 32));
+                const int copies = role == 1 ? (n * 64 + G - 1) / G : have;
+                const uint32_t bytes = role == 0 ? n * 512 : role == 1 ? walk.n * 32 : n * 128;
+                if (lane == 0) mbar_arrive_expect_tx(full(s), copies * bytes);
                 __syncwarp();
-                if (role == 1) {
-                    if (which < groups) moe_copy(stage(s) + dst, src + (int64_t)(c0 * 64 / G + which) * N * 2, walk.n * 32, full(s));
-                } else if (which < have) {
-                    moe_copy(stage(s) + dst, src + (int64_t)c0 * step, n * step, full(s));
-                }
+                if (lane < copies) moe_copy(stage(s) + dst, src + (role == 1 ? c0 * 64 / G : c0) * step, bytes, full(s));
             }
         }
         // copies still in flight must land before the CTA may exit (they have, unless a wait ran out)
@@ -242,6 +359,10 @@ static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(cons
     const uint32_t x_lane = C::W_BYTES + (lane & 7) * C::X_PITCH + chunk * 128 + (lane >> 3) * 16;
     const uint32_t w_lane = (half * kMoeHalf * kMoeChunks + chunk) * 512 + lane * 16;
     const uint32_t s_lane = C::W_BYTES + C::X_BYTES + (chunk * 64 / G) * C::S_ROW + half * kMoeHalf * 32 + g8 * 2;
+    if (!GATED) {
+        pdl_wait();                                      // the call before may still read what this one writes
+        pdl_launch_dependents();
+    }
     bool ok = true;
     while (walk.next()) {
         float acc[kMoeHalf][MT][4];
@@ -264,28 +385,48 @@ static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(cons
                     ldmatrix_x4(*reinterpret_cast<uint32_t(*)[4]>(&b[mt][0]), sb + x_lane + mt * 8 * C::X_PITCH);
                     ldmatrix_x4(*reinterpret_cast<uint32_t(*)[4]>(&b[mt][4]), sb + x_lane + mt * 8 * C::X_PITCH + 64);
                 }
+                // all four blocks of the half, there or not: the chains of a straight run interleave (sums of
+                // blocks past the batch, made of whatever the stage holds, are not read)
+                uint4 w4[kMoeHalf];
+                float scale[kMoeHalf][2];
 #pragma unroll
                 for (int blk = 0; blk < kMoeHalf; ++blk) {
-                    if (blk >= mine) break;
-                    const uint4 w4 = lds128(sb + w_lane + blk * (kMoeChunks * 512));
-                    const float lo = __half2float(__ushort_as_half(lds_u16(sb + s_lane + blk * 32)));
-                    const float hi = __half2float(__ushort_as_half(lds_u16(sb + s_lane + blk * 32 + 16)));
-                    float c[MT][4];
+                    w4[blk] = lds128(sb + w_lane + blk * (kMoeChunks * 512));
+                    scale[blk][0] = __half2float(__ushort_as_half(lds_u16(sb + s_lane + blk * 32)));
+                    scale[blk][1] = __half2float(__ushort_as_half(lds_u16(sb + s_lane + blk * 32 + 16)));
+                }
+                float c[kMoeHalf][MT][4], sum[MT][4];
 #pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) {
-                        uint32_t a[4];
-                        unscaled_word(ks == 0 ? w4.x : ks == 1 ? w4.y : ks == 2 ? w4.z : w4.w, a);
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            if (ks == 0) mma_16816_zero(c[mt], a, b[mt][0], b[mt][1]);
-                            else mma_16816(c[mt], a, b[mt][2 * ks], b[mt][2 * ks + 1]);
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        sum[mt][i] = 0.f;
+#pragma unroll
+                        for (int blk = 0; blk < kMoeHalf; ++blk) c[blk][mt][i] = 0.f;
                     }
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
+                for (int ks = 0; ks < 4; ++ks) {
+                    const uint32_t ones[4] = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[blk][mt][i] = fmaf(i < 2 ? lo : hi, c[mt][i], acc[blk][mt][i]);
+                    for (int mt = 0; mt < MT; ++mt) moe_mma(sum[mt], ones, b[mt][2 * ks], b[mt][2 * ks + 1]);
+#pragma unroll
+                    for (int blk = 0; blk < kMoeHalf; ++blk) {
+                        uint32_t a[4];
+                        code_word(ks == 0 ? w4[blk].x : ks == 1 ? w4[blk].y : ks == 2 ? w4[blk].z : w4[blk].w, a);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) moe_mma(c[blk][mt], a, b[mt][2 * ks], b[mt][2 * ks + 1]);
+                    }
                 }
+                // less 8 for every code, in the units of the rows
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float eight = sum[mt][i] * (i < 2 ? -0x1p-21f : -0x1p-17f);
+#pragma unroll
+                        for (int blk = 0; blk < kMoeHalf; ++blk)
+                            acc[blk][mt][i] = fmaf(scale[blk][i >> 1], c[blk][mt][i] + eight, acc[blk][mt][i]);
+                    }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(empty(s));
@@ -299,7 +440,7 @@ static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(cons
                 sts128(red + ((((half * kMoeHalf + blk) * kMoeChunks + chunk) * MT + mt) * 32 + lane) * 16,
                        make_float4(acc[blk][mt][0], acc[blk][mt][1], acc[blk][mt][2], acc[blk][mt][3]));
         bar_sync_named(2, kMoeConsumers * 32);
-        const int4 tile = __ldcg(moe_tiles(p) + walk.tile);
+        const int4 tile = tile_at(walk.tile);
         for (int i = warp; i < walk.n * MT; i += kMoeConsumers) {
             const int blk = i / MT, mt = i % MT;
             float v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -308,6 +449,7 @@ static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(cons
                 const float4 f = lds128f(red + (((blk * kMoeChunks + c) * MT + mt) * 32 + lane) * 16);
                 v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
             }
+            v[0] *= 0x1p24f; v[1] *= 0x1p24f; v[2] *= 0x1p20f; v[3] *= 0x1p20f;
             // elements 0, 1: row g8 of the block for rows 2 t4, 2 t4 + 1 of the tile; 2, 3: row g8 + 8
             const int nb = walk.block + blk;
 #pragma unroll
@@ -318,7 +460,7 @@ static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(cons
                     moe_inner(p)[(int64_t)(tile.y + row) * p.inner + nb * 8 + g8] =
                         __float2half_rn(activate(v[j], p.activation) * v[2 + j]);
                 } else {
-                    const int64_t entry = __ldcg(moe_order(p) + tile.y + row);
+                    const int64_t entry = entry_at(tile.y + row);
                     float* const o = moe_out(p) + ((int64_t)walk.split * p.entries + entry) * p.hidden + nb * 16 + g8;
                     __stcg(o, v[j]);
                     __stcg(o + 8, v[2 + j]);
@@ -330,33 +472,44 @@ static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(cons
 
 constexpr int kMoeFinishThreads = 256;
 
-// y = residual + the entries' results, weighted, in the order of the choices (K ranges first): four columns a thread.
+// y = residual + the entries' results, weighted, in the order of the choices and their K ranges: four columns a thread.
 static __global__ void __launch_bounds__(kMoeFinishThreads) moe_finish_kernel(const __grid_constant__ MoeParams p) {
-    pdl_launch_dependents();
-    pdl_wait();
     const int64_t token = blockIdx.x;
     const int col = (blockIdx.y * kMoeFinishThreads + threadIdx.x) * 4;
-    if (col >= p.hidden) return;
+    const bool in_row = col < p.hidden;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (p.residual) {
+    if (p.residual && in_row) {          // an input of the call: there before the products began
         const uint2 r = *reinterpret_cast<const uint2*>(p.residual + token * p.hidden + col);
         const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
         v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
     }
-    for (int j = 0; j < p.k; ++j) {
-        const int64_t entry = token * p.k + j;
-        const int e = __ldg(p.experts + entry);
-        if (e < 0 || e >= p.num_experts) continue;
-        const float w = __ldg(p.weights + entry);
-        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = 0; i < p.plan.splits; ++i) {
-            const float4 d = __ldcg(reinterpret_cast<const float4*>(moe_out(p) + ((int64_t)i * p.entries + entry) * p.hidden + col));
-            s.x += d.x; s.y += d.y; s.z += d.z; s.w += d.w;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (!in_row) return;
+    // eight (choice, K range) pairs' loads in flight at a time; what an expert outside the layer would have
+    // left is loaded too, and dropped
+    const int parts = p.k * p.plan.splits;
+    for (int i0 = 0; i0 < parts; i0 += 8) {
+        float4 d[8];
+        float w[8];
+        bool in[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int part = min(i0 + i, parts - 1), j = part / p.plan.splits, range = part - j * p.plan.splits;
+            const int64_t entry = token * p.k + j;
+            const int e = __ldg(p.experts + entry);
+            w[i] = __ldg(p.weights + entry);
+            d[i] = __ldcg(reinterpret_cast<const float4*>(moe_out(p) + (range * (int64_t)p.entries + entry) * p.hidden + col));
+            in[i] = i0 + i < parts && e >= 0 && e < p.num_experts;
         }
-        v[0] = fmaf(w, s.x, v[0]);
-        v[1] = fmaf(w, s.y, v[1]);
-        v[2] = fmaf(w, s.z, v[2]);
-        v[3] = fmaf(w, s.w, v[3]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (in[i]) {
+                v[0] = fmaf(w[i], d[i].x, v[0]);
+                v[1] = fmaf(w[i], d[i].y, v[1]);
+                v[2] = fmaf(w[i], d[i].z, v[2]);
+                v[3] = fmaf(w[i], d[i].w, v[3]);
+            }
     }
     const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
     *reinterpret_cast<uint2*>(p.y + token * p.hidden + col) =

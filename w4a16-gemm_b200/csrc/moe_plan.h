@@ -18,6 +18,8 @@ namespace w4a16 {
 constexpr int kMoeMaxExperts = 1024;
 constexpr int kMoeBlocks = 8;        // n16 blocks of a batch
 constexpr int kMoeChunks = 8;        // 64-wide K chunks of a stage
+// Up to this many entries every CTA of the products sorts them for itself; above, one kernel does it for all.
+constexpr int kMoeFewEntries = 1024;
 
 struct MoeTile {
     int32_t expert, start, count, pad;   // sorted entries [start, start + count)
@@ -34,6 +36,7 @@ struct MoePlan {
     int32_t rows;            // entries of a tile
     int32_t max_tiles;       // no routing makes more
     int32_t splits;          // K ranges of the second product
+    bool few;                // every CTA sorts the entries
     size_t tiles_at, order_at, inner_at, out_at, bytes;    // offsets in the workspace
 };
 
@@ -53,6 +56,7 @@ inline MoePlan moe_plan(int64_t tokens, int k, int experts, int hidden, int inne
     const int stages = (inner / 64 + kMoeChunks - 1) / kMoeChunks;
     p.splits = 1;
     while (p.splits < 4 && 2 * p.splits <= stages && units * p.splits < 8 * (int64_t)num_sms) p.splits *= 2;
+    p.few = entries <= kMoeFewEntries;
     p.tiles_at = sizeof(MoeHead);
     p.order_at = moe_align(p.tiles_at + (size_t)p.max_tiles * sizeof(MoeTile));
     p.inner_at = moe_align(p.order_at + (size_t)entries * 4);
