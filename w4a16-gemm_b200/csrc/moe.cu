@@ -62,8 +62,12 @@ cudaError_t launch_moe_experts(const w4a16_moe_args& a, const DeviceInfo& dev, v
     if (err == cudaSuccess) err = launch_product<true>(p, a.gate_up_group, dev.num_sms, stream, pdl);
     if (err == cudaSuccess) err = launch_product<false>(p, a.down_group, dev.num_sms, stream, pdl);
     if (err != cudaSuccess) return err;
-    const int cols = 4 * kMoeFinishThreads;
-    return launch(moe_finish_kernel, dim3((unsigned)a.tokens, (unsigned)((a.hidden + cols - 1) / cols)), kMoeFinishThreads, 0, stream, pdl, p);
+    const auto finish = [&](auto kern, int slices) {
+        const int cols = 4 * kMoeFinishThreads / slices;
+        return launch(kern, dim3((unsigned)a.tokens, (unsigned)((a.hidden + cols - 1) / cols)), kMoeFinishThreads, 0, stream, pdl, p);
+    };
+    // a few tokens' parts are spread over threads, a prompt's fill the machine as they are
+    return a.tokens <= 64 ? finish(moe_finish_kernel<4>, 4) : finish(moe_finish_kernel<1>, 1);
 }
 
 }  // namespace w4a16

@@ -13,20 +13,22 @@
 // its successor start only after its own wait for whatever ran before it.
 //
 // One CTA an SM takes a range of the (tile, n16 block of output channels) sequence and walks it in batches
-// of up to 8 blocks of one tile.  A batch runs over K in stages of 8 chunks of 64, filled by bulk copies onto
+// of up to 10 blocks of one tile.  A batch runs over K in stages of 8 chunks of 64, filled by bulk copies onto
 // one mbarrier: a block's 8 chunks are one run of 4 KB; the chunks' scales; 1 KB of each of the tile's rows.
 // Issuing a bulk copy takes about 30 ns and a producer's turn 0.3 us more, whatever their size, so the three kinds have
-// a warp each: 8 copies a turn bring 32 KB in 0.5 us, where an SM's share of the memory needs 0.7.  16 consumer warps: warp w takes chunk w % 8 of the stage for half of
-// the batch's blocks, so that K is summed over 8 warps, through shared memory, once a batch: sums are
-// whole where they are made, and the gate needs no second pass.
+// a warp each: 10 copies a turn bring 40 KB in 0.6 us, where an SM's share of the memory needs 0.9.  Consumer
+// warp w of 8 takes chunk w of a stage for all of the batch's blocks, so that K is summed over 8 warps, through
+// shared memory, once a batch: sums are whole where they are made, and the gate needs no second pass.  Few warps with
+// many independent chains each: what a warp does once a stage (waits, rows, the ones' product) counts
+// for 10 blocks; two warps a chunk with half of the blocks each took 5 % longer, three 12 %.
 //
 // The codes enter mma.m16n8k16 where they lie in their words, masked: four bits at the bottom of a half are the fp16
 // subnormal q 2^-24, the next four q 2^-20 (the first are rows 0-7 of a block, the others rows 8-15).  That
 // takes 5 instructions a word where making the fp16 numbers q - 8 takes 9.  The 8 is taken off a chunk's sums
 // with the sum of its x (a product with ones, shared by the blocks), the powers of two when a batch's sums are
-// joined.  A chunk's sums are multiplied by its scale in fp32:
-// the weight (q - 8) * s is never rounded.  The gated product's results are rounded to fp16 once, being
-// operands of the second product; its results stay fp32 until the weighted sum.
+// joined.  A chunk's sums are multiplied by its scale in fp32: the weight (q - 8) * s is never rounded.  The gated
+// product's results are rounded to fp16 once, being operands of the second product, whose results stay fp32
+// until the weighted sum.
 #pragma once
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -38,23 +40,23 @@
 
 namespace w4a16 {
 
-constexpr int kMoeConsumers = 16;                         // warps: 8 chunks x 2 halves of the blocks
+constexpr int kMoeConsumers = kMoeChunks;                 // warps: one for each chunk of a stage
 constexpr int kMoeProducers = 3;                          // warps: packed words, scales, rows
 constexpr int kMoeThreads = (kMoeConsumers + kMoeProducers) * 32;
-constexpr int kMoeHalf = kMoeBlocks / 2;                  // blocks of a consumer warp
 constexpr int kMoePlanThreads = 1024;
 
 template <int MT>
 struct MoeCfg {
     static constexpr int ROWS = 8 * MT;
+    static constexpr int BLOCKS = MT == 1 ? 10 : 6;                   // n16 blocks of a batch, at most
     static constexpr int X_PITCH = kMoeChunks * 128 + 16;             // rows 16 bytes apart in banks: ldmatrix without conflicts
-    static constexpr int W_BYTES = kMoeBlocks * kMoeChunks * 512;     // [block][chunk][32 lanes x 16 B]
+    static constexpr int W_BYTES = BLOCKS * kMoeChunks * 512;     // [block][chunk][32 lanes x 16 B]
     static constexpr int X_BYTES = ROWS * X_PITCH;
-    static constexpr int S_ROW = kMoeBlocks * 32;                     // scales of one group of K: [block][16]
+    static constexpr int S_ROW = BLOCKS * 32;                     // scales of one group of K: [block][16]
     static constexpr int S_BYTES = kMoeChunks * S_ROW;
     static constexpr int STAGE = W_BYTES + X_BYTES + S_BYTES;
-    static constexpr int STAGES = MT == 1 ? 4 : 3;
-    static constexpr int RED_BYTES = kMoeBlocks * kMoeChunks * MT * 512;   // [block][chunk warp][mt][lane] float4
+    static constexpr int STAGES = MT == 1 ? 3 : 4;
+    static constexpr int RED_BYTES = BLOCKS * kMoeChunks * MT * 512;   // [block][chunk warp][mt][lane] float4
     static constexpr int BARS = STAGES * STAGE + RED_BYTES;
     static constexpr int PLAN = BARS + 2 * STAGES * 8;                     // tiles of few entries, their order
     static constexpr int SMEM = 128 + PLAN + kMoeFewEntries * (8 + 2);
@@ -147,7 +149,7 @@ struct MoeSmallTile {
 // entries of one as they are numbered.  scratch: two words an expert, six bytes an entry.  Returns the number of tiles.
 template <int THREADS>
 __device__ __forceinline__ int moe_sort_few(const MoeParams& p, MoeSmallTile* tiles, uint16_t* order, char* scratch) {
-    static_assert(2 * THREADS >= kMoeMaxExperts, "two experts a thread");
+    constexpr int PER = (kMoeMaxExperts + THREADS - 1) / THREADS;
     constexpr int WARPS = THREADS / 32;
     __shared__ uint32_t sums[32];
     int32_t* const count = reinterpret_cast<int32_t*>(scratch);
@@ -177,10 +179,10 @@ __device__ __forceinline__ int moe_sort_few(const MoeParams& p, MoeSmallTile* ti
     }
     __syncthreads();
     // entries and tiles before each expert, 16 bits each, two experts a thread
-    uint32_t mine[2], v = 0;
+    uint32_t mine[PER], v = 0;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int e = 2 * t + j, n = e < kMoeMaxExperts ? count[e] : 0;
+    for (int j = 0; j < PER; ++j) {
+        const int e = PER * t + j, n = e < kMoeMaxExperts ? count[e] : 0;
         mine[j] = (uint32_t)n | (uint32_t)((n + p.plan.rows - 1) / p.plan.rows) << 16;
         v += mine[j];
     }
@@ -198,8 +200,8 @@ __device__ __forceinline__ int moe_sort_few(const MoeParams& p, MoeSmallTile* ti
         all += sums[w];
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int n = mine[j] & 0xffff, start = before & 0xffff, tile = before >> 16, e = 2 * t + j;
+    for (int j = 0; j < PER; ++j) {
+        const int n = mine[j] & 0xffff, start = before & 0xffff, tile = before >> 16, e = PER * t + j;
         if (e < kMoeMaxExperts) first[e] = start;
         for (int i = 0; i * p.plan.rows < n; ++i)
             tiles[tile + i] = {(uint16_t)e, (uint16_t)min(p.plan.rows, n - i * p.plan.rows), (uint32_t)(start + i * p.plan.rows)};
@@ -227,15 +229,127 @@ __device__ __forceinline__ void code_word(uint32_t q, uint32_t (&a)[4]) {
     a[3] = q8 & 0x00F000F0u;
 }
 
-// c += a * b.  Not volatile: chains of different blocks may be put between one another.
-__device__ __forceinline__ void moe_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// c += a * b, or c = a * b.  Not volatile: chains of different blocks may be put between one another.
+__device__ __forceinline__ void moe_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool fresh) {
+    if (fresh)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// What a warp takes out of a stage: its chunk's rows, the N blocks' words and scales.
+template <int MT, int N>
+struct MoeFragments {
+    uint32_t b[MT][8];
+    uint4 w[N];
+    uint16_t scale[N][2];
+    // x_at, w_at, s_at: this lane's shared-memory addresses
+    __device__ __forceinline__ void load(uint32_t x_at, uint32_t w_at, uint32_t s_at) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            ldmatrix_x4(*reinterpret_cast<uint32_t(*)[4]>(&b[mt][0]), x_at + mt * 8 * MoeCfg<MT>::X_PITCH);
+            ldmatrix_x4(*reinterpret_cast<uint32_t(*)[4]>(&b[mt][4]), x_at + mt * 8 * MoeCfg<MT>::X_PITCH + 64);
+        }
+#pragma unroll
+        for (int blk = 0; blk < N; ++blk) {
+            w[blk] = lds128(w_at + blk * (kMoeChunks * 512));
+            scale[blk][0] = lds_u16(s_at + blk * 32);
+            scale[blk][1] = lds_u16(s_at + blk * 32 + 16);
+        }
+    }
+    // Products of the chunk, added to the blocks' sums.
+    __device__ __forceinline__ void multiply(float (&acc)[N][MT][4]) const {
+        float c[N][MT][4], sum[MT][4];
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            const uint32_t ones[4] = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) moe_mma(sum[mt], ones, b[mt][2 * ks], b[mt][2 * ks + 1], ks == 0);
+#pragma unroll
+            for (int blk = 0; blk < N; ++blk) {
+                uint32_t a[4];
+                code_word(ks == 0 ? w[blk].x : ks == 1 ? w[blk].y : ks == 2 ? w[blk].z : w[blk].w, a);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) moe_mma(c[blk][mt], a, b[mt][2 * ks], b[mt][2 * ks + 1], ks == 0);
+            }
+        }
+        // less 8 for every code, in the units of the rows
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float eight = sum[mt][i] * (i < 2 ? -0x1p-21f : -0x1p-17f);
+#pragma unroll
+                for (int blk = 0; blk < N; ++blk)
+                    acc[blk][mt][i] = fmaf(__half2float(__ushort_as_half(scale[blk][i >> 1])), c[blk][mt][i] + eight, acc[blk][mt][i]);
+            }
+    }
+};
+
+// A place in the ring of stages.
+template <int STAGES>
+struct MoeRing {
+    int stage;
+    uint32_t phase;
+    __device__ __forceinline__ void next() {
+        if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+// One consumer warp's share of a batch of N blocks: its chunk of `stages` stages, the last of which holds `last` chunks.
+// A stage is given back as soon as it is in registers.  Leaves the sums in `red` (this lane's address of the first
+// block's).  False once a wait has run out; the ring is walked to the batch's end all the same.
+template <int MT, int N>
+__device__ __forceinline__ bool moe_batch(uint32_t base, MoeRing<MoeCfg<MT>::STAGES>& ring, int stages, int last, int chunk,
+                                          uint32_t x_lane, uint32_t w_lane, uint32_t s_lane, uint32_t red, bool ok) {
+    using C = MoeCfg<MT>;
+    float acc[N][MT][4];
+#pragma unroll
+    for (int blk = 0; blk < N; ++blk)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[blk][mt][i] = 0.f;
+#pragma unroll 1
+    for (int st = 0; st < stages; ++st) {
+        const uint32_t sb = base + (uint32_t)(ring.stage * C::STAGE);
+        const bool there = st + 1 < stages || chunk < last;
+        ok = ok && __all_sync(0xffffffffu, mbar_wait_sleep(base + (uint32_t)(C::BARS + ring.stage * 8), ring.phase, kDevTimeoutExperts));
+        const uint32_t empty = base + (uint32_t)(C::BARS + (C::STAGES + ring.stage) * 8);
+        ring.next();
+        // one straight run, with the fragments alive in it alone: they and the sums take 130 registers
+        if (ok && there) {
+            MoeFragments<MT, N> f;
+            f.load(sb + x_lane, sb + w_lane, sb + s_lane);
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) mbar_arrive(empty);
+            f.multiply(acc);
+        } else {
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) mbar_arrive(empty);
+        }
+    }
+    bar_sync_named(1, kMoeConsumers * 32);           // the last batch's sums have been read
+#pragma unroll
+    for (int blk = 0; blk < N; ++blk)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+            sts128(red + (blk * kMoeChunks * MT + mt) * 512, make_float4(acc[blk][mt][0], acc[blk][mt][1], acc[blk][mt][2], acc[blk][mt][3]));
+    return ok;
 }
 
 // A CTA's walk: batches of up to 8 blocks of one (tile, K range), over its range of units.  Unit u is block u % blocks
-// of K range u / blocks % splits of tile u / blocks / splits.
+// of K range u / blocks % splits of tile u / blocks / splits.  Batches of one range are of one size to within a block: a
+// short last one would take as many turns as a full one (25 blocks as 8 + 8 + 8 + 1 instead of 7 + 6 + 6 + 6 made
+// the slowest CTA 36 us late where the others took 29).
+template <int BLOCKS>
 struct MoeWalk {
     int unit, end, blocks, splits;
     int tile, split, block, n;         // of the current batch
@@ -246,7 +360,8 @@ struct MoeWalk {
         block = unit - line * blocks;
         tile = line / splits;
         split = line - tile * splits;
-        n = min(min(kMoeBlocks, blocks - block), end - unit);
+        const int left = min(blocks - block, end - unit), batches = (left + BLOCKS - 1) / BLOCKS;
+        n = (left + batches - 1) / batches;
         return true;
     }
 };
@@ -294,7 +409,7 @@ static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(cons
 
     const int K = GATED ? p.hidden : p.inner, N = GATED ? 2 * p.inner : p.hidden;
     const int chunks = K >> 6, all_stages = (chunks + kMoeChunks - 1) / kMoeChunks;
-    MoeWalk walk;
+    MoeWalk<C::BLOCKS> walk;
     walk.blocks = N >> 4;
     walk.splits = GATED ? 1 : p.plan.splits;
     const long long units = (long long)tiles * walk.splits * walk.blocks;
@@ -354,91 +469,30 @@ static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(cons
 
     // ---------------------------------------------------- consumers
     // After a wait that ran out a warp computes nothing more but keeps every barrier, so that none waits for it.
-    const int chunk = warp & (kMoeChunks - 1), half = warp / kMoeChunks;
-    const int g8 = lane >> 2, t4 = lane & 3;
+    const int chunk = warp, g8 = lane >> 2, t4 = lane & 3;
     const uint32_t x_lane = C::W_BYTES + (lane & 7) * C::X_PITCH + chunk * 128 + (lane >> 3) * 16;
-    const uint32_t w_lane = (half * kMoeHalf * kMoeChunks + chunk) * 512 + lane * 16;
-    const uint32_t s_lane = C::W_BYTES + C::X_BYTES + (chunk * 64 / G) * C::S_ROW + half * kMoeHalf * 32 + g8 * 2;
+    const uint32_t w_lane = chunk * 512 + lane * 16;
+    const uint32_t s_lane = C::W_BYTES + C::X_BYTES + (chunk * 64 / G) * C::S_ROW + g8 * 2;
+    const uint32_t red_lane = red + chunk * MT * 512 + lane * 16;
     if (!GATED) {
         pdl_wait();                                      // the call before may still read what this one writes
         pdl_launch_dependents();
     }
     bool ok = true;
+    MoeRing<C::STAGES> ring = {0, 0};
     while (walk.next()) {
-        float acc[kMoeHalf][MT][4];
-#pragma unroll
-        for (int b = 0; b < kMoeHalf; ++b)
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[b][mt][i] = 0.f;
-        const int mine = walk.n - half * kMoeHalf;       // blocks of this warp (may be 0 or less)
-        const int s1 = all_stages * (walk.split + 1) / walk.splits;
-        for (int st = all_stages * walk.split / walk.splits; st < s1; ++st, ++it) {
-            const int s = it % C::STAGES, n = min(kMoeChunks, chunks - st * kMoeChunks);
-            ok = ok && __all_sync(0xffffffffu, mbar_wait_sleep(full(s), (it / C::STAGES) & 1, kDevTimeoutExperts));
-            if (ok && chunk < n && mine > 0) {
-                const uint32_t sb = stage(s);
-                uint32_t b[MT][8];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    ldmatrix_x4(*reinterpret_cast<uint32_t(*)[4]>(&b[mt][0]), sb + x_lane + mt * 8 * C::X_PITCH);
-                    ldmatrix_x4(*reinterpret_cast<uint32_t(*)[4]>(&b[mt][4]), sb + x_lane + mt * 8 * C::X_PITCH + 64);
-                }
-                // all four blocks of the half, there or not: the chains of a straight run interleave (sums of
-                // blocks past the batch, made of whatever the stage holds, are not read)
-                uint4 w4[kMoeHalf];
-                float scale[kMoeHalf][2];
-#pragma unroll
-                for (int blk = 0; blk < kMoeHalf; ++blk) {
-                    w4[blk] = lds128(sb + w_lane + blk * (kMoeChunks * 512));
-                    scale[blk][0] = __half2float(__ushort_as_half(lds_u16(sb + s_lane + blk * 32)));
-                    scale[blk][1] = __half2float(__ushort_as_half(lds_u16(sb + s_lane + blk * 32 + 16)));
-                }
-                float c[kMoeHalf][MT][4], sum[MT][4];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        sum[mt][i] = 0.f;
-#pragma unroll
-                        for (int blk = 0; blk < kMoeHalf; ++blk) c[blk][mt][i] = 0.f;
-                    }
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks) {
-                    const uint32_t ones[4] = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) moe_mma(sum[mt], ones, b[mt][2 * ks], b[mt][2 * ks + 1]);
-#pragma unroll
-                    for (int blk = 0; blk < kMoeHalf; ++blk) {
-                        uint32_t a[4];
-                        code_word(ks == 0 ? w4[blk].x : ks == 1 ? w4[blk].y : ks == 2 ? w4[blk].z : w4[blk].w, a);
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) moe_mma(c[blk][mt], a, b[mt][2 * ks], b[mt][2 * ks + 1]);
-                    }
-                }
-                // less 8 for every code, in the units of the rows
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float eight = sum[mt][i] * (i < 2 ? -0x1p-21f : -0x1p-17f);
-#pragma unroll
-                        for (int blk = 0; blk < kMoeHalf; ++blk)
-                            acc[blk][mt][i] = fmaf(scale[blk][i >> 1], c[blk][mt][i] + eight, acc[blk][mt][i]);
-                    }
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(empty(s));
+        const int s0 = all_stages * walk.split / walk.splits, stages = all_stages * (walk.split + 1) / walk.splits - s0;
+        const int last = min(kMoeChunks, chunks - (s0 + stages - 1) * kMoeChunks);
+        switch (walk.n) {
+#define W4A16_MOE_BATCH(N) \
+            case N: \
+                if constexpr (N <= C::BLOCKS) \
+                    ok = moe_batch<MT, N>(base, ring, stages, last, chunk, x_lane, w_lane, s_lane, red_lane, ok); \
+                break;
+            W4A16_MOE_BATCH(1) W4A16_MOE_BATCH(2) W4A16_MOE_BATCH(3) W4A16_MOE_BATCH(4) W4A16_MOE_BATCH(5)
+            W4A16_MOE_BATCH(6) W4A16_MOE_BATCH(7) W4A16_MOE_BATCH(8) W4A16_MOE_BATCH(9) W4A16_MOE_BATCH(10)
+#undef W4A16_MOE_BATCH
         }
-        // the 8 warps' sums of each block, in their order
-        bar_sync_named(1, kMoeConsumers * 32);           // the last batch's sums have been read
-#pragma unroll
-        for (int blk = 0; blk < kMoeHalf; ++blk)
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-                sts128(red + ((((half * kMoeHalf + blk) * kMoeChunks + chunk) * MT + mt) * 32 + lane) * 16,
-                       make_float4(acc[blk][mt][0], acc[blk][mt][1], acc[blk][mt][2], acc[blk][mt][3]));
         bar_sync_named(2, kMoeConsumers * 32);
         const int4 tile = tile_at(walk.tile);
         for (int i = warp; i < walk.n * MT; i += kMoeConsumers) {
@@ -470,37 +524,41 @@ static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(cons
     }
 }
 
-constexpr int kMoeFinishThreads = 256;
+constexpr int kMoeFinishThreads = 128;
 
-// y = residual + the entries' results, weighted, in the order of the choices and their K ranges: four columns a thread.
+// y = residual + the entries' results, weighted, in the order of the choices and their K ranges: four columns a thread, and
+// SLICES threads (of different warps) to share those columns' parts, whose sums are added in order.  Bound by the
+// latency of its loads: each thread has 8 in flight.
+template <int SLICES>
 static __global__ void __launch_bounds__(kMoeFinishThreads) moe_finish_kernel(const __grid_constant__ MoeParams p) {
+    constexpr int QUADS = kMoeFinishThreads / SLICES;
+    __shared__ float4 shared[SLICES > 1 ? kMoeFinishThreads : 1];
     const int64_t token = blockIdx.x;
-    const int col = (blockIdx.y * kMoeFinishThreads + threadIdx.x) * 4;
+    const int slice = threadIdx.x / QUADS, col = (blockIdx.y * QUADS + threadIdx.x % QUADS) * 4;
     const bool in_row = col < p.hidden;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (p.residual && in_row) {          // an input of the call: there before the products began
+    if (p.residual && in_row && slice == 0) {          // an input of the call: there before the products began
         const uint2 r = *reinterpret_cast<const uint2*>(p.residual + token * p.hidden + col);
         const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
         v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
     }
+    const int parts = p.k * p.plan.splits, per = (parts + SLICES - 1) / SLICES;
+    const int end = min(parts, (slice + 1) * per);
     pdl_wait();
     pdl_launch_dependents();
-    if (!in_row) return;
-    // eight (choice, K range) pairs' loads in flight at a time; what an expert outside the layer would have
-    // left is loaded too, and dropped
-    const int parts = p.k * p.plan.splits;
-    for (int i0 = 0; i0 < parts; i0 += 8) {
+    // what an expert outside the layer would have left is loaded too, and dropped
+    for (int i0 = slice * per; i0 < end && in_row; i0 += 8) {
         float4 d[8];
         float w[8];
         bool in[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int part = min(i0 + i, parts - 1), j = part / p.plan.splits, range = part - j * p.plan.splits;
+            const int part = min(i0 + i, end - 1), j = part / p.plan.splits, range = part - j * p.plan.splits;
             const int64_t entry = token * p.k + j;
+            d[i] = __ldcg(reinterpret_cast<const float4*>(moe_out(p) + (range * (int64_t)p.entries + entry) * p.hidden + col));
             const int e = __ldg(p.experts + entry);
             w[i] = __ldg(p.weights + entry);
-            d[i] = __ldcg(reinterpret_cast<const float4*>(moe_out(p) + (range * (int64_t)p.entries + entry) * p.hidden + col));
-            in[i] = i0 + i < parts && e >= 0 && e < p.num_experts;
+            in[i] = i0 + i < end && e >= 0 && e < p.num_experts;
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -511,6 +569,17 @@ static __global__ void __launch_bounds__(kMoeFinishThreads) moe_finish_kernel(co
                 v[3] = fmaf(w[i], d[i].w, v[3]);
             }
     }
+    if constexpr (SLICES > 1) {
+        shared[threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
+        __syncthreads();
+        if (slice > 0) return;
+#pragma unroll
+        for (int i = 1; i < SLICES; ++i) {
+            const float4 f = shared[i * QUADS + threadIdx.x];
+            v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
+        }
+    }
+    if (!in_row) return;
     const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
     *reinterpret_cast<uint2*>(p.y + token * p.hidden + col) =
         make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));

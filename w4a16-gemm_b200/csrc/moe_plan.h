@@ -16,7 +16,6 @@
 namespace w4a16 {
 
 constexpr int kMoeMaxExperts = 1024;
-constexpr int kMoeBlocks = 8;        // n16 blocks of a batch
 constexpr int kMoeChunks = 8;        // 64-wide K chunks of a stage
 // Up to this many entries every CTA of the products sorts them for itself; above, one kernel does it for all.
 constexpr int kMoeFewEntries = 1024;
