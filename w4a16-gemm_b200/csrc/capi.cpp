@@ -14,7 +14,6 @@
 
 #include "../../include/w4a16.h"
 #include "internal.h"
-#include "moe_plan.h"
 
 namespace {
 

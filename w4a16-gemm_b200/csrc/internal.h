@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "../../include/w4a16.h"
+#include "moe_plan.h"
 
 namespace w4a16 {
 
@@ -94,6 +95,19 @@ struct PrefillPlan {
 // config 1..4 forces a token tile (32 / 64 / 128 / 256); 0 = choose from the shape.
 PrefillPlan plan_prefill(int M, int N, int K, int G, int config, const DeviceInfo& dev);
 cudaError_t launch_prefill(const GemmArgs& a, const PrefillPlan& p);
+
+// One product of an expert layer over rows sorted by expert (kernels.cu): [rows, K] times the expert's [N, K] each.
+struct GroupedArgs {
+    const void *wp, *x, *scales;   // all experts' words and scales, one expert after the other
+    void* y;                       // gated: fp16 [rows, N / 2]; else fp32 [rows, N]
+    int rows, experts, N, K, G;
+    bool gated;
+    int32_t activation;
+    MoeGroups groups;
+    cudaStream_t stream;
+    bool pdl;
+};
+cudaError_t launch_grouped(const GroupedArgs& a, const DeviceInfo& dev);
 
 // ---------------------------------------------------------------- load-time format kernels
 // codes uint8 [N, K] -> packed words (N % 16 == 0, K % 64 == 0, 16-byte aligned pointers).

@@ -15,6 +15,7 @@
 #include "ptx.cuh"
 #include "decode.cuh"
 #include "prefill.cuh"
+#include "moe_grouped.cuh"
 #include "dequant_kernel.cuh"
 #include "format_kernels.cuh"
 #include "tp_exchange.cuh"
@@ -185,6 +186,25 @@ cudaError_t make_prefill_tensor_maps(const GemmArgs& a, int tok, CUtensorMap* tx
         if ((err = encode_tiled(k, ts)) != cudaSuccess) return err;
     }
     return cudaSuccess;
+}
+
+cudaError_t make_grouped_tensor_maps(const GroupedArgs& a, CUtensorMap* tx, CUtensorMap* tw) {
+    cudaError_t err;
+    const int chunks = std::min(MgCfg::KCH, a.K / 64);
+    {
+        TmapKey k = tmap_key(a.x, 3, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_TENSOR_MAP_SWIZZLE_128B,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+        k.dims[0] = 64; k.dims[1] = (uint64_t)a.rows; k.dims[2] = (uint64_t)(a.K / 64);
+        k.strides[0] = (uint64_t)a.K * 2; k.strides[1] = 128;
+        k.box[0] = 64; k.box[1] = (uint32_t)MgCfg::TOK; k.box[2] = (uint32_t)chunks;
+        if ((err = encode_tiled(k, tx)) != cudaSuccess) return err;
+    }
+    TmapKey k = tmap_key(a.wp, 3, CU_TENSOR_MAP_DATA_TYPE_INT32, CU_TENSOR_MAP_SWIZZLE_NONE,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+    k.dims[0] = 128; k.dims[1] = (uint64_t)(a.K / 64); k.dims[2] = (uint64_t)a.experts * (uint64_t)(a.N / 16);
+    k.strides[0] = 512; k.strides[1] = (uint64_t)(a.K / 64) * 512;
+    k.box[0] = 128; k.box[1] = (uint32_t)chunks; k.box[2] = 8;
+    return encode_tiled(k, tw);
 }
 
 cudaError_t make_decode_tensor_maps(const GemmArgs& a, int box_blocks, int box_chunks, int mp, CUtensorMap* tw,

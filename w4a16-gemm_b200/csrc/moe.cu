@@ -24,19 +24,17 @@ size_t moe_workspace(const w4a16_moe_args& a, const DeviceInfo& dev) {
     return moe_plan(a.tokens, a.k, a.num_experts, a.hidden, a.inner, dev.num_sms).bytes;
 }
 
-template <int G, int MT, bool GATED>
+template <int G, bool GATED>
 static cudaError_t launch_product_t(const MoeParams& p, int grid, cudaStream_t stream, bool pdl) {
-    auto kern = moe_product_kernel<G, MT, GATED>;
+    auto kern = moe_product_kernel<G, GATED>;
     const cudaError_t err = ensure_max_dynamic_smem(reinterpret_cast<const void*>(kern));
     if (err != cudaSuccess) return err;
-    return launch(kern, dim3(grid), kMoeThreads, MoeCfg<MT>::SMEM, stream, pdl, p);
+    return launch(kern, dim3(grid), kMoeThreads, MoeCfg::SMEM, stream, pdl, p);
 }
 
 template <bool GATED>
 static cudaError_t launch_product(const MoeParams& p, int G, int grid, cudaStream_t stream, bool pdl) {
-    if (p.plan.rows == 8)
-        return G == 64 ? launch_product_t<64, 1, GATED>(p, grid, stream, pdl) : launch_product_t<128, 1, GATED>(p, grid, stream, pdl);
-    return G == 64 ? launch_product_t<64, 2, GATED>(p, grid, stream, pdl) : launch_product_t<128, 2, GATED>(p, grid, stream, pdl);
+    return G == 64 ? launch_product_t<64, GATED>(p, grid, stream, pdl) : launch_product_t<128, GATED>(p, grid, stream, pdl);
 }
 
 cudaError_t launch_moe_experts(const w4a16_moe_args& a, const DeviceInfo& dev, void* workspace, cudaStream_t stream, bool pdl) {
@@ -59,9 +57,32 @@ cudaError_t launch_moe_experts(const w4a16_moe_args& a, const DeviceInfo& dev, v
     p.inner = a.inner;
     p.activation = a.activation;
     cudaError_t err = p.plan.few ? cudaSuccess : launch(moe_plan_kernel, dim3(1), kMoePlanThreads, 0, stream, pdl, p);
-    if (err == cudaSuccess) err = launch_product<true>(p, a.gate_up_group, dev.num_sms, stream, pdl);
-    if (err == cudaSuccess) err = launch_product<false>(p, a.down_group, dev.num_sms, stream, pdl);
+    if (p.plan.grouped) {
+        constexpr int rows = kMoeGatherThreads / 32;
+        if (err == cudaSuccess)
+            err = launch(moe_gather_kernel, dim3((unsigned)((p.entries + rows - 1) / rows)), kMoeGatherThreads, 0, stream, pdl, p);
+        GroupedArgs g = {a.gate_up_wp, p.workspace + p.plan.rows_at, a.gate_up_scales, p.workspace + p.plan.inner_at, p.entries,
+                         a.num_experts, 2 * a.inner, a.hidden, a.gate_up_group, true, a.activation,
+                         {reinterpret_cast<MoeHead*>(p.workspace), reinterpret_cast<MoeTile*>(p.workspace + p.plan.tiles_at),
+                          2 * a.inner / 16, a.hidden / a.gate_up_group}, stream, pdl};
+        if (err == cudaSuccess) err = launch_grouped(g, dev);
+        g.wp = a.down_wp;
+        g.x = p.workspace + p.plan.inner_at;
+        g.scales = a.down_scales;
+        g.y = p.workspace + p.plan.out_at;
+        g.N = a.hidden;
+        g.K = a.inner;
+        g.G = a.down_group;
+        g.gated = false;
+        g.groups.blocks = a.hidden / 16;
+        g.groups.scale_rows = a.inner / a.down_group;
+        if (err == cudaSuccess) err = launch_grouped(g, dev);
+    } else {
+        if (err == cudaSuccess) err = launch_product<true>(p, a.gate_up_group, dev.num_sms, stream, pdl);
+        if (err == cudaSuccess) err = launch_product<false>(p, a.down_group, dev.num_sms, stream, pdl);
+    }
     if (err != cudaSuccess) return err;
+    if (p.plan.grouped) return launch(moe_grouped_finish_kernel, dim3((unsigned)a.tokens), kMoeFinishThreads, 0, stream, pdl, p);
     const auto finish = [&](auto kern, int slices) {
         const int cols = 4 * kMoeFinishThreads / slices;
         return launch(kern, dim3((unsigned)a.tokens, (unsigned)((a.hidden + cols - 1) / cols)), kMoeFinishThreads, 0, stream, pdl, p);

@@ -3,10 +3,13 @@
 //     h_tj = act(x_t Wg_e^T) * (x_t Wu_e^T),   e = experts[t][j]
 //     y_t  = residual_t + sum_j weights[t][j] (h_tj Wd_e^T)
 //
-// Three kernels, each launched behind the one before with programmatic dependent launch: the gated product,
-// the second product, the weighted sum.  The products stream the weights of the experts that were chosen, each once a
-// tile.  Which entries make which tile every CTA works out for itself, from up to 1024 entries (about 1 us, where a
-// kernel in front takes 4); above that a kernel does it once, in front.
+// Few entries an expert: three kernels, each launched behind the one before with programmatic dependent launch: the
+// gated product, the second product, the weighted sum.  The products stream the weights of the experts that
+// were chosen, each once a tile.  Which entries make which tile every CTA works out for itself, from up to 1024
+// entries (about 1 us, where a kernel in front takes 4); above that a kernel does it once, in front.
+//
+// Many entries an expert (more than 14 on average): the products of moe_grouped.cuh, over rows of x that a kernel puts
+// into sorted order first.
 //
 // The second product's CTAs start where the first one's leave, and fetch their first weights before the first
 // one has ended: what that reads was written before the call, or by the kernel in front, and the gated product lets
@@ -35,7 +38,6 @@
 
 #include "epilogue.cuh"
 #include "internal.h"
-#include "moe_plan.h"
 #include "ptx.cuh"
 
 namespace w4a16 {
@@ -45,23 +47,21 @@ constexpr int kMoeProducers = 3;                          // warps: packed words
 constexpr int kMoeThreads = (kMoeConsumers + kMoeProducers) * 32;
 constexpr int kMoePlanThreads = 1024;
 
-template <int MT>
 struct MoeCfg {
-    static constexpr int ROWS = 8 * MT;
-    static constexpr int BLOCKS = MT == 1 ? 10 : 6;                   // n16 blocks of a batch, at most
+    static constexpr int BLOCKS = 10;                                 // n16 blocks of a batch, at most
     static constexpr int X_PITCH = kMoeChunks * 128 + 16;             // rows 16 bytes apart in banks: ldmatrix without conflicts
     static constexpr int W_BYTES = BLOCKS * kMoeChunks * 512;     // [block][chunk][32 lanes x 16 B]
-    static constexpr int X_BYTES = ROWS * X_PITCH;
+    static constexpr int X_BYTES = kMoeRows * X_PITCH;
     static constexpr int S_ROW = BLOCKS * 32;                     // scales of one group of K: [block][16]
     static constexpr int S_BYTES = kMoeChunks * S_ROW;
     static constexpr int STAGE = W_BYTES + X_BYTES + S_BYTES;
-    static constexpr int STAGES = MT == 1 ? 3 : 4;
-    static constexpr int RED_BYTES = BLOCKS * kMoeChunks * MT * 512;   // [block][chunk warp][mt][lane] float4
+    static constexpr int STAGES = 3;
+    static constexpr int RED_BYTES = BLOCKS * kMoeChunks * 512;        // [block][chunk warp][lane] float4
     static constexpr int BARS = STAGES * STAGE + RED_BYTES;
     static constexpr int PLAN = BARS + 2 * STAGES * 8;                     // tiles of few entries, their order
     static constexpr int SMEM = 128 + PLAN + kMoeFewEntries * (8 + 2);
     static_assert(RED_BYTES >= kMoeMaxExperts * 8 + kMoeFewEntries * 6, "the sort's scratch");
-    static_assert(STAGE % 16 == 0 && SMEM <= 227 * 1024, "shared memory");
+    static_assert(BLOCKS == 10 && STAGE % 16 == 0 && SMEM <= 227 * 1024, "shared memory");
 };
 
 struct MoeParams {
@@ -80,6 +80,7 @@ struct MoeParams {
 __device__ __forceinline__ MoeHead* moe_head(const MoeParams& p) { return reinterpret_cast<MoeHead*>(p.workspace); }
 __device__ __forceinline__ int4* moe_tiles(const MoeParams& p) { return reinterpret_cast<int4*>(p.workspace + p.plan.tiles_at); }
 __device__ __forceinline__ int32_t* moe_order(const MoeParams& p) { return reinterpret_cast<int32_t*>(p.workspace + p.plan.order_at); }
+__device__ __forceinline__ int32_t* moe_place(const MoeParams& p) { return reinterpret_cast<int32_t*>(p.workspace + p.plan.place_at); }
 __device__ __forceinline__ __half* moe_inner(const MoeParams& p) { return reinterpret_cast<__half*>(p.workspace + p.plan.inner_at); }
 __device__ __forceinline__ float* moe_out(const MoeParams& p) { return reinterpret_cast<float*>(p.workspace + p.plan.out_at); }
 
@@ -117,9 +118,18 @@ static __global__ void __launch_bounds__(kMoePlanThreads) moe_plan_kernel(const 
     count[t] = 0;
     pdl_wait();
     __syncthreads();
-    for (int i = t; i < p.entries; i += kMoePlanThreads) {
-        const int e = __ldg(p.experts + i);
-        if (e >= 0 && e < p.num_experts) atomicAdd(&count[e], 1);
+    const auto expert_of = [&](int i) {
+        const int e = i < p.entries ? __ldg(p.experts + i) : -1;
+        return e >= 0 && e < p.num_experts ? e : -1;
+    };
+    constexpr int AHEAD = 8;                              // loads in flight
+    for (int i0 = t; i0 < p.entries; i0 += AHEAD * kMoePlanThreads) {
+        int e[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) e[j] = expert_of(i0 + j * kMoePlanThreads);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+            if (e[j] >= 0) atomicAdd(&count[e[j]], 1);
     }
     __syncthreads();
     const int mine = count[t], rows = p.plan.rows, tiles = (mine + rows - 1) / rows;
@@ -133,9 +143,39 @@ static __global__ void __launch_bounds__(kMoePlanThreads) moe_plan_kernel(const 
     }
     __syncthreads();
     int32_t* const order = moe_order(p);
-    for (int i = t; i < p.entries; i += kMoePlanThreads) {
-        const int e = __ldg(p.experts + i);
-        if (e >= 0 && e < p.num_experts) order[atomicAdd(&cursor[e], 1)] = i;
+    for (int i0 = t; i0 < p.entries; i0 += AHEAD * kMoePlanThreads) {
+        int e[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) e[j] = expert_of(i0 + j * kMoePlanThreads);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+            if (e[j] >= 0) {
+                const int i = i0 + j * kMoePlanThreads, at = atomicAdd(&cursor[e[j]], 1);
+                order[at] = i;
+                if (p.plan.grouped) moe_place(p)[i] = at;
+            }
+    }
+}
+
+// Rows of x in sorted order: a warp a row.
+constexpr int kMoeGatherThreads = 256;
+static __global__ void __launch_bounds__(kMoeGatherThreads) moe_gather_kernel(const __grid_constant__ MoeParams p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int64_t row = (int64_t)blockIdx.x * (kMoeGatherThreads / 32) + threadIdx.x / 32;
+    if (row >= __ldcg(&moe_head(p)->entries)) return;
+    const int64_t token = __ldcg(moe_order(p) + row) / p.k;
+    const uint4* const from = reinterpret_cast<const uint4*>(p.x + token * p.hidden);
+    uint4* const to = reinterpret_cast<uint4*>(p.workspace + p.plan.rows_at) + row * (p.hidden / 8);
+    const int units = p.hidden / 8;
+    for (int i = threadIdx.x & 31; i < units; i += 8 * 32) {      // eight loads in flight
+        uint4 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i + j * 32 < units) v[j] = from[i + j * 32];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i + j * 32 < units) to[i + j * 32] = v[j];
     }
 }
 
@@ -242,18 +282,15 @@ __device__ __forceinline__ void moe_mma(float (&c)[4], const uint32_t (&a)[4], u
 }
 
 // What a warp takes out of a stage: its chunk's rows, the N blocks' words and scales.
-template <int MT, int N>
+template <int N>
 struct MoeFragments {
-    uint32_t b[MT][8];
+    uint32_t b[8];
     uint4 w[N];
     uint16_t scale[N][2];
     // x_at, w_at, s_at: this lane's shared-memory addresses
     __device__ __forceinline__ void load(uint32_t x_at, uint32_t w_at, uint32_t s_at) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            ldmatrix_x4(*reinterpret_cast<uint32_t(*)[4]>(&b[mt][0]), x_at + mt * 8 * MoeCfg<MT>::X_PITCH);
-            ldmatrix_x4(*reinterpret_cast<uint32_t(*)[4]>(&b[mt][4]), x_at + mt * 8 * MoeCfg<MT>::X_PITCH + 64);
-        }
+        ldmatrix_x4(*reinterpret_cast<uint32_t(*)[4]>(&b[0]), x_at);
+        ldmatrix_x4(*reinterpret_cast<uint32_t(*)[4]>(&b[4]), x_at + 64);
 #pragma unroll
         for (int blk = 0; blk < N; ++blk) {
             w[blk] = lds128(w_at + blk * (kMoeChunks * 512));
@@ -262,31 +299,27 @@ struct MoeFragments {
         }
     }
     // Products of the chunk, added to the blocks' sums.
-    __device__ __forceinline__ void multiply(float (&acc)[N][MT][4]) const {
-        float c[N][MT][4], sum[MT][4];
+    __device__ __forceinline__ void multiply(float (&acc)[N][4]) const {
+        float c[N][4], sum[4];
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
             const uint32_t ones[4] = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) moe_mma(sum[mt], ones, b[mt][2 * ks], b[mt][2 * ks + 1], ks == 0);
+            moe_mma(sum, ones, b[2 * ks], b[2 * ks + 1], ks == 0);
 #pragma unroll
             for (int blk = 0; blk < N; ++blk) {
                 uint32_t a[4];
                 code_word(ks == 0 ? w[blk].x : ks == 1 ? w[blk].y : ks == 2 ? w[blk].z : w[blk].w, a);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) moe_mma(c[blk][mt], a, b[mt][2 * ks], b[mt][2 * ks + 1], ks == 0);
+                moe_mma(c[blk], a, b[2 * ks], b[2 * ks + 1], ks == 0);
             }
         }
         // less 8 for every code, in the units of the rows
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int i = 0; i < 4; ++i) {
+            const float eight = sum[i] * (i < 2 ? -0x1p-21f : -0x1p-17f);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float eight = sum[mt][i] * (i < 2 ? -0x1p-21f : -0x1p-17f);
-#pragma unroll
-                for (int blk = 0; blk < N; ++blk)
-                    acc[blk][mt][i] = fmaf(__half2float(__ushort_as_half(scale[blk][i >> 1])), c[blk][mt][i] + eight, acc[blk][mt][i]);
-            }
+            for (int blk = 0; blk < N; ++blk)
+                acc[blk][i] = fmaf(__half2float(__ushort_as_half(scale[blk][i >> 1])), c[blk][i] + eight, acc[blk][i]);
+        }
     }
 };
 
@@ -306,17 +339,15 @@ struct MoeRing {
 // One consumer warp's share of a batch of N blocks: its chunk of `stages` stages, the last of which holds `last` chunks.
 // A stage is given back as soon as it is in registers.  Leaves the sums in `red` (this lane's address of the first
 // block's).  False once a wait has run out; the ring is walked to the batch's end all the same.
-template <int MT, int N>
-__device__ __forceinline__ bool moe_batch(uint32_t base, MoeRing<MoeCfg<MT>::STAGES>& ring, int stages, int last, int chunk,
+template <int N>
+__device__ __forceinline__ bool moe_batch(uint32_t base, MoeRing<MoeCfg::STAGES>& ring, int stages, int last, int chunk,
                                           uint32_t x_lane, uint32_t w_lane, uint32_t s_lane, uint32_t red, bool ok) {
-    using C = MoeCfg<MT>;
-    float acc[N][MT][4];
+    using C = MoeCfg;
+    float acc[N][4];
 #pragma unroll
     for (int blk = 0; blk < N; ++blk)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[blk][mt][i] = 0.f;
+        for (int i = 0; i < 4; ++i) acc[blk][i] = 0.f;
 #pragma unroll 1
     for (int st = 0; st < stages; ++st) {
         const uint32_t sb = base + (uint32_t)(ring.stage * C::STAGE);
@@ -326,7 +357,7 @@ __device__ __forceinline__ bool moe_batch(uint32_t base, MoeRing<MoeCfg<MT>::STA
         ring.next();
         // one straight run, with the fragments alive in it alone: they and the sums take 130 registers
         if (ok && there) {
-            MoeFragments<MT, N> f;
+            MoeFragments<N> f;
             f.load(sb + x_lane, sb + w_lane, sb + s_lane);
             __syncwarp();
             if ((threadIdx.x & 31) == 0) mbar_arrive(empty);
@@ -339,9 +370,7 @@ __device__ __forceinline__ bool moe_batch(uint32_t base, MoeRing<MoeCfg<MT>::STA
     bar_sync_named(1, kMoeConsumers * 32);           // the last batch's sums have been read
 #pragma unroll
     for (int blk = 0; blk < N; ++blk)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-            sts128(red + (blk * kMoeChunks * MT + mt) * 512, make_float4(acc[blk][mt][0], acc[blk][mt][1], acc[blk][mt][2], acc[blk][mt][3]));
+        sts128(red + blk * kMoeChunks * 512, make_float4(acc[blk][0], acc[blk][1], acc[blk][2], acc[blk][3]));
     return ok;
 }
 
@@ -368,9 +397,9 @@ struct MoeWalk {
 
 // GATED: the first product (rows of x, gated, into the workspace in sorted order); else the second (rows of the
 // first's results, into the workspace by entry and K range).
-template <int G, int MT, bool GATED>
+template <int G, bool GATED>
 static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(const __grid_constant__ MoeParams p) {
-    using C = MoeCfg<MT>;
+    using C = MoeCfg;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 127u) & ~127u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -473,7 +502,7 @@ static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(cons
     const uint32_t x_lane = C::W_BYTES + (lane & 7) * C::X_PITCH + chunk * 128 + (lane >> 3) * 16;
     const uint32_t w_lane = chunk * 512 + lane * 16;
     const uint32_t s_lane = C::W_BYTES + C::X_BYTES + (chunk * 64 / G) * C::S_ROW + g8 * 2;
-    const uint32_t red_lane = red + chunk * MT * 512 + lane * 16;
+    const uint32_t red_lane = red + chunk * 512 + lane * 16;
     if (!GATED) {
         pdl_wait();                                      // the call before may still read what this one writes
         pdl_launch_dependents();
@@ -486,8 +515,7 @@ static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(cons
         switch (walk.n) {
 #define W4A16_MOE_BATCH(N) \
             case N: \
-                if constexpr (N <= C::BLOCKS) \
-                    ok = moe_batch<MT, N>(base, ring, stages, last, chunk, x_lane, w_lane, s_lane, red_lane, ok); \
+                ok = moe_batch<N>(base, ring, stages, last, chunk, x_lane, w_lane, s_lane, red_lane, ok); \
                 break;
             W4A16_MOE_BATCH(1) W4A16_MOE_BATCH(2) W4A16_MOE_BATCH(3) W4A16_MOE_BATCH(4) W4A16_MOE_BATCH(5)
             W4A16_MOE_BATCH(6) W4A16_MOE_BATCH(7) W4A16_MOE_BATCH(8) W4A16_MOE_BATCH(9) W4A16_MOE_BATCH(10)
@@ -495,12 +523,11 @@ static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(cons
         }
         bar_sync_named(2, kMoeConsumers * 32);
         const int4 tile = tile_at(walk.tile);
-        for (int i = warp; i < walk.n * MT; i += kMoeConsumers) {
-            const int blk = i / MT, mt = i % MT;
+        for (int blk = warp; blk < walk.n; blk += kMoeConsumers) {
             float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < kMoeChunks; ++c) {
-                const float4 f = lds128f(red + (((blk * kMoeChunks + c) * MT + mt) * 32 + lane) * 16);
+                const float4 f = lds128f(red + ((blk * kMoeChunks + c) * 32 + lane) * 16);
                 v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
             }
             v[0] *= 0x1p24f; v[1] *= 0x1p24f; v[2] *= 0x1p20f; v[3] *= 0x1p20f;
@@ -508,7 +535,7 @@ static __global__ void __launch_bounds__(kMoeThreads, 1) moe_product_kernel(cons
             const int nb = walk.block + blk;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int row = mt * 8 + 2 * t4 + j;
+                const int row = 2 * t4 + j;
                 if (row >= tile.z) continue;
                 if (GATED) {
                     moe_inner(p)[(int64_t)(tile.y + row) * p.inner + nb * 8 + g8] =
@@ -583,6 +610,52 @@ static __global__ void __launch_bounds__(kMoeFinishThreads) moe_finish_kernel(co
     const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
     *reinterpret_cast<uint2*>(p.y + token * p.hidden + col) =
         make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+// The same over the grouped products' results (in sorted order): a CTA a token, four columns a thread and turn.  Its
+// choices' rows and weights are looked up once; bound by the memory's bandwidth.
+static __global__ void __launch_bounds__(kMoeFinishThreads) moe_grouped_finish_kernel(const __grid_constant__ MoeParams p) {
+    __shared__ int32_t row[32];
+    __shared__ float weight[32];
+    const int64_t token = blockIdx.x;
+    pdl_wait();
+    pdl_launch_dependents();
+    if ((int)threadIdx.x < p.k) {
+        const int64_t entry = token * p.k + threadIdx.x;
+        const int e = __ldg(p.experts + entry);
+        const bool in = e >= 0 && e < p.num_experts;
+        row[threadIdx.x] = in ? __ldcg(moe_place(p) + entry) : -1;
+        weight[threadIdx.x] = in ? __ldg(p.weights + entry) : 0.f;
+    }
+    __syncthreads();
+    const float4* const out = reinterpret_cast<const float4*>(moe_out(p));
+    const int quads = p.hidden / 4;
+    for (int c = threadIdx.x; c < quads; c += kMoeFinishThreads) {
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (p.residual) {
+            const uint2 r = reinterpret_cast<const uint2*>(p.residual + token * p.hidden)[c];
+            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
+            v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+        }
+        for (int j0 = 0; j0 < p.k; j0 += 8) {
+            float4 d[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j0 + j < p.k && row[j0 + j] >= 0) d[j] = __ldcg(out + (int64_t)row[j0 + j] * quads + c);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j0 + j < p.k && row[j0 + j] >= 0) {
+                    const float w = weight[j0 + j];
+                    v[0] = fmaf(w, d[j].x, v[0]);
+                    v[1] = fmaf(w, d[j].y, v[1]);
+                    v[2] = fmaf(w, d[j].z, v[2]);
+                    v[3] = fmaf(w, d[j].w, v[3]);
+                }
+        }
+        const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+        reinterpret_cast<uint2*>(p.y + token * p.hidden)[c] =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
 }
 
 }  // namespace w4a16

@@ -17,6 +17,7 @@ namespace w4a16 {
 
 constexpr int kMoeMaxExperts = 1024;
 constexpr int kMoeChunks = 8;        // 64-wide K chunks of a stage
+constexpr int kMoeRows = 8;          // entries of a tile
 // Up to this many entries every CTA of the products sorts them for itself; above, one kernel does it for all.
 constexpr int kMoeFewEntries = 1024;
 
@@ -31,21 +32,41 @@ struct MoeHead {
     int32_t pad[62];
 };
 
+// What a grouped product reads of it: the tiles, and how far apart the experts' weights and scales are.
+struct MoeGroups {
+    const MoeHead* head;
+    const MoeTile* tiles;
+    int32_t blocks;          // n16 blocks of one expert's weight
+    int32_t scale_rows;      // rows of one expert's scales
+};
+
 struct MoePlan {
     int32_t rows;            // entries of a tile
     int32_t max_tiles;       // no routing makes more
     int32_t splits;          // K ranges of the second product
     bool few;                // every CTA sorts the entries
-    size_t tiles_at, order_at, inner_at, out_at, bytes;    // offsets in the workspace
+    bool grouped;            // many entries an expert: the tensor-core products of prompts over sorted rows
+    // offsets in the workspace: tiles, entries in sorted order, where each entry went (grouped), rows of x in sorted
+    // order (grouped), the gated product's results, the second one's
+    size_t tiles_at, order_at, place_at, rows_at, inner_at, out_at, bytes;
 };
+
+constexpr int kMoeGroupedEntries = 14;
+
+constexpr int kMoeGroupedRows = 64;  // entries of a grouped product's tile, at most
 
 W4A16_HD inline size_t moe_align(size_t n) { return (n + 255) / 256 * 256; }
 
 inline MoePlan moe_plan(int64_t tokens, int k, int experts, int hidden, int inner, int num_sms) {
     MoePlan p = {};
     const int64_t entries = tokens * k;
-    // 8 entries a tile where an expert seldom gets more (at most 8 tokens, or 4 entries for each expert), else 16
-    p.rows = tokens <= 8 || entries <= 4 * (int64_t)experts ? 8 : 16;
+    // more than 14 entries an expert: the experts' words are worth making into tensor-core operands for all of them (16
+    // entries an expert: 128 experts of 2048 x 768 262 us as few, 166 grouped; 64 of 2048 x 1408 186 and 165; 8 of 4096 x
+    // 14336 351 and 366; 24: 247 and 169, 467 and 367)
+    p.grouped = entries > kMoeGroupedEntries * (int64_t)experts;
+    // else 8, the width of mma.m16n8k16: with 16 a tile's two products for every word cost more than reading the words
+    // of an expert twice (64 experts, 3 entries each: 82 us and 102; 8 each: 118 and 128)
+    p.rows = p.grouped ? kMoeGroupedRows : kMoeRows;
     // every expert's last tile may be short; no tile is empty
     const int64_t most = entries / p.rows + (experts < entries ? experts : entries);
     p.max_tiles = (int32_t)(most < entries ? most : entries);
@@ -54,11 +75,13 @@ inline MoePlan moe_plan(int64_t tokens, int k, int experts, int hidden, int inne
     const int64_t units = (entries < experts ? entries : experts) * (hidden / 16);
     const int stages = (inner / 64 + kMoeChunks - 1) / kMoeChunks;
     p.splits = 1;
-    while (p.splits < 4 && 2 * p.splits <= stages && units * p.splits < 8 * (int64_t)num_sms) p.splits *= 2;
-    p.few = entries <= kMoeFewEntries;
+    while (!p.grouped && p.splits < 4 && 2 * p.splits <= stages && units * p.splits < 8 * (int64_t)num_sms) p.splits *= 2;
+    p.few = !p.grouped && entries <= kMoeFewEntries;
     p.tiles_at = sizeof(MoeHead);
     p.order_at = moe_align(p.tiles_at + (size_t)p.max_tiles * sizeof(MoeTile));
-    p.inner_at = moe_align(p.order_at + (size_t)entries * 4);
+    p.place_at = moe_align(p.order_at + (size_t)entries * 4);
+    p.rows_at = moe_align(p.place_at + (p.grouped ? (size_t)entries * 4 : 0));
+    p.inner_at = moe_align(p.rows_at + (p.grouped ? (size_t)entries * hidden * 2 : 0));
     p.out_at = moe_align(p.inner_at + (size_t)entries * inner * 2);
     p.bytes = moe_align(p.out_at + (size_t)p.splits * entries * hidden * 4);
     return p;
