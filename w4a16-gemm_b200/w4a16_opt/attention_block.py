@@ -1,12 +1,14 @@
 """An attention block served from 4-bit weights and a 4-bit cache, and a command that runs it.
 
-    PYTHONPATH=w4a16-gemm_b200 python -m w4a16_opt.attention_block [--batch B] [--prompt N] [--steps K]
+    PYTHONPATH=w4a16-gemm_b200 python -m w4a16_opt.attention_block [--batch B] [--prompt N] [--steps K] [--layer dense|experts]
 
 The block is what stands between two residual additions of a decoder: QKV projection
 (``w4a16_gemm``), rotary positions and the quantised write of keys and values (``cache_append``),
-attention over the cache (``cache_attention``), output projection.  The command fills a batch of
-prompts of different lengths in one call and then decodes token by token from a captured CUDA
-graph, with random weights of the Llama-3-8B attention shapes.
+attention over the cache (``cache_attention``), output projection.  With a norm it takes and returns the residual
+stream itself (``rms_norm`` before the first projection, the addition in the epilogue of the last, ``w4a16_linear``).
+The command fills a batch of prompts of different lengths in one call and then decodes token by token from a
+captured CUDA graph, with random weights of the Llama-3-8B attention shapes; ``--layer`` runs a whole decoder layer, with
+that model's dense products or with 64 experts of 1408 channels, 6 a token, behind the attention.
 """
 from __future__ import annotations
 
@@ -15,6 +17,7 @@ import argparse
 import torch
 
 from . import quantize_pack, w4a16_gemm
+from .layer import interleave_gate_up, rms_norm, w4a16_linear
 from .kvcache import Int4KVCache, cache_append, cache_attention
 
 
@@ -41,19 +44,28 @@ def slots_of(page_table: torch.Tensor, sequence: torch.Tensor, positions: torch.
 
 
 class AttentionBlock:
-    """Projections ``wqkv`` and ``wo`` as (packed words, scales), a cache, and a rotary table."""
+    """Projections ``wqkv`` and ``wo`` as (packed words, scales), a cache, and a rotary table.
 
-    def __init__(self, wqkv, wo, q_heads: int, cache: Int4KVCache, cos_sin: torch.Tensor):
+    With ``norm`` (the weight of a root-mean-square norm) the block is x + attention(norm x); without, attention(x).
+    """
+
+    def __init__(self, wqkv, wo, q_heads: int, cache: Int4KVCache, cos_sin: torch.Tensor, norm: torch.Tensor | None = None,
+                 eps: float = 1e-5):
         self.wqkv, self.wo, self.q_heads, self.cache, self.cos_sin = wqkv, wo, q_heads, cache, cos_sin
+        self.norm, self.eps = norm, eps
 
     def __call__(self, x, positions, slots, page_table, seq_lens, cu_q=None, max_q=None, **mask):
         """x fp16 [tokens, hidden] -> fp16 [tokens, hidden]; see cache_append and cache_attention."""
         hq, hk, d = self.q_heads, self.cache.kv_heads, self.cache.head_dim
-        qkv = w4a16_gemm(self.wqkv[0], x, self.wqkv[1]).view(x.shape[0], hq + 2 * hk, d)
+        h = x if self.norm is None else rms_norm(x, self.norm, self.eps)
+        qkv = w4a16_gemm(self.wqkv[0], h, self.wqkv[1]).view(x.shape[0], hq + 2 * hk, d)
         q = cache_append(self.cache, qkv[:, hq:hq + hk], qkv[:, hq + hk:], slots, q=qkv[:, :hq], positions=positions,
                          cos_sin=self.cos_sin)
         y = cache_attention(q, self.cache, page_table, seq_lens, cu_q=cu_q, max_q=max_q, **mask)
-        return w4a16_gemm(self.wo[0], y.view(x.shape[0], hq * d), self.wo[1])
+        y = y.view(x.shape[0], hq * d)
+        if self.norm is None:
+            return w4a16_gemm(self.wo[0], y, self.wo[1])
+        return w4a16_linear(self.wo[0], y, self.wo[1], residual=x)
 
 
 class DecodeLoop:
@@ -98,6 +110,22 @@ class DecodeLoop:
         return self.out
 
 
+def random_layer(attention: AttentionBlock, kind: str, hidden: int, rand):
+    """A decoder layer around ``attention`` with random weights: dense (14336 channels) or 64 experts of 1408, 6 a token."""
+    from .mlp_block import DecoderLayer, ExpertBlock, MLPBlock
+
+    def weights(inner):
+        gate_up = quantize_pack(interleave_gate_up(rand(inner, hidden) * 0.02, rand(inner, hidden) * 0.02), 128)
+        return gate_up, quantize_pack(rand(hidden, inner) * 0.02, 128)
+
+    norm = torch.ones(hidden, dtype=torch.float16, device="cuda")
+    if kind == "dense":
+        return DecoderLayer(attention, MLPBlock(*weights(14336), norm))
+    pairs = [weights(1408) for _ in range(64)]
+    gate_up, down = (tuple(torch.stack(t) for t in zip(*(p[i] for p in pairs))) for i in (0, 1))
+    return DecoderLayer(attention, ExpertBlock((rand(hidden, 64) * 0.02).half(), gate_up, down, 6, norm))
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
     ap.add_argument("--batch", type=int, default=8)
@@ -105,6 +133,7 @@ def main(argv=None):
     ap.add_argument("--steps", type=int, default=64)
     ap.add_argument("--page-size", type=int, default=64)
     ap.add_argument("--group-size", type=int, default=128)
+    ap.add_argument("--layer", choices=("none", "dense", "experts"), default="none", help="run a decoder layer around the block")
     args = ap.parse_args(argv)
     hidden, hq, hk, d, b = 4096, 32, 8, 128, args.batch
     gen = torch.Generator(device="cuda").manual_seed(0)
@@ -114,7 +143,10 @@ def main(argv=None):
     lens = [max(1, args.prompt - args.prompt * i // (2 * b)) for i in range(b)]
     pages = -(-(args.prompt + args.steps + 1) // args.page_size)
     cache = Int4KVCache(b * pages, hk, d, args.page_size, args.group_size)
-    block = AttentionBlock(wqkv, wo, hq, cache, rotary_table(args.prompt + args.steps + 1, d))
+    norm = None if args.layer == "none" else torch.ones(hidden, dtype=torch.float16, device="cuda")
+    block = AttentionBlock(wqkv, wo, hq, cache, rotary_table(args.prompt + args.steps + 1, d), norm)
+    if args.layer != "none":
+        block = random_layer(block, args.layer, hidden, rand)
     table = torch.randperm(b * pages, generator=gen, device="cuda").to(torch.int32).view(b, pages)
     seq_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
     cu_q = torch.tensor([0] + lens, device="cuda").cumsum(0).to(torch.int32)
