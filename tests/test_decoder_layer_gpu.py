@@ -47,8 +47,8 @@ def norm64(x, w):
 
 
 def gated(z):
-    z = z.view(len(z), -1, 2, 8)
-    return (act64(z[:, :, 0], "silu") * z[:, :, 1]).reshape(len(z), -1)
+    z = z.view(len(z), z.shape[1] // 16, 2, 8)
+    return (act64(z[:, :, 0], "silu") * z[:, :, 1]).flatten(1)
 
 
 def reference(layer, x, positions, sequences):

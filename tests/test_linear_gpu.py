@@ -27,7 +27,7 @@ EPILOGUES = [
 
 
 def act64(z, name):
-    t = torch.from_numpy(np.asarray(z))
+    t = torch.as_tensor(z)
     if name == "relu":
         return t.clamp_min(0)
     if name == "silu":

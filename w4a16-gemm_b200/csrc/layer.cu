@@ -9,19 +9,20 @@
 
 namespace w4a16 {
 
-// Widths by who owns a row: a warp up to 256 values, then as few threads as hold it in one or two vectors
-// each, since a row's barrier costs more the more warps meet there.
+// Widths by who owns a row: up to a warp for 256 values, then as few threads as hold it in two vectors each, since
+// fewer threads a row are more rows in flight.
 template <typename T, typename R>
 static cudaError_t launch_norm_t(const NormArgs& a, cudaStream_t stream, bool pdl) {
     const int vecs = a.dim / 8;
     const auto grid = [&](int rows) { return dim3((unsigned)((a.rows + rows - 1) / rows)); };
-    if (vecs <= 8) return launch(rms_norm_kernel<T, R, 8, 1, 16>, grid(16), 128, 0, stream, pdl, a);
-    if (vecs <= 16) return launch(rms_norm_kernel<T, R, 16, 1, 8>, grid(8), 128, 0, stream, pdl, a);
-    if (vecs <= 32) return launch(rms_norm_kernel<T, R, 32, 1, 4>, grid(4), 128, 0, stream, pdl, a);
-    if (vecs <= 128) return launch(rms_norm_kernel<T, R, 128, 1, 1>, grid(1), 128, 0, stream, pdl, a);
-    if (vecs <= 256) return launch(rms_norm_kernel<T, R, 256, 1, 1>, grid(1), 256, 0, stream, pdl, a);
-    if (vecs <= 512) return launch(rms_norm_kernel<T, R, 512, 1, 1>, grid(1), 512, 0, stream, pdl, a);
+    if (vecs <= 8) return launch(rms_norm_kernel<T, R, 8, 1, 32>, grid(32), 256, 0, stream, pdl, a);
+    if (vecs <= 16) return launch(rms_norm_kernel<T, R, 16, 1, 16>, grid(16), 256, 0, stream, pdl, a);
+    if (vecs <= 32) return launch(rms_norm_kernel<T, R, 32, 1, 8>, grid(8), 256, 0, stream, pdl, a);
+    if (vecs <= 128) return launch(rms_norm_kernel<T, R, 64, 2, 1>, grid(1), 64, 0, stream, pdl, a);
+    if (vecs <= 256) return launch(rms_norm_kernel<T, R, 128, 2, 1>, grid(1), 128, 0, stream, pdl, a);
+    if (vecs <= 512) return launch(rms_norm_kernel<T, R, 256, 2, 1>, grid(1), 256, 0, stream, pdl, a);
     if (vecs <= 1024) return launch(rms_norm_kernel<T, R, 512, 2, 1>, grid(1), 512, 0, stream, pdl, a);
+    if (vecs <= 2048) return launch(rms_norm_kernel<T, R, 1024, 2, 1>, grid(1), 1024, 0, stream, pdl, a);
     return launch(rms_norm_kernel<T, R, 1024, 4, 1>, grid(1), 1024, 0, stream, pdl, a);
 }
 
