@@ -118,3 +118,21 @@ def test_order_of_gated_rows():
         interleave_gate_up(gate[:12], up[:12])
     with pytest.raises(RuntimeError, match="one shape"):
         interleave_gate_up(gate, up[:8])
+
+
+def test_structures_are_laid_out_as_the_header_says(tmp_path):
+    import os
+    import subprocess
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    lines = []
+    for c, struct in (("w4a16_epilogue", capi.Epilogue), ("w4a16_norm_args", capi.NormArgs), ("w4a16_moe_args", capi.MoeArgs)):
+        lines.append(f'printf("%zu\\n", sizeof({c}));')
+        lines += [f'printf("%zu\\n", offsetof({c}, {name}));' for name, _ in struct._fields_]
+    (tmp_path / "s.c").write_text("#include <stddef.h>\n#include <stdio.h>\n#include \"w4a16.h\"\nint main(void) {\n" + "\n".join(lines) + "\nreturn 0; }\n")
+    subprocess.run(["gcc", "-std=c99", "-pedantic", "-Wall", "-Werror", "-I", include, str(tmp_path / "s.c"), "-o", str(tmp_path / "s")], check=True)
+    got = [int(v) for v in subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.split()]
+    want = []
+    for struct in (capi.Epilogue, capi.NormArgs, capi.MoeArgs):
+        want.append(ctypes.sizeof(struct))
+        want += [getattr(struct, name).offset for name, _ in struct._fields_]
+    assert got == want

@@ -18,7 +18,8 @@ pytestmark = pytest.mark.gpu
 # tokens, experts, k, hidden, inner, groups of both products
 SHAPES = [(1, 1, 1, 64, 64, 64, 64), (1, 8, 2, 256, 192, 128, 64), (1, 128, 8, 512, 128, 128, 128), (3, 4, 4, 384, 320, 128, 64), (5, 3, 1, 64, 1216, 64, 64),
           (8, 16, 2, 1024, 512, 128, 128), (33, 64, 6, 256, 128, 64, 128), (20, 8, 3, 512, 448, 128, 64), (70, 5, 2, 384, 384, 64, 128),
-          (200, 12, 4, 256, 128, 128, 64), (700, 8, 2, 128, 192, 64, 64)]
+          (200, 12, 4, 256, 128, 128, 64), (700, 8, 2, 128, 192, 64, 64),
+          (200, 128, 8, 64, 64, 64, 64), (2, 40, 32, 128, 64, 64, 64), (40, 40, 32, 64, 128, 64, 128), (120, 6, 2, 448, 320, 64, 64), (31, 1, 1, 64, 64, 64, 64)]
 
 
 def make(T, E, k, H, I, G1, G2, seed=0):

@@ -16,7 +16,10 @@
 // 128 rows took 242; 192 entries: the same).  A tile's rows come from a list; a tile of fewer rows is multiplied as the
 // narrowest product that holds them.  A stage is two 64-wide K chunks in two copies, rows and words.
 //
-// Bound by the rows: every 128 channels read the tile's rows again, 8 KB a chunk beside 4 KB of words, about 8 TB/s from L2.
+// Bound by the tensor cores' products: one of 128 channels with A from TMEM takes about 106 clocks for 16 K, be it 16 or 64
+// rows wide (256 rows take 128; clocks of the issuing thread: 1700 of a chain's 2100 a stage are the products', the
+// waits come to 420).  Wider tiles need accumulators that two chains an SM have no room for; measured and slower were one chain
+// of 128 rows (above) and one of 64 rows and 256 channels (192 entries: 517 -> 582 us).
 #pragma once
 #include <cuda.h>
 #include <cuda_fp16.h>
