@@ -191,7 +191,7 @@ w4a16_status w4a16_gemm_ex(const int32_t* Wp, const void* x, const void* scales,
 
 w4a16_status w4a16_linear(const int32_t* Wp, const void* x, const void* scales, void* y, int64_t M, int64_t N, int64_t K,
                           int64_t groups, int64_t wp_words, const w4a16_epilogue* epilogue, int32_t variant,
-                          uint32_t flags, void* workspace, uint64_t workspace_bytes, void* stream) {
+                          uint32_t flags, void* workspace, uint64_t workspace_bytes, void* stream) try {
     w4a16_status s = w4a16_validate(Wp, x, scales, M, N, K, groups, wp_words, variant);
     if (s != W4A16_OK) return s;
     if (N == 0) return fail(W4A16_ERR_N_MULTIPLE, "N must be at least 16");
@@ -214,6 +214,8 @@ w4a16_status w4a16_linear(const int32_t* Wp, const void* x, const void* scales, 
                         plain ? w4a16::kEpiNone : e.gated ? w4a16::kEpiGated : w4a16::kEpiPlain,
                         {e.bias, e.residual, e.activation}},
                        variant);
+} catch (...) {
+    return W4A16_ERR_CUDA;      // out of host memory: no exception crosses the boundary
 }
 
 w4a16_status w4a16_gemm(const int32_t* Wp, const void* x, const void* scales, void* y, int64_t M, int64_t N,
@@ -692,7 +694,7 @@ bool rows_apart(const View& v, int64_t tokens, int64_t heads, int64_t dim) {
 
 }  // namespace
 
-w4a16_status w4a16_rms_norm(const w4a16_norm_args* args, void* stream) {
+w4a16_status w4a16_rms_norm(const w4a16_norm_args* args, void* stream) try {
     if (!args) return fail(W4A16_ERR_NULL_POINTER, "args must be non-null");
     const w4a16_norm_args& n = *args;
     w4a16_status s = check_act_dtype(n.dtype);
@@ -732,10 +734,12 @@ w4a16_status w4a16_rms_norm(const w4a16_norm_args* args, void* stream) {
     if ((s = check_device(&d)) != W4A16_OK) return s;
     const cudaError_t err = w4a16::launch_rms_norm(n, static_cast<cudaStream_t>(stream), pdl_enabled());
     return err == cudaSuccess ? ok() : cuda_fail(err);
+} catch (...) {
+    return W4A16_ERR_CUDA;      // out of host memory: no exception crosses the boundary
 }
 
 w4a16_status w4a16_moe_route(const void* logits, int32_t dtype, int64_t row_stride, int64_t tokens, int32_t num_experts,
-                             int32_t k, int32_t renormalize, float* weights, int32_t* experts, void* stream) {
+                             int32_t k, int32_t renormalize, float* weights, int32_t* experts, void* stream) try {
     if (dtype < W4A16_LOGITS_F16 || dtype > W4A16_LOGITS_F32)
         return fail(W4A16_ERR_ACT_DTYPE, "dtype of the logits must be 0 (fp16), 1 (bf16) or 2 (fp32)");
     if (num_experts < 1 || num_experts > w4a16::kRouteMaxExperts)
@@ -758,6 +762,8 @@ w4a16_status w4a16_moe_route(const void* logits, int32_t dtype, int64_t row_stri
     const cudaError_t err = w4a16::launch_moe_route(logits, dtype, row_stride, tokens, num_experts, k, renormalize != 0,
                                                     weights, experts, static_cast<cudaStream_t>(stream), pdl_enabled());
     return err == cudaSuccess ? ok() : cuda_fail(err);
+} catch (...) {
+    return W4A16_ERR_CUDA;      // out of host memory: no exception crosses the boundary
 }
 
 // ------------------------------------------------------------------ expert layer
@@ -788,7 +794,7 @@ w4a16_status check_moe_sizes(const w4a16_moe_args* args) {
 
 }  // namespace
 
-w4a16_status w4a16_moe_workspace(const w4a16_moe_args* args, uint64_t* bytes) {
+w4a16_status w4a16_moe_workspace(const w4a16_moe_args* args, uint64_t* bytes) try {
     w4a16_status s = check_moe_sizes(args);
     if (s != W4A16_OK) return s;
     if (!bytes) return fail(W4A16_ERR_NULL_POINTER, "bytes must be non-null");
@@ -798,9 +804,11 @@ w4a16_status w4a16_moe_workspace(const w4a16_moe_args* args, uint64_t* bytes) {
     if ((s = check_device(&d)) != W4A16_OK) return s;
     *bytes = w4a16::moe_workspace(*args, d);
     return ok();
+} catch (...) {
+    return W4A16_ERR_CUDA;      // out of host memory: no exception crosses the boundary
 }
 
-w4a16_status w4a16_moe_experts(const w4a16_moe_args* args, void* workspace, uint64_t workspace_bytes, void* stream) {
+w4a16_status w4a16_moe_experts(const w4a16_moe_args* args, void* workspace, uint64_t workspace_bytes, void* stream) try {
     w4a16_status s = check_moe_sizes(args);
     if (s != W4A16_OK) return s;
     const w4a16_moe_args& a = *args;
@@ -828,6 +836,8 @@ w4a16_status w4a16_moe_experts(const w4a16_moe_args* args, void* workspace, uint
     if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(W4A16_ERR_WORKSPACE, "workspace must be 256-byte aligned");
     const cudaError_t err = w4a16::launch_moe_experts(a, d, workspace, static_cast<cudaStream_t>(stream), pdl_enabled());
     return err == cudaSuccess ? ok() : cuda_fail(err);
+} catch (...) {
+    return W4A16_ERR_CUDA;      // out of host memory: no exception crosses the boundary
 }
 
 w4a16_status w4a16_device_status(int32_t* code, int32_t reset) {

@@ -402,9 +402,8 @@ __global__ void __launch_bounds__(kDcCols) decode_combine_kernel(void* __restric
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int c = cc + i;
-            const float* const q = p + (size_t)(c == cf ? slot_f : 2 * c) * kDcSlotFloats;
-            v[i] = c <= cl ? __ldcg(q) : 0.f;
-            if (EPI == kEpiGated) u[i] = c <= cl ? __ldcg(q + 8) : 0.f;
+            v[i] = c <= cl ? __ldcg(p + (size_t)(c == cf ? slot_f : 2 * c) * kDcSlotFloats) : 0.f;
+            if (EPI == kEpiGated) u[i] = c <= cl ? __ldcg(p + 8 + (size_t)(c == cf ? slot_f : 2 * c) * kDcSlotFloats) : 0.f;
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {

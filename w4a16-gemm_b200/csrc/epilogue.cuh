@@ -17,6 +17,9 @@
 
 namespace w4a16 {
 
+// The activations in fp32.  erf is CUDA's: below z = -3, where 1 + erf cancels, gelu is off by up to |z| 2^-24, a step or
+// two of fp16's smallest.
+//
 // z * sigmoid(t).  exp and the division are the fast ones: a few fp32 ulps for |t| up to 88 (where the
 // result has vanished in 16 bits), against the 2^-11 of the rounding that follows.
 __device__ __forceinline__ float times_sigmoid(float z, float t) {

@@ -114,9 +114,9 @@ __device__ __forceinline__ int scan_threads(int v, int* shared) {
 static __global__ void __launch_bounds__(kMoePlanThreads) moe_plan_kernel(const __grid_constant__ MoeParams p) {
     __shared__ int count[kMoeMaxExperts], cursor[kMoeMaxExperts], warps[32];
     const int t = threadIdx.x;
-    pdl_launch_dependents();
     count[t] = 0;
     pdl_wait();
+    pdl_launch_dependents();
     __syncthreads();
     const auto expert_of = [&](int i) {
         const int e = i < p.entries ? __ldg(p.experts + i) : -1;
@@ -186,7 +186,7 @@ struct MoeSmallTile {
 };
 
 // The same for up to kMoeFewEntries entries, by every CTA in its shared memory, in one order: expert by expert, the
-// entries of one as they are numbered.  scratch: two words an expert, six bytes an entry.  Returns the number of tiles.
+// entries of one as they are numbered (the CTAs of a call have to agree).  scratch: two words an expert, six bytes an entry.  Returns the number of tiles.
 template <int THREADS>
 __device__ __forceinline__ int moe_sort_few(const MoeParams& p, MoeSmallTile* tiles, uint16_t* order, char* scratch) {
     constexpr int PER = (kMoeMaxExperts + THREADS - 1) / THREADS;
@@ -197,6 +197,31 @@ __device__ __forceinline__ int moe_sort_few(const MoeParams& p, MoeSmallTile* ti
     int32_t* const expert = first + kMoeMaxExperts;
     uint16_t* const rank = reinterpret_cast<uint16_t*>(expert + kMoeFewEntries);
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    if (p.entries <= 32) {               // one warp, in registers: experts by their first entry
+        if (warp == 0) {
+            const int raw = lane < p.entries ? __ldg(p.experts + lane) : -1;
+            const int e = raw >= 0 && raw < p.num_experts ? raw : -1;
+            const uint32_t same = __match_any_sync(0xffffffffu, e);
+            const int n = __popc(same), leader = __ffs(same) - 1;
+            const bool leads = e >= 0 && leader == lane;
+            const uint32_t mine = leads ? (uint32_t)n | (uint32_t)((n + p.plan.rows - 1) / p.plan.rows) << 16 : 0u;
+            uint32_t end = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t u = __shfl_up_sync(0xffffffffu, end, o);
+                if (lane >= o) end += u;
+            }
+            const uint32_t before = end - mine;
+            const int start = __shfl_sync(0xffffffffu, before, leader) & 0xffff;
+            if (e >= 0) order[start + __popc(same & ((1u << lane) - 1))] = (uint16_t)lane;
+            if (leads)
+                for (int i = 0; i * p.plan.rows < n; ++i)
+                    tiles[(before >> 16) + i] = {(uint16_t)e, (uint16_t)min(p.plan.rows, n - i * p.plan.rows), (uint32_t)(start + i * p.plan.rows)};
+            if (lane == 31) sums[0] = end;
+        }
+        __syncthreads();
+        return (int)(sums[0] >> 16);
+    }
     for (int i = t; i < kMoeMaxExperts; i += THREADS) count[i] = 0;
     for (int i = t; i < p.entries; i += THREADS) {
         const int e = __ldg(p.experts + i);

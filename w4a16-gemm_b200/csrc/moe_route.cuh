@@ -48,8 +48,8 @@ __device__ __forceinline__ float logit_at(const __nv_bfloat16* p, int64_t i) { r
 
 template <typename T, int VALUES>
 __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(RouteArgs a) {
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();      // after the wait: the next kernel may read ahead what the one before this wrote
     const int lane = threadIdx.x & 31;
     const int64_t token = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
     if (token >= a.tokens) return;

@@ -110,8 +110,8 @@ template <typename T, typename R, int THREADS, int VPT, int ROWS>
 __global__ void __launch_bounds__(THREADS * ROWS, VPT <= 2 ? 2048 / (THREADS * ROWS) : 1) rms_norm_kernel(NormArgs a) {
     constexpr bool ADD = !std::is_same_v<R, void>;
     __shared__ float shared[THREADS > 32 ? THREADS / 32 : 1];
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();      // after the wait: the next kernel may read ahead what the one before this wrote
     const int64_t row = (int64_t)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x / THREADS : 0);
     const int dim = row < a.rows ? a.dim : 0;     // past the last row: nothing is read or written
     const int64_t token = row / a.heads, head = row - token * a.heads;
