@@ -16,10 +16,10 @@
 // 128 rows took 242; 192 entries: the same).  A tile's rows come from a list; a tile of fewer rows is multiplied as the
 // narrowest product that holds them.  A stage is two 64-wide K chunks in two copies, rows and words.
 //
-// Bound by the tensor cores' products: one of 128 channels with A from TMEM takes about 106 clocks for 16 K, be it 16 or 64
-// rows wide (256 rows take 128; clocks of the issuing thread: 1700 of a chain's 2100 a stage are the products', the
-// waits come to 420).  Wider tiles need accumulators that two chains an SM have no room for; measured and slower were one chain
-// of 128 rows (above) and one of 64 rows and 256 channels (192 entries: 517 -> 582 us).
+// Bound by the hand-overs of a chain, not by the tensor cores (leaving out three products of four: 518 -> 444 us, and the
+// drains: 463).  With groups of 128 by the issuing warp (2100 clocks a stage when one lane polled its barriers one after
+// the other; three lanes at once, one commit less and one descriptor: 192 entries an expert 517 -> 462 us), with groups
+// of 64 by the drain, 630 clocks of its warps' own for each 64 K.  One chain of 64 rows and 256 channels was slower (582).
 #pragma once
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -86,7 +86,7 @@ moe_grouped_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     if (threadIdx.x == 0) {
         for (int s = 0; s < ST; ++s) {
             mbar_init(full(s), 1);
-            mbar_init(empty(s), kMgDqWarps + 1);   // the dequantising warps + the MMA commit
+            mbar_init(empty(s), kMgDqWarps);       // the dequantising warps, for the MMAs too
         }
         for (int a = 0; a < NA; ++a) {
             mbar_init(afull(a), kMgDqWarps);
@@ -138,40 +138,48 @@ moe_grouped_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
-        if (lane == 0) {
-            int it = 0, gi = 0;
-            bool ok = true;
-            for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
-                const MgTile t = mg_tile(tile, n_tiles, groups);
-                const uint32_t idesc = (pf_idesc<TOK>() & ~(63u << 17)) | ((uint32_t)((t.rows + 15) / 16 * 2) << 17);
-                for (int kt = 0; kt < KT && ok; ++kt, ++it) {
-                    const int s = it % ST, a = it % NA;
-                    if (!mbar_wait(full(s), (it / ST) & 1, kDevTimeoutPipeline) ||
-                        !mbar_wait(afull(a), (it / NA) & 1, kDevTimeoutPipeline)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint32_t xa = base + s * C::STAGE, at = tmem + (uint32_t)(C::A_COL0 + a * C::A_COLS);
-                    const int nch = KC - kt * C::KCH < C::KCH ? KC - kt * C::KCH : C::KCH;
-                    for (int j = 0; j < nch; ++j) {
-                        // a group is a chunk (G = 64) or two, wherever the stages end
-                        const bool first = G == 64 || (kt * C::KCH + j) % 2 == 0;
-                        if (first) {
-                            if (!mbar_wait(accempty(gi & 1), ((gi >> 1) & 1) ^ 1, kDevTimeoutPipeline)) { ok = false; break; }
-                            tc_fence_after();
-                        }
+        // This warp's instructions are what a stage waits for, so they are few: a stage's three barriers are polled by three
+        // lanes at once, and one descriptor is counted up (its 14 address bits never carry).
+        int it = 0, gi = 0;
+        bool ok = true;
+        const uint64_t desc0 = pf_sw128_desc(base);
+        const auto products = [&](int s, int a, int j, uint32_t idesc, bool first) {      // of one chunk
+            const uint32_t d = tmem + (uint32_t)((gi & 1) * TOK), at = tmem + (uint32_t)(C::A_COL0 + a * C::A_COLS + j * 32);
+            const uint64_t x = desc0 + (uint32_t)((s * C::STAGE + j * TOK * 128) >> 4);
 #pragma unroll
-                        for (int k16 = 0; k16 < 4; ++k16)
-                            tc_mma_ts(tmem + (uint32_t)((gi & 1) * TOK), at + j * 32 + k16 * 8,
-                                      pf_sw128_desc(xa + j * TOK * 128 + k16 * 32), idesc, !(first && k16 == 0));
-                        if (G == 64 || !first) {
-                            tc_commit(accfull(gi & 1));
-                            ++gi;
-                        }
-                    }
-                    if (!ok) break;
-                    tc_commit(empty(s));
-                    tc_commit(aempty(a));
+            for (int k16 = 0; k16 < 4; ++k16) tc_mma_ts(d, at + k16 * 8, x + k16 * 2, idesc, !(first && k16 == 0));
+        };
+        for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
+            const MgTile t = mg_tile(tile, n_tiles, groups);
+            const uint32_t idesc = (pf_idesc<TOK>() & ~(63u << 17)) | ((uint32_t)((t.rows + 15) / 16 * 2) << 17);
+            for (int kt = 0; kt < KT; ++kt, ++it) {
+                const int s = it % ST, a = it % NA;
+                const bool both = kt * C::KCH + 1 < KC;
+                const uint32_t bar = lane == 0 ? full(s) : lane == 1 ? afull(a) : accempty(gi & 1);
+                const uint32_t parity = lane == 0 ? (it / ST) & 1 : lane == 1 ? (it / NA) & 1 : ((gi >> 1) & 1) ^ 1;
+                ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, kDevTimeoutPipeline));
+                if (!ok) break;
+                tc_fence_after();
+                if (lane == 0) {
+                    products(s, a, 0, idesc, true);
+                    if (G == 128) products(s, a, 1, idesc, false);      // K has whole groups
+                    tc_commit(accfull(gi & 1));
                 }
+                ++gi;
+                if (G == 64 && both) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(accempty(gi & 1), ((gi >> 1) & 1) ^ 1, kDevTimeoutPipeline));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        products(s, a, 1, idesc, true);
+                        tc_commit(accfull(gi & 1));
+                    }
+                    ++gi;
+                }
+                if (lane == 0) tc_commit(aempty(a));
             }
+        }
+        if (lane == 0) {
             tc_commit(done_bar);   // every MMA of this CTA retired before TMEM is released
             mbar_wait(done_bar, 0, kDevTimeoutDrain);
         }
@@ -196,8 +204,9 @@ moe_grouped_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
 #pragma unroll
                     for (int j = 0; j < C::KCH; ++j)
                         if (j < nch) w[b][j] = lds128(sbw + (uint32_t)(((nbl + b) * KB + j) * 512 + lane * 16));
+                // the products of the stage whose A slot this is are done, and so is everyone with that stage
                 __syncwarp();
-                if (lane == 0) mbar_arrive(empty(s));      // this warp is done with the stage's packed words
+                if (lane == 0 && it >= NA) mbar_arrive(empty((it - NA) % ST));
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
