@@ -212,3 +212,20 @@ def test_refusals(cuda_device):
     refused("activation must be", activation="tanh")
     refused("apart from every input", out=g["s2"].view(-1)[:4 * 128].view(4, 128))
     refused("workspace too small", workspace=torch.zeros(256, dtype=torch.uint8, device="cuda"))
+
+
+@pytest.mark.parametrize("T", [2, 900])
+def test_weights_past_4_gb(cuda_device, T):
+    """The last expert of a layer of 5 GB gives what it gives alone: few entries, and more than 14 for each expert."""
+    from w4a16_opt import moe_experts
+    E, H, I = 60, 4096, 14336
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    words = lambda n: torch.randint(-(1 << 31), 1 << 31, (E, n), dtype=torch.int32, device="cuda", generator=gen)      # noqa: E731
+    scales = lambda *s: ((0.5 + torch.rand(*s, device="cuda", generator=gen)) / 500).half()                            # noqa: E731
+    gate_up, down = (words(2 * I * H // 8), scales(E, H // 128, 2 * I)), (words(H * I // 8), scales(E, I // 128, H))
+    x = torch.randn(T, H, device="cuda", generator=gen).half()
+    last, ones = torch.full((T, 1), E - 1, dtype=torch.int32, device="cuda"), torch.ones(T, 1, device="cuda")
+    y = moe_experts(x, gate_up, down, last, ones).float()
+    alone = moe_experts(x, tuple(t[-1:] for t in gate_up), tuple(t[-1:] for t in down), torch.zeros_like(last), ones).float()
+    # the same sums, perhaps in other pieces of K: half a step of fp16 each, and the inner results are the same
+    assert bool(((y - alone).abs() <= 2.0 ** -10 * alone.abs() + 2.0 ** -16 * alone.abs().max()).all()) and float(alone.abs().max()) > 0.1

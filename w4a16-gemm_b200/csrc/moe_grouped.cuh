@@ -126,7 +126,7 @@ moe_grouped_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 const MgTile t = mg_tile(tile, n_tiles, groups);
                 for (int kt = 0; kt < KT; ++kt, ++it) {
                     const int s = it % ST;
-                    if (!mbar_wait(empty(s), ((it / ST) & 1) ^ 1, kDevTimeoutPipeline)) { ok = false; break; }
+                    if (!mbar_wait(empty(s), ((it / ST) & 1) ^ 1, kDevTimeoutExperts)) { ok = false; break; }
                     const uint32_t sb = base + s * C::STAGE;
                     mbar_arrive_expect_tx(full(s), (uint32_t)(KB * (TOK * 128 + kPfWBytes)));
                     tma_load_3d(sb, &tm_x, 0, t.row0, kt * C::KCH, full(s));
@@ -134,7 +134,7 @@ moe_grouped_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 }
             }
             if (!ok)      // the last stages that were issued may still be landing
-                for (int j = max(0, it - ST); j < it; ++j) mbar_wait(full(j % ST), (j / ST) & 1, kDevTimeoutDrain);
+                for (int j = max(0, it - ST); j < it; ++j) mbar_wait(full(j % ST), (j / ST) & 1, kDevTimeoutExperts);
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
@@ -157,7 +157,7 @@ moe_grouped_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 const bool both = kt * C::KCH + 1 < KC;
                 const uint32_t bar = lane == 0 ? full(s) : lane == 1 ? afull(a) : accempty(gi & 1);
                 const uint32_t parity = lane == 0 ? (it / ST) & 1 : lane == 1 ? (it / NA) & 1 : ((gi >> 1) & 1) ^ 1;
-                ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, kDevTimeoutPipeline));
+                ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, kDevTimeoutExperts));
                 if (!ok) break;
                 tc_fence_after();
                 if (lane == 0) {
@@ -167,7 +167,7 @@ moe_grouped_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 }
                 ++gi;
                 if (G == 64 && both) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(accempty(gi & 1), ((gi >> 1) & 1) ^ 1, kDevTimeoutPipeline));
+                    ok = __all_sync(0xffffffffu, mbar_wait(accempty(gi & 1), ((gi >> 1) & 1) ^ 1, kDevTimeoutExperts));
                     if (!ok) break;
                     tc_fence_after();
                     if (lane == 0) {
@@ -181,7 +181,7 @@ moe_grouped_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         }
         if (lane == 0) {
             tc_commit(done_bar);   // every MMA of this CTA retired before TMEM is released
-            mbar_wait(done_bar, 0, kDevTimeoutDrain);
+            mbar_wait(done_bar, 0, kDevTimeoutExperts);
         }
     } else if (warp < kMgEpiWarp0) {
         // ------------------------------------------------------------ codes -> TMEM A ring (q - 8, exact)
@@ -192,8 +192,8 @@ moe_grouped_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         for (int tile = blockIdx.x; tile < total && ok; tile += gridDim.x) {
             for (int kt = 0; kt < KT; ++kt, ++it) {
                 const int s = it % ST, a = it % NA;
-                bool w_ok = mbar_wait(full(s), (it / ST) & 1, kDevTimeoutPipeline);
-                w_ok = w_ok && mbar_wait(aempty(a), ((it / NA) & 1) ^ 1, kDevTimeoutPipeline);
+                bool w_ok = mbar_wait(full(s), (it / ST) & 1, kDevTimeoutExperts);
+                w_ok = w_ok && mbar_wait(aempty(a), ((it / NA) & 1) ^ 1, kDevTimeoutExperts);
                 if (!__all_sync(0xffffffffu, w_ok)) { ok = false; break; }
                 tc_fence_after();
                 const int nch = KC - kt * C::KCH < C::KCH ? KC - kt * C::KCH : C::KCH;
@@ -249,7 +249,7 @@ moe_grouped_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 const float scale = __half2float(next);
                 next = after;
                 if (g + 2 < scale_groups) after = __ldg(s_at + (int64_t)(g + 2) * N);
-                ok = __all_sync(0xffffffffu, mbar_wait(accfull(gi & 1), (gi >> 1) & 1, kDevTimeoutPipeline));
+                ok = __all_sync(0xffffffffu, mbar_wait(accfull(gi & 1), (gi >> 1) & 1, kDevTimeoutExperts));
                 if (!ok) break;
                 tc_fence_after();
                 if (rows_here) {
