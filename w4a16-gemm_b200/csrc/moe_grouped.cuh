@@ -254,14 +254,12 @@ moe_grouped_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 tc_fence_after();
                 if (rows_here) {
                     const uint32_t at = tcol + (uint32_t)((gi & 1) * TOK);
+uint32_t r[CW];       // all of the warp's columns in one wait
+                    tmem_ld_cols<16>(at, *reinterpret_cast<uint32_t(*)[16]>(&r[0]));
+                    tmem_ld_cols<16>(at + 16, *reinterpret_cast<uint32_t(*)[16]>(&r[16]));
+                    tc_wait_ld();
 #pragma unroll
-                    for (int c0 = 0; c0 < CW; c0 += 16) {
-                        uint32_t r[16];
-                        tmem_ld_cols<16>(at + (uint32_t)c0, r);
-                        tc_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) sum[c0 + i] = fmaf(scale, __uint_as_float(r[i]), sum[c0 + i]);
-                    }
+                    for (int i = 0; i < CW; ++i) sum[i] = fmaf(scale, __uint_as_float(r[i]), sum[i]);
                 }
                 tc_fence_before();
                 __syncwarp();
