@@ -465,7 +465,7 @@ typedef struct w4a16_moe_args {
 /* A mixture-of-experts layer: with e = experts[t][j],
  *     h_tj = act(x_t Wg_e^T) * (x_t Wu_e^T),   y_t = residual_t + sum_j weights[t][j] (h_tj Wd_e^T).
  * Rows of the gated weights alternate as in w4a16_epilogue; a weight is (q - 8) * scale.  Sums are fp32; h is
- * rounded to fp16, y once.  Pointers are 16-byte aligned (experts and weights 4-byte).  The workspace is scratch, 256-byte
+ * rounded to fp16, y once: an |h| of 65520 or more becomes infinite, and its token's y is not finite.  Pointers are 16-byte aligned (experts and weights 4-byte).  The workspace is scratch, 256-byte
  * aligned, one per concurrent call. */
 w4a16_status w4a16_moe_experts(const w4a16_moe_args* args, void* workspace, uint64_t workspace_bytes, void* stream);
 

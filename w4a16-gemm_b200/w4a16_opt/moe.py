@@ -36,7 +36,8 @@ def moe_experts(x: torch.Tensor, gate_up, down, experts: torch.Tensor, weights: 
     group size (64 or 128); at most 1024 experts.  ``experts`` int32 and ``weights`` fp32 [tokens, k], as ``moe_route``
     gives them; an expert outside [0, experts) adds nothing (another device's, say), the same one twice counts twice.
 
-    Sums are fp32; the inner results are rounded to fp16, y once.  ``out`` may be ``residual`` or ``x``.
+    Sums are fp32; the inner results act(gate) * up are rounded to fp16, as ``w4a16_linear`` would return them, and y once: where
+    an inner result passes fp16's 65504, its token's y is not finite.  ``out`` may be ``residual`` or ``x``.
     ``workspace``: optional scratch CUDA buffer (256-byte aligned); without it the binding keeps one per (device, stream).
     """
     return _C.moe_experts(x, gate_up[0], gate_up[1], down[0], down[1], experts, weights, activation_code(activation),
