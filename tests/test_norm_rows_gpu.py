@@ -1,0 +1,44 @@
+"""GPU tests of the norm's rows that share a warp (dim up to 128: four or two of them), where some need their squares summed again
+at another scale and their neighbours do not.  Tolerances as in test_norm_gpu, derived there."""
+import pytest
+import torch
+
+from test_norm_gpu import check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("pattern", ["alternate", "first", "last", "pairs"])
+@pytest.mark.parametrize("kind", ["bf16", "bf16 + bf16", "bf16 + fp32", "fp16 + fp32"])
+@pytest.mark.parametrize("rows,dim", [(37, 8), (64, 40), (66, 64), (35, 72), (34, 128), (20, 136), (9, 256), (6, 1024)])
+def test_large_rows_beside_ordinary_ones(cuda_device, rows, dim, kind, pattern):
+    from w4a16_opt import rms_norm
+    gen = torch.Generator().manual_seed(rows + dim)
+    dtype = torch.float16 if kind.startswith("fp16") else torch.bfloat16
+    rtype = torch.float32 if kind.endswith("fp32") else dtype
+    x = torch.randn(rows, dim, generator=gen).to(dtype).cuda()
+    r = torch.randn(rows, dim, generator=gen).to(rtype).cuda() if "+" in kind else None
+    w = (1 + 0.3 * torch.randn(dim, generator=gen)).to(dtype).cuda()
+    at = torch.arange(rows)
+    large = {"alternate": at % 2 == 1, "first": at % 4 == 0, "last": at == rows - 1, "pairs": at % 4 > 1}[pattern].cuda()
+    norm = lambda x, r: (rms_norm(x, w), x) if r is None else rms_norm(x, w, residual=r)      # noqa: E731
+    clean, h_clean = norm(x, r)
+    target = x if r is None else r
+    target[large] = (target[large].float() * 1e37).to(target.dtype)
+    y, h = norm(x, r)
+    assert torch.equal(y[~large], clean[~large]) and torch.equal(h[~large], h_clean[~large])
+    full = x.cpu().double() if r is None else x.cpu().double() + r.cpu().double()
+    check(y, full, w, 1e-5)
+
+
+@pytest.mark.parametrize("dim", [8, 64, 128])
+def test_infinities_and_nan_beside_ordinary_rows(cuda_device, dim):
+    from w4a16_opt import rms_norm
+    gen = torch.Generator().manual_seed(dim)
+    x, w = torch.randn(11, dim, generator=gen).half().cuda(), torch.ones(dim).half().cuda()
+    clean = rms_norm(x, w)
+    x[1, 5], x[6, 2] = float("inf"), float("nan")
+    y = rms_norm(x, w)
+    keep = [t for t in range(11) if t not in (1, 6)]
+    assert torch.equal(y[keep], clean[keep])
+    assert y[1, 5].isnan() and (y[1, :5] == 0).all() and y[6].isnan().all()

@@ -142,17 +142,22 @@ __global__ void __launch_bounds__(THREADS * ROWS, VPT <= 2 ? 2048 / (THREADS * R
     sum = row_sum<THREADS>(sum, shared);
     const float n = (float)a.dim;
     // squares of large finite values (bf16 and fp32 reach 3e38) pass fp32: then the row is scaled by 2^-80 for
-    // its sum, which keeps every square of 2^127 finite and loses none that counts beside it
+    // its sum, which keeps every square of 2^127 finite and loses none that counts beside it.  Rows that share a warp
+    // share its shuffles, so a warp sums again if one of its rows has to, and the others keep their first sum.
     float scale = rsqrtf(sum / n + a.eps), shrink = 1.f;
-    if (!(sum < INFINITY)) {
-        shrink = 0x1p-80f;
+    const bool large = !(sum < INFINITY);
+    if (THREADS < 32 ? __any_sync(0xffffffffu, large) : large) {
+        constexpr float S = 0x1p-80f;
         sum = 0.f;
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j] * shrink, h[i][j] * shrink, sum);
+            for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j] * S, h[i][j] * S, sum);
         sum = row_sum<THREADS>(sum, shared);
-        scale = rsqrtf(sum / n);                  // eps vanishes beside it
+        if (large) {
+            shrink = S;
+            scale = rsqrtf(sum / n);              // eps vanishes beside it
+        }
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
