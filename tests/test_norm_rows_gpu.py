@@ -31,6 +31,31 @@ def test_large_rows_beside_ordinary_ones(cuda_device, rows, dim, kind, pattern):
     check(y, full, w, 1e-5)
 
 
+# the means of squares leave fp32 where eps is at the ends of its range too: rows from subnormals to near the largest value, each its own size
+@pytest.mark.parametrize("eps", [0.0, 1e-45, 1e-38, 1e-30, 1e-19, 1.0, 1e30, 1e38, 3e38])
+@pytest.mark.parametrize("residual", [None, "same", "fp32"])
+@pytest.mark.parametrize("dim", [8, 64, 128, 264, 2048, 16640])
+def test_rows_of_every_size_with_every_eps(cuda_device, dim, residual, eps):
+    from w4a16_opt import rms_norm
+    gen = torch.Generator().manual_seed(dim)
+    sizes = torch.logspace(-39, 37, 39).double()[:, None]
+    x = (torch.randn(39, dim, generator=gen).double() * sizes).bfloat16().cuda()
+    w = (1 + 0.3 * torch.randn(dim, generator=gen)).bfloat16().cuda()
+    if residual is None:
+        y, h = rms_norm(x, w, eps), x.cpu().double()
+    else:
+        r = (torch.randn(39, dim, generator=gen).double() * sizes).to(torch.bfloat16 if residual == "same" else torch.float32).cuda()
+        y, _ = rms_norm(x, w, eps, residual=r)
+        h = (x.float() + r.float()).cpu().double()        # the sum itself is one fp32 addition
+    eps = torch.tensor(eps, dtype=torch.float32).double().item()      # as the entry point takes it
+    want = h / torch.sqrt((h * h).mean(-1, keepdim=True) + eps) * w.cpu().double()
+    # results below bf16's normal numbers: half a step of its subnormals, 2^-134, and fp32's own steps on the way there (2^-149 of a
+    # scaled value, times a scale of at most 2^19 and a weight of at most 2^2: 2^-128)
+    tol = want.abs() * (2.0 ** -8 + 2.0 ** -17) + 2.0 ** -127
+    off = (y.cpu().double() - want).abs() / tol
+    assert bool((off <= 1).all()), (off.max(), off.max(1).values)
+
+
 @pytest.mark.parametrize("dim", [8, 64, 128])
 def test_infinities_and_nan_beside_ordinary_rows(cuda_device, dim):
     from w4a16_opt import rms_norm

@@ -6,7 +6,8 @@
 // unrounded h.  Bound by the memory's bandwidth: a row is read once and stays in registers between its
 // sum and its scaling.  8 values (16 bytes) a load; THREADS threads own a row, each VPT such vectors.  What a
 // row takes is its latency (loads, two barriers, stores), so the rows in flight count: 32 registers a thread, 2048
-// threads an SM (8192 rows of 8192 with a residual, bf16: 118 -> 91 us, 5.9 TB/s).  Rows of up to 256 values go to one
+// threads an SM, a few bytes of spills included (8192 rows of 8192 with a residual, bf16: 118 -> 91 us; in a graph 85, 6.3 TB/s).
+// The sum x + residual is stored as soon as it is made, so that what is kept of it may be scaled.  Rows of up to 256 values go to one
 // warp or to a part of one (8 lanes a row of 64 values, 16 of 128): no shared memory, no barrier.
 #pragma once
 #include <cuda_bf16.h>
@@ -128,6 +129,7 @@ __global__ void __launch_bounds__(THREADS * ROWS, VPT <= 2 ? 2048 / (THREADS * R
                 load8<R>(a.residual, token * a.residual_token + head * a.residual_head + at, r);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) h[i][j] += r[j];
+                store8<R>(a.residual_out, token * a.out_token + head * a.out_head + at, h[i]);
             }
         } else {
 #pragma unroll
@@ -141,33 +143,37 @@ __global__ void __launch_bounds__(THREADS * ROWS, VPT <= 2 ? 2048 / (THREADS * R
         for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
     sum = row_sum<THREADS>(sum, shared);
     const float n = (float)a.dim;
-    // squares of large finite values (bf16 and fp32 reach 3e38) pass fp32: then the row is scaled by 2^-80 for
-    // its sum, which keeps every square of 2^127 finite and loses none that counts beside it.  Rows that share a warp
-    // share its shuffles, so a warp sums again if one of its rows has to, and the others keep their first sum.
-    float scale = rsqrtf(sum / n + a.eps), shrink = 1.f;
-    const bool large = !(sum < INFINITY);
-    if (THREADS < 32 ? __any_sync(0xffffffffu, large) : large) {
-        constexpr float S = 0x1p-80f;
+    // squares of large finite values (bf16 and fp32 reach 3e38) pass fp32, and those of values below 2^-60 or so, which count
+    // where eps is as small, fall out of it: then the row is scaled by 2^-80 or 2^80 for its sum.  The first keeps every square of
+    // 2^127 finite and loses none that counts beside it; with the second, for means below 2^-64, a row's squares stay
+    // below 2^111, and full down to values of 2^-143.  Rows that share a warp share its shuffles, so a warp sums again if one of its
+    // rows has to, and the others keep their first sum.
+    const float mean = sum / n + a.eps;
+    float scale = rsqrtf(mean);
+    const bool again = !(mean >= 0x1p-64f && mean < INFINITY);
+    if (THREADS < 32 ? __any_sync(0xffffffffu, again) : again) {
+        const float s = mean < 1.f ? 0x1p80f : 0x1p-80f;
         sum = 0.f;
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j] * S, h[i][j] * S, sum);
+            for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j] * s, h[i][j] * s, sum);
         sum = row_sum<THREADS>(sum, shared);
-        if (large) {
-            shrink = S;
-            scale = rsqrtf(sum / n);              // eps vanishes beside it
+        if (again) {
+            scale = rsqrtf(sum / n + a.eps * s * s);
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[i][j] *= s;
         }
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
         const int at = (i * THREADS + t) * 8;
         if (at < dim) {
-            if constexpr (ADD)
-                store8<R>(a.residual_out, token * a.out_token + head * a.out_head + at, h[i]);
             load8<T>(a.weight, at, w[i]);      // the same for every row: there in L1
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * shrink * scale * w[i][j];
+            for (int j = 0; j < 8; ++j) h[i][j] = h[i][j] * scale * w[i][j];
             store8<T>(a.y, yo + at, h[i]);
         }
     }
