@@ -17,20 +17,38 @@
 
 namespace w4a16 {
 
-// The activations in fp32.  erf is CUDA's: below z = -3, where 1 + erf cancels, gelu is off by up to |z| 2^-24, a step or
-// two of fp16's smallest.
+// The activations in fp32, each good to 2^-16 or so of its own value down to z = -9: with a gate the other factor may be large
+// where the activation is small.  exp and the division are the fast ones; exp's error grows with its argument t, 2 + 1.2 |t|
+// fp32 ulps (26 at 20, where the factor is 2e-9), against the 2^-11 of the rounding that follows.
 //
-// z * sigmoid(t).  exp and the division are the fast ones: a few fp32 ulps for |t| up to 88 (where the
-// result has vanished in 16 bits), against the 2^-11 of the rounding that follows.
+// z * sigmoid(t).
 __device__ __forceinline__ float times_sigmoid(float z, float t) {
     return __fdividef(z, 1.f + __expf(-t));
+}
+
+// The normal distribution's Phi(z).  1 + erf(z / sqrt 2) would cancel below -3 (7 % off at -5, all of it from -5.5 on), so the
+// smaller tail is made, Phi(-a) = exp(-a^2 / 2) r(a) at a = |z|: r falls from 1/2 as 1 / (a sqrt(2 pi)), and r / t is a polynomial of
+// t = 1 / (1 + 0.3625 a), of degree 6 for a relative error of 7.7e-7 up to a = 14 (a weighted least-squares fit, the weights
+// repeated until the error was level; 2.7e-6 in fp32).  erfcf is as good but longer:
+// a prompt's plain product with bias and gelu, 2048 x 14336 x 4096, takes 341 us with it, 289 with erff, 260 with this.
+__device__ __forceinline__ float normal_below(float z) {
+    const float a = fabsf(z), t = __fdividef(1.f, fmaf(a, 0.3625f, 1.f));
+    float q = 0.0480628535f;
+    q = fmaf(q, t, -0.179742277f);
+    q = fmaf(q, t, 0.175103799f);
+    q = fmaf(q, t, 0.029682558f);
+    q = fmaf(q, t, 0.139256671f);
+    q = fmaf(q, t, 0.142936394f);
+    q = fmaf(q, t, 0.144700378f);
+    q *= t * __expf(-0.5f * a * a);
+    return z < 0.f ? q : 1.f - q;
 }
 
 __device__ __forceinline__ float activate(float z, int activation) {
     switch (activation) {
         case W4A16_ACTIVATION_RELU: return z < 0.f ? 0.f : z;          // NaN stays
         case W4A16_ACTIVATION_SILU: return times_sigmoid(z, z);
-        case W4A16_ACTIVATION_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678f));
+        case W4A16_ACTIVATION_GELU: return z * normal_below(z);
         case W4A16_ACTIVATION_GELU_TANH:                               // (1 + tanh u) / 2 = sigmoid(2u)
             return times_sigmoid(z, 1.5957691f * (z + 0.044715f * z * z * z));
         default: return z;
