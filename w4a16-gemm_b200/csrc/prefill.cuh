@@ -369,16 +369,18 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__
         for (int tile = blockIdx.x; tile < total; tile += gridDim.x, ++tc) {
             const int tt = tile / n_tiles, tn = tile % n_tiles;
             const int b = tc % NACC;
+            if (EPI == kEpiNone && !__all_sync(0xffffffffu, mbar_wait(accfull(b), (tc / NACC) & 1, kDevTimeoutPipeline))) break;
             const int n = tn * kPfRows + 32 * q + lane;
             const int tok0 = tt * TOK + h * CW;
-            // what is added to the sums: fetched before the wait for them
             float bias = 0.f;
             uint32_t hv[EPI == kEpiGated ? CW / 4 : CW / 2];
+            // what is added to the sums is fetched before the wait for them (the plain store has nothing to fetch, and
+            // registers that live across a wait would be spilled)
             if constexpr (EPI != kEpiNone) {
                 if (epi.bias && n < N) bias = half_at(epi.bias, n);
                 load_residual<EPI, CW>(hv, epi, tok0, M, n, N);
+                if (!__all_sync(0xffffffffu, mbar_wait(accfull(b), (tc / NACC) & 1, kDevTimeoutPipeline))) break;
             }
-            if (!__all_sync(0xffffffffu, mbar_wait(accfull(b), (tc / NACC) & 1, kDevTimeoutPipeline))) break;
             tc_fence_after();
             const uint32_t tcol = tmem + lane_field + (uint32_t)(b * TOK + h * CW);
             if (OUT_F32) {
