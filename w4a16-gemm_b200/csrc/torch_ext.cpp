@@ -524,6 +524,11 @@ std::tuple<torch::Tensor, torch::Tensor> moe_route_py(torch::Tensor logits, int6
     return {weights, experts};
 }
 
+// A prompt's expert layer takes 2 * inner + 6 * hidden bytes a (token, choice), gigabytes for long ones.  Above this size the
+// workspace is the call's own: it goes back to torch's allocator (which reuses it in stream order), instead of staying
+// with the stream for good.  Such calls run for 200 us and more, and an allocation costs the host two.
+constexpr uint64_t kMoeKeptWorkspace = 64ull << 20;
+
 torch::Tensor moe_experts_py(torch::Tensor x, torch::Tensor gate_up_wp, torch::Tensor gate_up_scales, torch::Tensor down_wp,
                              torch::Tensor down_scales, torch::Tensor experts, torch::Tensor weights, int64_t activation,
                              c10::optional<torch::Tensor> residual, c10::optional<torch::Tensor> out,
@@ -588,7 +593,7 @@ torch::Tensor moe_experts_py(torch::Tensor x, torch::Tensor gate_up_wp, torch::T
         ws_bytes = (uint64_t)ws.numel() * ws.element_size();
     } else {
         check(w4a16_moe_workspace(&a, &ws_bytes));
-        ws = workspace_for(x, ws_bytes, stream);
+        ws = ws_bytes > kMoeKeptWorkspace ? fresh({(int64_t)ws_bytes}, torch::kUInt8, x) : workspace_for(x, ws_bytes, stream);
     }
     check(w4a16_moe_experts(&a, ws.defined() ? ws.data_ptr() : nullptr, ws_bytes, stream));
     return y;

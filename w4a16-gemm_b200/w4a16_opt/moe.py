@@ -37,8 +37,11 @@ def moe_experts(x: torch.Tensor, gate_up, down, experts: torch.Tensor, weights: 
     gives them; an expert outside [0, experts) adds nothing (another device's, say), the same one twice counts twice.
 
     Sums are fp32; the inner results act(gate) * up are rounded to fp16, as ``w4a16_linear`` would return them, and y once: where
-    an inner result passes fp16's 65504, its token's y is not finite.  For a given number of tokens a token's y depends on its own inputs alone, bit for bit.  ``out`` may be ``residual`` or ``x``.
-    ``workspace``: optional scratch CUDA buffer (256-byte aligned); without it the binding keeps one per (device, stream).
+    an inner result passes fp16's 65504, its token's y is not finite.  For a given number of tokens a token's y depends on
+    its own inputs alone, bit for bit.  tokens * k * max(inner / 8, hidden / 4) must be below 2^31.
+
+    ``out`` may be ``residual`` or ``x``.  ``workspace``: optional scratch CUDA buffer (256-byte aligned); without it the binding
+    keeps one per (device, stream) for calls that need up to 64 MB, and takes a larger one from torch's allocator for the call.
     """
     return _C.moe_experts(x, gate_up[0], gate_up[1], down[0], down[1], experts, weights, activation_code(activation),
                           residual, out, workspace)
