@@ -246,7 +246,7 @@ __device__ __forceinline__ int moe_sort_few(const MoeParams& p, MoeSmallTile* ti
         }
     }
     __syncthreads();
-    // entries and tiles before each expert, 16 bits each, two experts a thread
+    // entries and tiles before each expert, 16 bits each, PER experts a thread
     uint32_t mine[PER], v = 0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
@@ -402,9 +402,9 @@ __device__ __forceinline__ bool moe_batch(uint32_t base, MoeRing<MoeCfg::STAGES>
     return ok;
 }
 
-// A CTA's walk: batches of up to 8 blocks of one (tile, K range), over its range of units.  Unit u is block u % blocks
+// A CTA's walk: batches of up to BLOCKS blocks of one (tile, K range), over its range of units.  Unit u is block u % blocks
 // of K range u / blocks % splits of tile u / blocks / splits.  Batches of one range are of one size to within a block: a
-// short last one would take as many turns as a full one (25 blocks as 8 + 8 + 8 + 1 instead of 7 + 6 + 6 + 6 made
+// short last one would take as many turns as a full one (25 blocks by 8, as 8 + 8 + 8 + 1 instead of 7 + 6 + 6 + 6, made
 // the slowest CTA 36 us late where the others took 29).
 template <int BLOCKS>
 struct MoeWalk {

@@ -254,7 +254,7 @@ moe_grouped_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 tc_fence_after();
                 if (rows_here) {
                     const uint32_t at = tcol + (uint32_t)((gi & 1) * TOK);
-uint32_t r[CW];       // all of the warp's columns in one wait
+                    uint32_t r[CW];       // all of the warp's columns in one wait
                     tmem_ld_cols<16>(at, *reinterpret_cast<uint32_t(*)[16]>(&r[0]));
                     tmem_ld_cols<16>(at + 16, *reinterpret_cast<uint32_t(*)[16]>(&r[16]));
                     tc_wait_ld();
@@ -301,7 +301,7 @@ uint32_t r[CW];       // all of the warp's columns in one wait
 }
 
 // ------------------------------------------------------------------ host side
-// x [K/64][rows][64] in boxes of a stage's chunks and 64 or 128 rows; the experts' words as one tall weight [experts * N /
+// x [K/64][rows][64] in boxes of a stage's chunks and a tile's rows; the experts' words as one tall weight [experts * N /
 // 16][K/64][128] in boxes of 8 blocks.
 cudaError_t make_grouped_tensor_maps(const GroupedArgs& a, CUtensorMap* tx, CUtensorMap* tw);
 
