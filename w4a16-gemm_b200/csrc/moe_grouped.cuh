@@ -269,19 +269,27 @@ moe_grouped_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
             const int row = t.row0 + h * CW, end = t.row0 + t.rows;
             if constexpr (GATED) {
                 // lanes l and l + 8 of a half warp hold the two factors: of each pair of rows the gate's lane makes the
-                // first one's result, the other lane the second one's (see prefill.cuh)
+                // first one's result, the other lane the second one's (see prefill.cuh).  Which activation it is is asked
+                // once, not for every value (2048 tokens of 6 of 64: groups of 64 588 -> 571 us, of 128 456 -> 441).
                 const bool up = lane >> 3 & 1;
                 uint32_t hv[CW / 4];
 #pragma unroll
-                for (int i = 0; i < CW / 4; ++i) {
-                    float v[2];
+                for (int i = 0; i < CW / 2; ++i) {
+                    const float z0 = sum[2 * i], z1 = sum[2 * i + 1];
+                    const float got = __shfl_xor_sync(0xffffffffu, up ? z0 : z1, 8);
+                    sum[2 * i] = up ? got : z0;
+                    sum[2 * i + 1] = up ? z1 : got;
+                }
+                if (activation == W4A16_ACTIVATION_SILU) {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float z0 = sum[4 * i + 2 * j], z1 = sum[4 * i + 2 * j + 1];
-                        const float got = __shfl_xor_sync(0xffffffffu, up ? z0 : z1, 8);
-                        v[j] = activate(up ? got : z0, activation) * (up ? z1 : got);
-                    }
-                    const __half2 p = __floats2half2_rn(v[0], v[1]);
+                    for (int i = 0; i < CW / 2; ++i) sum[2 * i] = times_sigmoid(sum[2 * i], sum[2 * i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < CW / 2; ++i) sum[2 * i] = activate(sum[2 * i], activation);
+                }
+#pragma unroll
+                for (int i = 0; i < CW / 4; ++i) {
+                    const __half2 p = __floats2half2_rn(sum[4 * i] * sum[4 * i + 1], sum[4 * i + 2] * sum[4 * i + 3]);
                     hv[i] = *reinterpret_cast<const uint32_t*>(&p);
                 }
                 store_gated<CW>(hv, static_cast<__half*>(yv), row, end, n, N);
