@@ -20,9 +20,11 @@ cudaError_t run_moe_wait_limit_check() {
     return err != cudaSuccess ? err : cudaDeviceSynchronize();
 }
 
-size_t moe_workspace(const w4a16_moe_args& a, const DeviceInfo& dev) {
-    return moe_plan(a.tokens, a.k, a.num_experts, a.hidden, a.inner, dev.num_sms).bytes;
+static MoePlan plan_of(const w4a16_moe_args& a, const DeviceInfo& dev) {
+    return moe_plan(a.tokens, a.k, a.num_experts, a.hidden, a.inner, dev.num_sms, a.gate_up_group == 128 && a.down_group == 128);
 }
+
+size_t moe_workspace(const w4a16_moe_args& a, const DeviceInfo& dev) { return plan_of(a, dev).bytes; }
 
 template <int G, bool GATED>
 static cudaError_t launch_product_t(const MoeParams& p, int grid, cudaStream_t stream, bool pdl) {
@@ -49,7 +51,7 @@ cudaError_t launch_moe_experts(const w4a16_moe_args& a, const DeviceInfo& dev, v
     p.residual = static_cast<const __half*>(a.residual);
     p.y = static_cast<__half*>(a.y);
     p.workspace = static_cast<char*>(workspace);
-    p.plan = moe_plan(a.tokens, a.k, a.num_experts, a.hidden, a.inner, dev.num_sms);
+    p.plan = plan_of(a, dev);
     p.entries = (int32_t)(a.tokens * a.k);
     p.k = a.k;
     p.num_experts = a.num_experts;

@@ -8,7 +8,7 @@
 // were chosen, each once a tile.  Which entries make which tile every CTA works out for itself, from up to 1024
 // entries (about 1 us, where a kernel in front takes 4); above that a kernel does it once, in front.
 //
-// Many entries an expert (more than 14 on average): the products of moe_grouped.cuh, over rows of x that a kernel puts
+// Many entries an expert (more than 14 on average, 10 with groups of 128): the products of moe_grouped.cuh, over rows of x that a kernel puts
 // into sorted order first.
 //
 // The second product's CTAs start where the first one's leave, and fetch their first weights before the first

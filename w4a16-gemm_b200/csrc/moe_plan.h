@@ -51,19 +51,27 @@ struct MoePlan {
     size_t tiles_at, order_at, place_at, rows_at, inner_at, out_at, bytes;
 };
 
-constexpr int kMoeGroupedEntries = 14;
+// More entries an expert than this, on average, are grouped; the second if both products have groups of 128.
+constexpr int kMoeGroupedEntries = 14, kMoeGroupedEntriesWide = 10;
 
 constexpr int kMoeGroupedRows = 64;  // entries of a grouped product's tile, at most
 
 W4A16_HD inline size_t moe_align(size_t n) { return (n + 255) / 256 * 256; }
 
-inline MoePlan moe_plan(int64_t tokens, int k, int experts, int hidden, int inner, int num_sms) {
+// wide_groups: both products' scales are of groups of 128.
+inline MoePlan moe_plan(int64_t tokens, int k, int experts, int hidden, int inner, int num_sms, bool wide_groups = false) {
     MoePlan p = {};
     const int64_t entries = tokens * k;
-    // more than 14 entries an expert: the experts' words are worth making into tensor-core operands for all of them (16
-    // entries an expert: 128 experts of 2048 x 768 262 us as few, 166 grouped; 64 of 2048 x 1408 186 and 165; 8 of 4096 x
-    // 14336 351 and 366; 24: 247 and 169, 467 and 367)
-    p.grouped = entries > kMoeGroupedEntries * (int64_t)experts;
+    // many entries an expert: its words are worth making into tensor-core operands for all of them.  As few and grouped, us from
+    // a graph, even loads, 8, 10, 12, 16 and 24 entries an expert:
+    //     128 experts of 2048 x 768, groups of 128     139 144   160 144   180 145   221 147   301 151
+    //      64 of 2048 x 1408, 128                      108 126   124 126   143 126   178 127   244 132
+    //       8 of 4096 x 14336, 128                     213 281   270 281   280 281   367 282   539 283
+    //      64 of 2048 x 1408, 64                       108 162   128 163   144 164   176 166   250 172
+    // With groups of 64 the grouped products drain twice as often, and the forms meet at 15 instead of 9 to 12.  Entries and experts
+    // are the call's, as it is told them: entries of experts outside the layer count (a slice of 8 of 64 experts, 32 tokens of 6:
+    // grouped 39 us, as few 23), and how they are spread does not (96 tokens to the same 6 of 64: as few 86, grouped 44).
+    p.grouped = entries > (wide_groups ? kMoeGroupedEntriesWide : kMoeGroupedEntries) * (int64_t)experts;
     // else 8, the width of mma.m16n8k16: with 16 a tile's two products for every word cost more than reading the words
     // of an expert twice (64 experts, 3 entries each: 82 us and 102; 8 each: 118 and 128)
     p.rows = p.grouped ? kMoeGroupedRows : kMoeRows;
