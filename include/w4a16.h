@@ -427,7 +427,10 @@ typedef struct w4a16_norm_args {
 
 /* Root-mean-square norm of rows: with h = x + residual (fp32), y = h * weight / sqrt(mean(h^2) + eps), and
  * residual_out = h; each rounded once (y from the unrounded h).  Pointers are 16-byte aligned, strides not
- * negative; the rows of an output must not overlap one another. */
+ * negative; the rows of an output must not overlap one another.  Where an output is not an input's very view, no
+ * address between its first and its last element may lie between an input's or the other output's: views that alternate in one buffer
+ * are refused.  eps is in [0, 3e38], and rows may be of any size: means of squares that fp32 does not hold are made at
+ * another scale. */
 w4a16_status w4a16_rms_norm(const w4a16_norm_args* args, void* stream);
 
 typedef enum w4a16_logits_dtype {
@@ -465,7 +468,8 @@ typedef struct w4a16_moe_args {
 /* A mixture-of-experts layer: with e = experts[t][j],
  *     h_tj = act(x_t Wg_e^T) * (x_t Wu_e^T),   y_t = residual_t + sum_j weights[t][j] (h_tj Wd_e^T).
  * Rows of the gated weights alternate as in w4a16_epilogue; a weight is (q - 8) * scale.  Sums are fp32; h is
- * rounded to fp16, y once: an |h| of 65520 or more becomes infinite, and its token's y is not finite.  Pointers are 16-byte aligned (experts and weights 4-byte).  The workspace is scratch, 256-byte
+ * rounded to fp16, y once: an |h| of 65520 or more becomes infinite, and its token's y is not finite.  How the work is cut goes by
+ * tokens * k over num_experts: a slice of a larger layer with most entries outside it is cut as if all were inside.  Pointers are 16-byte aligned (experts and weights 4-byte).  The workspace is scratch, 256-byte
  * aligned, one per concurrent call. */
 w4a16_status w4a16_moe_experts(const w4a16_moe_args* args, void* workspace, uint64_t workspace_bytes, void* stream);
 

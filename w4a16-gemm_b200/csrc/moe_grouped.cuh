@@ -12,14 +12,16 @@
 //
 // Tiles of 64 rows and 128 channels, two CTAs an SM, each with half of TMEM (two accumulators, two slots of A) and its own
 // chain of copies, operands, products and sums: a stage of one chain takes about 0.8 us whatever its tile, so two chains
-// are worth more than tiles of twice the rows (16 entries an expert: 64 experts of 2048 x 1408 165 us where one CTA with
+// were worth more than tiles of twice the rows (16 entries an expert: 64 experts of 2048 x 1408 165 us where one CTA with
 // 128 rows took 242; 192 entries: the same).  A tile's rows come from a list; a tile of fewer rows is multiplied as the
 // narrowest product that holds them.  A stage is two 64-wide K chunks in two copies, rows and words.
 //
 // Bound by the hand-overs of a chain, not by the tensor cores (leaving out three products of four: 518 -> 444 us, and the
 // drains: 463).  With groups of 128 by the issuing warp (2100 clocks a stage when one lane polled its barriers one after
-// the other; three lanes at once, one commit less and one descriptor: 192 entries an expert 517 -> 462 us), with groups
-// of 64 by the drain, 630 clocks of its warps' own for each 64 K.  One chain of 64 rows and 256 channels was slower (582).
+// the other; three lanes at once, one commit less and one descriptor: 192 entries an expert 517 -> 462 us, 441 today), with
+// groups of 64 by the drain, 630 clocks of its warps' own for each 64 K (571 us).  The other shapes, one CTA of 128 rows and one chain of
+// 64 rows and 256 channels (582), were timed before the issuing warp was shortened, which they have more of a tile for, and
+// not since.
 #pragma once
 #include <cuda.h>
 #include <cuda_fp16.h>

@@ -61,7 +61,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, *, residu
     last dimension, other strides multiples of 8; dim a multiple of 8 up to 32768.  ``weight`` [dim] of x's dtype.
     ``residual`` of x's shape, in x's dtype or fp32; the sum is returned in its type, and the norm
     taken of the unrounded sum.  ``out`` and ``residual_out``, where the results go, may be ``x`` or ``residual``
-    themselves (the very same view) and otherwise must not overlap an input.
+    themselves (the very same view) and otherwise lie apart from every input, from first address to last (views that alternate in
+    one buffer are refused).
     """
     y, h = _C.rms_norm(x, weight, eps, residual, out, residual_out)
     return y if residual is None else (y, h)
