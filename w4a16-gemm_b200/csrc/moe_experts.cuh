@@ -33,8 +33,9 @@
 // product's results are rounded to fp16 once, being operands of the second product, whose results stay fp32
 // until the weighted sum.  That rounding is what a product with a gate returns on its own, its range with it (beyond 65504
 // an inner result is infinite); it is the only one before y's, and takes the error against 64 bits from 2.1e-4, what
-// y's rounding makes alone, to 2.9e-4.  Two halves for every value would keep fp32's bits for twice the products of
-// the second weight and twice the bytes of its rows.
+// y's rounding makes alone, to 2.9e-4.  Two fp16 numbers for every inner result keep fp32's bits (built, in both forms: 2.1e-4) for
+// twice the second weight's products and twice the bytes of its rows, and the same range: one token of 2 of 8 experts 47.0 ->
+// 50.7 us, 32 of 6 of 64 78.7 -> 86.7, 2048 of 6 of 64 560 -> 618 with groups of 64 and 440 -> 530 with groups of 128.  Not kept.
 #pragma once
 #include <cuda_fp16.h>
 #include <stdint.h>
