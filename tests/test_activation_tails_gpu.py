@@ -67,3 +67,22 @@ def test_experts(cuda_device, T, activation):
                     torch.ones(T, 1, device="cuda"), activation=activation)
     ref, tol = expected(-zg, torch.full((I,), 64.0), activation)
     close(y, (ref.expand(T, I), tol.expand(T, I) * 2))       # the inner result's rounding, y's
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("M", [2, 40])
+def test_infinite_and_not_a_number(cuda_device, M, gated):
+    """z of +inf passes, large negative z vanishes, NaN stays, beside ordinary columns."""
+    from w4a16_opt import interleave_gate_up, pack_int4, w4a16_linear
+    cols, K, inf = 16, 128, float("inf")
+    zg = torch.tensor([inf, -60000.0, float("nan"), 60000.0, 0.0, 1.0, -1.0, 30.0] * 2).half()
+    N = 2 * cols if gated else cols
+    Wp = pack_int4(torch.full((N, K), 8, dtype=torch.uint8)).cuda()
+    x, scales = torch.ones(M, K).half().cuda(), torch.ones(K // 64, N).half().cuda()
+    bias = interleave_gate_up(zg, torch.ones(cols).half()) if gated else zg
+    for activation in ("gelu", "silu", "gelu_tanh"):
+        y = w4a16_linear(Wp, x, scales, bias=bias.cuda(), activation=activation, gated=gated).cpu()
+        assert (y[:, ::8] == inf).all() and (y[:, 1::8] == 0).all() and y[:, 2::8].isnan().all() and (y[:, 3::8] == 60000).all()
+        assert (y[:, 4::8] == 0).all() and (y[:, 7::8] == 30).all()
+        one = act64(torch.tensor([1.0, -1.0]).double(), activation)
+        assert ((y[:, 5:7].double() - one).abs() <= 2.0 ** -10 * one.abs()).all()

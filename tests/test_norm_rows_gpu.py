@@ -67,3 +67,23 @@ def test_infinities_and_nan_beside_ordinary_rows(cuda_device, dim):
     keep = [t for t in range(11) if t not in (1, 6)]
     assert torch.equal(y[keep], clean[keep])
     assert y[1, 5].isnan() and (y[1, :5] == 0).all() and y[6].isnan().all()
+
+
+@pytest.mark.parametrize("large", [False, True])
+@pytest.mark.parametrize("rows,dim", [(9, 64), (5, 136), (4, 2048), (3, 8200), (2, 20480)])
+def test_outputs_in_each_others_inputs(cuda_device, rows, dim, large):
+    """The norm over the residual's place and the sum over x's; one tensor as both inputs and the sum."""
+    from w4a16_opt import rms_norm
+    gen = torch.Generator().manual_seed(dim)
+    draw = lambda: torch.randn(rows, dim, generator=gen).bfloat16().cuda()      # noqa: E731
+    x, r, w = draw(), draw(), draw()[0]
+    if large:
+        r[::2] *= 1e37
+    y, h = rms_norm(x, w, residual=r)
+    x2, r2 = x.clone(), r.clone()
+    rms_norm(x2, w, residual=r2, out=r2, residual_out=x2)
+    assert torch.equal(r2, y) and torch.equal(x2, h)
+    y, h = rms_norm(r, w, residual=r)
+    r2 = r.clone()
+    y2, _ = rms_norm(r2, w, residual=r2, residual_out=r2)
+    assert torch.equal(y2, y) and torch.equal(r2, h)
